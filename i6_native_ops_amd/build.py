@@ -1,5 +1,5 @@
-"""Builds the native parts in-tree: libi6fbw.so (HIP kernels + C ABI, hipcc, gfx950) and the
-PyTorch-ROCm bindings fbw_core and fast_viterbi_core (both link libi6fbw.so).  Takes the place of the reference's
+"""Builds the native parts in-tree: libi6fbw.so and libi6train.so (HIP kernels + C ABI, hipcc, gfx950) and the
+PyTorch-ROCm bindings fbw_core and fast_viterbi_core (both link libi6fbw.so) and training_core (links both).  Takes the place of the reference's
 setup.py FBW entry (setup.py:29-33) and its import-time JIT fallback (fbw/__init__.py:10-24):
 nothing is compiled at import time, and nothing is hipified."""
 import os
@@ -9,6 +9,8 @@ import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
+TRAINING = os.path.join(CSRC, "training")
+TRAINING_SOURCES = ("cross_entropy.hip", "recurrence.hip", "adamw.hip", "status.hip")
 OUT = os.path.join(PKG, "fbw")
 LIB = os.path.join(OUT, "libi6fbw.so")
 EXT = os.path.join(OUT, "fbw_core" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
@@ -42,27 +44,27 @@ def kernel_resources(remarks):
     return out
 
 
-def sources_digest():
+def sources_digest(folder=CSRC):
     """sha256 over the device sources and the compiler flags: kept inside kernel_resources.json, so that a record
     made from other sources than the ones present is recognised as such"""
     import hashlib
     h = hashlib.sha256(" ".join(HIP_FLAGS).encode())
-    for name in sorted(os.listdir(CSRC)):
+    for name in sorted(os.listdir(folder)):
         if name.endswith((".hip", ".inc", ".h")):
             h.update(name.encode())
-            h.update(open(os.path.join(CSRC, name), "rb").read())
+            h.update(open(os.path.join(folder, name), "rb").read())
     return h.hexdigest()
 
 
-def build_lib(out_root=PKG):
-    """libi6fbw.so into <out_root>/fbw (out_root: this package in the source tree, or its copy in a build tree),
-    and beside it kernel_resources.json: registers, scratch and occupancy of every kernel as the compiler reports
+def build_lib(out_root=PKG, sub="fbw", name="libi6fbw.so", folder=CSRC, sources=("fbw_kernels.hip",)):
+    """A library of kernels (libi6fbw.so) into <out_root>/<sub> (out_root: this package in the source tree, or its copy
+    in a build tree), and beside it kernel_resources.json: registers, scratch and occupancy of every kernel as the compiler reports
     them (a kernel that outgrows its register budget spills without a word and runs at half its speed;
     tests/test_boundary_cpu.py reads this record)."""
     import json
-    lib = os.path.join(out_root, "fbw", "libi6fbw.so")
+    lib = os.path.join(out_root, sub, name)
     os.makedirs(os.path.dirname(lib), exist_ok=True)
-    cmd = [HIPCC, *HIP_FLAGS, "-shared", "-Rpass-analysis=kernel-resource-usage", os.path.join(CSRC, "fbw_kernels.hip"), "-o", lib]
+    cmd = [HIPCC, *HIP_FLAGS, "-shared", "-Rpass-analysis=kernel-resource-usage", *(os.path.join(folder, s) for s in sources), "-o", lib]
     print(" ".join(cmd), flush=True)
     done = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     remarks = done.stdout
@@ -74,13 +76,18 @@ def build_lib(out_root=PKG):
     if done.returncode != 0:
         raise subprocess.CalledProcessError(done.returncode, cmd)
     record = kernel_resources(remarks)
-    record["_sources_sha256"] = sources_digest()
-    with open(os.path.join(out_root, "fbw", "kernel_resources.json"), "w") as f:
+    record["_sources_sha256"] = sources_digest(folder)
+    with open(os.path.join(out_root, sub, "kernel_resources.json"), "w") as f:
         json.dump(record, f, indent=1, sort_keys=True)
     return lib
 
 
-def build_ext(name="fbw_core", source="fbw_torch.cpp", out_dir=None, lib_dir=None):
+def build_training_lib(out_root=PKG):
+    """libi6train.so, with a record of its own"""
+    return build_lib(out_root, "training", "libi6train.so", TRAINING, TRAINING_SOURCES)
+
+
+def build_ext(name="fbw_core", source="fbw_torch.cpp", out_dir=None, lib_dir=None, more_libs=()):
     import torch
     from torch.utils import cpp_extension
     inc = cpp_extension.include_paths()
@@ -96,7 +103,7 @@ def build_ext(name="fbw_core", source="fbw_torch.cpp", out_dir=None, lib_dir=Non
     cmd += [os.path.join(CSRC, source), "-o", ext,
             "-L" + (lib_dir or OUT), "-li6fbw", "-L" + torch_lib, "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip",
             "-ltorch_python", "-L/opt/rocm/lib", "-lamdhip64",
-            "-Wl,-rpath,$ORIGIN", "-Wl,-rpath,$ORIGIN/../fbw", "-Wl,-rpath," + torch_lib, "-Wl,-rpath,/opt/rocm/lib", "-Wno-attributes"]
+            *more_libs, "-Wl,-rpath,$ORIGIN", "-Wl,-rpath,$ORIGIN/../fbw", "-Wl,-rpath," + torch_lib, "-Wl,-rpath,/opt/rocm/lib", "-Wno-attributes"]
     _run(cmd)
     return ext
 
@@ -107,6 +114,14 @@ def build_all(out_root=PKG):
     lib_dir = os.path.join(out_root, "fbw")
     build_ext("fbw_core", "fbw_torch.cpp", lib_dir, lib_dir)
     build_ext("fast_viterbi_core", "viterbi_torch.cpp", os.path.join(out_root, "fast_viterbi"), lib_dir)
+    build_training(out_root)
+
+
+def build_training(out_root=PKG):
+    """The operators around the losses; libi6fbw.so has to be there."""
+    build_training_lib(out_root)
+    out = os.path.join(out_root, "training")
+    build_ext("training_core", os.path.join("training", "training_torch.cpp"), out, os.path.join(out_root, "fbw"), ("-L" + out, "-li6train"))
 
 
 if __name__ == "__main__":

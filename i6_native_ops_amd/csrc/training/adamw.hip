@@ -1,0 +1,306 @@
+// AdamW over many tensors in one launch, states in 32 bits or in 8 (include/i6train.h).
+//
+// Bound by memory: a value in 32 bits moves 28 bytes (parameter and two states both ways, gradient one way), with
+// states in 8 bits 16.06.  The table of tensors travels in the kernel's arguments, so a step is one launch for up to kMaxTensors
+// tensors, copies nothing to the device and can be captured into a graph.  A workgroup takes kChunk consecutive values of one
+// tensor; which tensor, it finds by bisection over the first workgroup of each.
+#include <cmath>
+
+#include "train_common.h"
+
+// Sums and products are rounded one by one, as the definition states them: what is stored in 8 bits depends on
+// comparisons, and a contracted multiply-add would make them depend on the compiler.
+#pragma clang fp contract(off)
+
+namespace i6train {
+namespace {
+
+constexpr int kMaxTensors = 56;          // x 64 bytes: the arguments of a kernel may have 4 KB
+constexpr int kChunk = 4096;
+constexpr int kThreads = 256;
+constexpr float kE4m3Max = 448.f, kPerMax = 1.f / 448.f;
+constexpr float kLeastScale = 0x1p-100f;
+constexpr uint32_t kPhi = 2654435769u, kRoot = 1779033703u;
+
+struct Table {
+    i6train_adamw_tensor t[kMaxTensors];
+    int first[kMaxTensors];              // first workgroup of each tensor
+    int n;
+};
+static_assert(sizeof(Table) <= 3800, "kernel arguments");
+
+struct Factors {
+    float beta1, rest1, beta2, rest2, keep, rate, root_correction, eps;
+    uint32_t turn_m, turn_v;             // step ROOT and step PHI
+};
+
+__device__ __forceinline__ int find(const Table& tab, int wg) {
+    int lo = 0, hi = tab.n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (tab.first[mid] <= wg) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+template <typename T> using vec4 = T __attribute__((ext_vector_type(4)));
+using f32x4 = vec4<float>;
+
+// Four consecutive values; kAligned: the tensor's addresses allow one access.  `left` values are there.
+template <bool kAligned, typename T> __device__ __forceinline__ f32x4 load4(const T* p, int64_t left) {
+    if (kAligned && left >= 4) {
+        const vec4<T> v = *reinterpret_cast<const vec4<T>*>(p);
+        return f32x4{(float)v.x, (float)v.y, (float)v.z, (float)v.w};
+    }
+    f32x4 v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (i < left) v[i] = (float)p[i];
+    return v;
+}
+
+template <bool kAligned, typename T> __device__ __forceinline__ void store4(T* p, f32x4 v, int64_t left) {
+    if (kAligned && left >= 4) {
+        *reinterpret_cast<vec4<T>*>(p) = vec4<T>{(T)v.x, (T)v.y, (T)v.z, (T)v.w};
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (i < left) p[i] = (T)v[i];
+}
+
+// m, v and p of one value.
+__device__ __forceinline__ void update(const Factors& k, float g, float& p, float& m, float& v, float& root) {
+    m = m * k.beta1 + g * k.rest1;
+    v = v * k.beta2 + g * g * k.rest2;
+    root = sqrtf(v);
+    const float size = root * k.root_correction + k.eps;
+    p = p * k.keep - m / size * k.rate;
+}
+
+template <typename T, bool kAligned>
+__device__ __forceinline__ void chunk32(const i6train_adamw_tensor& t, const Factors& k, int64_t base) {
+    T* p = static_cast<T*>(t.param);
+    const T* g = static_cast<const T*>(t.grad);
+    float* m = static_cast<float*>(t.exp_avg);
+    float* v = static_cast<float*>(t.exp_avg_sq);
+#pragma unroll
+    for (int r = 0; r < kChunk / (4 * kThreads); r++) {
+        const int64_t at = base + (r * kThreads + threadIdx.x) * 4, left = t.n - at;
+        if (left <= 0) continue;
+        f32x4 pv = load4<kAligned>(p + at, left), mv = load4<kAligned>(m + at, left), vv = load4<kAligned>(v + at, left);
+        const f32x4 gv = load4<kAligned>(g + at, left);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float pi = pv[i], mi = mv[i], vi = vv[i], root;
+            update(k, gv[i], pi, mi, vi, root);
+            pv[i] = pi; mv[i] = mi; vv[i] = vi;
+        }
+        store4<kAligned>(p + at, pv, left);
+        store4<kAligned>(m + at, mv, left);
+        store4<kAligned>(v + at, vv, left);
+    }
+}
+
+// The largest of 64 lanes' values, in all of them.  The values are bit patterns of magnitudes, whose order as whole numbers is that of
+// the magnitudes with NaN on top, so a NaN in a block is not lost.
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+#define I6_STEP(ctrl, rows)                                                                                   \
+    {                                                                                                         \
+        const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xf, false);          \
+        x = y > x ? y : x;                                                                                    \
+    }
+    I6_STEP(0x111, 0xf)      // from 1, 2, 4, 8 lanes below within rows of 16
+    I6_STEP(0x112, 0xf)
+    I6_STEP(0x114, 0xf)
+    I6_STEP(0x118, 0xf)
+    I6_STEP(0x142, 0xa)      // the last lane of rows 0 and 2 to rows 1 and 3
+    I6_STEP(0x143, 0xc)      // that of row 1 to rows 2 and 3
+#undef I6_STEP
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+
+__device__ __forceinline__ float scale_of(uint32_t bits) {
+    const float s = __uint_as_float(bits) * kPerMax;
+    return s < kLeastScale ? kLeastScale : s;      // (NaN stays)
+}
+
+// Distance of the 8-bit values around y >= 0: 2^(e - 3), e the exponent, -6 at least.
+__device__ __forceinline__ float quantum(float y) {
+    uint32_t e = (__float_as_uint(y) >> 23) & 255u;
+    e = e < 121u ? 121u : e;
+    return __uint_as_float((e - 3u) << 23);
+}
+// 1 / quantum(y), a power of two as well
+__device__ __forceinline__ float per_quantum(float y) {
+    uint32_t e = (__float_as_uint(y) >> 23) & 255u;
+    e = e < 121u ? 121u : e;
+    return __uint_as_float((257u - e) << 23);
+}
+
+// m / scale rounded up with the probability that keeps its mean: floor(|y| / q + u) q.
+__device__ __forceinline__ float round_m(float y, float u) {
+    const float a = fabsf(y), q = quantum(a);
+    float k = floorf(a * per_quantum(a) + u) * q;
+    k = k > kE4m3Max ? kE4m3Max : k;
+    return copysignf(k, y);
+}
+
+// The root so that its square keeps its mean: up where y^2 - low^2 > u (high^2 - low^2).  The square would otherwise grow by the variance of
+// the rounding, up to 0.4 %, at every step, more than a step with beta2 = 0.999 forgets.  A root under the smallest value is rounded up:
+// what divides by it stays bounded.
+__device__ __forceinline__ float round_root(float y, float u) {
+    const float q = quantum(y);
+    const float low = floorf(y * per_quantum(y)) * q;
+    const bool up = (y * y - low * low > u * (q * (low + low + q))) || (low == 0.f && y > 0.f);
+    const float k = up ? low + q : low;
+    return k > kE4m3Max ? kE4m3Max : k;
+}
+
+__device__ __forceinline__ f32x4 from_fp8(uint32_t w) {
+    return f32x4{__builtin_amdgcn_cvt_f32_fp8((int)w, 0), __builtin_amdgcn_cvt_f32_fp8((int)w, 1), __builtin_amdgcn_cvt_f32_fp8((int)w, 2),
+                 __builtin_amdgcn_cvt_f32_fp8((int)w, 3)};
+}
+__device__ __forceinline__ uint32_t to_fp8(f32x4 v) {        // values of the format: nothing is rounded here
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v.x, v.y, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v.z, v.w, w, true);
+}
+
+template <bool kAligned> __device__ __forceinline__ uint32_t load_bytes(const uint8_t* p, int64_t left) {
+    if (kAligned && left >= 4) return *reinterpret_cast<const uint32_t*>(p);
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (i < left) w |= (uint32_t)p[i] << (8 * i);
+    return w;
+}
+template <bool kAligned> __device__ __forceinline__ void store_bytes(uint8_t* p, uint32_t w, int64_t left) {
+    if (kAligned && left >= 4) {
+        *reinterpret_cast<uint32_t*>(p) = w;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (i < left) p[i] = (uint8_t)(w >> (8 * i));
+}
+
+// A wave has a block of 256 values, four in each lane: the scale of a block is a reduction within the wave.
+template <typename T, bool kAligned>
+__device__ __forceinline__ void chunk8(const i6train_adamw_tensor& t, const Factors& k, int64_t base) {
+    T* p = static_cast<T*>(t.param);
+    const T* g = static_cast<const T*>(t.grad);
+    uint8_t* m8 = static_cast<uint8_t*>(t.exp_avg);
+    uint8_t* v8 = static_cast<uint8_t*>(t.exp_avg_sq);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    f32x4 um, uv;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t j = lane * 4 + i;
+        um[i] = (float)((j * kPhi + k.turn_m) >> 16) * 0x1p-16f;
+        uv[i] = (float)((j * kRoot + k.turn_v) >> 16) * 0x1p-16f;
+    }
+#pragma unroll
+    for (int r = 0; r < kChunk / (4 * kThreads); r++) {
+        const int64_t block = base / I6TRAIN_BLOCK + r * (kThreads / kWave) + wave;
+        if (block * I6TRAIN_BLOCK >= t.n) continue;          // the same for the whole wave
+        const int64_t at = block * I6TRAIN_BLOCK + lane * 4, left = t.n - at;
+        f32x4 pv = load4<kAligned>(p + at, left), gv = load4<kAligned>(g + at, left);
+        f32x4 mv = from_fp8(load_bytes<kAligned>(m8 + at, left)) * t.exp_avg_scale[block];
+        f32x4 vv = from_fp8(load_bytes<kAligned>(v8 + at, left)) * t.exp_avg_sq_scale[block];
+        f32x4 rv;
+        uint32_t most_m = 0, most_r = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float pi = pv[i], mi = mv[i], vi = vv[i] * vv[i], root;
+            update(k, gv[i], pi, mi, vi, root);
+            pv[i] = pi; mv[i] = mi; rv[i] = root;
+            const uint32_t bm = __float_as_uint(fabsf(mi)), br = __float_as_uint(fabsf(root));
+            most_m = bm > most_m ? bm : most_m;
+            most_r = br > most_r ? br : most_r;
+        }
+        const float sm = scale_of(wave_max(most_m)), sr = scale_of(wave_max(most_r));
+        const float per_m = 1.f / sm, per_r = 1.f / sr;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            mv[i] = round_m(mv[i] * per_m, um[i]);
+            rv[i] = round_root(rv[i] * per_r, uv[i]);
+        }
+        store4<kAligned>(p + at, pv, left);
+        store_bytes<kAligned>(m8 + at, to_fp8(mv), left);
+        store_bytes<kAligned>(v8 + at, to_fp8(rv), left);
+        if (lane == 0) {
+            t.exp_avg_scale[block] = sm;
+            t.exp_avg_sq_scale[block] = sr;
+        }
+    }
+}
+
+template <typename T, int BITS>
+__global__ __launch_bounds__(kThreads) void adamw_step(Table tab, Factors k) {
+    const int i = find(tab, blockIdx.x);
+    const i6train_adamw_tensor& t = tab.t[i];
+    const int64_t base = (int64_t)(blockIdx.x - tab.first[i]) * kChunk;
+    // one access for four values needs their size as alignment; views into a larger buffer may not have it
+    const uintptr_t whole = (uintptr_t)t.param | (uintptr_t)t.grad, state = (uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq;
+    const bool aligned = whole % (4 * sizeof(T)) == 0 && state % (BITS == 8 ? 4 : 16) == 0;
+    if (BITS == 8) {
+        if (aligned) chunk8<T, true>(t, k, base); else chunk8<T, false>(t, k, base);
+    } else {
+        if (aligned) chunk32<T, true>(t, k, base); else chunk32<T, false>(t, k, base);
+    }
+}
+
+template <typename T> void launch(const Table& tab, const Factors& k, int bits, int wgs, hipStream_t s) {
+    if (bits == 8) adamw_step<T, 8><<<dim3(wgs), dim3(kThreads), 0, s>>>(tab, k);
+    else adamw_step<T, 32><<<dim3(wgs), dim3(kThreads), 0, s>>>(tab, k);
+}
+
+}  // namespace
+}  // namespace i6train
+
+extern "C" int i6train_adamw(const i6train_adamw_tensor* tensors, int n_tensors, int dtype, int state_bits, int64_t step, double lr,
+                             double beta1, double beta2, double eps, double weight_decay, void* stream) {
+    using namespace i6train;
+    if (n_tensors < 0 || (n_tensors > 0 && !tensors) || !valid_dtype(dtype) || (state_bits != 8 && state_bits != 32) || step < 1 ||
+        !(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1) || !(eps >= 0) || !std::isfinite(lr) || !std::isfinite(weight_decay))
+        return I6TRAIN_ERR_INVALID_ARGUMENT;
+    for (int i = 0; i < n_tensors; i++) {
+        const i6train_adamw_tensor& t = tensors[i];
+        if (t.n < 0) return I6TRAIN_ERR_INVALID_ARGUMENT;
+        if (t.n == 0) continue;
+        if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq) return I6TRAIN_ERR_INVALID_ARGUMENT;
+        if (state_bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)) return I6TRAIN_ERR_INVALID_ARGUMENT;
+        if (t.n > ((int64_t)1 << 40)) return I6TRAIN_ERR_TOO_LARGE;
+    }
+    Factors k;
+    k.beta1 = (float)beta1; k.rest1 = (float)(1.0 - beta1);
+    k.beta2 = (float)beta2; k.rest2 = (float)(1.0 - beta2);
+    k.keep = (float)(1.0 - lr * weight_decay);
+    k.rate = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
+    k.root_correction = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
+    k.eps = (float)eps;
+    k.turn_m = (uint32_t)step * kRoot;
+    k.turn_v = (uint32_t)step * kPhi;
+    constexpr int64_t kMostGroups = 0x7fffffff;
+    Table tab;
+    tab.n = 0;
+    int64_t wgs = 0;
+    const auto flush = [&]() {
+        if (tab.n == 0) return I6TRAIN_OK;
+        if (dtype == I6TRAIN_BF16) launch<bf16>(tab, k, state_bits, (int)wgs, (hipStream_t)stream);
+        else launch<float>(tab, k, state_bits, (int)wgs, (hipStream_t)stream);
+        tab.n = 0;
+        wgs = 0;
+        return launched();
+    };
+    for (int i = 0; i < n_tensors; i++) {
+        if (tensors[i].n == 0) continue;
+        const int64_t need = ceil_div(tensors[i].n, (int64_t)kChunk);
+        if (tab.n == kMaxTensors || wgs + need > kMostGroups) I6TRAIN_TRY(flush());
+        tab.t[tab.n] = tensors[i];
+        tab.first[tab.n] = (int)wgs;
+        tab.n++;
+        wgs += need;
+    }
+    return flush();
+}

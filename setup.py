@@ -49,7 +49,7 @@ setup(
     version=_version(),
     description="Full-sum forward-backward (FBW) loss and best-path alignment of rwth-i6/i6_native_ops for AMD MI355X (gfx950)",
     packages=find_packages(include=["i6_native_ops_amd", "i6_native_ops_amd.*"]),
-    package_data={"i6_native_ops_amd": ["csrc/*.hip", "csrc/*.inc", "csrc/*.cpp", "csrc/*.h", "fbw/*.so", "fast_viterbi/*.so"]},
+    package_data={"i6_native_ops_amd": ["csrc/*.hip", "csrc/*.inc", "csrc/*.cpp", "csrc/*.h", "csrc/training/*", "fbw/*.so", "fast_viterbi/*.so", "training/*.so"]},
     cmdclass={"build_py": BuildWithNative},
     distclass=BinaryDistribution,
     python_requires=">=3.9",
