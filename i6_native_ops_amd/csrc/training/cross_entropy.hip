@@ -5,17 +5,21 @@
 //   backward   for one piece of the vocabulary after another: z again, G = g (softmax(z) - [f = y]) rounded to the operands'
 //              precision, then  dh += G W  and  dW = G^T h
 //
-// All three products run through one kernel, product(): C[m][n] = sum_k A[m][k] B[n][k] on the matrix units, both operands with
-// consecutive k, which differs in what becomes of a finished tile.  So that k is consecutive, G is written in both layouts, and h
-// and W are transposed once per backward call.
+// All three products run through one kernel, product(): C[m][n] = sum_k A[m][k] B[n][k] on the matrix units.  An operand lies in memory
+// with consecutive k (W and h for the logits, G for dh) or with consecutive m or n (W for dh, G and h for dW) and is turned
+// as it is read from LDS, so nothing is transposed or written twice.
 //
 // The frames of a batch are packed first: only frames that belong to a sequence are rows of the products, and what the others
-// hold is not read.  How many there are is known on the device alone: tiles behind the last row return at once.
+// hold is not read.  How many there are is known on the device alone: workgroups without a tile return at once.
 //
-// 32-bit operands.  The matrix units have 16-bit operands at sixteen times the rate of 32-bit ones.  A value x is split into x1 = f16(s x)
-// and x2 = f16(2^11 (s x - x1)), s a power of two that brings the tensor's largest value to 2^14..2^15: 22 bits down to 2^-29 of the largest
-// value.  Of (x1 + x2 2^-11)(y1 + y2 2^-11) the last term is below the precision and left out: the k-loop runs over x1 y2 and x2 y1,
-// scales the accumulators by 2^-11, and goes on with x1 y1.
+// Operands.  All products have 16-bit floating-point operands with 11 bits of precision, and sums in 32 bits.  Tensors are scaled by a
+// power of two that brings their largest finite value to 2^14 .. 2^15.  bfloat16 values (8 bits) are then held exactly down to 2^-29 of the
+// largest, and G to 2^-12 of each value instead of the 2^-9 that bfloat16 would leave.  A 32-bit value x is split into x1 = f16(s x) and
+// x2 = f16(2^11 (s x - x1)): 22 bits.  Of (x1 + x2 2^-11)(y1 + y2 2^-11) the last term is below the precision and left out: the k-loop runs
+// over x1 y2 and x2 y1, scales the accumulators by 2^-11, and goes on with x1 y1: three times the work, on units whose rate for 16-bit operands
+// is sixteen times that for 32-bit ones.
+//
+// Logits are in units of log 2 from the accumulators on: exponentials and logarithms are single instructions.
 #include <cmath>
 
 #include "train_common.h"
@@ -23,415 +27,597 @@
 namespace i6train {
 namespace {
 
-constexpr int kTile = 128;           // rows and columns of a workgroup's tile
-constexpr int kStep = 64;            // k of one turn: 128 bytes of a row
+constexpr int kM = 256, kN = 128;    // a workgroup's tile of C: four waves, 128 x 64 each
+constexpr int kK = 32;               // k of one stage
+constexpr int kStages = 3;
 constexpr int kThreads = 256;
+constexpr int kParts = 256;          // partial maxima of a tensor
+constexpr int kPad = 64;             // rows and columns of operands are padded with zeros to multiples of this
 constexpr float kLow = 0x1p-11f;     // weight of the second half of a 32-bit value
 
-template <typename T> struct Frag;
-template <> struct Frag<bf16> { using type = bf16 __attribute__((ext_vector_type(8))); };
-template <> struct Frag<f16> { using type = f16 __attribute__((ext_vector_type(8))); };
+using f16x2 = f16 __attribute__((ext_vector_type(2)));
+using f16x4 = f16 __attribute__((ext_vector_type(4)));
+using f16x8 = f16 __attribute__((ext_vector_type(8)));
+using s16x4 = short __attribute__((ext_vector_type(4)));
 using acc_t = float __attribute__((ext_vector_type(16)));
 using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ acc_t mfma(Frag<bf16>::type a, Frag<bf16>::type b, acc_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ acc_t mfma(Frag<f16>::type a, Frag<f16>::type b, acc_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+template <typename N, typename M> __host__ __device__ constexpr N round_up(N n, M to) { return (n + (N)to - 1) / (N)to * (N)to; }
 
-// What the kernels tell each other: at the start of the forward workspace.
+// At the start of the forward workspace.
 struct Header {
-    int rows;                 // frames that belong to a sequence
-    uint32_t most_x, most_w;  // largest finite magnitudes, as bit patterns (32-bit operands)
+    int rows, unused[3];                                   // frames that belong to a sequence
+    alignas(16) uint32_t most_x[kParts], most_w[kParts];   // largest finite magnitudes, as bit patterns
 };
+// At the start of the backward workspace.
 struct BackHeader {
-    uint32_t most_g;
+    alignas(16) uint32_t most_g[kParts];
 };
 
-// The power of two that brings `most` to 2^14 .. 2^15, and its inverse.
-__device__ __forceinline__ int scale_exponent(uint32_t most) {
-    if (most == 0) return 0;
-    const int e = (int)(most >> 23) - 127;         // (subnormals: -127)
-    const int k = 14 - e;
-    return k > 100 ? 100 : k;
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t wave_most(uint32_t m) {
+    for (int d = 32; d; d >>= 1) m = umax(m, (uint32_t)__shfl_xor((int)m, d));
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)m);
 }
-
-// ------------------------------------------------------------------------------------------------------------- rows
-
-// offsets[b]: the first row of sequence b.  One workgroup.
-__global__ __launch_bounds__(1024) void ce_begin(const int32_t* lens, int B, int T, int* offsets, Header* header) {
-    __shared__ int sums[16];
-    __shared__ int carry;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (threadIdx.x == 0) carry = 0;
-    __syncthreads();
-    for (int base = 0; base < B; base += 1024) {
-        const int b = base + threadIdx.x;
-        int n = b < B ? lens[b] : 0;
-        n = n < 0 ? 0 : (n > T ? T : n);
-        int sum = n;
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(sum, d);
-            if (lane >= d) sum += o;
-        }
-        if (lane == 63) sums[wave] = sum;
-        __syncthreads();
-        int before = carry;
-        for (int w = 0; w < wave; w++) before += sums[w];
-        if (b < B) offsets[b] = before + sum - n;
-        __syncthreads();
-        if (threadIdx.x == 1023) carry = before + sum;
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) {
-        header->rows = carry;
-        header->most_x = 0;
-        header->most_w = 0;
-    }
-}
-
 __device__ __forceinline__ uint32_t finite_bits(float x) {
     const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
     return b < 0x7f800000u ? b : 0u;
 }
-__device__ __forceinline__ void most_of(uint32_t m, uint32_t* to) {
-    for (int d = 32; d; d >>= 1) {
-        const uint32_t o = (uint32_t)__shfl_xor((int)m, d);
-        m = o > m ? o : m;
-    }
-    if ((threadIdx.x & 63) == 0 && m) atomicMax(to, m);       // a maximum: the order does not matter
+
+// The exponent of the power of two that brings a tensor's largest value to 2^14 .. 2^15, from its partial maxima: in every lane of a whole wave.
+__device__ __forceinline__ int scale_exponent(const uint32_t* parts) {
+    const u32x4 p = reinterpret_cast<const u32x4*>(parts)[threadIdx.x & 63];
+    const uint32_t most = wave_most(umax(umax(p.x, p.y), umax(p.z, p.w)));
+    if (most == 0) return 0;
+    const int k = 14 - ((int)(most >> 23) - 127);          // (subnormals: as 2^-127)
+    return k > 100 ? 100 : k;
 }
 
 __device__ __forceinline__ bool has_target(int y, int classes) { return y >= 0 && y < classes; }
 
-// Largest magnitude of a matrix of floats; `lens`: its rows are frames (b, t), and those without a target do not count.
-__global__ __launch_bounds__(256) void ce_most(const float* x, int64_t stride_b, int64_t stride_t, int64_t rows, int T, int D, const int32_t* lens, const int32_t* targets,
-                                               int64_t tgt_b, int64_t tgt_t, int classes, uint32_t* most) {
-    uint32_t m = 0;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)gridDim.x * 4) {
-        const int64_t b = r / T, t = r % T;
-        if (lens && (t >= lens[b] || !has_target(targets[b * tgt_b + t * tgt_t], classes))) continue;
-        const float* row = x + b * stride_b + t * stride_t;
-        for (int d = threadIdx.x & 63; d < D; d += 64) {
-            const uint32_t v = finite_bits(row[d]);
-            m = v > m ? v : m;
+// ------------------------------------------------------------------------------------------------------ preparation
+
+struct Frames {
+    const void* hidden;  int64_t stride_b, stride_t;
+    const int32_t* lens;
+    const int32_t* targets;  int64_t tgt_b, tgt_t;
+    int B, T, F, D, Kp;
+};
+struct Weights {
+    const void* p;  int64_t stride;
+    const void* bias;
+};
+
+// Eight values from column c on; zeros behind column D.
+template <typename In> __device__ __forceinline__ void load8(const In* row, int c, int D, bool aligned, float (&v)[8]) {
+    if (aligned && c + 8 <= D) {
+        if constexpr (sizeof(In) == 2) {
+            using V = In __attribute__((ext_vector_type(8)));
+            const V x = *reinterpret_cast<const V*>(row + c);
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = (float)x[i];
+        } else {
+            using V = In __attribute__((ext_vector_type(4)));
+            const V x = *reinterpret_cast<const V*>(row + c), y = *reinterpret_cast<const V*>(row + c + 4);
+#pragma unroll
+            for (int i = 0; i < 4; i++) { v[i] = x[i]; v[4 + i] = y[i]; }
         }
+        return;
     }
-    most_of(m, most);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = c + i < D ? (float)row[c + i] : 0.f;
 }
 
-// x as one 16-bit value or two.
-__device__ __forceinline__ void split(float x, int exponent, f16& high, f16& low) {
-    const float s = ldexpf(x, exponent);
+// Workgroup 0: offsets[b], the first row of sequence b.  The next kParts: largest magnitudes of the frames with a target; the
+// last kParts: those of the weights.
+template <typename In>
+__global__ __launch_bounds__(kThreads) void ce_look(Frames f, Weights w, int* offsets, Header* header) {
+    __shared__ int sums[4];
+    __shared__ uint32_t most_of[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (blockIdx.x == 0) {
+        int carry = 0;
+        for (int base = 0; base < f.B; base += kThreads) {
+            const int b = base + threadIdx.x;
+            int n = b < f.B ? f.lens[b] : 0;
+            n = n < 0 ? 0 : (n > f.T ? f.T : n);
+            int sum = n;
+            for (int d = 1; d < 64; d <<= 1) {
+                const int o = __shfl_up(sum, d);
+                if (lane >= d) sum += o;
+            }
+            if (lane == 63) sums[wave] = sum;
+            __syncthreads();
+            int before = carry;
+            for (int i = 0; i < wave; i++) before += sums[i];
+            if (b < f.B) offsets[b] = before + sum - n;
+            carry += sums[0] + sums[1] + sums[2] + sums[3];
+            __syncthreads();
+        }
+        if (threadIdx.x == 0) header->rows = carry;
+        return;
+    }
+    const bool weights = blockIdx.x > kParts;
+    const int part = (blockIdx.x - 1) % kParts;
+    const In* base = static_cast<const In*>(weights ? w.p : f.hidden);
+    const int64_t rows = weights ? f.F : (int64_t)f.B * f.T;
+    uint32_t most = 0;
+    for (int64_t r = (int64_t)part * 4 + wave; r < rows; r += kParts * 4) {
+        const In* row;
+        if (weights) {
+            row = base + r * w.stride;
+        } else {
+            const int b = (int)(r / f.T), t = (int)(r % f.T);
+            if (t >= f.lens[b] || !has_target(f.targets[b * f.tgt_b + t * f.tgt_t], f.F)) continue;
+            row = base + b * f.stride_b + t * f.stride_t;
+        }
+        const bool aligned = (uintptr_t)row % 16 == 0;
+        for (int c = lane * 8; c < f.D; c += 512) {
+            float v[8];
+            load8(row, c, f.D, aligned, v);
+#pragma unroll
+            for (int i = 0; i < 8; i++) most = umax(most, finite_bits(v[i]));
+        }
+    }
+    most = wave_most(most);
+    if (lane == 0) most_of[wave] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) (weights ? header->most_w : header->most_x)[part] = umax(umax(most_of[0], most_of[1]), umax(most_of[2], most_of[3]));
+}
+
+// x as one operand or as two halves.
+__device__ __forceinline__ void split(float s, f16& high, f16& low) {
     high = (f16)s;
     low = fabsf(s) < 65504.f ? (f16)((s - (float)high) * 0x1p11f) : (f16)0.f;       // infinities and NaN are in the first half alone
 }
+template <int S> __device__ __forceinline__ void store_operand(f16* out, int Kp, int c, const float (&v)[8], int exponent) {
+    f16x8 high, low;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float s = ldexpf(v[i], exponent);
+        if (S == 2) {
+            f16 h, l;
+            split(s, h, l);
+            high[i] = h;
+            low[i] = l;
+        } else {
+            high[i] = (f16)s;
+        }
+    }
+    *reinterpret_cast<f16x8*>(out + c) = high;
+    if (S == 2) *reinterpret_cast<f16x8*>(out + Kp + c) = low;
+}
 
-// Frames and weights as operands: [row][halves][Kp], zeros behind column D.
-struct PackArgs {
-    const void* x;  int64_t stride_b, stride_t;
-    int64_t rows;  int T, D, Kp, classes;
-    const int32_t *lens, *offsets, *targets;  int64_t tgt_b, tgt_t;      // null for weights
-    const uint32_t* most;
-    void* out;
+struct Packed {
+    f16 *x, *w;                      // [row][halves][Kp], zeros behind column D and in rows up to a multiple of kPad
     int *row_frame, *row_target;
+    float* target_logit;             // in units of log 2
     float* loss;
 };
 
-template <typename In, typename T>
-__global__ __launch_bounds__(256) void ce_pack(PackArgs a) {
+// A wave per row: frames as operands, with the logit of their target in 32 bits; then weights.
+template <typename In>
+__global__ __launch_bounds__(kThreads) void ce_pack(Frames f, Weights w, const int* offsets, const Header* header, Packed o) {
     constexpr int S = sizeof(In) == 4 ? 2 : 1;
     const int lane = threadIdx.x & 63;
-    const int exponent = S == 2 ? scale_exponent(*a.most) : 0;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < a.rows; r += (int64_t)gridDim.x * 4) {
-        const int64_t b = r / a.T, t = r % a.T;
-        int64_t row = r;
-        bool used = true;
-        if (a.lens) {
-            if (t >= a.lens[b]) {
-                if (lane == 0) a.loss[r] = 0.f;
-                continue;
+    const int ex = scale_exponent(header->most_x), ew = scale_exponent(header->most_w);
+    const int64_t frames = (int64_t)f.B * f.T, n_weights = round_up(f.F, kPad), all = frames + kPad + n_weights;
+    const int64_t row_size = S * (int64_t)f.Kp;
+    const float none[8] = {};
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < all; r += (int64_t)gridDim.x * 4) {
+        if (r >= frames + kPad) {
+            const int64_t row = r - frames - kPad;
+            const In* x = static_cast<const In*>(w.p) + row * w.stride;
+            const bool aligned = (uintptr_t)x % 16 == 0;
+            for (int c = lane * 8; c < f.Kp; c += 512) {
+                float v[8];
+                if (row < f.F) load8(x, c, f.D, aligned, v);
+                store_operand<S>(o.w + row * row_size, f.Kp, c, row < f.F ? v : none, ew);
             }
-            row = a.offsets[b] + t;
-            const int target = a.targets[b * a.tgt_b + t * a.tgt_t];
-            used = has_target(target, a.classes);      // a frame without a target: zeros, whatever it holds
-            if (lane == 0) {
-                a.row_frame[row] = (int)r;
-                a.row_target[row] = target;
-            }
+            continue;
         }
-        const In* x = static_cast<const In*>(a.x) + b * a.stride_b + t * a.stride_t;
-        T* out = static_cast<T*>(a.out) + row * (S * (int64_t)a.Kp);
-        for (int d = lane; d < a.Kp; d += 64) {
-            if constexpr (S == 2) {
-                f16 high = (f16)0.f, low = (f16)0.f;
-                if (used && d < a.D) split(x[d], exponent, high, low);
-                out[d] = high;
-                out[a.Kp + d] = low;
-            } else {
-                out[d] = used && d < a.D ? x[d] : (T)0.f;
-            }
+        if (r >= frames) {
+            const int64_t row = header->rows + (r - frames);
+            if (row < round_up((int64_t)header->rows, kPad))
+                for (int c = lane * 8; c < f.Kp; c += 512) store_operand<S>(o.x + row * row_size, f.Kp, c, none, 0);
+            continue;
         }
-    }
-}
-
-// out[h][c][r] = in[r][h][c] for 16-bit values, rows r < *n_rows (or `rows`); zeros up to Rp.  Tiles of 64 x 64.
-struct TransposeArgs {
-    const uint16_t* in;  int64_t row_stride, half_stride;
-    int rows;  const int* n_rows;  int cols;
-    uint16_t* out;  int64_t col_stride, out_half;       // of the transposed matrix
-};
-__global__ __launch_bounds__(256) void ce_transpose(TransposeArgs a) {
-    __shared__ uint16_t tile[64][66];
-    const int rows = a.n_rows ? *a.n_rows : a.rows;
-    const int64_t r0 = (int64_t)blockIdx.x * 64;
-    const int c0 = blockIdx.y * 64, half = blockIdx.z;
-    if (r0 >= ceil_div(rows, 64) * (int64_t)64) return;
-    const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-    for (int i = y; i < 64; i += 4) {
-        const int64_t r = r0 + i;
-        const int c = c0 + x;
-        tile[i][x] = r < rows && c < a.cols ? a.in[r * a.row_stride + half * a.half_stride + c] : (uint16_t)0;
-    }
-    __syncthreads();
-    for (int i = y; i < 64; i += 4) {
-        const int c = c0 + i;
-        if (c < a.cols) a.out[c * a.col_stride + half * a.out_half + r0 + x] = tile[x][i];
+        const int b = (int)(r / f.T), t = (int)(r % f.T);
+        if (t >= f.lens[b]) {
+            if (lane == 0) o.loss[r] = 0.f;
+            continue;
+        }
+        const int64_t row = offsets[b] + t;
+        const int target = f.targets[b * f.tgt_b + t * f.tgt_t];
+        const bool used = has_target(target, f.F);      // a frame without a target: zeros, whatever it holds
+        const In* x = static_cast<const In*>(f.hidden) + b * f.stride_b + t * f.stride_t;
+        const In* y = static_cast<const In*>(w.p) + (used ? target : 0) * w.stride;
+        const bool aligned = (uintptr_t)x % 16 == 0, aligned_y = (uintptr_t)y % 16 == 0;
+        float dot = 0.f;
+        for (int c = lane * 8; c < f.Kp; c += 512) {
+            float v[8], u[8];
+            if (used) {
+                load8(x, c, f.D, aligned, v);
+                load8(y, c, f.D, aligned_y, u);
+#pragma unroll
+                for (int i = 0; i < 8; i++) dot = fmaf(v[i], u[i], dot);
+            }
+            store_operand<S>(o.x + row * row_size, f.Kp, c, used ? v : none, ex);
+        }
+        for (int d = 32; d; d >>= 1) dot += __shfl_xor(dot, d);
+        if (lane == 0) {
+            o.row_frame[row] = (int)r;
+            o.row_target[row] = target;
+            o.target_logit[row] = used ? dot + (w.bias ? (float)static_cast<const In*>(w.bias)[target] : 0.f) : 0.f;
+        }
     }
 }
 
 // ---------------------------------------------------------------------------------------------------------- product
 
 struct Operand {
-    const void* p;
-    int64_t row_stride;       // elements
+    const f16* p;
+    int64_t row_stride;       // elements between rows; a row has consecutive k, or consecutive m (n)
     int64_t half_stride;      // elements to the second halves
-    int rows;                 // rows that may be read
-    const int* n_rows;        // if they are known on the device alone
+    int64_t bytes;            // of the buffer, from p on
+    int rows;                 // m (n) that there are
+    const int* n_rows;        // if that is known on the device alone
 };
 struct ProductArgs {
     Operand a, b;
-    int K;                    // of one half; multiple of kStep
-    const int* n_k;           // K = n_k rounded up to kStep, where it is known on the device alone
-    int splits;               // blockIdx.z takes one of so many ranges of k
+    int K;                    // of one half; a multiple of kK
+    const int* n_k;           // K = *n_k rounded up to kK, where it is known on the device alone
+    int splits;               // ranges of k, one tile of C each
 };
 
-enum Kind { kStatistics, kGradient, kStore };
+enum Kind { kStatistics, kGradient, kHidden, kWeight };
 
 struct EpilogueArgs {
-    // kStatistics, kGradient: m is the class, n the row (frame)
-    const void* bias;  int bias_f32;
+    // kStatistics, kGradient: m is the class, n the row
+    const void* bias;
     const Header* header;  const BackHeader* back;
-    int first_class, classes;              // of this piece; classes of the layer
+    int first_class;                       // of this piece
     const int* row_target;
-    float2* part;  float* target_logit;    // [tile of classes][rows_p], [rows_p]
+    float2* part;                          // [tile of classes][rows_p]: maximum, sum
     int64_t rows_p;
-    const float *lse, *row_scale;
-    void* g;  int64_t g_stride, g_half;    // [row][halves][piece]
-    void* gt;  int64_t gt_stride, gt_half; // [class][halves][rows_p]
-    // kStore: m, n as they are; float [split][m][n]
+    const float *target_logit, *lse, *row_scale;
+    f16* g;  int64_t g_stride, g_half;     // [row][halves][piece]
+    float* column_sums;                    // [tile of rows][classes]; of G, may be null
+    int64_t column_stride;
+    // kHidden, kWeight: float [split][m][n]
     float* out;  int64_t out_stride, out_split;
     int add;
 };
 
-template <typename T, int KIND>
-__global__ __launch_bounds__(kThreads) void product(ProductArgs p, EpilogueArgs e) {
-    constexpr int S = sizeof(T) == 2 && __is_same(T, f16) ? 2 : 1;
-    using F = typename Frag<T>::type;
-    __shared__ u32x4 lds[2][kTile * kStep / 8];              // A and B: rows of 8 chunks of 16 bytes, chunk c of row r at place c ^ (r & 7)
-    __shared__ float join[2][2][kTile];
+__device__ __forceinline__ void wait_for_loads(int left) {        // the number of this wave's loads that may still be on their way
+    if (left) __builtin_amdgcn_s_waitcnt(0x0f70 | 6); else __builtin_amdgcn_s_waitcnt(0x0f70);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 
-    const int rows_a = p.a.n_rows ? *p.a.n_rows : p.a.rows, rows_b = p.b.n_rows ? *p.b.n_rows : p.b.rows;
-    const int m0 = blockIdx.x * kTile, n0 = blockIdx.y * kTile;
-    if (m0 >= rows_a || n0 >= rows_b) return;
+using lds_ptr = __attribute__((address_space(3))) void*;
+
+// One operand's part of a stage: R rows of the tile by kK.  LDS is filled by loads that bypass the registers and write 64 lanes x 16 bytes in
+// order; which 16 bytes a lane asks for is free, and places them so that reading has no bank conflicts.
+//   consecutive k:   row r has 4 chunks of 8 k; chunk c lies at place c ^ ((r >> 1) & 3) of the row.  A fragment is one read of 16 bytes.
+//   consecutive m:   k has R / 8 chunks of 8 m; chunk c lies at place c ^ ((k & 3) << 1).  A fragment is two reads that
+//                    transpose 4 k x 16 m within 16 lanes.
+template <int R, bool kConsecutiveK> struct Side {
+    static constexpr int kLoads = R * kK * 2 / 16 / kThreads;      // per thread and stage
+    static constexpr int kBytes = R * kK * 2;
+    __amdgpu_buffer_rsrc_t rsrc;
+    uint32_t from[kLoads];       // byte offsets of this lane's chunks at k = 0
+    uint32_t step, half;         // bytes from stage to stage, and to the second halves
+    int read[2];                 // byte offsets of this lane's fragments
+
+    __device__ __forceinline__ void set(const Operand& o, int rows, int first, int k0, int base_row) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int64_t origin = kConsecutiveK ? first * o.row_stride + k0 : k0 * o.row_stride + first;
+        const int64_t left = o.bytes - origin * 2;
+        rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(o.p + origin), 0, left > 0xffffffffll ? 0xffffffffu : (uint32_t)left, 0x00020000);
+        half = (uint32_t)(o.half_stride * 2);
+        step = kConsecutiveK ? kK * 2 : (uint32_t)(kK * o.row_stride * 2);
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+            const int slot = (i * 4 + wave) * 64 + lane;
+            if (kConsecutiveK) {
+                const int r = slot >> 2, c = (slot & 3) ^ ((r >> 1) & 3);
+                from[i] = (uint32_t)(min(r, rows - 1 - first) * o.row_stride * 2 + c * 16);      // rows behind the last are the last again
+            } else {
+                const int k = slot / (R / 8), c = (slot % (R / 8)) ^ ((k & 3) << 1);
+                const int last = (int)((o.row_stride - first) / 8 - 1);                          // columns behind the row's end as well
+                from[i] = (uint32_t)(k * o.row_stride * 2 + min(c, last) * 16);
+            }
+        }
+        if (kConsecutiveK) {
+            const int r = base_row + (lane & 31), x = (r >> 1) & 3;
+            read[0] = r * 64 + (((lane >> 5) ^ x) * 16);
+            read[1] = r * 64 + (((2 + (lane >> 5)) ^ x) * 16);
+        } else {
+            const int k = (lane >> 5) * 8 + ((lane & 15) >> 2), m = base_row / 8 + ((lane >> 4) & 1) * 2;
+#pragma unroll
+            for (int i = 0; i < 2; i++) read[i] = k * (R * 2) + (((m + i * 4) ^ ((k & 3) << 1)) + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
+        }
+    }
+    __device__ __forceinline__ void fetch(char* lds, uint32_t offset) const {
+        const int wave = threadIdx.x >> 6;
+#pragma unroll
+        for (int i = 0; i < kLoads; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(lds + (i * 4 + wave) * 1024), 16, from[i], offset, 0, 0);
+    }
+    // block b of 32 rows, k of kk * 16 .. + 15
+    __device__ __forceinline__ f16x8 fragment(const char* lds, int b, int kk) const {
+        if constexpr (kConsecutiveK) {
+            return *reinterpret_cast<const f16x8*>(lds + read[kk] + b * 32 * 64);
+        } else {
+            const char* at = lds + read[b & 1] + (b >> 1) * 128 + kk * 16 * (R * 2);
+            using P = __attribute__((address_space(3))) s16x4*;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(at + 4 * (R * 2)));
+            return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
+};
+
+constexpr int kGStride = kM * 2 + 16;      // bytes of a row of G in LDS
+constexpr int kStageBytes = (kM + kN) * kK * 2;
+constexpr int kLdsBytes = kStages * kStageBytes;
+static_assert(kN * kGStride <= kLdsBytes, "G goes through the stages' LDS");
+
+// In           type of the user's tensors: two halves where it has 32 bits
+// KIND         what becomes of a tile
+template <typename In, int KIND>
+__global__ __launch_bounds__(kThreads, 2) void product(ProductArgs p, EpilogueArgs e) {
+#if __HIP_DEVICE_COMPILE__      // the buffer descriptors are types of the device
+    constexpr int S = sizeof(In) == 4 ? 2 : 1;
+    constexpr bool kAk = KIND != kWeight, kBk = KIND == kStatistics || KIND == kGradient;
+    __shared__ alignas(16) char lds[kLdsBytes];
+    __shared__ float bias[KIND == kStatistics || KIND == kGradient ? kM : 1];
+    __shared__ float join[KIND == kStatistics || KIND == kGradient ? 4 : 1][kM];
+
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave & 1, wn = wave >> 1;
-    int K = p.n_k ? ceil_div(*p.n_k, kStep) * kStep : p.K;
+    const int rows_a = p.a.n_rows ? *p.a.n_rows : p.a.rows, rows_b = p.b.n_rows ? *p.b.n_rows : p.b.rows;
+
+    // Workgroups go round the eight dies; each die has an L2 of its own, so it gets a range of tiles of its own, in groups of eight tiles of A:
+    // the 64 tiles that a die works on at a time have 8 + 8 operand tiles among them, not 64 + 1.
+    const int tiles_m = ceil_div(rows_a, kM), tiles_n = ceil_div(rows_b, kN), tiles = tiles_m * tiles_n * p.splits;
+    const int each = ceil_div(tiles, 8);
+    int tile = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= each || tile >= tiles) return;
+    const int part_of_k = tile / (tiles_m * tiles_n);
+    tile -= part_of_k * tiles_m * tiles_n;
+    const int group = tile / (8 * tiles_n), in_group = min(8, tiles_m - group * 8);
+    tile -= group * 8 * tiles_n;
+    const int tile_m = group * 8 + tile % in_group, tile_n = tile / in_group;
+    const int m0 = tile_m * kM, n0 = tile_n * kN;
+
+    int K = p.n_k ? round_up(*p.n_k, kK) : p.K;
     int k0 = 0;
     if (p.splits > 1) {
-        const int each = ceil_div(ceil_div(K, kStep), p.splits) * kStep;
-        k0 = min(K, (int)blockIdx.z * each);
-        K = min(K, k0 + each);
+        const int range = ceil_div(ceil_div(K, kK), p.splits) * kK;
+        k0 = min(K, part_of_k * range);
+        K = min(K, k0 + range);
+    }
+    const int steps = (K - k0) / kK, all = S == 2 ? 3 * steps : steps;
+
+    Side<kM, kAk> A;
+    Side<kN, kBk> B;
+    A.set(p.a, rows_a, m0, k0, wm * 128);
+    B.set(p.b, rows_b, n0, k0, wn * 64);
+    if constexpr (KIND == kStatistics || KIND == kGradient) {
+        const int m = m0 + tid;       // classes behind the last: -inf, no probability
+        float v = m < rows_a ? 0.f : -INFINITY;
+        if (e.bias && m < rows_a) v = (float)static_cast<const In*>(e.bias)[e.first_class + m] * kLog2e;
+        bias[tid] = v;
     }
 
-    acc_t acc[2][2];
+    acc_t acc[4][2];
 #pragma unroll
-    for (int i = 0; i < 2; i++)
+    for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
             for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
 
-    // rows behind the last are the last one again: read, and never stored
-    const T *pa[4], *pb[4];
-    int place[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int at = i * kThreads + tid, r = at >> 3, c = at & 7;
-        pa[i] = static_cast<const T*>(p.a.p) + (int64_t)min(m0 + r, rows_a - 1) * p.a.row_stride + c * 8;
-        pb[i] = static_cast<const T*>(p.b.p) + (int64_t)min(n0 + r, rows_b - 1) * p.b.row_stride + c * 8;
-        place[i] = r * 8 + (c ^ (r & 7));
-    }
-    const auto segment = [&](int64_t off_a, int64_t off_b) {
-        for (int k = k0; k < K; k += kStep) {
-            u32x4 ra[4], rb[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                ra[i] = *reinterpret_cast<const u32x4*>(pa[i] + off_a + k);
-                rb[i] = *reinterpret_cast<const u32x4*>(pb[i] + off_b + k);
-            }
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                lds[0][place[i]] = ra[i];
-                lds[1][place[i]] = rb[i];
-            }
-            __syncthreads();
-#pragma unroll
-            for (int kk = 0; kk < kStep / 16; kk++) {
-                F fa[2], fb[2];
-                const int c = kk * 2 + (lane >> 5);
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int rm = wm * 64 + i * 32 + (lane & 31), rn = wn * 64 + i * 32 + (lane & 31);
-                    fa[i] = __builtin_bit_cast(F, lds[0][rm * 8 + (c ^ (rm & 7))]);
-                    fb[i] = __builtin_bit_cast(F, lds[1][rn * 8 + (c ^ (rn & 7))]);
-                }
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++) acc[i][j] = mfma(fa[i], fb[j], acc[i][j]);
-            }
+    const auto fetch = [&](int it) {
+        char* at = lds + (it % kStages) * kStageBytes;
+        uint32_t oa, ob;
+        if constexpr (S == 2) {
+            const int part = it / steps, k = it - part * steps;       // high x low, low x high, high x high
+            oa = k * A.step + (part == 1 ? A.half : 0);
+            ob = k * B.step + (part == 0 ? B.half : 0);
+        } else {
+            oa = it * A.step;
+            ob = it * B.step;
         }
+        A.fetch(at, oa);
+        B.fetch(at + A.kBytes, ob);
     };
-    if constexpr (S == 2) {
-        segment(0, p.b.half_stride);
-        segment(p.a.half_stride, 0);
+    if (all > 0) fetch(0);
+    if (all > 1) fetch(1);
+    for (int it = 0; it < all; it++) {
+        wait_for_loads(it + 1 < all);          // this stage is there for everyone, and nobody reads the one before it any more
+        if (it + 2 < all) fetch(it + 2);
+        if (S == 2 && it == 2 * steps) {
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+            for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int j = 0; j < 2; j++) acc[i][j] *= kLow;
+                for (int j = 0; j < 2; j++) acc[i][j] *= kLow;
+        }
+        const char* at = lds + (it % kStages) * kStageBytes;
+#pragma unroll
+        for (int kk = 0; kk < kK / 16; kk++) {
+            f16x8 fa[4], fb[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) fb[j] = B.fragment(at + A.kBytes, j, kk);
+#pragma unroll
+            for (int i = 0; i < 4; i++) fa[i] = A.fragment(at, i, kk);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+        }
     }
-    segment(0, 0);
 
     // register r of a 32 x 32 block: row (r & 3) + 8 (r >> 2) + 4 (lane >> 5), column lane & 31
-    const int row_in = 4 * (lane >> 5), col_in = lane & 31;
+    const int row_in = wm * 128 + 4 * (lane >> 5), col_in = wn * 64 + (lane & 31);
 
-    if constexpr (KIND == kStore) {
-        float* out = e.out + (int64_t)blockIdx.z * e.out_split;
+    if constexpr (KIND == kHidden || KIND == kWeight) {
+        float* out = e.out + part_of_k * e.out_split + (int64_t)m0 * e.out_stride + n0;
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+        for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const int n = n0 + wn * 64 + j * 32 + col_in;
+                const int n = col_in + j * 32;
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    const int m = m0 + wm * 64 + i * 32 + row_in + (r & 3) + 8 * (r >> 2);
-                    if (m < rows_a && n < rows_b) {
-                        float* at = out + (int64_t)m * e.out_stride + n;
-                        *at = e.add ? *at + acc[i][j][r] : acc[i][j][r];
+                    const int m = row_in + i * 32 + (r & 3) + 8 * (r >> 2);
+                    if (m0 + m < rows_a && n0 + n < rows_b) {
+                        float* to = out + (int64_t)m * e.out_stride + n;
+                        *to = e.add ? *to + acc[i][j][r] : acc[i][j][r];
                     }
                 }
             }
         return;
     }
 
-    // logits: the scales of 32-bit operands go, the bias comes
-    const int down = S == 2 ? -(scale_exponent(e.header->most_x)) : 0, down_w = S == 2 ? -(scale_exponent(e.header->most_w)) : 0;
-    const int classes = min(e.classes - e.first_class, rows_a);
-    float bias[2][16];
+    const int down = scale_exponent(e.header->most_x) + scale_exponent(e.header->most_w);
+    const float per = fminf(ldexpf(kLog2e, -down), 0x1p127f);
+    __syncthreads();
+    // logits in units of log 2
 #pragma unroll
-    for (int i = 0; i < 2; i++)
+    for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-            const int m = m0 + wm * 64 + i * 32 + row_in + (r & 3) + 8 * (r >> 2);
-            float v = 0.f;
-            if (e.bias && m < classes)
-                v = e.bias_f32 ? static_cast<const float*>(e.bias)[e.first_class + m] : (float)static_cast<const bf16*>(e.bias)[e.first_class + m];
-            bias[i][r] = v;
-        }
+        for (int q = 0; q < 4; q++) {
+            const float4 b = *reinterpret_cast<const float4*>(&bias[row_in + i * 32 + 8 * q]);
 #pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                float z = acc[i][j][r];
-                if (S == 2) z = ldexpf(ldexpf(z, down), down_w);
-                acc[i][j][r] = z + bias[i][r];
+            for (int j = 0; j < 2; j++) {
+                acc[i][j][4 * q] = fmaf(acc[i][j][4 * q], per, b.x);
+                acc[i][j][4 * q + 1] = fmaf(acc[i][j][4 * q + 1], per, b.y);
+                acc[i][j][4 * q + 2] = fmaf(acc[i][j][4 * q + 2], per, b.z);
+                acc[i][j][4 * q + 3] = fmaf(acc[i][j][4 * q + 3], per, b.w);
             }
+        }
 
     if constexpr (KIND == kStatistics) {
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            const int col = wn * 64 + j * 32 + col_in, n = n0 + col;
-            const int target = n < rows_b ? e.row_target[n] : -1;
             float most = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int m = m0 + wm * 64 + i * 32 + row_in + (r & 3) + 8 * (r >> 2);
-                    if (m >= classes) acc[i][j][r] = -INFINITY;
-                    else if (e.first_class + m == target) e.target_logit[n] = acc[i][j][r];
-                    most = fmaxf(most, acc[i][j][r]);
-                }
+                for (int r = 0; r < 16; r++) most = fmaxf(most, acc[i][j][r]);
             most = fmaxf(most, __shfl_xor(most, 32));
-            const float base = most == -INFINITY ? 0.f : most;        // a tile of classes that are all -inf: the sum is 0, not NaN
+            const float base = most == -INFINITY ? 0.f : most;        // classes that are all ruled out: the sum is 0, not NaN
             float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) sum += exp2_fast((acc[i][j][r] - base) * kLog2e);
+                for (int r = 0; r < 16; r++) sum += exp2_fast(acc[i][j][r] - base);
             sum += __shfl_xor(sum, 32);
             if (lane < 32) {
-                join[wm][0][col] = most;
-                join[wm][1][col] = sum;
+                join[wm * 2][col_in + j * 32] = most;
+                join[wm * 2 + 1][col_in + j * 32] = sum;
             }
         }
         __syncthreads();
-        if (tid < kTile && n0 + tid < rows_b) {
-            const float ma = join[0][0][tid], mb = join[1][0][tid], most = fmaxf(ma, mb), base = most == -INFINITY ? 0.f : most;
-            const float sum = join[0][1][tid] * exp2_fast((ma - base) * kLog2e) + join[1][1][tid] * exp2_fast((mb - base) * kLog2e);
-            e.part[(int64_t)blockIdx.x * e.rows_p + n0 + tid] = make_float2(most, sum);
+        if (tid < kN && n0 + tid < rows_b) {
+            const float ma = join[0][tid], mb = join[2][tid], most = fmaxf(ma, mb), base = most == -INFINITY ? 0.f : most;
+            const float sum = join[1][tid] * exp2_fast(ma - base) + join[3][tid] * exp2_fast(mb - base);
+            e.part[(int64_t)tile_m * e.rows_p + n0 + tid] = make_float2(most, sum);
         }
-        return;
     }
 
     if constexpr (KIND == kGradient) {
-        const int g_exponent = S == 2 ? scale_exponent(e.back->most_g) : 0;
-        T* g = static_cast<T*>(e.g);
-        T* gt = static_cast<T*>(e.gt);
+        const int up = scale_exponent(e.back->most_g);
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            const int n = n0 + wn * 64 + j * 32 + col_in;
-            const bool there = n < rows_b;
-            const int target = there ? e.row_target[n] : -1;
-            const float lse = there ? e.lse[n] : 0.f, scale = there ? e.row_scale[n] : 0.f;
+            const int n = n0 + col_in + j * 32;
+            const float lse = n < rows_b ? e.lse[n] : INFINITY, scale = n < rows_b ? ldexpf(e.row_scale[n], up) : 0.f;
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int i = 0; i < 4; i++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    const int m = m0 + wm * 64 + i * 32 + row_in + (r & 3) + 8 * (r >> 2);
-                    float v = exp2_fast((acc[i][j][r] - lse) * kLog2e) * scale;
-                    if (e.first_class + m == target) v -= scale;
-                    if (m >= classes || !there) v = 0.f;
-                    // columns up to the end of the tile are there in both, zero behind the last class or row
+                    const float v = exp2_fast(acc[i][j][r] - lse) * scale;
                     if constexpr (S == 2) {
+                        f16x2 halves;      // both in the accumulator's register
                         f16 high, low;
-                        split(v, g_exponent, high, low);
-                        if (there) {
-                            g[(int64_t)n * e.g_stride + m] = high;
-                            g[(int64_t)n * e.g_stride + e.g_half + m] = low;
-                        }
-                        if (m < classes) {
-                            gt[(int64_t)m * e.gt_stride + n] = high;
-                            gt[(int64_t)m * e.gt_stride + e.gt_half + n] = low;
-                        }
+                        split(v, high, low);
+                        halves[0] = high;
+                        halves[1] = low;
+                        acc[i][j][r] = __builtin_bit_cast(float, halves);
                     } else {
-                        if (there) g[(int64_t)n * e.g_stride + m] = (T)v;
-                        if (m < classes) gt[(int64_t)m * e.gt_stride + n] = (T)v;
+                        acc[i][j][r] = v;
                     }
                 }
         }
+        // the target's value of each row, in the place it has in this tile
+        int place = -1;
+        float at_target = 0.f;
+        if (tid < kN && n0 + tid < rows_b) {
+            const int y = e.row_target[n0 + tid] - e.first_class - m0;
+            if (y >= 0 && y < min(kM, rows_a - m0)) {
+                place = y;
+                at_target = (exp2_fast(fmaf(e.target_logit[n0 + tid], kLog2e, -e.lse[n0 + tid])) - 1.f) * ldexpf(e.row_scale[n0 + tid], up);
+            }
+        }
+        float column[4] = {};
+#pragma unroll 1
+        for (int h = 0; h < S; h++) {
+            // through LDS, so that whole rows of the tile are written at once
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        f16x4 v;
+                        if constexpr (S == 2) {
+                            const uint32_t which = h ? 0x07060302u : 0x05040100u;       // upper or lower 16 bits of two registers
+                            uint32_t pair[2];
+#pragma unroll
+                            for (int r = 0; r < 2; r++)
+                                pair[r] = __builtin_amdgcn_perm(__float_as_uint(acc[i][j][4 * q + 2 * r + 1]), __float_as_uint(acc[i][j][4 * q + 2 * r]), which);
+                            v = __builtin_bit_cast(f16x4, pair);
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 4; r++) v[r] = (f16)acc[i][j][4 * q + r];
+                        }
+                        *reinterpret_cast<f16x4*>(lds + (col_in + j * 32) * kGStride + (row_in + i * 32 + 8 * q) * 2) = v;
+                    }
+            __syncthreads();
+            if (place >= 0) {
+                f16 high, low;
+                split(at_target, high, low);
+                *reinterpret_cast<f16*>(lds + tid * kGStride + place * 2) = h == 0 ? high : low;
+            }
+            __syncthreads();
+            f16* g = e.g + n0 * e.g_stride + h * e.g_half + m0;
+#pragma unroll 4
+            for (int i = 0; i < kN / 8; i++) {
+                const int r = i * 8 + (tid >> 5), c = tid & 31;
+                *reinterpret_cast<u32x4*>(g + r * e.g_stride + c * 8) = *reinterpret_cast<const u32x4*>(lds + r * kGStride + c * 16);
+            }
+            if (e.column_sums) {
+                float sum[4] = {};
+                for (int r = wave * 32; r < wave * 32 + 32; r++) {
+                    const f16x4 v = *reinterpret_cast<const f16x4*>(lds + r * kGStride + lane * 8);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sum[i] += (float)v[i];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) column[i] += h == 0 ? sum[i] : sum[i] * kLow;
+            }
+            if (h + 1 < S) __syncthreads();
+        }
+        if (e.column_sums) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) join[wave][lane * 4 + i] = column[i];
+            __syncthreads();
+            if (m0 + tid < rows_a) e.column_sums[tile_n * e.column_stride + e.first_class + m0 + tid] = join[0][tid] + join[1][tid] + join[2][tid] + join[3][tid];
+        }
     }
+#endif
 }
 
 // ---------------------------------------------------------------------------------------------------------- the rest
@@ -445,15 +631,15 @@ __global__ __launch_bounds__(256) void ce_finish(const Header* header, const flo
     for (int i = 0; i < tiles; i++) {
         const float2 p = part[i * rows_p + row];
         const float m = fmaxf(most, p.x), base = m == -INFINITY ? 0.f : m;
-        sum = sum * exp2_fast((most - base) * kLog2e) + p.y * exp2_fast((p.x - base) * kLog2e);
+        sum = sum * exp2_fast(most - base) + p.y * exp2_fast(p.x - base);
         most = m;
     }
-    const float l = most + log2_fast(sum) * kLn2;
+    const float l = most + log2_fast(sum);
     lse[row] = l;
     const int y = row_target[row], frame = row_frame[row];
     float v = 0.f;
-    if (y >= 0 && y < F) {
-        v = l - target_logit[row];
+    if (has_target(y, F)) {
+        v = l * kLn2 - target_logit[row];
     } else if (y >= F) {
         v = __builtin_nanf("");
         if (report) {
@@ -464,37 +650,37 @@ __global__ __launch_bounds__(256) void ce_finish(const Header* header, const flo
     loss[frame] = v;
 }
 
-__global__ void ce_clear(BackHeader* back) { back->most_g = 0; }
-
-// The incoming gradient of each row; rows without a target, or with one that is out of range, have none.
+// The incoming gradient of each row; rows without a target, or with one that is out of range, have none.  kParts workgroups.
 __global__ __launch_bounds__(256) void ce_row_scale(const Header* header, const int* row_frame, const int* row_target, const float* grad_loss, int64_t stride_b,
-                                                    int64_t stride_t, int T, int F, float* row_scale, uint32_t* most) {
-    const int row = blockIdx.x * 256 + threadIdx.x;
-    float g = 0.f;
-    if (row < header->rows) {
-        const int frame = row_frame[row], y = row_target[row];
-        if (y >= 0 && y < F) g = grad_loss[(int64_t)(frame / T) * stride_b + (int64_t)(frame % T) * stride_t];
+                                                    int64_t stride_t, int T, int F, float* row_scale, BackHeader* back) {
+    __shared__ uint32_t most_of[4];
+    uint32_t most = 0;
+    for (int row = blockIdx.x * 256 + threadIdx.x; row < header->rows; row += kParts * 256) {
+        float g = 0.f;
+        const int frame = row_frame[row];
+        if (has_target(row_target[row], F)) g = grad_loss[(int64_t)(frame / T) * stride_b + (int64_t)(frame % T) * stride_t];
         row_scale[row] = g;
+        most = umax(most, finite_bits(g));
     }
-    most_of(finite_bits(g), most);
+    most = wave_most(most);
+    if ((threadIdx.x & 63) == 0) most_of[threadIdx.x >> 6] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) back->most_g[blockIdx.x] = umax(umax(most_of[0], most_of[1]), umax(most_of[2], most_of[3]));
 }
 
 // grad_hidden: rows back to their frames.
 template <typename Out>
-__global__ __launch_bounds__(256) void ce_store_hidden(const Header* header, const BackHeader* back, const int* offsets, const int32_t* lens, const int32_t* targets,
-                                                       int64_t tgt_b, int64_t tgt_t, const float* acc, int B, int T, int F, int D, Out* out) {
+__global__ __launch_bounds__(256) void ce_store_hidden(const Header* header, const BackHeader* back, Frames f, const int* offsets, const float* acc, Out* out) {
     const int lane = threadIdx.x & 63;
-    const bool scaled = sizeof(Out) == 4;
-    const int down = scaled ? -scale_exponent(back->most_g) : 0, down_w = scaled ? -scale_exponent(header->most_w) : 0;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < (int64_t)B * T; r += (int64_t)gridDim.x * 4) {
-        const int64_t b = r / T, t = r % T;
-        const bool live = t < lens[b];
-        const float* row = acc + (live ? (int64_t)(offsets[b] + t) * D : 0);
-        const bool bad = live && targets[b * tgt_b + t * tgt_t] >= F;
-        for (int d = lane; d < D; d += 64) {
-            float v = live ? row[d] : 0.f;
-            if (scaled) v = ldexpf(ldexpf(v, down), down_w);
-            out[r * D + d] = (Out)(bad ? __builtin_nanf("") : v);
+    const int down = -scale_exponent(back->most_g), down_w = -scale_exponent(header->most_w);
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < (int64_t)f.B * f.T; r += (int64_t)gridDim.x * 4) {
+        const int64_t b = r / f.T, t = r % f.T;
+        const bool live = t < f.lens[b];
+        const float* row = acc + (live ? (int64_t)(offsets[b] + t) * f.D : 0);
+        const bool bad = live && f.targets[b * f.tgt_b + t * f.tgt_t] >= f.F;
+        for (int d = lane; d < f.D; d += 64) {
+            const float v = live ? ldexpf(ldexpf(row[d], down), down_w) : 0.f;
+            out[r * f.D + d] = (Out)(bad ? __builtin_nanf("") : v);
         }
     }
 }
@@ -502,48 +688,36 @@ __global__ __launch_bounds__(256) void ce_store_hidden(const Header* header, con
 // One piece of grad_weight: the ranges of k joined.
 template <typename Out>
 __global__ __launch_bounds__(256) void ce_store_weight(const Header* header, const BackHeader* back, const float* part, int splits, int64_t split_stride, int64_t n, Out* out) {
+    const int down = -scale_exponent(back->most_g), down_x = -scale_exponent(header->most_x);
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
     float v = 0.f;
     for (int s = 0; s < splits; s++) v += part[s * split_stride + i];
-    if (sizeof(Out) == 4) v = ldexpf(ldexpf(v, -scale_exponent(back->most_g)), -scale_exponent(header->most_x));
-    out[i] = (Out)v;
+    out[i] = (Out)ldexpf(ldexpf(v, down), down_x);
 }
 
-// grad_bias: sums over the rows.  One workgroup per class.
-template <typename T, typename Out>
-__global__ __launch_bounds__(256) void ce_store_bias(const Header* header, const BackHeader* back, const T* gt, int64_t stride, int64_t half, Out* out) {
-    constexpr int S = sizeof(Out) == 4 ? 2 : 1;
-    __shared__ float sums[4];
-    const T* row = gt + blockIdx.x * stride;
+// grad_bias: sums over the tiles of rows.
+template <typename Out>
+__global__ __launch_bounds__(256) void ce_store_bias(const Header* header, const BackHeader* back, const float* sums, int64_t stride, int F, Out* out) {
+    const int down = -scale_exponent(back->most_g);
+    const int f = blockIdx.x * 256 + threadIdx.x;
+    if (f >= F) return;
+    const int tiles = ceil_div(header->rows, kN);
     float v = 0.f;
-    for (int i = threadIdx.x; i < header->rows; i += 256) {
-        v += (float)row[i];
-        if (S == 2) v += (float)row[half + i] * kLow;
-    }
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = v;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        v = sums[0] + sums[1] + sums[2] + sums[3];
-        if (S == 2) v = ldexpf(v, -scale_exponent(back->most_g));
-        out[blockIdx.x] = (Out)v;
-    }
+    for (int i = 0; i < tiles; i++) v += sums[i * stride + f];
+    out[f] = (Out)ldexpf(v, down);
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
 
-constexpr size_t kPieceBytes = (size_t)256 << 20;      // of G, both layouts: the caches in front of the memory hold 256 MB
-
-template <typename N> N round_up(N n, N to) { return ceil_div(n, to) * to; }
+constexpr size_t kPieceBytes = (size_t)256 << 20;      // of G: the caches in front of the memory hold 256 MB
 
 // Where things are in the workspaces.
 struct Layout {
     int S, Kp, row_tiles, class_tiles, piece, splits;
-    int64_t rows_p;
-    bool own_weight;                    // weights are copied as operands
-    size_t header, offsets, row_frame, row_target, target_logit, lse, x, w, part, forward;
-    size_t back, row_scale, xt, wt, g, gt, dx, dw, backward;
+    int64_t rows, rows_p, weights_p;
+    size_t header, offsets, row_frame, row_target, target_logit, lse, x, w, part, x_bytes, w_bytes, forward;
+    size_t back, row_scale, g, dx, dw, sums, g_bytes, backward;
 };
 
 bool valid(const i6train_ce_problem* p) {
@@ -551,14 +725,14 @@ bool valid(const i6train_ce_problem* p) {
 }
 
 int layout(const i6train_ce_problem& p, Layout& l) {
-    const int64_t rows = (int64_t)p.B * p.T;
-    if (rows > (1 << 22) || p.F > (1 << 22) || p.D > (1 << 16)) return I6TRAIN_ERR_TOO_LARGE;
+    l.rows = (int64_t)p.B * p.T;
+    if (l.rows > (1 << 22) || p.F > (1 << 22) || p.D > (1 << 14)) return I6TRAIN_ERR_TOO_LARGE;
     l.S = p.dtype == I6TRAIN_F32 ? 2 : 1;
-    l.Kp = round_up(p.D, kStep);
-    l.row_tiles = (int)ceil_div(rows, (int64_t)kTile);
-    l.class_tiles = ceil_div(p.F, kTile);
-    l.rows_p = (int64_t)l.row_tiles * kTile;
-    l.own_weight = !(p.dtype == I6TRAIN_BF16 && p.D % kStep == 0 && (uintptr_t)p.weight % 16 == 0 && p.weight_stride_f % 8 == 0);
+    l.Kp = round_up(p.D, kPad);
+    l.row_tiles = (int)ceil_div(l.rows, (int64_t)kN);
+    l.class_tiles = ceil_div(p.F, kM);
+    l.rows_p = (int64_t)l.row_tiles * kN;
+    l.weights_p = round_up(p.F, kPad);
     size_t at = 0;
     const auto take = [&](size_t bytes) { const size_t here = at; at += align256(bytes); return here; };
     l.header = take(sizeof(Header));
@@ -567,133 +741,114 @@ int layout(const i6train_ce_problem& p, Layout& l) {
     l.row_target = take(4 * l.rows_p);
     l.target_logit = take(4 * l.rows_p);
     l.lse = take(4 * l.rows_p);
-    l.x = take((size_t)rows * l.S * l.Kp * 2);
-    l.w = l.own_weight ? take((size_t)p.F * l.S * l.Kp * 2) : 0;
+    l.x_bytes = (size_t)l.rows_p * l.S * l.Kp * 2;
+    l.w_bytes = (size_t)l.weights_p * l.S * l.Kp * 2;
+    l.x = take(l.x_bytes);
+    l.w = take(l.w_bytes);
     l.part = take(sizeof(float2) * l.class_tiles * l.rows_p);
     l.forward = at;
 
     at = 0;
-    int64_t piece = (int64_t)(kPieceBytes / (4 * (size_t)l.S * l.rows_p)) / kTile * kTile;
-    const int64_t all = (int64_t)l.class_tiles * kTile;
-    piece = piece < kTile ? kTile : (piece > all ? all : piece);
-    l.piece = (int)piece;
-    const int64_t tiles = piece / kTile * ceil_div(p.D, kTile);
-    l.splits = (int)ceil_div((int64_t)512, tiles);
-    const int most = (int)ceil_div(rows, (int64_t)512);
-    if (l.splits > most) l.splits = most;
+    int64_t piece = (int64_t)(kPieceBytes / (2 * (size_t)l.S * l.rows_p)) / kM * kM;
+    const int64_t classes = (int64_t)l.class_tiles * kM;
+    piece = piece < kM ? kM : (piece > classes ? classes : piece);
+    l.piece = (int)round_up(ceil_div(classes, ceil_div(classes, piece)), kM);      // pieces of one size
+    const int64_t tiles = (int64_t)l.piece / kM * ceil_div(p.D, kN);
+    int64_t splits = ceil_div((int64_t)512, tiles);
+    const int64_t most = ceil_div(l.rows, (int64_t)512), least = ceil_div((int64_t)l.rows_p * l.S * (l.piece > l.Kp ? l.piece : l.Kp) * 2, (int64_t)1 << 31);
+    splits = splits > most ? most : splits;
+    l.splits = (int)(splits < least ? least : splits);      // offsets within a range of k have 32 bits
     l.back = take(sizeof(BackHeader));
     l.row_scale = take(4 * l.rows_p);
-    l.xt = take((size_t)p.D * l.S * l.rows_p * 2);
-    l.wt = take((size_t)p.D * l.S * all * 2);
-    l.g = take((size_t)l.rows_p * l.S * piece * 2);
-    l.gt = take((size_t)piece * l.S * l.rows_p * 2);
+    l.g_bytes = (size_t)l.rows_p * l.S * l.piece * 2;
+    l.g = take(l.g_bytes);
     l.dx = take(4 * (size_t)l.rows_p * p.D);
-    l.dw = take(4 * (size_t)l.splits * piece * p.D);
+    l.dw = take(4 * (size_t)l.splits * l.piece * p.D);
+    l.sums = take(4 * (size_t)l.row_tiles * p.F);
     l.backward = at;
     return I6TRAIN_OK;
 }
 
 int groups_for(int64_t rows) { return (int)(rows < 16384 ? ceil_div(rows, (int64_t)4) : 4096); }
 
-template <typename In, typename T>
+Frames frames_of(const i6train_ce_problem& p, const Layout& l) {
+    return {p.hidden, p.hidden_stride_b, p.hidden_stride_t, p.seq_lens, p.targets, p.targets_stride_b, p.targets_stride_t, p.B, p.T, p.F, p.D, l.Kp};
+}
+
+template <typename In, int KIND> void launch_product(const ProductArgs& q, const EpilogueArgs& e, int tiles_m, int tiles_n, hipStream_t s) {
+    product<In, KIND><<<dim3(round_up(tiles_m * tiles_n * q.splits, 8)), dim3(kThreads), 0, s>>>(q, e);
+}
+
+template <typename In>
 int forward(const i6train_ce_problem& p, const Layout& l, float* loss, char* ws, hipStream_t s) {
-    constexpr int S = sizeof(In) == 4 ? 2 : 1;
-    const int64_t rows = (int64_t)p.B * p.T;
+    const Frames f = frames_of(p, l);
+    const Weights w{p.weight, p.weight_stride_f, p.bias};
     Header* header = (Header*)(ws + l.header);
     int* offsets = (int*)(ws + l.offsets);
-    ce_begin<<<dim3(1), dim3(1024), 0, s>>>(p.seq_lens, p.B, p.T, offsets, header);
-    if (S == 2) {
-        ce_most<<<dim3(groups_for(rows)), dim3(256), 0, s>>>((const float*)p.hidden, p.hidden_stride_b, p.hidden_stride_t, rows, p.T, p.D, p.seq_lens, p.targets, p.targets_stride_b,
-                                                                p.targets_stride_t, p.F, &header->most_x);
-        ce_most<<<dim3(groups_for(p.F)), dim3(256), 0, s>>>((const float*)p.weight, 0, p.weight_stride_f, p.F, p.F, p.D, nullptr, nullptr, 0, 0, 0, &header->most_w);
-    }
-    PackArgs a{};
-    a.x = p.hidden; a.stride_b = p.hidden_stride_b; a.stride_t = p.hidden_stride_t;
-    a.rows = rows; a.T = p.T; a.D = p.D; a.Kp = l.Kp; a.classes = p.F;
-    a.lens = p.seq_lens; a.offsets = offsets; a.targets = p.targets; a.tgt_b = p.targets_stride_b; a.tgt_t = p.targets_stride_t;
-    a.most = &header->most_x;
-    a.out = ws + l.x; a.row_frame = (int*)(ws + l.row_frame); a.row_target = (int*)(ws + l.row_target); a.loss = loss;
-    ce_pack<In, T><<<dim3(groups_for(rows)), dim3(256), 0, s>>>(a);
-    if (l.own_weight) {
-        PackArgs w{};
-        w.x = p.weight; w.stride_t = p.weight_stride_f;
-        w.rows = p.F; w.T = p.F; w.D = p.D; w.Kp = l.Kp;
-        w.most = &header->most_w; w.out = ws + l.w;
-        ce_pack<In, T><<<dim3(groups_for(p.F)), dim3(256), 0, s>>>(w);
-    }
-    const void* weight = l.own_weight ? ws + l.w : p.weight;
-    const int64_t weight_stride = l.own_weight ? S * (int64_t)l.Kp : p.weight_stride_f;
+    ce_look<In><<<dim3(1 + 2 * kParts), dim3(kThreads), 0, s>>>(f, w, offsets, header);
+    const Packed o{(f16*)(ws + l.x), (f16*)(ws + l.w), (int*)(ws + l.row_frame), (int*)(ws + l.row_target), (float*)(ws + l.target_logit), loss};
+    ce_pack<In><<<dim3(groups_for(l.rows + kPad + l.weights_p)), dim3(kThreads), 0, s>>>(f, w, offsets, header, o);
     ProductArgs q{};
-    q.a = {weight, weight_stride, l.Kp, p.F, nullptr};
-    q.b = {ws + l.x, S * (int64_t)l.Kp, l.Kp, 0, &header->rows};
+    q.a = {o.w, l.S * (int64_t)l.Kp, l.Kp, (int64_t)l.w_bytes, p.F, nullptr};
+    q.b = {o.x, l.S * (int64_t)l.Kp, l.Kp, (int64_t)l.x_bytes, 0, &header->rows};
     q.K = l.Kp; q.splits = 1;
     EpilogueArgs e{};
-    e.bias = p.bias; e.bias_f32 = p.dtype == I6TRAIN_F32; e.header = header; e.classes = p.F;
-    e.row_target = (int*)(ws + l.row_target); e.part = (float2*)(ws + l.part); e.target_logit = (float*)(ws + l.target_logit); e.rows_p = l.rows_p;
-    product<T, kStatistics><<<dim3(l.class_tiles, l.row_tiles), dim3(kThreads), 0, s>>>(q, e);
-    ce_finish<<<dim3(ceil_div(rows, (int64_t)256)), dim3(256), 0, s>>>(header, e.part, l.class_tiles, l.rows_p, (int*)(ws + l.row_frame), e.row_target, e.target_logit, p.T, p.F,
-                                                                       (float*)(ws + l.lse), loss, status_slot());
+    e.bias = p.bias; e.header = header; e.part = (float2*)(ws + l.part); e.rows_p = l.rows_p;
+    launch_product<In, kStatistics>(q, e, l.class_tiles, l.row_tiles, s);
+    ce_finish<<<dim3(ceil_div(l.rows, (int64_t)256)), dim3(256), 0, s>>>(header, e.part, l.class_tiles, l.rows_p, o.row_frame, o.row_target, o.target_logit, p.T, p.F,
+                                                                         (float*)(ws + l.lse), loss, status_slot());
     return launched();
 }
 
-template <typename In, typename T>
+template <typename In>
 int backward(const i6train_ce_problem& p, const Layout& l, const float* grad_loss, int64_t gs_b, int64_t gs_t, void* grad_hidden, void* grad_weight, void* grad_bias,
              const char* fw, char* ws, hipStream_t s) {
-    constexpr int S = sizeof(In) == 4 ? 2 : 1;
-    const int64_t rows = (int64_t)p.B * p.T;
     const Header* header = (const Header*)(fw + l.header);
     BackHeader* back = (BackHeader*)(ws + l.back);
     const int* row_target = (const int*)(fw + l.row_target);
     float* row_scale = (float*)(ws + l.row_scale);
-    const int64_t all = (int64_t)l.class_tiles * kTile;
-    ce_clear<<<dim3(1), dim3(1), 0, s>>>(back);
-    ce_row_scale<<<dim3(ceil_div(rows, (int64_t)256)), dim3(256), 0, s>>>(header, (const int*)(fw + l.row_frame), row_target, grad_loss, gs_b, gs_t, p.T, p.F, row_scale, &back->most_g);
-    const void* weight = l.own_weight ? fw + l.w : p.weight;
-    const int64_t weight_stride = l.own_weight ? S * (int64_t)l.Kp : p.weight_stride_f;
-    TransposeArgs x{(const uint16_t*)(fw + l.x), S * (int64_t)l.Kp, l.Kp, 0, &header->rows, p.D, (uint16_t*)(ws + l.xt), S * l.rows_p, l.rows_p};
-    if (grad_weight) ce_transpose<<<dim3(l.rows_p / 64, ceil_div(p.D, 64), S), dim3(256), 0, s>>>(x);
-    TransposeArgs w{(const uint16_t*)weight, weight_stride, l.Kp, p.F, nullptr, p.D, (uint16_t*)(ws + l.wt), S * all, all};
-    if (grad_hidden) ce_transpose<<<dim3(ceil_div(p.F, 64), ceil_div(p.D, 64), S), dim3(256), 0, s>>>(w);
-
+    const f16 *x = (const f16*)(fw + l.x), *w = (const f16*)(fw + l.w);
+    f16* g = (f16*)(ws + l.g);
+    float *dx = (float*)(ws + l.dx), *dw = (float*)(ws + l.dw), *sums = grad_bias ? (float*)(ws + l.sums) : nullptr;
+    const int64_t row_size = l.S * (int64_t)l.Kp, g_stride = l.S * (int64_t)l.piece;
+    ce_row_scale<<<dim3(kParts), dim3(256), 0, s>>>(header, (const int*)(fw + l.row_frame), row_target, grad_loss, gs_b, gs_t, p.T, p.F, row_scale, back);
     for (int first = 0; first < p.F; first += l.piece) {
-        const int classes = p.F - first < l.piece ? p.F - first : l.piece;
-        const int Kc = round_up(classes, kStep);
+        const int classes = p.F - first < l.piece ? p.F - first : l.piece, class_tiles = ceil_div(classes, kM);
+        const Operand piece_w{w + first * row_size, row_size, l.Kp, (int64_t)l.w_bytes - first * row_size * 2, classes, nullptr};
         ProductArgs q{};
-        q.a = {(const T*)weight + first * weight_stride, weight_stride, l.Kp, classes, nullptr};
-        q.b = {fw + l.x, S * (int64_t)l.Kp, l.Kp, 0, &header->rows};
+        q.a = piece_w;
+        q.b = {x, row_size, l.Kp, (int64_t)l.x_bytes, 0, &header->rows};
         q.K = l.Kp; q.splits = 1;
         EpilogueArgs e{};
-        e.bias = p.bias; e.bias_f32 = p.dtype == I6TRAIN_F32; e.header = header; e.back = back; e.first_class = first; e.classes = p.F;
-        e.row_target = row_target; e.rows_p = l.rows_p; e.lse = (const float*)(fw + l.lse); e.row_scale = row_scale;
-        e.g = ws + l.g; e.g_stride = S * (int64_t)l.piece; e.g_half = l.piece;
-        e.gt = ws + l.gt; e.gt_stride = S * l.rows_p; e.gt_half = l.rows_p;
-        product<T, kGradient><<<dim3(ceil_div(classes, kTile), l.row_tiles), dim3(kThreads), 0, s>>>(q, e);
+        e.bias = p.bias; e.header = header; e.back = back; e.first_class = first;
+        e.row_target = row_target; e.target_logit = (const float*)(fw + l.target_logit); e.lse = (const float*)(fw + l.lse); e.row_scale = row_scale;
+        e.g = g; e.g_stride = g_stride; e.g_half = l.piece;
+        e.column_sums = sums; e.column_stride = p.F;
+        launch_product<In, kGradient>(q, e, class_tiles, l.row_tiles, s);
         if (grad_hidden) {
             ProductArgs d{};
-            d.a = {ws + l.g, S * (int64_t)l.piece, l.piece, 0, &header->rows};
-            d.b = {(const T*)(ws + l.wt) + first, S * all, all, p.D, nullptr};
-            d.K = Kc; d.splits = 1;
+            d.a = {g, g_stride, l.piece, (int64_t)l.g_bytes, 0, &header->rows};
+            d.b = piece_w;
+            d.b.rows = p.D;
+            d.K = round_up(classes, kK); d.splits = 1;
             EpilogueArgs o{};
-            o.out = (float*)(ws + l.dx); o.out_stride = p.D; o.add = first > 0;
-            product<T, kStore><<<dim3(l.row_tiles, ceil_div(p.D, kTile)), dim3(kThreads), 0, s>>>(d, o);
+            o.out = dx; o.out_stride = p.D; o.add = first > 0;
+            launch_product<In, kHidden>(d, o, ceil_div(l.rows, (int64_t)kM), ceil_div(p.D, kN), s);
         }
         if (grad_weight) {
             ProductArgs d{};
-            d.a = {ws + l.gt, S * l.rows_p, l.rows_p, classes, nullptr};
-            d.b = {ws + l.xt, S * l.rows_p, l.rows_p, p.D, nullptr};
+            d.a = {g, g_stride, l.piece, (int64_t)l.g_bytes, classes, nullptr};
+            d.b = {x, row_size, l.Kp, (int64_t)l.x_bytes, p.D, nullptr};
             d.n_k = &header->rows; d.splits = l.splits;
             EpilogueArgs o{};
-            o.out = (float*)(ws + l.dw); o.out_stride = p.D; o.out_split = (int64_t)l.piece * p.D;
-            product<T, kStore><<<dim3(ceil_div(classes, kTile), ceil_div(p.D, kTile), l.splits), dim3(kThreads), 0, s>>>(d, o);
+            o.out = dw; o.out_stride = p.D; o.out_split = (int64_t)l.piece * p.D;
+            launch_product<In, kWeight>(d, o, class_tiles, ceil_div(p.D, kN), s);
             const int64_t n = (int64_t)classes * p.D;
-            ce_store_weight<In><<<dim3(ceil_div(n, (int64_t)256)), dim3(256), 0, s>>>(header, back, o.out, l.splits, o.out_split, n, (In*)grad_weight + (int64_t)first * p.D);
+            ce_store_weight<In><<<dim3(ceil_div(n, (int64_t)256)), dim3(256), 0, s>>>(header, back, dw, l.splits, o.out_split, n, (In*)grad_weight + (int64_t)first * p.D);
         }
-        if (grad_bias)
-            ce_store_bias<T, In><<<dim3(classes), dim3(256), 0, s>>>(header, back, (const T*)(ws + l.gt), S * l.rows_p, l.rows_p, (In*)grad_bias + first);
     }
-    if (grad_hidden)
-        ce_store_hidden<In><<<dim3(groups_for(rows)), dim3(256), 0, s>>>(header, back, (const int*)(fw + l.offsets), p.seq_lens, p.targets, p.targets_stride_b, p.targets_stride_t,
-                                                                         (const float*)(ws + l.dx), p.B, p.T, p.F, p.D, (In*)grad_hidden);
+    if (grad_hidden) ce_store_hidden<In><<<dim3(groups_for(l.rows)), dim3(256), 0, s>>>(header, back, frames_of(p, l), (const int*)(fw + l.offsets), dx, (In*)grad_hidden);
+    if (grad_bias) ce_store_bias<In><<<dim3(ceil_div(p.F, 256)), dim3(256), 0, s>>>(header, back, sums, p.F, p.F, (In*)grad_bias);
     return launched();
 }
 
@@ -718,8 +873,8 @@ int i6train_ce_forward(const i6train_ce_problem* p, float* loss, void* workspace
     Layout l;
     I6TRAIN_TRY(layout(*p, l));
     if (workspace_bytes < l.forward) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
-    if (p->dtype == I6TRAIN_F32) return forward<float, f16>(*p, l, loss, (char*)workspace, (hipStream_t)stream);
-    return forward<bf16, bf16>(*p, l, loss, (char*)workspace, (hipStream_t)stream);
+    if (p->dtype == I6TRAIN_F32) return forward<float>(*p, l, loss, (char*)workspace, (hipStream_t)stream);
+    return forward<bf16>(*p, l, loss, (char*)workspace, (hipStream_t)stream);
 }
 
 int i6train_ce_backward(const i6train_ce_problem* p, const float* grad_loss, int64_t grad_stride_b, int64_t grad_stride_t, void* grad_hidden, void* grad_weight, void* grad_bias,
@@ -728,9 +883,8 @@ int i6train_ce_backward(const i6train_ce_problem* p, const float* grad_loss, int
     Layout l;
     I6TRAIN_TRY(layout(*p, l));
     if (forward_bytes < l.forward || workspace_bytes < l.backward) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
-    if (p->dtype == I6TRAIN_F32)
-        return backward<float, f16>(*p, l, grad_loss, grad_stride_b, grad_stride_t, grad_hidden, grad_weight, grad_bias, (const char*)forward_workspace, (char*)workspace, (hipStream_t)stream);
-    return backward<bf16, bf16>(*p, l, grad_loss, grad_stride_b, grad_stride_t, grad_hidden, grad_weight, grad_bias, (const char*)forward_workspace, (char*)workspace, (hipStream_t)stream);
+    const auto run = p->dtype == I6TRAIN_F32 ? backward<float> : backward<bf16>;
+    return run(*p, l, grad_loss, grad_stride_b, grad_stride_t, grad_hidden, grad_weight, grad_bias, (const char*)forward_workspace, (char*)workspace, (hipStream_t)stream);
 }
 
 }  // extern "C"
