@@ -300,8 +300,8 @@ using lds_ptr = __attribute__((address_space(3))) void*;
 
 // One operand's part of a stage: R rows of the tile by kK.  LDS is filled by loads that bypass the registers and write 64 lanes x 16 bytes in
 // order; which 16 bytes a lane asks for is free, and places them so that reading has no bank conflicts.
-//   consecutive k:   row r has 4 chunks of 8 k; chunk c lies at place c ^ ((r >> 1) & 3) of the row.  A fragment is one read of 16 bytes.
-//   consecutive m:   k has R / 8 chunks of 8 m; chunk c lies at place c ^ ((k & 3) << 1).  A fragment is two reads that
+//   consecutive k:   row r has 4 chunks of 8 k; chunk c lies at place c ^ ((r >> 2) & 3) of the row.  A fragment is one read of 16 bytes.
+//   consecutive m:   k has R / 8 chunks of 8 m; chunk c lies at place c ^ ((k & 3) << 2).  A fragment is two reads that
 //                    transpose 4 k x 16 m within 16 lanes.
 template <int R, bool kConsecutiveK> struct Side {
     static constexpr int kLoads = R * kK * 2 / 16 / kThreads;      // per thread and stage
@@ -309,7 +309,7 @@ template <int R, bool kConsecutiveK> struct Side {
     __amdgpu_buffer_rsrc_t rsrc;
     uint32_t from[kLoads];       // byte offsets of this lane's chunks at k = 0
     uint32_t step, half;         // bytes from stage to stage, and to the second halves
-    int read[2];                 // byte offsets of this lane's fragments
+    int read[4];                 // byte offsets of this lane's fragments
 
     __device__ __forceinline__ void set(const Operand& o, int rows, int first, int k0, int base_row) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -322,22 +322,22 @@ template <int R, bool kConsecutiveK> struct Side {
         for (int i = 0; i < kLoads; i++) {
             const int slot = (i * 4 + wave) * 64 + lane;
             if (kConsecutiveK) {
-                const int r = slot >> 2, c = (slot & 3) ^ ((r >> 1) & 3);
+                const int r = slot >> 2, c = (slot & 3) ^ ((r >> 2) & 3);
                 from[i] = (uint32_t)(min(r, rows - 1 - first) * o.row_stride * 2 + c * 16);      // rows behind the last are the last again
             } else {
-                const int k = slot / (R / 8), c = (slot % (R / 8)) ^ ((k & 3) << 1);
+                const int k = slot / (R / 8), c = (slot % (R / 8)) ^ ((k & 3) << 2);
                 const int last = (int)((o.row_stride - first) / 8 - 1);                          // columns behind the row's end as well
                 from[i] = (uint32_t)(k * o.row_stride * 2 + min(c, last) * 16);
             }
         }
         if (kConsecutiveK) {
-            const int r = base_row + (lane & 31), x = (r >> 1) & 3;
+            const int r = base_row + (lane & 31), x = (r >> 2) & 3;
             read[0] = r * 64 + (((lane >> 5) ^ x) * 16);
             read[1] = r * 64 + (((2 + (lane >> 5)) ^ x) * 16);
         } else {
             const int k = (lane >> 5) * 8 + ((lane & 15) >> 2), m = base_row / 8 + ((lane >> 4) & 1) * 2;
 #pragma unroll
-            for (int i = 0; i < 2; i++) read[i] = k * (R * 2) + (((m + i * 4) ^ ((k & 3) << 1)) + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
+            for (int i = 0; i < 4; i++) read[i] = k * (R * 2) + (((m + i * 4) ^ ((k & 3) << 2)) + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
         }
     }
     __device__ __forceinline__ void fetch(char* lds, uint32_t offset) const {
@@ -351,7 +351,7 @@ template <int R, bool kConsecutiveK> struct Side {
         if constexpr (kConsecutiveK) {
             return *reinterpret_cast<const f16x8*>(lds + read[kk] + b * 32 * 64);
         } else {
-            const char* at = lds + read[b & 1] + (b >> 1) * 128 + kk * 16 * (R * 2);
+            const char* at = lds + read[b] + kk * 16 * (R * 2);
             using P = __attribute__((address_space(3))) s16x4*;
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(at + 4 * (R * 2)));
             return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
