@@ -27,7 +27,8 @@
 namespace i6train {
 namespace {
 
-constexpr int kM = 256, kN = 128;    // a workgroup's tile of C: four waves, 128 x 64 each
+constexpr int kM = 256;              // rows of a workgroup's tile of C, and, per two waves of 128 x 64 each, 64 columns
+constexpr int kN = 128;              // its columns where the tile's logits are worked on
 constexpr int kK = 32;               // k of one stage
 constexpr int kStages = 3;
 constexpr int kThreads = 256;
@@ -289,38 +290,56 @@ struct EpilogueArgs {
     int add;
 };
 
-__device__ __forceinline__ void wait_for_loads(int left) {        // the number of this wave's loads that may still be on their way
-    if (left) __builtin_amdgcn_s_waitcnt(0x0f70 | 6); else __builtin_amdgcn_s_waitcnt(0x0f70);
+// Waits for this wave's reads of LDS, and for its loads but the last `kLeft`; then for the other waves.
+template <int kLeft> __device__ __forceinline__ void wait_and_meet() {
+    static_assert(kLeft < 16, "one field of the instruction");
     asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070 | kLeft);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
 
-using lds_ptr = __attribute__((address_space(3))) void*;
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p; }
+
+// A description of `bytes` bytes from p on; reads behind them give 0.
+using descriptor = uint32_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ descriptor describe(const void* p, int64_t bytes) {
+    const uint64_t at = (uint64_t)p;
+    const auto uniform = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
+    return descriptor{uniform((uint32_t)at), uniform((uint32_t)(at >> 32) & 0xffffu), uniform(bytes > 0xffffffffll ? 0xffffffffu : (uint32_t)bytes), 0x00020000u};
+}
+
+// 64 lanes x 16 bytes from the described memory, at `from` + `offset`, to LDS from address `to` on, lane after lane.  Written out because the compiler
+// takes every later read of LDS to depend on it and waits for all loads there; wait_and_meet() counts them instead.  No register receives
+// anything; m0, which takes the address in LDS, is used by nothing else here.
+__device__ __forceinline__ void load_to_lds(descriptor d, uint32_t to, uint32_t from, uint32_t offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(from), "s"(d), "s"(offset) : "memory");
+}
 
 // One operand's part of a stage: R rows of the tile by kK.  LDS is filled by loads that bypass the registers and write 64 lanes x 16 bytes in
 // order; which 16 bytes a lane asks for is free, and places them so that reading has no bank conflicts.
 //   consecutive k:   row r has 4 chunks of 8 k; chunk c lies at place c ^ ((r >> 2) & 3) of the row.  A fragment is one read of 16 bytes.
 //   consecutive m:   k has R / 8 chunks of 8 m; chunk c lies at place c ^ ((k & 3) << 2).  A fragment is two reads that
 //                    transpose 4 k x 16 m within 16 lanes.
-template <int R, bool kConsecutiveK> struct Side {
-    static constexpr int kLoads = R * kK * 2 / 16 / kThreads;      // per thread and stage
+template <int R, bool kConsecutiveK, int kWaves> struct Side {
+    static constexpr int kLoads = R * kK * 2 / 1024 / kWaves;      // per wave and stage
     static constexpr int kBytes = R * kK * 2;
-    __amdgpu_buffer_rsrc_t rsrc;
+    descriptor source;
     uint32_t from[kLoads];       // byte offsets of this lane's chunks at k = 0
     uint32_t step, half;         // bytes from stage to stage, and to the second halves
     int read[4];                 // byte offsets of this lane's fragments
 
     __device__ __forceinline__ void set(const Operand& o, int rows, int first, int k0, int base_row) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int lane = threadIdx.x & 63, wave = wave_index();
         const int64_t origin = kConsecutiveK ? first * o.row_stride + k0 : k0 * o.row_stride + first;
-        const int64_t left = o.bytes - origin * 2;
-        rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(o.p + origin), 0, left > 0xffffffffll ? 0xffffffffu : (uint32_t)left, 0x00020000);
+        source = describe(o.p + origin, o.bytes - origin * 2);
         half = (uint32_t)(o.half_stride * 2);
         step = kConsecutiveK ? kK * 2 : (uint32_t)(kK * o.row_stride * 2);
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
-            const int slot = (i * 4 + wave) * 64 + lane;
+            const int slot = (i * kWaves + wave) * 64 + lane;
             if (kConsecutiveK) {
                 const int r = slot >> 2, c = (slot & 3) ^ ((r >> 2) & 3);
                 from[i] = (uint32_t)(min(r, rows - 1 - first) * o.row_stride * 2 + c * 16);      // rows behind the last are the last again
@@ -340,11 +359,10 @@ template <int R, bool kConsecutiveK> struct Side {
             for (int i = 0; i < 4; i++) read[i] = k * (R * 2) + (((m + i * 4) ^ ((k & 3) << 2)) + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
         }
     }
-    __device__ __forceinline__ void fetch(char* lds, uint32_t offset) const {
-        const int wave = threadIdx.x >> 6;
+    __device__ __forceinline__ void fetch(uint32_t lds, uint32_t offset) const {
+        const int wave = wave_index();
 #pragma unroll
-        for (int i = 0; i < kLoads; i++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(lds + (i * 4 + wave) * 1024), 16, from[i], offset, 0, 0);
+        for (int i = 0; i < kLoads; i++) load_to_lds(source, lds + (i * kWaves + wave) * 1024, from[i], offset);
     }
     // block b of 32 rows, k of kk * 16 .. + 15
     __device__ __forceinline__ f16x8 fragment(const char* lds, int b, int kk) const {
@@ -360,27 +378,29 @@ template <int R, bool kConsecutiveK> struct Side {
 };
 
 constexpr int kGStride = kM * 2 + 16;      // bytes of a row of G in LDS
-constexpr int kStageBytes = (kM + kN) * kK * 2;
-constexpr int kLdsBytes = kStages * kStageBytes;
-static_assert(kN * kGStride <= kLdsBytes, "G goes through the stages' LDS");
 
 // In           type of the user's tensors: two halves where it has 32 bits
 // KIND         what becomes of a tile
-template <typename In, int KIND>
-__global__ __launch_bounds__(kThreads, 2) void product(ProductArgs p, EpilogueArgs e) {
-#if __HIP_DEVICE_COMPILE__      // the buffer descriptors are types of the device
+// NW           pairs of waves: a tile has 64 NW columns
+template <typename In, int KIND, int NW>
+__global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueArgs e) {
+#if __HIP_DEVICE_COMPILE__
     constexpr int S = sizeof(In) == 4 ? 2 : 1;
-    constexpr bool kAk = KIND != kWeight, kBk = KIND == kStatistics || KIND == kGradient;
-    __shared__ alignas(16) char lds[kLdsBytes];
-    __shared__ float bias[KIND == kStatistics || KIND == kGradient ? kM : 1];
-    __shared__ float join[KIND == kStatistics || KIND == kGradient ? 4 : 1][kM];
+    constexpr bool kAk = KIND != kWeight, kBk = KIND == kStatistics || KIND == kGradient;      // consecutive k
+    constexpr int kWaves = 2 * NW, kCols = 64 * NW;
+    constexpr int kStageBytes = (kM + kCols) * kK * 2;
+    constexpr bool kLogits = KIND == kStatistics || KIND == kGradient;
+    static_assert(!kLogits || (kCols == kN && kN * kGStride <= kStages * kStageBytes), "G goes through the stages' LDS");
+    __shared__ alignas(16) char lds[kStages * kStageBytes];
+    __shared__ float bias[kLogits ? kM : 1];
+    __shared__ float join[kLogits ? 4 : 1][kM];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave & 1, wn = wave >> 1;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), wm = wave & 1, wn = wave >> 1;
     const int rows_a = p.a.n_rows ? *p.a.n_rows : p.a.rows, rows_b = p.b.n_rows ? *p.b.n_rows : p.b.rows;
 
     // Workgroups go round the eight dies; each die has an L2 of its own, so it gets a range of tiles of its own, in groups of eight tiles of A:
     // the 64 tiles that a die works on at a time have 8 + 8 operand tiles among them, not 64 + 1.
-    const int tiles_m = ceil_div(rows_a, kM), tiles_n = ceil_div(rows_b, kN), tiles = tiles_m * tiles_n * p.splits;
+    const int tiles_m = ceil_div(rows_a, kM), tiles_n = ceil_div(rows_b, kCols), tiles = tiles_m * tiles_n * p.splits;
     const int each = ceil_div(tiles, 8);
     int tile = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= each || tile >= tiles) return;
@@ -389,7 +409,7 @@ __global__ __launch_bounds__(kThreads, 2) void product(ProductArgs p, EpilogueAr
     const int group = tile / (8 * tiles_n), in_group = min(8, tiles_m - group * 8);
     tile -= group * 8 * tiles_n;
     const int tile_m = group * 8 + tile % in_group, tile_n = tile / in_group;
-    const int m0 = tile_m * kM, n0 = tile_n * kN;
+    const int m0 = tile_m * kM, n0 = tile_n * kCols;
 
     int K = p.n_k ? round_up(*p.n_k, kK) : p.K;
     int k0 = 0;
@@ -400,69 +420,108 @@ __global__ __launch_bounds__(kThreads, 2) void product(ProductArgs p, EpilogueAr
     }
     const int steps = (K - k0) / kK, all = S == 2 ? 3 * steps : steps;
 
-    Side<kM, kAk> A;
-    Side<kN, kBk> B;
+    Side<kM, kAk, kWaves> A;
+    Side<kCols, kBk, kWaves> B;
     A.set(p.a, rows_a, m0, k0, wm * 128);
     B.set(p.b, rows_b, n0, k0, wn * 64);
-    if constexpr (KIND == kStatistics || KIND == kGradient) {
+    if constexpr (kLogits) {
         const int m = m0 + tid;       // classes behind the last: -inf, no probability
         float v = m < rows_a ? 0.f : -INFINITY;
         if (e.bias && m < rows_a) v = (float)static_cast<const In*>(e.bias)[e.first_class + m] * kLog2e;
         bias[tid] = v;
     }
 
+    // register r of a 32 x 32 block: row (r & 3) + 8 (r >> 2) + 4 (lane >> 5), column lane & 31
+    const int row_in = wm * 128 + 4 * (lane >> 5), col_in = wn * 64 + (lane & 31);
     acc_t acc[4][2];
+    if (!kLogits && e.add) {
+        const float* out = e.out + (int64_t)m0 * e.out_stride + n0;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+        for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < 2; j++)
+            for (int j = 0; j < 2; j++) {
+                const int n = min(col_in + j * 32, rows_b - n0 - 1);
 #pragma unroll
-            for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
+                for (int r = 0; r < 16; r++) {
+                    const int m = min(row_in + i * 32 + (r & 3) + 8 * (r >> 2), rows_a - m0 - 1);
+                    acc[i][j][r] = out[(int64_t)m * e.out_stride + n] * (S == 2 ? 1.f / kLow : 1.f);       // scaled on the way, below
+                }
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
+    }
 
-    const auto fetch = [&](int it) {
-        char* at = lds + (it % kStages) * kStageBytes;
+    const uint32_t stages = lds_address(lds);
+    const auto fetch = [&](int it, int at) {
         uint32_t oa, ob;
         if constexpr (S == 2) {
-            const int part = it / steps, k = it - part * steps;       // high x low, low x high, high x high
+            const int part = it >= 2 * steps ? 2 : (it >= steps ? 1 : 0), k = it - part * steps;       // high x low, low x high, high x high
             oa = k * A.step + (part == 1 ? A.half : 0);
             ob = k * B.step + (part == 0 ? B.half : 0);
         } else {
             oa = it * A.step;
             ob = it * B.step;
         }
-        A.fetch(at, oa);
-        B.fetch(at + A.kBytes, ob);
+        A.fetch(stages + at, __builtin_amdgcn_readfirstlane(oa));
+        B.fetch(stages + at + A.kBytes, __builtin_amdgcn_readfirstlane(ob));
     };
-    if (all > 0) fetch(0);
-    if (all > 1) fetch(1);
-    for (int it = 0; it < all; it++) {
-        wait_for_loads(it + 1 < all);          // this stage is there for everyone, and nobody reads the one before it any more
-        if (it + 2 < all) fetch(it + 2);
-        if (S == 2 && it == 2 * steps) {
+    // Three stages of LDS and two sets of fragments: while the first half of a stage is multiplied its second half is read, and while that is
+    // multiplied the first half of the next stage.  In between the waves meet: this stage is in registers and its LDS free for the loads of the stage
+    // after the next two, and the next stage has come in, whose loads have had the time of more than two stages.
+    f16x8 fa[2][4], fb[2][2];
+    const auto read = [&](int at, int kk) {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+        for (int j = 0; j < 2; j++) fb[kk][j] = B.fragment(lds + at + A.kBytes, j, kk);
 #pragma unroll
-                for (int j = 0; j < 2; j++) acc[i][j] *= kLow;
+        for (int i = 0; i < 4; i++) fa[kk][i] = A.fragment(lds + at, i, kk);
+    };
+    const auto multiply = [&](int kk) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[kk][i], fb[kk][j], acc[i][j], 0, 0, 0);
+        // one product, then its share of the reads, and so on
+        constexpr int kReads = (kAk ? 4 : 8) + (kBk ? 2 : 4);
+#pragma unroll
+        for (int i = 0; i < 6; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, kReads / 6, 0);
         }
-        const char* at = lds + (it % kStages) * kStageBytes;
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+    };
+    constexpr int kPerStage = Side<kM, kAk, kWaves>::kLoads + Side<kCols, kBk, kWaves>::kLoads;
+    if (all > 0) {
+        fetch(0, 0);
+        if (all > 1) fetch(1, kStageBytes);
+        if (all > 2) fetch(2, 2 * kStageBytes);
+        if (all > 2) wait_and_meet<2 * kPerStage>();
+        else wait_and_meet<0>();
+        read(0, 0);
+        int at = 0;
+        for (int it = 0; it < all; it++) {
+            if (S == 2 && it == 2 * steps) {
 #pragma unroll
-        for (int kk = 0; kk < kK / 16; kk++) {
-            f16x8 fa[4], fb[2];
+                for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int j = 0; j < 2; j++) fb[j] = B.fragment(at + A.kBytes, j, kk);
-#pragma unroll
-            for (int i = 0; i < 4; i++) fa[i] = A.fragment(at, i, kk);
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < 2; j++) acc[i][j] *= kLow;
+            }
+            read(at, 1);
+            multiply(0);
+            if (it + 2 < all) wait_and_meet<kPerStage>();
+            else wait_and_meet<0>();
+            if (it + 3 < all) fetch(it + 3, at);
+            at = at == 2 * kStageBytes ? 0 : at + kStageBytes;
+            read(at, 0);         // behind the last stage: what is there, and not used
+            multiply(1);
         }
     }
 
-    // register r of a 32 x 32 block: row (r & 3) + 8 (r >> 2) + 4 (lane >> 5), column lane & 31
-    const int row_in = wm * 128 + 4 * (lane >> 5), col_in = wn * 64 + (lane & 31);
-
-    if constexpr (KIND == kHidden || KIND == kWeight) {
+    if constexpr (!kLogits) {
         float* out = e.out + part_of_k * e.out_split + (int64_t)m0 * e.out_stride + n0;
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -472,10 +531,7 @@ __global__ __launch_bounds__(kThreads, 2) void product(ProductArgs p, EpilogueAr
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     const int m = row_in + i * 32 + (r & 3) + 8 * (r >> 2);
-                    if (m0 + m < rows_a && n0 + n < rows_b) {
-                        float* to = out + (int64_t)m * e.out_stride + n;
-                        *to = e.add ? *to + acc[i][j][r] : acc[i][j][r];
-                    }
+                    if (m0 + m < rows_a && n0 + n < rows_b) out[(int64_t)m * e.out_stride + n] = acc[i][j][r];
                 }
             }
         return;
@@ -775,8 +831,9 @@ Frames frames_of(const i6train_ce_problem& p, const Layout& l) {
     return {p.hidden, p.hidden_stride_b, p.hidden_stride_t, p.seq_lens, p.targets, p.targets_stride_b, p.targets_stride_t, p.B, p.T, p.F, p.D, l.Kp};
 }
 
-template <typename In, int KIND> void launch_product(const ProductArgs& q, const EpilogueArgs& e, int tiles_m, int tiles_n, hipStream_t s) {
-    product<In, KIND><<<dim3(round_up(tiles_m * tiles_n * q.splits, 8)), dim3(kThreads), 0, s>>>(q, e);
+template <typename In, int KIND, int NW> void launch_product(const ProductArgs& q, const EpilogueArgs& e, int64_t rows_a, int64_t rows_b, hipStream_t s) {
+    const int64_t tiles = ceil_div(rows_a, (int64_t)kM) * ceil_div(rows_b, (int64_t)(64 * NW)) * q.splits;
+    product<In, KIND, NW><<<dim3((unsigned)round_up(tiles, 8)), dim3(128 * NW), 0, s>>>(q, e);
 }
 
 template <typename In>
@@ -794,7 +851,7 @@ int forward(const i6train_ce_problem& p, const Layout& l, float* loss, char* ws,
     q.K = l.Kp; q.splits = 1;
     EpilogueArgs e{};
     e.bias = p.bias; e.header = header; e.part = (float2*)(ws + l.part); e.rows_p = l.rows_p;
-    launch_product<In, kStatistics>(q, e, l.class_tiles, l.row_tiles, s);
+    launch_product<In, kStatistics, 2>(q, e, p.F, l.rows, s);
     ce_finish<<<dim3(ceil_div(l.rows, (int64_t)256)), dim3(256), 0, s>>>(header, e.part, l.class_tiles, l.rows_p, o.row_frame, o.row_target, o.target_logit, p.T, p.F,
                                                                          (float*)(ws + l.lse), loss, status_slot());
     return launched();
@@ -813,7 +870,7 @@ int backward(const i6train_ce_problem& p, const Layout& l, const float* grad_los
     const int64_t row_size = l.S * (int64_t)l.Kp, g_stride = l.S * (int64_t)l.piece;
     ce_row_scale<<<dim3(kParts), dim3(256), 0, s>>>(header, (const int*)(fw + l.row_frame), row_target, grad_loss, gs_b, gs_t, p.T, p.F, row_scale, back);
     for (int first = 0; first < p.F; first += l.piece) {
-        const int classes = p.F - first < l.piece ? p.F - first : l.piece, class_tiles = ceil_div(classes, kM);
+        const int classes = p.F - first < l.piece ? p.F - first : l.piece;
         const Operand piece_w{w + first * row_size, row_size, l.Kp, (int64_t)l.w_bytes - first * row_size * 2, classes, nullptr};
         ProductArgs q{};
         q.a = piece_w;
@@ -824,7 +881,7 @@ int backward(const i6train_ce_problem& p, const Layout& l, const float* grad_los
         e.row_target = row_target; e.target_logit = (const float*)(fw + l.target_logit); e.lse = (const float*)(fw + l.lse); e.row_scale = row_scale;
         e.g = g; e.g_stride = g_stride; e.g_half = l.piece;
         e.column_sums = sums; e.column_stride = p.F;
-        launch_product<In, kGradient>(q, e, class_tiles, l.row_tiles, s);
+        launch_product<In, kGradient, 2>(q, e, classes, l.rows, s);
         if (grad_hidden) {
             ProductArgs d{};
             d.a = {g, g_stride, l.piece, (int64_t)l.g_bytes, 0, &header->rows};
@@ -833,7 +890,7 @@ int backward(const i6train_ce_problem& p, const Layout& l, const float* grad_los
             d.K = round_up(classes, kK); d.splits = 1;
             EpilogueArgs o{};
             o.out = dx; o.out_stride = p.D; o.add = first > 0;
-            launch_product<In, kHidden>(d, o, ceil_div(l.rows, (int64_t)kM), ceil_div(p.D, kN), s);
+            launch_product<In, kHidden, 2>(d, o, l.rows, p.D, s);
         }
         if (grad_weight) {
             ProductArgs d{};
@@ -842,7 +899,7 @@ int backward(const i6train_ce_problem& p, const Layout& l, const float* grad_los
             d.n_k = &header->rows; d.splits = l.splits;
             EpilogueArgs o{};
             o.out = dw; o.out_stride = p.D; o.out_split = (int64_t)l.piece * p.D;
-            launch_product<In, kWeight>(d, o, class_tiles, ceil_div(p.D, kN), s);
+            launch_product<In, kWeight, 2>(d, o, classes, p.D, s);
             const int64_t n = (int64_t)classes * p.D;
             ce_store_weight<In><<<dim3(ceil_div(n, (int64_t)256)), dim3(256), 0, s>>>(header, back, dw, l.splits, o.out_split, n, (In*)grad_weight + (int64_t)first * p.D);
         }
