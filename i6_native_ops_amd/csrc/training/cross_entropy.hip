@@ -30,7 +30,6 @@ namespace {
 constexpr int kM = 256;              // rows of a workgroup's tile of C, and, per two waves of 128 x 64 each, 64 columns
 constexpr int kN = 128;              // its columns where the tile's logits are worked on
 constexpr int kK = 32;               // k of one stage
-constexpr int kStages = 3;
 constexpr int kThreads = 256;
 constexpr int kParts = 256;          // partial maxima of a tensor
 constexpr int kPad = 64;             // rows and columns of operands are padded with zeros to multiples of this
@@ -329,6 +328,7 @@ template <int R, bool kConsecutiveK, int kWaves> struct Side {
     descriptor source;
     uint32_t from[kLoads];       // byte offsets of this lane's chunks at k = 0
     uint32_t step, half;         // bytes from stage to stage, and to the second halves
+    uint32_t to;                 // this wave's place in a stage
     int read[4];                 // byte offsets of this lane's fragments
 
     __device__ __forceinline__ void set(const Operand& o, int rows, int first, int k0, int base_row) {
@@ -336,6 +336,7 @@ template <int R, bool kConsecutiveK, int kWaves> struct Side {
         const int64_t origin = kConsecutiveK ? first * o.row_stride + k0 : k0 * o.row_stride + first;
         source = describe(o.p + origin, o.bytes - origin * 2);
         half = (uint32_t)(o.half_stride * 2);
+        to = wave * 1024;
         step = kConsecutiveK ? kK * 2 : (uint32_t)(kK * o.row_stride * 2);
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
@@ -359,10 +360,8 @@ template <int R, bool kConsecutiveK, int kWaves> struct Side {
             for (int i = 0; i < 4; i++) read[i] = k * (R * 2) + (((m + i * 4) ^ ((k & 3) << 2)) + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
         }
     }
-    __device__ __forceinline__ void fetch(uint32_t lds, uint32_t offset) const {
-        const int wave = wave_index();
-#pragma unroll
-        for (int i = 0; i < kLoads; i++) load_to_lds(source, lds + (i * kWaves + wave) * 1024, from[i], offset);
+    __device__ __forceinline__ void fetch(int i, uint32_t lds, uint32_t offset) const {
+        load_to_lds(source, lds + to + i * kWaves * 1024, from[i], offset);
     }
     // block b of 32 rows, k of kk * 16 .. + 15
     __device__ __forceinline__ f16x8 fragment(const char* lds, int b, int kk) const {
@@ -387,10 +386,10 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
 #if __HIP_DEVICE_COMPILE__
     constexpr int S = sizeof(In) == 4 ? 2 : 1;
     constexpr bool kAk = KIND != kWeight, kBk = KIND == kStatistics || KIND == kGradient;      // consecutive k
-    constexpr int kWaves = 2 * NW, kCols = 64 * NW;
+    constexpr int kWaves = 2 * NW, kCols = 64 * NW, kStages = NW == 2 ? 3 : 4;
     constexpr int kStageBytes = (kM + kCols) * kK * 2;
     constexpr bool kLogits = KIND == kStatistics || KIND == kGradient;
-    static_assert(!kLogits || (kCols == kN && kN * kGStride <= kStages * kStageBytes), "G goes through the stages' LDS");
+    static_assert(KIND != kGradient || (kCols == kN && kN * kGStride <= kStages * kStageBytes), "G goes through the stages' LDS");
     __shared__ alignas(16) char lds[kStages * kStageBytes];
     __shared__ float bias[kLogits ? kM : 1];
     __shared__ float join[kLogits ? 4 : 1][kM];
@@ -425,16 +424,18 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
     A.set(p.a, rows_a, m0, k0, wm * 128);
     B.set(p.b, rows_b, n0, k0, wn * 64);
     if constexpr (kLogits) {
+        if (tid < kM) {
         const int m = m0 + tid;       // classes behind the last: -inf, no probability
         float v = m < rows_a ? 0.f : -INFINITY;
         if (e.bias && m < rows_a) v = (float)static_cast<const In*>(e.bias)[e.first_class + m] * kLog2e;
         bias[tid] = v;
+        }
     }
 
     // register r of a 32 x 32 block: row (r & 3) + 8 (r >> 2) + 4 (lane >> 5), column lane & 31
     const int row_in = wm * 128 + 4 * (lane >> 5), col_in = wn * 64 + (lane & 31);
     acc_t acc[4][2];
-    if (!kLogits && e.add) {
+    if (KIND == kHidden && e.add) {
         const float* out = e.out + (int64_t)m0 * e.out_stride + n0;
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -447,6 +448,8 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
                     acc[i][j][r] = out[(int64_t)m * e.out_stride + n] * (S == 2 ? 1.f / kLow : 1.f);       // scaled on the way, below
                 }
             }
+        // here, or the compiler waits for all loads before the products of every stage
+        __builtin_amdgcn_s_waitcnt(0x0f70);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -457,51 +460,43 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
     }
 
     const uint32_t stages = lds_address(lds);
-    const auto fetch = [&](int it, int at) {
-        uint32_t oa, ob;
+    constexpr int kLoadsA = Side<kM, kAk, kWaves>::kLoads, kPerStage = kLoadsA + Side<kCols, kBk, kWaves>::kLoads;
+    uint32_t next_a = 0, next_b = 0;           // offsets of the stage that is fetched next
+    const auto place_of = [&](int it) {
         if constexpr (S == 2) {
             const int part = it >= 2 * steps ? 2 : (it >= steps ? 1 : 0), k = it - part * steps;       // high x low, low x high, high x high
-            oa = k * A.step + (part == 1 ? A.half : 0);
-            ob = k * B.step + (part == 0 ? B.half : 0);
+            next_a = __builtin_amdgcn_readfirstlane(k * A.step + (part == 1 ? A.half : 0));
+            next_b = __builtin_amdgcn_readfirstlane(k * B.step + (part == 0 ? B.half : 0));
         } else {
-            oa = it * A.step;
-            ob = it * B.step;
+            next_a = it * A.step;
+            next_b = it * B.step;
         }
-        A.fetch(stages + at, __builtin_amdgcn_readfirstlane(oa));
-        B.fetch(stages + at + A.kBytes, __builtin_amdgcn_readfirstlane(ob));
     };
-    // Three stages of LDS and two sets of fragments: while the first half of a stage is multiplied its second half is read, and while that is
-    // multiplied the first half of the next stage.  In between the waves meet: this stage is in registers and its LDS free for the loads of the stage
-    // after the next two, and the next stage has come in, whose loads have had the time of more than two stages.
+    const auto fetch = [&](int i, int at) {    // load i of a stage
+        if (i < kLoadsA) A.fetch(i, stages + at, next_a);
+        else B.fetch(i - kLoadsA, stages + at + A.kBytes, next_b);
+    };
     f16x8 fa[2][4], fb[2][2];
-    const auto read = [&](int at, int kk) {
-#pragma unroll
-        for (int j = 0; j < 2; j++) fb[kk][j] = B.fragment(lds + at + A.kBytes, j, kk);
-#pragma unroll
-        for (int i = 0; i < 4; i++) fa[kk][i] = A.fragment(lds + at, i, kk);
+    const auto read = [&](int i, int at, int kk) {      // fragment i of a half stage
+        if (i < 2) fb[kk][i] = B.fragment(lds + at + A.kBytes, i, kk);
+        else fa[kk][i - 2] = A.fragment(lds + at, i - 2, kk);
     };
-    const auto multiply = [&](int kk) {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[kk][i], fb[kk][j], acc[i][j], 0, 0, 0);
-        // one product, then its share of the reads, and so on
-        constexpr int kReads = (kAk ? 4 : 8) + (kBk ? 2 : 4);
-#pragma unroll
-        for (int i = 0; i < 6; i++) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, kReads / 6, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-    };
-    constexpr int kPerStage = Side<kM, kAk, kWaves>::kLoads + Side<kCols, kBk, kWaves>::kLoads;
+    // Stages of LDS and two sets of fragments: while the first half of a stage is multiplied its second half is read, and while that is
+    // multiplied the first half of the next stage.  In between the waves meet: this stage is in registers and its LDS free for another one, and the
+    // next stage has come in.  Reads and loads are spread over the products: issued all at once, the loads of eight waves fill the queue
+    // of the compute unit, and no product starts until they have gone through.
     if (all > 0) {
-        fetch(0, 0);
-        if (all > 1) fetch(1, kStageBytes);
-        if (all > 2) fetch(2, 2 * kStageBytes);
-        if (all > 2) wait_and_meet<2 * kPerStage>();
+#pragma unroll
+        for (int n = 0; n < kStages; n++) {
+            if (n >= all) break;
+            place_of(n);
+#pragma unroll
+            for (int i = 0; i < kPerStage; i++) fetch(i, n * kStageBytes);
+        }
+        if (all >= kStages) wait_and_meet<(kStages - 1) * kPerStage>();
         else wait_and_meet<0>();
-        read(0, 0);
+#pragma unroll
+        for (int i = 0; i < 6; i++) read(i, 0, 0);
         int at = 0;
         for (int it = 0; it < all; it++) {
             if (S == 2 && it == 2 * steps) {
@@ -510,14 +505,25 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
 #pragma unroll
                     for (int j = 0; j < 2; j++) acc[i][j] *= kLow;
             }
-            read(at, 1);
-            multiply(0);
-            if (it + 2 < all) wait_and_meet<kPerStage>();
+#pragma unroll
+            for (int n = 0; n < 8; n++) {
+                acc[n >> 1][n & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][n >> 1], fb[0][n & 1], acc[n >> 1][n & 1], 0, 0, 0);
+                if (n < 6) read(n, at, 1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (it + kStages - 1 < all) wait_and_meet<(kStages - 2) * kPerStage>();
             else wait_and_meet<0>();
-            if (it + 3 < all) fetch(it + 3, at);
-            at = at == 2 * kStageBytes ? 0 : at + kStageBytes;
-            read(at, 0);         // behind the last stage: what is there, and not used
-            multiply(1);
+            const int free = at;
+            const bool more = it + kStages < all;
+            if (more) place_of(it + kStages);
+            at = at == (kStages - 1) * kStageBytes ? 0 : at + kStageBytes;
+#pragma unroll
+            for (int n = 0; n < 8; n++) {
+                acc[n >> 1][n & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[1][n >> 1], fb[1][n & 1], acc[n >> 1][n & 1], 0, 0, 0);
+                if (n < 6) read(n, at, 0);         // behind the last stage: what is there, and not used
+                if (more && n >= 1 && n - 1 < kPerStage) fetch(n - 1, free);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     }
 
@@ -577,7 +583,7 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
             }
         }
         __syncthreads();
-        if (tid < kN && n0 + tid < rows_b) {
+        if (tid < kCols && n0 + tid < rows_b) {
             const float ma = join[0][tid], mb = join[2][tid], most = fmaxf(ma, mb), base = most == -INFINITY ? 0.f : most;
             const float sum = join[1][tid] * exp2_fast(ma - base) + join[3][tid] * exp2_fast(mb - base);
             e.part[(int64_t)tile_m * e.rows_p + n0 + tid] = make_float2(most, sum);
@@ -809,8 +815,8 @@ int layout(const i6train_ce_problem& p, Layout& l) {
     const int64_t classes = (int64_t)l.class_tiles * kM;
     piece = piece < kM ? kM : (piece > classes ? classes : piece);
     l.piece = (int)round_up(ceil_div(classes, ceil_div(classes, piece)), kM);      // pieces of one size
-    const int64_t tiles = (int64_t)l.piece / kM * ceil_div(p.D, kN);
-    int64_t splits = ceil_div((int64_t)512, tiles);
+    const int64_t tiles = (int64_t)l.piece / kM * ceil_div(p.D, 256);
+    int64_t splits = 256 / tiles < 1 ? 1 : 256 / tiles;
     const int64_t most = ceil_div(l.rows, (int64_t)512), least = ceil_div((int64_t)l.rows_p * l.S * (l.piece > l.Kp ? l.piece : l.Kp) * 2, (int64_t)1 << 31);
     splits = splits > most ? most : splits;
     l.splits = (int)(splits < least ? least : splits);      // offsets within a range of k have 32 bits
@@ -851,7 +857,7 @@ int forward(const i6train_ce_problem& p, const Layout& l, float* loss, char* ws,
     q.K = l.Kp; q.splits = 1;
     EpilogueArgs e{};
     e.bias = p.bias; e.header = header; e.part = (float2*)(ws + l.part); e.rows_p = l.rows_p;
-    launch_product<In, kStatistics, 2>(q, e, p.F, l.rows, s);
+    launch_product<In, kStatistics, 4>(q, e, p.F, l.rows, s);
     ce_finish<<<dim3(ceil_div(l.rows, (int64_t)256)), dim3(256), 0, s>>>(header, e.part, l.class_tiles, l.rows_p, o.row_frame, o.row_target, o.target_logit, p.T, p.F,
                                                                          (float*)(ws + l.lse), loss, status_slot());
     return launched();
@@ -890,7 +896,7 @@ int backward(const i6train_ce_problem& p, const Layout& l, const float* grad_los
             d.K = round_up(classes, kK); d.splits = 1;
             EpilogueArgs o{};
             o.out = dx; o.out_stride = p.D; o.add = first > 0;
-            launch_product<In, kHidden, 2>(d, o, l.rows, p.D, s);
+            launch_product<In, kHidden, 4>(d, o, l.rows, p.D, s);
         }
         if (grad_weight) {
             ProductArgs d{};
@@ -899,7 +905,7 @@ int backward(const i6train_ce_problem& p, const Layout& l, const float* grad_los
             d.n_k = &header->rows; d.splits = l.splits;
             EpilogueArgs o{};
             o.out = dw; o.out_stride = p.D; o.out_split = (int64_t)l.piece * p.D;
-            launch_product<In, kWeight, 2>(d, o, classes, p.D, s);
+            launch_product<In, kWeight, 4>(d, o, classes, p.D, s);
             const int64_t n = (int64_t)classes * p.D;
             ce_store_weight<In><<<dim3(ceil_div(n, (int64_t)256)), dim3(256), 0, s>>>(header, back, dw, l.splits, o.out_split, n, (In*)grad_weight + (int64_t)first * p.D);
         }
