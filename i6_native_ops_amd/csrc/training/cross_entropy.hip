@@ -32,6 +32,7 @@ constexpr int kN = 128;              // its columns where the tile's logits are 
 constexpr int kK = 32;               // k of one stage
 constexpr int kThreads = 256;
 constexpr int kParts = 256;          // partial maxima of a tensor
+constexpr int kLookThreads = 1024;   // every wave waits for lengths, targets and rows in turn: many waves, few rows each
 constexpr int kPad = 64;             // rows and columns of operands are padded with zeros to multiples of this
 constexpr float kLow = 0x1p-11f;     // weight of the second half of a 32-bit value
 
@@ -111,13 +112,14 @@ template <typename In> __device__ __forceinline__ void load8(const In* row, int 
 // Workgroup 0: offsets[b], the first row of sequence b.  The next kParts: largest magnitudes of the frames with a target; the
 // last kParts: those of the weights.
 template <typename In>
-__global__ __launch_bounds__(kThreads) void ce_look(Frames f, Weights w, int* offsets, Header* header) {
-    __shared__ int sums[4];
-    __shared__ uint32_t most_of[4];
+__global__ __launch_bounds__(kLookThreads) void ce_look(Frames f, Weights w, int* offsets, Header* header) {
+    constexpr int kWaves = kLookThreads / kWave;
+    __shared__ int sums[kWaves];
+    __shared__ uint32_t most_of[kWaves];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (blockIdx.x == 0) {
         int carry = 0;
-        for (int base = 0; base < f.B; base += kThreads) {
+        for (int base = 0; base < f.B; base += kLookThreads) {
             const int b = base + threadIdx.x;
             int n = b < f.B ? f.lens[b] : 0;
             n = n < 0 ? 0 : (n > f.T ? f.T : n);
@@ -131,7 +133,7 @@ __global__ __launch_bounds__(kThreads) void ce_look(Frames f, Weights w, int* of
             int before = carry;
             for (int i = 0; i < wave; i++) before += sums[i];
             if (b < f.B) offsets[b] = before + sum - n;
-            carry += sums[0] + sums[1] + sums[2] + sums[3];
+            for (int i = 0; i < kWaves; i++) carry += sums[i];
             __syncthreads();
         }
         if (threadIdx.x == 0) header->rows = carry;
@@ -142,7 +144,7 @@ __global__ __launch_bounds__(kThreads) void ce_look(Frames f, Weights w, int* of
     const In* base = static_cast<const In*>(weights ? w.p : f.hidden);
     const int64_t rows = weights ? f.F : (int64_t)f.B * f.T;
     uint32_t most = 0;
-    for (int64_t r = (int64_t)part * 4 + wave; r < rows; r += kParts * 4) {
+    for (int64_t r = (int64_t)part * kWaves + wave; r < rows; r += kParts * kWaves) {
         const In* row;
         if (weights) {
             row = base + r * w.stride;
@@ -162,7 +164,10 @@ __global__ __launch_bounds__(kThreads) void ce_look(Frames f, Weights w, int* of
     most = wave_most(most);
     if (lane == 0) most_of[wave] = most;
     __syncthreads();
-    if (threadIdx.x == 0) (weights ? header->most_w : header->most_x)[part] = umax(umax(most_of[0], most_of[1]), umax(most_of[2], most_of[3]));
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < kWaves; i++) most = umax(most, most_of[i]);
+        (weights ? header->most_w : header->most_x)[part] = most;
+    }
 }
 
 // x as one operand or as two halves.
@@ -282,11 +287,15 @@ struct EpilogueArgs {
     int64_t rows_p;
     const float *target_logit, *lse, *row_scale;
     f16* g;  int64_t g_stride, g_half;     // [row][halves][piece]
-    float* column_sums;                    // [tile of rows][classes]; of G, may be null
-    int64_t column_stride;
-    // kHidden, kWeight: float [split][m][n]
-    float* out;  int64_t out_stride, out_split;
-    int add;
+    // kHidden: m is the row, n the feature
+    float* sum;  int64_t sum_stride;       // [m][n] over the pieces so far
+    int add, last;                         // to what is there; the last piece, which goes to `out`
+    const int* row_frame;
+    int classes;
+    void* out;
+    // kWeight: m is the class, n the feature; ranges of k one after another
+    float* part_out;  int64_t part_stride;
+    float* bias_out;  int64_t bias_stride; // [range][class], sums of G over the rows
 };
 
 // Waits for this wave's reads of LDS, and for its loads but the last `kLeft`; then for the other waves.
@@ -436,7 +445,7 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
     const int row_in = wm * 128 + 4 * (lane >> 5), col_in = wn * 64 + (lane & 31);
     acc_t acc[4][2];
     if (KIND == kHidden && e.add) {
-        const float* out = e.out + (int64_t)m0 * e.out_stride + n0;
+        const float* sum = e.sum + (int64_t)m0 * e.sum_stride + n0;
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -445,7 +454,7 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     const int m = min(row_in + i * 32 + (r & 3) + 8 * (r >> 2), rows_a - m0 - 1);
-                    acc[i][j][r] = out[(int64_t)m * e.out_stride + n] * (S == 2 ? 1.f / kLow : 1.f);       // scaled on the way, below
+                    acc[i][j][r] = sum[(int64_t)m * e.sum_stride + n] * (S == 2 ? 1.f / kLow : 1.f);       // scaled on the way, below
                 }
             }
         // here, or the compiler waits for all loads before the products of every stage
@@ -481,6 +490,17 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
         if (i < 2) fb[kk][i] = B.fragment(lds + at + A.kBytes, i, kk);
         else fa[kk][i - 2] = A.fragment(lds + at, i - 2, kk);
     };
+    // kWeight: the fragments of A are G with the rows along k; the gradient of the bias is their sum
+    const bool with_bias = KIND == kWeight && e.bias_out && tile_n == 0 && wn == 0;
+    float bias_sum[4] = {};
+    const auto add_up = [&](int kk) {
+        if (KIND == kWeight && with_bias) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int r = 0; r < 8; r++) bias_sum[i] += (float)fa[kk][i][r];
+        }
+    };
     // Stages of LDS and two sets of fragments: while the first half of a stage is multiplied its second half is read, and while that is
     // multiplied the first half of the next stage.  In between the waves meet: this stage is in registers and its LDS free for another one, and the
     // next stage has come in.  Reads and loads are spread over the products: issued all at once, the loads of eight waves fill the queue
@@ -504,7 +524,10 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
                 for (int i = 0; i < 4; i++)
 #pragma unroll
                     for (int j = 0; j < 2; j++) acc[i][j] *= kLow;
+#pragma unroll
+                for (int i = 0; i < 4; i++) bias_sum[i] *= kLow;
             }
+            if (S == 1 || it >= steps) add_up(0);
 #pragma unroll
             for (int n = 0; n < 8; n++) {
                 acc[n >> 1][n & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][n >> 1], fb[0][n & 1], acc[n >> 1][n & 1], 0, 0, 0);
@@ -517,6 +540,7 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
             const bool more = it + kStages < all;
             if (more) place_of(it + kStages);
             at = at == (kStages - 1) * kStageBytes ? 0 : at + kStageBytes;
+            if (S == 1 || it >= steps) add_up(1);
 #pragma unroll
             for (int n = 0; n < 8; n++) {
                 acc[n >> 1][n & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[1][n >> 1], fb[1][n & 1], acc[n >> 1][n & 1], 0, 0, 0);
@@ -527,8 +551,8 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
         }
     }
 
-    if constexpr (!kLogits) {
-        float* out = e.out + part_of_k * e.out_split + (int64_t)m0 * e.out_stride + n0;
+    if constexpr (KIND == kWeight) {
+        float* out = e.part_out + part_of_k * e.part_stride + (int64_t)m0 * rows_b + n0;
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -537,7 +561,57 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     const int m = row_in + i * 32 + (r & 3) + 8 * (r >> 2);
-                    if (m0 + m < rows_a && n0 + n < rows_b) out[(int64_t)m * e.out_stride + n] = acc[i][j][r];
+                    if (m0 + m < rows_a && n0 + n < rows_b) out[(int64_t)m * rows_b + n] = acc[i][j][r];
+                }
+            }
+        if (with_bias) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float v = bias_sum[i] + __shfl_xor(bias_sum[i], 32);
+                const int m = m0 + wm * 128 + i * 32 + lane;
+                if (lane < 32 && m < rows_a) e.bias_out[part_of_k * e.bias_stride + m] = v;
+            }
+        }
+        return;
+    }
+
+    if constexpr (KIND == kHidden) {
+        if (!e.last) {
+            float* sum = e.sum + (int64_t)m0 * e.sum_stride + n0;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int n = col_in + j * 32;
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const int m = row_in + i * 32 + (r & 3) + 8 * (r >> 2);
+                        if (m0 + m < rows_a && n0 + n < rows_b) sum[(int64_t)m * e.sum_stride + n] = acc[i][j][r];
+                    }
+                }
+            return;
+        }
+        // back to the frames, scales off; where the target is out of range, NaN
+        int* frames = reinterpret_cast<int*>(lds);
+        __syncthreads();
+        for (int i = tid; i < kM; i += 128 * NW) {
+            const int m = m0 + i;
+            frames[i] = m < rows_a ? (e.row_target[m] >= e.classes ? ~e.row_frame[m] : e.row_frame[m]) : 0;
+        }
+        __syncthreads();
+        const int down = -scale_exponent(e.back->most_g), down_w = -scale_exponent(e.header->most_w);
+        In* out = static_cast<In*>(e.out) + n0;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int m = row_in + i * 32 + (r & 3) + 8 * (r >> 2), frame = frames[m];
+                In* row = out + (int64_t)(frame < 0 ? ~frame : frame) * rows_b;
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int n = col_in + j * 32;
+                    const float v = ldexpf(ldexpf(acc[i][j][r], down), down_w);
+                    if (m0 + m < rows_a && n0 + n < rows_b) row[n] = (In)(frame < 0 ? __builtin_nanf("") : v);
                 }
             }
         return;
@@ -623,7 +697,6 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
                 at_target = (exp2_fast(fmaf(e.target_logit[n0 + tid], kLog2e, -e.lse[n0 + tid])) - 1.f) * ldexpf(e.row_scale[n0 + tid], up);
             }
         }
-        float column[4] = {};
 #pragma unroll 1
         for (int h = 0; h < S; h++) {
             // through LDS, so that whole rows of the tile are written at once
@@ -660,23 +733,7 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
                 const int r = i * 8 + (tid >> 5), c = tid & 31;
                 *reinterpret_cast<u32x4*>(g + r * e.g_stride + c * 8) = *reinterpret_cast<const u32x4*>(lds + r * kGStride + c * 16);
             }
-            if (e.column_sums) {
-                float sum[4] = {};
-                for (int r = wave * 32; r < wave * 32 + 32; r++) {
-                    const f16x4 v = *reinterpret_cast<const f16x4*>(lds + r * kGStride + lane * 8);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) sum[i] += (float)v[i];
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) column[i] += h == 0 ? sum[i] : sum[i] * kLow;
-            }
             if (h + 1 < S) __syncthreads();
-        }
-        if (e.column_sums) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) join[wave][lane * 4 + i] = column[i];
-            __syncthreads();
-            if (m0 + tid < rows_a) e.column_sums[tile_n * e.column_stride + e.first_class + m0 + tid] = join[0][tid] + join[1][tid] + join[2][tid] + join[3][tid];
         }
     }
 #endif
@@ -685,15 +742,23 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
 // ---------------------------------------------------------------------------------------------------------- the rest
 
 // Statistics of the tiles joined: loss and log sum of a row.
-__global__ __launch_bounds__(256) void ce_finish(const Header* header, const float2* part, int tiles, int64_t rows_p, const int* row_frame,
+__global__ __launch_bounds__(64) void ce_finish(const Header* header, const float2* part, int tiles, int64_t rows_p, const int* row_frame,
                                                  const int* row_target, const float* target_logit, int T, int F, float* lse, float* loss, int* report) {
-    const int row = blockIdx.x * 256 + threadIdx.x;
+    const int row = blockIdx.x * 64 + threadIdx.x;
     if (row >= header->rows) return;
     float most = -INFINITY, sum = 0.f;
-    for (int i = 0; i < tiles; i++) {
-        const float2 p = part[i * rows_p + row];
-        const float m = fmaxf(most, p.x), base = m == -INFINITY ? 0.f : m;
-        sum = sum * exp2_fast(most - base) + p.y * exp2_fast(p.x - base);
+    for (int i = 0; i < tiles; i += 8) {
+        float2 p[8];
+        float m = most;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            p[k] = i + k < tiles ? part[(i + k) * rows_p + row] : make_float2(-INFINITY, 0.f);
+            m = fmaxf(m, p[k].x);
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        sum *= exp2_fast(most - base);
+#pragma unroll
+        for (int k = 0; k < 8; k++) sum += p[k].y * exp2_fast(p[k].x - base);
         most = m;
     }
     const float l = most + log2_fast(sum);
@@ -712,62 +777,65 @@ __global__ __launch_bounds__(256) void ce_finish(const Header* header, const flo
     loss[frame] = v;
 }
 
-// The incoming gradient of each row; rows without a target, or with one that is out of range, have none.  kParts workgroups.
+// The first kParts workgroups: the incoming gradient of each row; rows without a target, or with one that is out of range, have none.  The
+// others: zeros in the frames behind the ends.
+template <typename Out>
 __global__ __launch_bounds__(256) void ce_row_scale(const Header* header, const int* row_frame, const int* row_target, const float* grad_loss, int64_t stride_b,
-                                                    int64_t stride_t, int T, int F, float* row_scale, BackHeader* back) {
+                                                    int64_t stride_t, Frames f, float* row_scale, BackHeader* back, Out* grad_hidden) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (blockIdx.x >= kParts) {
+        const int64_t frames = (int64_t)f.B * f.T;
+        for (int64_t r = (int64_t)(blockIdx.x - kParts) * 4 + wave; r < frames; r += (int64_t)(gridDim.x - kParts) * 4) {
+            const int b = (int)(r / f.T), t = (int)(r % f.T);
+            if (t < f.lens[b]) continue;
+            for (int d = lane; d < f.D; d += 64) grad_hidden[r * f.D + d] = (Out)0.f;
+        }
+        return;
+    }
     __shared__ uint32_t most_of[4];
     uint32_t most = 0;
     for (int row = blockIdx.x * 256 + threadIdx.x; row < header->rows; row += kParts * 256) {
         float g = 0.f;
         const int frame = row_frame[row];
-        if (has_target(row_target[row], F)) g = grad_loss[(int64_t)(frame / T) * stride_b + (int64_t)(frame % T) * stride_t];
+        if (has_target(row_target[row], f.F)) g = grad_loss[(int64_t)(frame / f.T) * stride_b + (int64_t)(frame % f.T) * stride_t];
         row_scale[row] = g;
         most = umax(most, finite_bits(g));
     }
     most = wave_most(most);
-    if ((threadIdx.x & 63) == 0) most_of[threadIdx.x >> 6] = most;
+    if (lane == 0) most_of[wave] = most;
     __syncthreads();
     if (threadIdx.x == 0) back->most_g[blockIdx.x] = umax(umax(most_of[0], most_of[1]), umax(most_of[2], most_of[3]));
 }
 
-// grad_hidden: rows back to their frames.
+// One piece of grad_weight and grad_bias: the ranges of k joined, scales off.
 template <typename Out>
-__global__ __launch_bounds__(256) void ce_store_hidden(const Header* header, const BackHeader* back, Frames f, const int* offsets, const float* acc, Out* out) {
-    const int lane = threadIdx.x & 63;
-    const int down = -scale_exponent(back->most_g), down_w = -scale_exponent(header->most_w);
-    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < (int64_t)f.B * f.T; r += (int64_t)gridDim.x * 4) {
-        const int64_t b = r / f.T, t = r % f.T;
-        const bool live = t < f.lens[b];
-        const float* row = acc + (live ? (int64_t)(offsets[b] + t) * f.D : 0);
-        const bool bad = live && f.targets[b * f.tgt_b + t * f.tgt_t] >= f.F;
-        for (int d = lane; d < f.D; d += 64) {
-            const float v = live ? ldexpf(ldexpf(row[d], down), down_w) : 0.f;
-            out[r * f.D + d] = (Out)(bad ? __builtin_nanf("") : v);
-        }
-    }
-}
-
-// One piece of grad_weight: the ranges of k joined.
-template <typename Out>
-__global__ __launch_bounds__(256) void ce_store_weight(const Header* header, const BackHeader* back, const float* part, int splits, int64_t split_stride, int64_t n, Out* out) {
+__global__ __launch_bounds__(256) void ce_store_weight(const Header* header, const BackHeader* back, const float* part, int splits, int64_t split_stride, int64_t n, Out* out,
+                                                       const float* bias_part, int64_t bias_stride, int classes, Out* bias) {
     const int down = -scale_exponent(back->most_g), down_x = -scale_exponent(header->most_x);
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    float v = 0.f;
-    for (int s = 0; s < splits; s++) v += part[s * split_stride + i];
-    out[i] = (Out)ldexpf(ldexpf(v, down), down_x);
-}
-
-// grad_bias: sums over the tiles of rows.
-template <typename Out>
-__global__ __launch_bounds__(256) void ce_store_bias(const Header* header, const BackHeader* back, const float* sums, int64_t stride, int F, Out* out) {
-    const int down = -scale_exponent(back->most_g);
-    const int f = blockIdx.x * 256 + threadIdx.x;
-    if (f >= F) return;
-    const int tiles = ceil_div(header->rows, kN);
-    float v = 0.f;
-    for (int i = 0; i < tiles; i++) v += sums[i * stride + f];
-    out[f] = (Out)ldexpf(v, down);
+    int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i < n) {
+        if (!out) return;
+        using V = float __attribute__((ext_vector_type(4)));
+        V v = 0.f;
+        if (i + 4 <= n && n % 4 == 0) {
+#pragma unroll 4
+            for (int s = 0; s < splits; s++) v += *reinterpret_cast<const V*>(part + s * split_stride + i);
+        } else {
+            for (int s = 0; s < splits; s++)
+                for (int k = 0; k < 4 && i + k < n; k++) v[k] += part[s * split_stride + i + k];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (i + k < n) out[i + k] = (Out)ldexpf(ldexpf(v[k], down), down_x);
+        return;
+    }
+    i -= round_up(n, 1024);         // the last workgroups
+    if (!bias || i < 0) return;
+    for (int k = 0; k < 4 && i + k < classes; k++) {
+        float v = 0.f;
+        for (int s = 0; s < splits; s++) v += bias_part[s * bias_stride + i + k];
+        bias[i + k] = (Out)ldexpf(v, down);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
@@ -779,7 +847,7 @@ struct Layout {
     int S, Kp, row_tiles, class_tiles, piece, splits;
     int64_t rows, rows_p, weights_p;
     size_t header, offsets, row_frame, row_target, target_logit, lse, x, w, part, x_bytes, w_bytes, forward;
-    size_t back, row_scale, g, dx, dw, sums, g_bytes, backward;
+    size_t back, row_scale, g, dx, dw, db, g_bytes, backward;
 };
 
 bool valid(const i6train_ce_problem* p) {
@@ -824,9 +892,9 @@ int layout(const i6train_ce_problem& p, Layout& l) {
     l.row_scale = take(4 * l.rows_p);
     l.g_bytes = (size_t)l.rows_p * l.S * l.piece * 2;
     l.g = take(l.g_bytes);
-    l.dx = take(4 * (size_t)l.rows_p * p.D);
+    l.dx = take(l.piece < p.F ? 4 * (size_t)l.rows_p * p.D : 0);
     l.dw = take(4 * (size_t)l.splits * l.piece * p.D);
-    l.sums = take(4 * (size_t)l.row_tiles * p.F);
+    l.db = take(4 * (size_t)l.splits * l.piece);
     l.backward = at;
     return I6TRAIN_OK;
 }
@@ -848,7 +916,7 @@ int forward(const i6train_ce_problem& p, const Layout& l, float* loss, char* ws,
     const Weights w{p.weight, p.weight_stride_f, p.bias};
     Header* header = (Header*)(ws + l.header);
     int* offsets = (int*)(ws + l.offsets);
-    ce_look<In><<<dim3(1 + 2 * kParts), dim3(kThreads), 0, s>>>(f, w, offsets, header);
+    ce_look<In><<<dim3(1 + 2 * kParts), dim3(kLookThreads), 0, s>>>(f, w, offsets, header);
     const Packed o{(f16*)(ws + l.x), (f16*)(ws + l.w), (int*)(ws + l.row_frame), (int*)(ws + l.row_target), (float*)(ws + l.target_logit), loss};
     ce_pack<In><<<dim3(groups_for(l.rows + kPad + l.weights_p)), dim3(kThreads), 0, s>>>(f, w, offsets, header, o);
     ProductArgs q{};
@@ -857,8 +925,8 @@ int forward(const i6train_ce_problem& p, const Layout& l, float* loss, char* ws,
     q.K = l.Kp; q.splits = 1;
     EpilogueArgs e{};
     e.bias = p.bias; e.header = header; e.part = (float2*)(ws + l.part); e.rows_p = l.rows_p;
-    launch_product<In, kStatistics, 4>(q, e, p.F, l.rows, s);
-    ce_finish<<<dim3(ceil_div(l.rows, (int64_t)256)), dim3(256), 0, s>>>(header, e.part, l.class_tiles, l.rows_p, o.row_frame, o.row_target, o.target_logit, p.T, p.F,
+    launch_product<In, kStatistics, 2>(q, e, p.F, l.rows, s);
+    ce_finish<<<dim3(ceil_div(l.rows, (int64_t)64)), dim3(64), 0, s>>>(header, e.part, l.class_tiles, l.rows_p, o.row_frame, o.row_target, o.target_logit, p.T, p.F,
                                                                          (float*)(ws + l.lse), loss, status_slot());
     return launched();
 }
@@ -872,9 +940,10 @@ int backward(const i6train_ce_problem& p, const Layout& l, const float* grad_los
     float* row_scale = (float*)(ws + l.row_scale);
     const f16 *x = (const f16*)(fw + l.x), *w = (const f16*)(fw + l.w);
     f16* g = (f16*)(ws + l.g);
-    float *dx = (float*)(ws + l.dx), *dw = (float*)(ws + l.dw), *sums = grad_bias ? (float*)(ws + l.sums) : nullptr;
+    float *dx = (float*)(ws + l.dx), *dw = (float*)(ws + l.dw), *db = grad_bias ? (float*)(ws + l.db) : nullptr;
     const int64_t row_size = l.S * (int64_t)l.Kp, g_stride = l.S * (int64_t)l.piece;
-    ce_row_scale<<<dim3(kParts), dim3(256), 0, s>>>(header, (const int*)(fw + l.row_frame), row_target, grad_loss, gs_b, gs_t, p.T, p.F, row_scale, back);
+    const int zeros = grad_hidden ? (int)(l.rows < 4096 ? ceil_div(l.rows, (int64_t)4) : 1024) : 0;
+    ce_row_scale<In><<<dim3(kParts + zeros), dim3(256), 0, s>>>(header, (const int*)(fw + l.row_frame), row_target, grad_loss, gs_b, gs_t, frames_of(p, l), row_scale, back, (In*)grad_hidden);
     for (int first = 0; first < p.F; first += l.piece) {
         const int classes = p.F - first < l.piece ? p.F - first : l.piece;
         const Operand piece_w{w + first * row_size, row_size, l.Kp, (int64_t)l.w_bytes - first * row_size * 2, classes, nullptr};
@@ -886,7 +955,6 @@ int backward(const i6train_ce_problem& p, const Layout& l, const float* grad_los
         e.bias = p.bias; e.header = header; e.back = back; e.first_class = first;
         e.row_target = row_target; e.target_logit = (const float*)(fw + l.target_logit); e.lse = (const float*)(fw + l.lse); e.row_scale = row_scale;
         e.g = g; e.g_stride = g_stride; e.g_half = l.piece;
-        e.column_sums = sums; e.column_stride = p.F;
         launch_product<In, kGradient, 2>(q, e, classes, l.rows, s);
         if (grad_hidden) {
             ProductArgs d{};
@@ -895,23 +963,24 @@ int backward(const i6train_ce_problem& p, const Layout& l, const float* grad_los
             d.b.rows = p.D;
             d.K = round_up(classes, kK); d.splits = 1;
             EpilogueArgs o{};
-            o.out = dx; o.out_stride = p.D; o.add = first > 0;
+            o.header = header; o.back = back; o.row_target = row_target; o.row_frame = (const int*)(fw + l.row_frame); o.classes = p.F;
+            o.sum = dx; o.sum_stride = p.D; o.add = first > 0; o.last = first + l.piece >= p.F; o.out = grad_hidden;
             launch_product<In, kHidden, 4>(d, o, l.rows, p.D, s);
         }
-        if (grad_weight) {
+        if (grad_weight || grad_bias) {
             ProductArgs d{};
             d.a = {g, g_stride, l.piece, (int64_t)l.g_bytes, classes, nullptr};
             d.b = {x, row_size, l.Kp, (int64_t)l.x_bytes, p.D, nullptr};
             d.n_k = &header->rows; d.splits = l.splits;
             EpilogueArgs o{};
-            o.out = dw; o.out_stride = p.D; o.out_split = (int64_t)l.piece * p.D;
+            o.part_out = dw; o.part_stride = (int64_t)l.piece * p.D; o.bias_out = db; o.bias_stride = l.piece;
             launch_product<In, kWeight, 4>(d, o, classes, p.D, s);
             const int64_t n = (int64_t)classes * p.D;
-            ce_store_weight<In><<<dim3(ceil_div(n, (int64_t)256)), dim3(256), 0, s>>>(header, back, dw, l.splits, o.out_split, n, (In*)grad_weight + (int64_t)first * p.D);
+            ce_store_weight<In><<<dim3((unsigned)(ceil_div(n, (int64_t)1024) + ceil_div(classes, 1024))), dim3(256), 0, s>>>(
+                header, back, dw, l.splits, o.part_stride, n, grad_weight ? (In*)grad_weight + (int64_t)first * p.D : nullptr, db, o.bias_stride, classes,
+                grad_bias ? (In*)grad_bias + first : nullptr);
         }
     }
-    if (grad_hidden) ce_store_hidden<In><<<dim3(groups_for(l.rows)), dim3(256), 0, s>>>(header, back, frames_of(p, l), (const int*)(fw + l.offsets), dx, (In*)grad_hidden);
-    if (grad_bias) ce_store_bias<In><<<dim3(ceil_div(p.F, 256)), dim3(256), 0, s>>>(header, back, sums, p.F, p.F, (In*)grad_bias);
     return launched();
 }
 
