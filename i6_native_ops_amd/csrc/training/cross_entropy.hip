@@ -518,6 +518,7 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
 #pragma unroll
         for (int i = 0; i < 6; i++) read(i, 0, 0);
         int at = 0;
+        __builtin_amdgcn_s_setprio(1);
         for (int it = 0; it < all; it++) {
             if (S == 2 && it == 2 * steps) {
 #pragma unroll
@@ -549,6 +550,7 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
     }
 
     if constexpr (KIND == kWeight) {
@@ -840,7 +842,7 @@ __global__ __launch_bounds__(256) void ce_store_weight(const Header* header, con
 
 // ------------------------------------------------------------------------------------------------------------- host
 
-constexpr size_t kPieceBytes = (size_t)256 << 20;      // of G: the caches in front of the memory hold 256 MB
+constexpr size_t kPieceBytes = (size_t)512 << 20;      // of G: the caches in front of the memory hold 256 MB
 
 // Where things are in the workspaces.
 struct Layout {
