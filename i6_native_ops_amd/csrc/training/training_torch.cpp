@@ -1,11 +1,13 @@
-// PyTorch-ROCm binding of libi6train.so: module `training_core`.  torch is used for device memory and the current
-// stream only; all arithmetic is behind the C ABI declared in include/i6train.h.
+// PyTorch-ROCm binding of libi6train.so: module `training_core`.  torch is used for device memory, the current
+// stream and the autograd graph; all arithmetic is behind the C ABI declared in include/i6train.h.  The graph's nodes
+// are C++: the smallest training steps take as long as their host work, of which nodes in Python would be the larger part.
 #include <optional>
 #include <tuple>
 #include <vector>
 
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include "../../../include/i6fbw.h"
@@ -71,7 +73,7 @@ i6train_ce_problem ce_problem(int64_t B, int64_t T, int64_t D, const torch::Tens
     return p;
 }
 
-std::vector<torch::Tensor> linear_cross_entropy_forward(const torch::Tensor& hidden, const torch::Tensor& weight, const torch::Tensor& targets, const torch::Tensor& seq_lens,
+std::tuple<torch::Tensor, torch::Tensor> linear_cross_entropy_forward(const torch::Tensor& hidden, const torch::Tensor& weight, const torch::Tensor& targets, const torch::Tensor& seq_lens,
                                                         const Optional& bias) {
     CHECK_CUDA(hidden);
     dtype_of(hidden, "hidden");
@@ -115,6 +117,7 @@ std::vector<Optional> linear_cross_entropy_backward(const torch::Tensor& grad_lo
                                                     bool need_weight, bool need_bias) {
     CHECK_CUDA(grad_loss);
     CHECK_TYPE(grad_loss, torch::kFloat32);
+    CHECK_DEVICE(grad_loss, weight);
     TORCH_CHECK(grad_loss.sizes() == targets.sizes(), "grad_loss must have shape (B, T)");
     CHECK_CUDA(forward_workspace);
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(weight.device());
@@ -131,6 +134,55 @@ std::vector<Optional> linear_cross_entropy_backward(const torch::Tensor& grad_lo
     check("linear_cross_entropy", i6train_ce_backward(&p, grad_loss.data_ptr<float>(), grad_loss.stride(0), grad_loss.stride(1), ptr(grad_hidden), ptr(grad_weight), ptr(grad_bias),
                                                       forward_workspace.data_ptr(), forward_workspace.numel(), workspace.data_ptr(), backward_bytes, (void*)current_stream()));
     return {grad_hidden, grad_weight, grad_bias};
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+torch::Tensor rows(const torch::Tensor& x) { return x.dim() == 0 || x.stride(-1) == 1 ? x : x.contiguous(); }
+Optional given(const torch::Tensor& x) { return x.defined() ? Optional(x) : Optional(); }
+torch::Tensor or_none(const Optional& x) { return x ? *x : torch::Tensor(); }
+bool wants_gradient(std::initializer_list<torch::Tensor> inputs) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const torch::Tensor& x : inputs)
+        if (x.defined() && x.requires_grad()) return true;
+    return false;
+}
+
+// Gradients of gradients are refused as they are asked for, not as create_graph is.
+variable_list once(const char* op, const variable_list& incoming, variable_list outgoing) {
+    if (!at::GradMode::is_enabled()) return outgoing;
+    bool tracked = false;
+    for (const torch::Tensor& g : incoming) tracked = tracked || (g.defined() && g.requires_grad());
+    if (!tracked) return outgoing;
+    for (torch::Tensor& g : outgoing)
+        if (g.defined()) g = g.detach().requires_grad_();
+    return (*std::make_shared<torch::autograd::DelayedError>(std::string(op) + " can be differentiated once", (int64_t)outgoing.size()))(std::move(outgoing));
+}
+
+struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
+    static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& hidden, const torch::Tensor& weight, const Optional& bias, const torch::Tensor& targets,
+                                 const torch::Tensor& seq_lens) {
+        auto [loss, workspace] = linear_cross_entropy_forward(hidden, weight, targets, seq_lens, bias);
+        ctx->save_for_backward({weight, or_none(bias), targets, seq_lens, workspace});
+        ctx->saved_data["features"] = hidden.size(2);
+        return loss;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        const std::vector<Optional> got = linear_cross_entropy_backward(grads[0], ctx->saved_data["features"].toInt(), saved[0], saved[2], saved[3], given(saved[1]), saved[4],
+                                                                        ctx->needs_input_grad(0), ctx->needs_input_grad(1), saved[1].defined() && ctx->needs_input_grad(2));      // (a missing bias has no number)
+        variable_list out(5);
+        for (int i = 0; i < 3; i++)
+            if (got[i]) out[i] = *got[i];
+        return once("linear_cross_entropy", grads, std::move(out));
+    }
+};
+
+torch::Tensor linear_cross_entropy(const torch::Tensor& hidden, const torch::Tensor& weight, const torch::Tensor& targets, const torch::Tensor& seq_lens, const Optional& bias) {
+    if (wants_gradient({hidden, weight, or_none(bias)}))
+        return LinearCrossEntropy::apply(rows(hidden), rows(weight), bias, targets, seq_lens);
+    return std::get<0>(linear_cross_entropy_forward(rows(hidden), rows(weight), targets, seq_lens, bias));
 }
 
 // --------------------------------------------------------------------------------------------------------- recurrence
@@ -206,6 +258,31 @@ std::vector<torch::Tensor> gated_recurrence_backward(const Optional& grad_h, con
     return {grad_x, grad_gate, grad_initial};
 }
 
+struct GatedRecurrence : torch::autograd::Function<GatedRecurrence> {
+    static variable_list forward(AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& gate, const Optional& initial, const Optional& seq_lens) {
+        std::vector<Optional> got = gated_recurrence_forward(x, gate, seq_lens, initial, true);
+        ctx->save_for_backward({x, gate, or_none(seq_lens), *got[2]});
+        ctx->saved_data["with_state"] = initial.has_value();
+        ctx->set_materialize_grads(false);
+        return {*got[0], *got[1]};
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        const Optional grad_h = grads[0].defined() ? Optional(rows(grads[0])) : Optional(), grad_last = grads[1].defined() ? Optional(grads[1].contiguous()) : Optional();
+        const std::vector<torch::Tensor> got = gated_recurrence_backward(grad_h, grad_last, saved[0], saved[1], given(saved[2]), saved[3]);
+        return once("gated_recurrence", grads, {got[0], got[1], ctx->saved_data["with_state"].toBool() && ctx->needs_input_grad(2) ? got[2] : torch::Tensor(), torch::Tensor()});
+    }
+};
+
+std::tuple<torch::Tensor, torch::Tensor> gated_recurrence(const torch::Tensor& x, const torch::Tensor& gate, const Optional& seq_lens, const Optional& initial) {
+    if (wants_gradient({x, gate, or_none(initial)})) {
+        const variable_list out = GatedRecurrence::apply(rows(x), rows(gate), initial, seq_lens);
+        return {out[0], out[1]};
+    }
+    std::vector<Optional> got = gated_recurrence_forward(rows(x), rows(gate), seq_lens, initial, false);
+    return {*got[0], *got[1]};
+}
+
 // -------------------------------------------------------------------------------------------------------------- AdamW
 
 void adamw_step(const std::vector<torch::Tensor>& params, const std::vector<torch::Tensor>& grads, const std::vector<torch::Tensor>& exp_avgs,
@@ -247,10 +324,8 @@ void adamw_step(const std::vector<torch::Tensor>& params, const std::vector<torc
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-    m.def("linear_cross_entropy_forward", &linear_cross_entropy_forward, "[loss (B, T), workspace the backward call needs]");
-    m.def("linear_cross_entropy_backward", &linear_cross_entropy_backward, "[grad_hidden, grad_weight, grad_bias], None where not asked for");
-    m.def("gated_recurrence_forward", &gated_recurrence_forward, "[h (B, T, D), last (B, D), states the backward call needs or None]");
-    m.def("gated_recurrence_backward", &gated_recurrence_backward, "[grad_x, grad_gate, grad_initial]");
+    m.def("linear_cross_entropy", &linear_cross_entropy, "loss (B, T)");
+    m.def("gated_recurrence", &gated_recurrence, "h (B, T, D), last (B, D)");
     m.def("adamw_step", &adamw_step, "One AdamW step over lists of tensors, in place");
     m.def("check_status", &check_status, "Waits for the device and raises the first problem that kernels of earlier calls reported");
 }

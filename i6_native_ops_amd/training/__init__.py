@@ -15,7 +15,6 @@ according to ``i6_native_ops_amd.fbw.set_status_mode``.  The reference has none 
 from typing import Iterable, Optional, Sequence, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .._version import __version__  # noqa: F401
 
@@ -32,28 +31,6 @@ BLOCK = 256     # values that share a scale where AdamW's states are held in 8 b
 check_status = core.check_status
 
 __all__ = ["linear_cross_entropy", "gated_recurrence", "adamw_step", "AdamW", "check_status", "core", "BLOCK"]
-
-
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    return x if x.dim() == 0 or x.stride(-1) == 1 else x.contiguous()
-
-
-class _LinearCrossEntropy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden, weight, bias, targets, seq_lens):
-        loss, workspace = core.linear_cross_entropy_forward(hidden, weight, targets, seq_lens, bias)
-        ctx.save_for_backward(weight, bias, targets, seq_lens, workspace)
-        ctx.features = hidden.shape[2]
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_loss):
-        weight, bias, targets, seq_lens, workspace = ctx.saved_tensors
-        hidden_grad, weight_grad, bias_grad = core.linear_cross_entropy_backward(
-            grad_loss, ctx.features, weight, targets, seq_lens, bias, workspace, *ctx.needs_input_grad[:3]
-        )
-        return hidden_grad, weight_grad, bias_grad, None, None
 
 
 def linear_cross_entropy(
@@ -74,28 +51,7 @@ def linear_cross_entropy(
     :return: float32 [B, T]; 0 in frames behind the end or without a target, NaN (and an error raised later) where a
         target is F or more
     """
-    hidden, weight = _rows(hidden), _rows(weight)
-    return _LinearCrossEntropy.apply(hidden, weight, bias, targets, seq_lens)
-
-
-class _GatedRecurrence(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, gate, initial_state, seq_lens):
-        h, last, states = core.gated_recurrence_forward(x, gate, seq_lens, initial_state, True)
-        ctx.save_for_backward(x, gate, seq_lens, states)
-        ctx.set_materialize_grads(False)
-        return h, last
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_h, grad_last):
-        x, gate, seq_lens, states = ctx.saved_tensors
-        if grad_h is not None:
-            grad_h = _rows(grad_h)
-        if grad_last is not None:
-            grad_last = grad_last.contiguous()
-        grad_x, grad_gate, grad_initial = core.gated_recurrence_backward(grad_h, grad_last, x, gate, seq_lens, states)
-        return grad_x, grad_gate, grad_initial if ctx.needs_input_grad[2] else None, None
+    return core.linear_cross_entropy(hidden, weight, targets, seq_lens, bias)
 
 
 def gated_recurrence(
@@ -114,11 +70,7 @@ def gated_recurrence(
     :return: h [B, T, D] in the type of x, 0 behind the end, and the state after the last frame of every sequence, float32
         [B, D].  The next frames of the same streams start from it: ``h, state = gated_recurrence(x, gate, initial_state=state)``
     """
-    x, gate = _rows(x), _rows(gate)
-    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (initial_state is not None and initial_state.requires_grad)):
-        return _GatedRecurrence.apply(x, gate, initial_state, seq_lens)
-    h, last, _ = core.gated_recurrence_forward(x, gate, seq_lens, initial_state, False)
-    return h, last
+    return core.gated_recurrence(x, gate, seq_lens, initial_state)
 
 
 def adamw_step(

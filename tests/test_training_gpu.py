@@ -694,3 +694,17 @@ def test_operators_on_another_stream_and_in_a_graph():
         want = work(*again)
         for a, b in zip(captured + list(buffers), want + list(again)):
             assert torch.equal(a, b), turn
+
+
+def test_gradients_of_gradients_are_refused():
+    from i6_native_ops_amd.training import gated_recurrence, linear_cross_entropy
+    hidden, weight, bias, targets, lens, grad = ce_problem(2, 5, 7, 8, torch.float32)
+    leaf = hidden.detach().requires_grad_()
+    got, = torch.autograd.grad(linear_cross_entropy(leaf, weight, targets, lens, bias=bias), leaf, grad.requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError, match="linear_cross_entropy can be differentiated once"):
+        got.sum().backward()
+    leaf = hidden.detach().requires_grad_()
+    h, _ = gated_recurrence(leaf, hidden)
+    got, = torch.autograd.grad(h, leaf, torch.ones_like(h).requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError, match="gated_recurrence can be differentiated once"):
+        got.sum().backward()
