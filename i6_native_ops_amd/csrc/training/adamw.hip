@@ -102,24 +102,6 @@ __device__ __forceinline__ void chunk32(const i6train_adamw_tensor& t, const Fac
     }
 }
 
-// The largest of 64 lanes' values, in all of them.  The values are bit patterns of magnitudes, whose order as whole numbers is that of
-// the magnitudes with NaN on top, so a NaN in a block is not lost.
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-#define I6_STEP(ctrl, rows)                                                                                   \
-    {                                                                                                         \
-        const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xf, false);          \
-        x = y > x ? y : x;                                                                                    \
-    }
-    I6_STEP(0x111, 0xf)      // from 1, 2, 4, 8 lanes below within rows of 16
-    I6_STEP(0x112, 0xf)
-    I6_STEP(0x114, 0xf)
-    I6_STEP(0x118, 0xf)
-    I6_STEP(0x142, 0xa)      // the last lane of rows 0 and 2 to rows 1 and 3
-    I6_STEP(0x143, 0xc)      // that of row 1 to rows 2 and 3
-#undef I6_STEP
-    return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
-}
-
 __device__ __forceinline__ float scale_of(uint32_t bits) {
     const float s = __uint_as_float(bits) * kPerMax;
     return s < kLeastScale ? kLeastScale : s;      // (NaN stays)
@@ -218,6 +200,7 @@ __device__ __forceinline__ void chunk8(const i6train_adamw_tensor& t, const Fact
             most_m = bm > most_m ? bm : most_m;
             most_r = br > most_r ? br : most_r;
         }
+        // as bit patterns: a NaN in a block is not lost
         const float sm = scale_of(wave_max(most_m)), sr = scale_of(wave_max(most_r));
         const float per_m = 1.f / sm, per_r = 1.f / sr;
 #pragma unroll

@@ -56,10 +56,6 @@ struct BackHeader {
 };
 
 __device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
-__device__ __forceinline__ uint32_t wave_most(uint32_t m) {
-    for (int d = 32; d; d >>= 1) m = umax(m, (uint32_t)__shfl_xor((int)m, d));
-    return (uint32_t)__builtin_amdgcn_readfirstlane((int)m);
-}
 __device__ __forceinline__ uint32_t finite_bits(float x) {
     const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
     return b < 0x7f800000u ? b : 0u;
@@ -68,7 +64,7 @@ __device__ __forceinline__ uint32_t finite_bits(float x) {
 // The exponent of the power of two that brings a tensor's largest value to 2^14 .. 2^15, from its partial maxima: in every lane of a whole wave.
 __device__ __forceinline__ int scale_exponent(const uint32_t* parts) {
     const u32x4 p = reinterpret_cast<const u32x4*>(parts)[threadIdx.x & 63];
-    const uint32_t most = wave_most(umax(umax(p.x, p.y), umax(p.z, p.w)));
+    const uint32_t most = wave_max(umax(umax(p.x, p.y), umax(p.z, p.w)));
     if (most == 0) return 0;
     const int k = 14 - ((int)(most >> 23) - 127);          // (subnormals: as 2^-127)
     return k > 100 ? 100 : k;
@@ -161,7 +157,7 @@ __global__ __launch_bounds__(kLookThreads) void ce_look(Frames f, Weights w, int
             for (int i = 0; i < 8; i++) most = umax(most, finite_bits(v[i]));
         }
     }
-    most = wave_most(most);
+    most = wave_max(most);
     if (lane == 0) most_of[wave] = most;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -249,7 +245,7 @@ __global__ __launch_bounds__(kThreads) void ce_pack(Frames f, Weights w, const i
             }
             store_operand<S>(o.x + row * row_size, f.Kp, c, used ? v : none, ex);
         }
-        for (int d = 32; d; d >>= 1) dot += __shfl_xor(dot, d);
+        dot = wave_sum(dot);
         if (lane == 0) {
             o.row_frame[row] = (int)r;
             o.row_target[row] = target;
@@ -387,6 +383,36 @@ template <int R, bool kConsecutiveK, int kWaves> struct Side {
 
 constexpr int kGStride = kM * 2 + 16;      // bytes of a row of G in LDS
 
+// A wave's block of 32 x 64 of C to memory, times two powers of two, through LDS of the wave's own: rows of 64 values in accesses of 16 bytes instead of one
+// value a lane.  row(r) is where row r begins, or null; `cols` of the columns are there; `whole`: every 16 bytes of a row are aligned.
+constexpr int kBlockBytes = 32 * (64 * 4 + 16);
+template <typename Out, typename Row>
+__device__ __forceinline__ void store_block(char* lds, const acc_t (&c)[2], float by, float by_too, int cols, bool whole, Row row) {
+    constexpr int kStride = 64 * sizeof(Out) + 16, kPer = 16 / sizeof(Out), kLanes = 64 / kPer, kRows = 64 / kLanes;
+    const int lane = threadIdx.x & 63;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+            *reinterpret_cast<Out*>(lds + (4 * (lane >> 5) + (r & 3) + 8 * (r >> 2)) * kStride + (j * 32 + (lane & 31)) * sizeof(Out)) = (Out)(c[j][r] * by * by_too);
+    __builtin_amdgcn_wave_barrier();        // the wave's reads of LDS follow its writes
+#pragma unroll
+    for (int k = 0; k < 32 / kRows; k++) {
+        const int r = k * kRows + lane / kLanes, n = lane % kLanes * kPer;
+        const u32x4 v = *reinterpret_cast<const u32x4*>(lds + r * kStride + n * sizeof(Out));
+        Out* to = row(r);
+        if (!to || n >= cols) continue;
+        if (whole && n + kPer <= cols) {
+            *reinterpret_cast<u32x4*>(to + n) = v;
+        } else {
+            Out w[kPer];
+            __builtin_memcpy(w, &v, 16);
+            for (int i = 0; i < kPer && n + i < cols; i++) to[n + i] = w[i];
+        }
+    }
+}
+
 // In           type of the user's tensors: two halves where it has 32 bits
 // KIND         what becomes of a tile
 // NW           pairs of waves: a tile has 64 NW columns
@@ -428,6 +454,9 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
     }
     const int steps = (K - k0) / kK, all = S == 2 ? 3 * steps : steps;
 
+    int up = 0, down = 0;      // what the tensors' scales come to
+    if constexpr (kLogits) down = scale_exponent(e.header->most_x) + scale_exponent(e.header->most_w);
+    if constexpr (KIND == kGradient) up = scale_exponent(e.back->most_g);
     Side<kM, kAk, kWaves> A;
     Side<kCols, kBk, kWaves> B;
     A.set(p.a, rows_a, m0, k0, wm * 128);
@@ -554,18 +583,14 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
     }
 
     if constexpr (KIND == kWeight) {
-        float* out = e.part_out + part_of_k * e.part_stride + (int64_t)m0 * rows_b + n0;
+        __syncthreads();
+        float* out = e.part_out + part_of_k * e.part_stride + n0 + wn * 64;
 #pragma unroll
         for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int n = col_in + j * 32;
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int m = row_in + i * 32 + (r & 3) + 8 * (r >> 2);
-                    if (m0 + m < rows_a && n0 + n < rows_b) out[(int64_t)m * rows_b + n] = acc[i][j][r];
-                }
-            }
+            store_block<float>(lds + wave * kBlockBytes, acc[i], 1.f, 1.f, rows_b - n0 - wn * 64, rows_b % 4 == 0, [&](int r) -> float* {
+                const int m = m0 + wm * 128 + i * 32 + r;
+                return m < rows_a ? out + (int64_t)m * rows_b : nullptr;
+            });
         if (with_bias) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -579,47 +604,40 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
 
     if constexpr (KIND == kHidden) {
         if (!e.last) {
-            float* sum = e.sum + (int64_t)m0 * e.sum_stride + n0;
+            __syncthreads();
+            float* sum = e.sum + n0 + wn * 64;
 #pragma unroll
             for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const int n = col_in + j * 32;
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const int m = row_in + i * 32 + (r & 3) + 8 * (r >> 2);
-                        if (m0 + m < rows_a && n0 + n < rows_b) sum[(int64_t)m * e.sum_stride + n] = acc[i][j][r];
-                    }
-                }
+                store_block<float>(lds + wave * kBlockBytes, acc[i], 1.f, 1.f, rows_b - n0 - wn * 64, rows_b % 4 == 0, [&](int r) -> float* {
+                    const int m = m0 + wm * 128 + i * 32 + r;
+                    return m < rows_a ? sum + (int64_t)m * e.sum_stride : nullptr;
+                });
             return;
         }
         // back to the frames, scales off; where the target is out of range, NaN
-        int* frames = reinterpret_cast<int*>(lds);
+        int* frames = reinterpret_cast<int*>(lds + kWaves * kBlockBytes);
         __syncthreads();
-        for (int i = tid; i < kM; i += 128 * NW) {
+        for (int i = tid; i < kM; i += 64 * kWaves) {
             const int m = m0 + i;
             frames[i] = m < rows_a ? (e.row_target[m] >= e.classes ? ~e.row_frame[m] : e.row_frame[m]) : 0;
         }
+        const float unscale = ldexpf(1.f, -scale_exponent(e.back->most_g)), unscale_w = ldexpf(1.f, -scale_exponent(e.header->most_w));
         __syncthreads();
-        const int down = -scale_exponent(e.back->most_g), down_w = -scale_exponent(e.header->most_w);
-        In* out = static_cast<In*>(e.out) + n0;
+        In* out = static_cast<In*>(e.out) + n0 + wn * 64;
+        const bool whole = rows_b % (16 / (int)sizeof(In)) == 0;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < 4; i++) {
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int m = row_in + i * 32 + (r & 3) + 8 * (r >> 2), frame = frames[m];
-                In* row = out + (int64_t)(frame < 0 ? ~frame : frame) * rows_b;
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const int n = col_in + j * 32;
-                    const float v = ldexpf(ldexpf(acc[i][j][r], down), down_w);
-                    if (m0 + m < rows_a && n0 + n < rows_b) row[n] = (In)(frame < 0 ? __builtin_nanf("") : v);
-                }
-            }
+            for (int r = 0; r < 16; r++)
+                if (frames[row_in + i * 32 + (r & 3) + 8 * (r >> 2)] < 0) acc[i][0][r] = acc[i][1][r] = __builtin_nanf("");
+            store_block<In>(lds + wave * kBlockBytes, acc[i], unscale, unscale_w, rows_b - n0 - wn * 64, whole, [&](int r) -> In* {
+                const int m = wm * 128 + i * 32 + r, frame = frames[m];
+                return m0 + m < rows_a ? out + (int64_t)(frame < 0 ? ~frame : frame) * rows_b : nullptr;
+            });
+        }
         return;
     }
 
-    const int down = scale_exponent(e.header->most_x) + scale_exponent(e.header->most_w);
     const float per = fminf(ldexpf(kLog2e, -down), 0x1p127f);
     __syncthreads();
     // logits in units of log 2
@@ -667,7 +685,6 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
     }
 
     if constexpr (KIND == kGradient) {
-        const int up = scale_exponent(e.back->most_g);
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             const int n = n0 + col_in + j * 32;
@@ -803,41 +820,41 @@ __global__ __launch_bounds__(256) void ce_row_scale(const Header* header, const 
         row_scale[row] = g;
         most = umax(most, finite_bits(g));
     }
-    most = wave_most(most);
+    most = wave_max(most);
     if (lane == 0) most_of[wave] = most;
     __syncthreads();
     if (threadIdx.x == 0) back->most_g[blockIdx.x] = umax(umax(most_of[0], most_of[1]), umax(most_of[2], most_of[3]));
 }
 
-// One piece of grad_weight and grad_bias: the ranges of k joined, scales off.
+// One piece of grad_weight and grad_bias: the ranges of k joined, scales off.  A workgroup has 256 values, a quarter of the ranges for each wave.
 template <typename Out>
 __global__ __launch_bounds__(256) void ce_store_weight(const Header* header, const BackHeader* back, const float* part, int splits, int64_t split_stride, int64_t n, Out* out,
                                                        const float* bias_part, int64_t bias_stride, int classes, Out* bias) {
-    const int down = -scale_exponent(back->most_g), down_x = -scale_exponent(header->most_x);
-    int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i < n) {
-        if (!out) return;
-        using V = float __attribute__((ext_vector_type(4)));
-        V v = 0.f;
-        if (i + 4 <= n && n % 4 == 0) {
-#pragma unroll 4
-            for (int s = 0; s < splits; s++) v += *reinterpret_cast<const V*>(part + s * split_stride + i);
-        } else {
-            for (int s = 0; s < splits; s++)
-                for (int k = 0; k < 4 && i + k < n; k++) v[k] += part[s * split_stride + i + k];
-        }
+    using V = float __attribute__((ext_vector_type(4)));
+    __shared__ V sums[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const float down = ldexpf(1.f, -scale_exponent(back->most_g)), down_x = ldexpf(1.f, -scale_exponent(header->most_x));
+    const int64_t groups = ceil_div(n, (int64_t)256);
+    const bool of_bias = blockIdx.x >= groups;            // the last workgroups
+    const int64_t i = (of_bias ? blockIdx.x - groups : blockIdx.x) * 256 + lane * 4, all = of_bias ? classes : n, stride = of_bias ? bias_stride : split_stride;
+    const float* from = of_bias ? bias_part : part;
+    Out* to = of_bias ? bias : out;
+    if (!to) return;
+    V v = 0.f;
+    if (i + 4 <= all && stride % 4 == 0) {
+#pragma unroll 8
+        for (int s = wave; s < splits; s += 4) v += *reinterpret_cast<const V*>(from + s * stride + i);
+    } else {
+        for (int s = wave; s < splits; s += 4)
+            for (int k = 0; k < 4 && i + k < all; k++) v[k] += from[s * stride + i + k];
+    }
+    sums[wave][lane] = v;
+    __syncthreads();
+    if (wave != 0) return;
+    v = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (i + k < n) out[i + k] = (Out)ldexpf(ldexpf(v[k], down), down_x);
-        return;
-    }
-    i -= round_up(n, 1024);         // the last workgroups
-    if (!bias || i < 0) return;
-    for (int k = 0; k < 4 && i + k < classes; k++) {
-        float v = 0.f;
-        for (int s = 0; s < splits; s++) v += bias_part[s * bias_stride + i + k];
-        bias[i + k] = (Out)ldexpf(v, down);
-    }
+    for (int k = 0; k < 4; k++)
+        if (i + k < all) to[i + k] = (Out)(v[k] * down * (of_bias ? 1.f : down_x));
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
@@ -978,13 +995,15 @@ int backward(const i6train_ce_problem& p, const Layout& l, const float* grad_los
             o.part_out = dw; o.part_stride = (int64_t)l.piece * p.D; o.bias_out = db; o.bias_stride = l.piece;
             launch_product<In, kWeight, 4>(d, o, classes, p.D, s);
             const int64_t n = (int64_t)classes * p.D;
-            ce_store_weight<In><<<dim3((unsigned)(ceil_div(n, (int64_t)1024) + ceil_div(classes, 1024))), dim3(256), 0, s>>>(
+            ce_store_weight<In><<<dim3((unsigned)(ceil_div(n, (int64_t)256) + ceil_div(classes, 256))), dim3(256), 0, s>>>(
                 header, back, dw, l.splits, o.part_stride, n, grad_weight ? (In*)grad_weight + (int64_t)first * p.D : nullptr, db, o.bias_stride, classes,
                 grad_bias ? (In*)grad_bias + first : nullptr);
         }
     }
     return launched();
 }
+
+#include "cross_entropy_small.inc"
 
 }  // namespace
 }  // namespace i6train
@@ -995,6 +1014,11 @@ extern "C" {
 
 int i6train_ce_workspace_size(const i6train_ce_problem* p, size_t* forward_bytes, size_t* backward_bytes) {
     if (!valid(p) || !forward_bytes || !backward_bytes) return I6TRAIN_ERR_INVALID_ARGUMENT;
+    if (is_small(*p)) {
+        *forward_bytes = small_forward_bytes(*p);
+        *backward_bytes = small_backward_bytes(*p);
+        return I6TRAIN_OK;
+    }
     Layout l;
     I6TRAIN_TRY(layout(*p, l));
     *forward_bytes = l.forward;
@@ -1004,6 +1028,11 @@ int i6train_ce_workspace_size(const i6train_ce_problem* p, size_t* forward_bytes
 
 int i6train_ce_forward(const i6train_ce_problem* p, float* loss, void* workspace, size_t workspace_bytes, void* stream) {
     if (!valid(p) || !p->hidden || !loss || !workspace || (uintptr_t)workspace % 256) return I6TRAIN_ERR_INVALID_ARGUMENT;
+    if (is_small(*p)) {
+        if (workspace_bytes < small_forward_bytes(*p)) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
+        const auto run = p->dtype == I6TRAIN_F32 ? small_forward<float> : small_forward<bf16>;
+        return run(*p, loss, (char*)workspace, (hipStream_t)stream);
+    }
     Layout l;
     I6TRAIN_TRY(layout(*p, l));
     if (workspace_bytes < l.forward) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
@@ -1014,6 +1043,12 @@ int i6train_ce_forward(const i6train_ce_problem* p, float* loss, void* workspace
 int i6train_ce_backward(const i6train_ce_problem* p, const float* grad_loss, int64_t grad_stride_b, int64_t grad_stride_t, void* grad_hidden, void* grad_weight, void* grad_bias,
                         const void* forward_workspace, size_t forward_bytes, void* workspace, size_t workspace_bytes, void* stream) {
     if (!valid(p) || !grad_loss || !forward_workspace || !workspace || (uintptr_t)workspace % 256) return I6TRAIN_ERR_INVALID_ARGUMENT;
+    if (is_small(*p)) {
+        if (!p->hidden) return I6TRAIN_ERR_INVALID_ARGUMENT;
+        if (forward_bytes < small_forward_bytes(*p) || workspace_bytes < small_backward_bytes(*p)) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
+        const auto run = p->dtype == I6TRAIN_F32 ? small_backward<float> : small_backward<bf16>;
+        return run(*p, grad_loss, grad_stride_b, grad_stride_t, grad_hidden, grad_weight, grad_bias, (const char*)forward_workspace, (char*)workspace, (hipStream_t)stream);
+    }
     Layout l;
     I6TRAIN_TRY(layout(*p, l));
     if (forward_bytes < l.forward || workspace_bytes < l.backward) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;

@@ -61,10 +61,11 @@ torch::Tensor bytes(size_t n, const torch::Tensor& like) {
 
 // ------------------------------------------------------------------------------------------------------ cross entropy
 
-i6train_ce_problem ce_problem(int64_t B, int64_t T, int64_t D, const torch::Tensor& weight, const torch::Tensor& targets, const torch::Tensor& seq_lens,
+i6train_ce_problem ce_problem(const torch::Tensor& hidden, const torch::Tensor& weight, const torch::Tensor& targets, const torch::Tensor& seq_lens,
                               const Optional& bias) {
     i6train_ce_problem p{};
-    p.B = (int)B; p.T = (int)T; p.D = (int)D; p.F = (int)weight.size(0);
+    p.B = (int)hidden.size(0); p.T = (int)hidden.size(1); p.D = (int)hidden.size(2); p.F = (int)weight.size(0);
+    p.hidden = hidden.data_ptr(); p.hidden_stride_b = hidden.stride(0); p.hidden_stride_t = hidden.stride(1);
     p.dtype = dtype_of(weight, "weight");
     p.weight = weight.data_ptr(); p.weight_stride_f = weight.stride(0);
     p.bias = bias ? bias->data_ptr() : nullptr;
@@ -100,8 +101,7 @@ std::tuple<torch::Tensor, torch::Tensor> linear_cross_entropy_forward(const torc
     TORCH_CHECK(hidden.size(0) < (1 << 30) && hidden.size(1) < (1 << 30) && hidden.size(2) < (1 << 30) && weight.size(0) < (1 << 30), "NativeOp: linear_cross_entropy: ",
                 i6train_strerror(I6TRAIN_ERR_TOO_LARGE));
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(hidden.device());
-    i6train_ce_problem p = ce_problem(hidden.size(0), hidden.size(1), hidden.size(2), weight, targets, seq_lens, bias);
-    p.hidden = hidden.data_ptr(); p.hidden_stride_b = hidden.stride(0); p.hidden_stride_t = hidden.stride(1);
+    const i6train_ce_problem p = ce_problem(hidden, weight, targets, seq_lens, bias);
     size_t forward_bytes = 0, backward_bytes = 0;
     check("linear_cross_entropy", i6train_ce_workspace_size(&p, &forward_bytes, &backward_bytes));
     torch::Tensor workspace = bytes(forward_bytes, hidden);
@@ -112,7 +112,7 @@ std::tuple<torch::Tensor, torch::Tensor> linear_cross_entropy_forward(const torc
     return {loss, workspace};
 }
 
-std::vector<Optional> linear_cross_entropy_backward(const torch::Tensor& grad_loss, int64_t D, const torch::Tensor& weight, const torch::Tensor& targets,
+std::vector<Optional> linear_cross_entropy_backward(const torch::Tensor& grad_loss, const torch::Tensor& hidden, const torch::Tensor& weight, const torch::Tensor& targets,
                                                     const torch::Tensor& seq_lens, const Optional& bias, const torch::Tensor& forward_workspace, bool need_hidden,
                                                     bool need_weight, bool need_bias) {
     CHECK_CUDA(grad_loss);
@@ -121,7 +121,7 @@ std::vector<Optional> linear_cross_entropy_backward(const torch::Tensor& grad_lo
     TORCH_CHECK(grad_loss.sizes() == targets.sizes(), "grad_loss must have shape (B, T)");
     CHECK_CUDA(forward_workspace);
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(weight.device());
-    const i6train_ce_problem p = ce_problem(targets.size(0), targets.size(1), D, weight, targets, seq_lens, bias);
+    const i6train_ce_problem p = ce_problem(hidden, weight, targets, seq_lens, bias);
     size_t forward_bytes = 0, backward_bytes = 0;
     check("linear_cross_entropy", i6train_ce_workspace_size(&p, &forward_bytes, &backward_bytes));
     torch::Tensor workspace = bytes(backward_bytes, weight);
@@ -164,14 +164,13 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& hidden, const torch::Tensor& weight, const Optional& bias, const torch::Tensor& targets,
                                  const torch::Tensor& seq_lens) {
         auto [loss, workspace] = linear_cross_entropy_forward(hidden, weight, targets, seq_lens, bias);
-        ctx->save_for_backward({weight, or_none(bias), targets, seq_lens, workspace});
-        ctx->saved_data["features"] = hidden.size(2);
+        ctx->save_for_backward({hidden, weight, or_none(bias), targets, seq_lens, workspace});
         return loss;
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
         const variable_list saved = ctx->get_saved_variables();
-        const std::vector<Optional> got = linear_cross_entropy_backward(grads[0], ctx->saved_data["features"].toInt(), saved[0], saved[2], saved[3], given(saved[1]), saved[4],
-                                                                        ctx->needs_input_grad(0), ctx->needs_input_grad(1), saved[1].defined() && ctx->needs_input_grad(2));      // (a missing bias has no number)
+        const std::vector<Optional> got = linear_cross_entropy_backward(grads[0], saved[0], saved[1], saved[3], saved[4], given(saved[2]), saved[5],
+                                                                        ctx->needs_input_grad(0), ctx->needs_input_grad(1), saved[2].defined() && ctx->needs_input_grad(2));      // (a missing bias has no number)
         variable_list out(5);
         for (int i = 0; i < 3; i++)
             if (got[i]) out[i] = *got[i];

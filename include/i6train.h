@@ -54,7 +54,7 @@ int i6train_poll_status(int* code, int* seq);
  *   loss   float [B, T]
  *
  * The forward call leaves in `workspace` what the backward call needs: keep it until then (it may be used for several
- * backward calls, which do not look at `hidden`).  Logits exist in registers only; the backward call forms them again, in pieces of the
+ * backward calls; hidden, weight and bias have to be what they were).  Logits exist in registers only; the backward call forms them again, in pieces of the
  * vocabulary.  Sums and statistics are held in 32 bits.  bfloat16 operands are multiplied as they are; 32-bit
  * operands as two halves of 11 bits each.  The gradient with respect to the logits is rounded to the operands' precision (bfloat16, or
  * 22 bits) before it is multiplied.
