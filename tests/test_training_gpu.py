@@ -708,3 +708,27 @@ def test_gradients_of_gradients_are_refused():
     got, = torch.autograd.grad(h, leaf, torch.ones_like(h).requires_grad_(), create_graph=True)
     with pytest.raises(RuntimeError, match="gated_recurrence can be differentiated once"):
         got.sum().backward()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_large_steps(bits):
+    """Steps that go past the caches come to the same as small ones, bit for bit: the large tensor repeats a small one."""
+    from i6_native_ops_amd.training import adamw_step
+    small, times = 1 << 16, 640
+    g = gen(2)
+    p, gr = torch.randn(small, generator=g, device="cuda"), torch.randn(small, generator=g, device="cuda")
+    if bits == 8:
+        m, v = (torch.zeros(small, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2))
+        scales = [(torch.ones(small // 256, device="cuda"), torch.ones(small // 256, device="cuda"))]
+    else:
+        m, v, scales = torch.zeros(small, device="cuda"), torch.zeros(small, device="cuda"), None
+
+    def repeated(x):
+        return x.view(torch.uint8).repeat(times).view(x.dtype)
+
+    big = [repeated(x) for x in (p, gr, m, v)]
+    big_scales = [tuple(repeated(s) for s in pair) for pair in scales] if scales else None
+    adamw_step([p], [gr], [m], [v], step=1, lr=1e-2, scales=scales)
+    adamw_step(*([x] for x in big), step=1, lr=1e-2, scales=big_scales)
+    for a, b in zip([p, m, v] + (list(scales[0]) if scales else []), [big[0], big[2], big[3]] + (list(big_scales[0]) if scales else [])):
+        assert torch.equal(repeated(a).view(torch.uint8), b.view(torch.uint8))
