@@ -83,7 +83,7 @@ template <typename T, int V, int W, int L, bool kPairs>
 __global__ __launch_bounds__(64 * W) void rec_forward(Args a) {
     using P = typename Pack<T, V>::type;
     __shared__ float lds[2][W][2 * V][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = blockIdx.y, seg = blockIdx.z;
     const int ch = (blockIdx.x * 64 + lane) * V;
     const bool mine = ch < a.D;
@@ -91,8 +91,9 @@ __global__ __launch_bounds__(64 * W) void rec_forward(Args a) {
     const int len = clamp_len(a, b);
     const int begin = seg * a.seg_frames, stop = min(a.T, begin + a.seg_frames);
     const int end = min(len, stop);                       // frames of the sequence in this segment: begin .. end - 1
-    const T* x = static_cast<const T*>(a.x) + (int64_t)b * a.x_b + at;
-    const T* g = static_cast<const T*>(a.gate) + (int64_t)b * a.g_b + at;
+    // rows begin at addresses that are the same for a whole wave; the lanes add their channel
+    const T* x = static_cast<const T*>(a.x) + (int64_t)b * a.x_b;
+    const T* g = static_cast<const T*>(a.gate) + (int64_t)b * a.g_b;
 
     float c[V], total_a[V];
 #pragma unroll
@@ -113,8 +114,8 @@ __global__ __launch_bounds__(64 * W) void rec_forward(Args a) {
 #pragma unroll
         for (int l = 0; l < L; l++) {
             const int t = min(t0 + wave * L + l, len - 1);      // frames behind the end are not looked at
-            xr[l] = *reinterpret_cast<const P*>(x + (int64_t)t * a.x_t);
-            gr[l] = *reinterpret_cast<const P*>(g + (int64_t)t * a.g_t);
+            xr[l] = *reinterpret_cast<const P*>(x + (int64_t)t * a.x_t + at);
+            gr[l] = *reinterpret_cast<const P*>(g + (int64_t)t * a.g_t + at);
         }
     };
     if (begin < end) fetch(begin);
@@ -169,7 +170,7 @@ __global__ __launch_bounds__(64 * W) void rec_forward(Args a) {
 #pragma unroll
             for (int v = 0; v < V; v++) a.states[i + v] = mine_c[v];
         }
-        T* h = static_cast<T*>(a.h) + ((int64_t)b * a.T + t1) * a.D + at;
+        T* h = static_cast<T*>(a.h) + ((int64_t)b * a.T + t1) * a.D;
 #pragma unroll
         for (int l = 0; l < L; l++) {
             const int t = t1 + l;
@@ -179,7 +180,7 @@ __global__ __launch_bounds__(64 * W) void rec_forward(Args a) {
                 mine_c[v] = fmaf(f[l][v], mine_c[v], u[l][v]);
                 hv[v] = t < end ? mine_c[v] : 0.f;
             }
-            if (mine && t < stop) put<T, V>(h + (int64_t)l * a.D, hv);
+            if (mine && t < stop) put<T, V>(h + (int64_t)l * a.D + at, hv);
         }
     }
     if (kPairs) {
@@ -216,7 +217,7 @@ __global__ __launch_bounds__(64 * W) void rec_backward(Args a) {
     using P = typename Pack<T, V>::type;
     static_assert(kStateSpan % (W * L) == 0, "a turn starts from a kept state, or from the one the last turn left");
     __shared__ float lds[2][W][3 * V][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = blockIdx.y, seg = blockIdx.z;
     const int ch = (blockIdx.x * 64 + lane) * V;
     const bool mine = ch < a.D;
@@ -224,10 +225,11 @@ __global__ __launch_bounds__(64 * W) void rec_backward(Args a) {
     const int len = clamp_len(a, b);
     const int begin = seg * a.seg_frames, stop = min(a.T, begin + a.seg_frames);
     const int end = min(len, stop);
-    const T* x = static_cast<const T*>(a.x) + (int64_t)b * a.x_b + at;
-    const T* g = static_cast<const T*>(a.gate) + (int64_t)b * a.g_b + at;
+    // rows begin at addresses that are the same for a whole wave; the lanes add their channel
+    const T* x = static_cast<const T*>(a.x) + (int64_t)b * a.x_b;
+    const T* g = static_cast<const T*>(a.gate) + (int64_t)b * a.g_b;
     const bool has_dh = a.dh;                             // without: the gate is read in its place, and not used
-    const T* dh = has_dh ? static_cast<const T*>(a.dh) + (int64_t)b * a.dh_b + at : g;
+    const T* dh = has_dh ? static_cast<const T*>(a.dh) + (int64_t)b * a.dh_b : g;
     const int64_t dh_t = has_dh ? a.dh_t : a.g_t;
 
     float c[V], total_a[V];        // c: the gradient of the state behind the frames that are still to come
@@ -260,9 +262,9 @@ __global__ __launch_bounds__(64 * W) void rec_backward(Args a) {
 #pragma unroll
         for (int l = 0; l < L; l++) {
             const int t = min(t0 + wave * L + l, len - 1);
-            gr[l] = *reinterpret_cast<const P*>(g + (int64_t)t * a.g_t);
-            if (!kPairs) xr[l] = *reinterpret_cast<const P*>(x + (int64_t)t * a.x_t);
-            dr[l] = *reinterpret_cast<const P*>(dh + (int64_t)t * dh_t);
+            gr[l] = *reinterpret_cast<const P*>(g + (int64_t)t * a.g_t + at);
+            if (!kPairs) xr[l] = *reinterpret_cast<const P*>(x + (int64_t)t * a.x_t + at);
+            dr[l] = *reinterpret_cast<const P*>(dh + (int64_t)t * dh_t + at);
         }
         if (!kPairs) {
             const int64_t i = ((int64_t)b * a.n_states + t0 / kStateSpan) * a.D + at;
@@ -332,7 +334,7 @@ __global__ __launch_bounds__(64 * W) void rec_backward(Args a) {
                 before[l][v] = hc[v];
                 hc[v] = fmaf(f[l][v], hc[v], rest[l][v] * xv[l][v]);
             }
-        const int64_t row = ((int64_t)b * a.T + t0 + wave * L) * a.D + at;
+        const int64_t row = ((int64_t)b * a.T + t0 + wave * L) * a.D;
 #pragma unroll
         for (int l = L - 1; l >= 0; l--) {
             float dx[V], dg[V];
@@ -344,8 +346,8 @@ __global__ __launch_bounds__(64 * W) void rec_backward(Args a) {
                 mine_c[v] = f[l][v] * dv;
             }
             if (mine && t0 + wave * L + l < end) {
-                put<T, V>(static_cast<T*>(a.dx) + row + (int64_t)l * a.D, dx);
-                put<T, V>(static_cast<T*>(a.dgate) + row + (int64_t)l * a.D, dg);
+                put<T, V>(static_cast<T*>(a.dx) + row + (int64_t)l * a.D + at, dx);
+                put<T, V>(static_cast<T*>(a.dgate) + row + (int64_t)l * a.D + at, dg);
             }
         }
     }
