@@ -364,23 +364,30 @@ __global__ __launch_bounds__(64 * W) void rec_backward(Args a) {
 
 // ------------------------------------------------------------------------------------------------------------- host
 
-constexpr int kMostSegments = 64, kWantedGroups = 512, kLeastSegment = 256;
+constexpr int kUnits = 256;             // compute units
+constexpr int kMostSegments = 64, kLeastSegment = 128;
 
+// Channels of a lane.  64 floats are a row of 256 bytes for a wave; of bfloat16, pairs are, unless the workgroups are then fewer than the compute
+// units: single channels are twice as many with half the work each (training, 16 x 2000 x 1024: 147 us, pairs 164 us; 1 x 4000 x 512: 42 and 55 us; but
+// 32 x 1000 x 1024: 124 and 110 us).
 int vector_width(const i6train_rec_problem& p, const void* dh, int64_t dh_b, int64_t dh_t) {
-    if (p.dtype != I6TRAIN_BF16) return 1;          // 64 floats are a row of 256 bytes for a wave
+    if (p.dtype != I6TRAIN_BF16 || (int64_t)p.B * ceil_div(p.D, 128) < kUnits) return 1;
     const auto even = [](const void* q, int64_t sb, int64_t st) { return (uintptr_t)q % 4 == 0 && sb % 2 == 0 && st % 2 == 0; };
     return p.D % 2 == 0 && even(p.x, p.x_stride_b, p.x_stride_t) && even(p.gate, p.gate_stride_b, p.gate_stride_t) && even(dh, dh_b, dh_t) ? 2 : 1;
 }
 
-// Segments of whole state spans: one, unless the (sequence, channel) groups leave much of the chip idle.
+// Segments of whole state spans: one, unless the (sequence, channel) groups leave compute units idle; then enough for two workgroups on each, of at least
+// kLeastSegment frames, and at least three, as the first launch goes through all of them as well.  (Training, float, 1 x 1000 x 512: 27 us, 38 us with 256 frames at least, 66 us in one
+// piece; 19 x 437 x 321, where there is little to gain: 44 us, and 40 us in one piece.)
 void cut(const i6train_rec_problem& p, int V, int& segments, int& seg_frames) {
     const int64_t groups = (int64_t)p.B * ceil_div(p.D, 64 * V);
     int64_t n = 1;
-    if (groups < kWantedGroups / 2) {
-        n = ceil_div((int64_t)kWantedGroups, groups);
+    if (groups < kUnits) {
+        n = ceil_div((int64_t)2 * kUnits, groups);
         n = n < kMostSegments ? n : kMostSegments;
         const int64_t room = ceil_div(p.T, kLeastSegment);
         n = n < room ? n : room;
+        if (n < 3) n = 1;
     }
     seg_frames = (int)(ceil_div(ceil_div((int64_t)p.T, n), (int64_t)128) * 128);
     segments = (int)ceil_div(p.T, seg_frames);
