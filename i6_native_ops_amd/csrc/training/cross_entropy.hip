@@ -284,13 +284,13 @@ struct EpilogueArgs {
     const float *target_logit, *lse, *row_scale;
     f16* g;  int64_t g_stride, g_half;     // [row][halves][piece]
     // kHidden: m is the row, n the feature
-    float* sum;  int64_t sum_stride;       // [m][n] over the pieces so far
+    float* sum;  int64_t sum_stride;       // [m][n] over the pieces so far, or [range of k][m][n]
     int add, last;                         // to what is there; the last piece, which goes to `out`
     const int* row_frame;
     int classes;
     void* out;
     // kWeight: m is the class, n the feature; ranges of k one after another
-    float* part_out;  int64_t part_stride;
+    float* part_out;  int64_t part_stride;      // (the stride for kHidden as well)
     float* bias_out;  int64_t bias_stride; // [range][class], sums of G over the rows
 };
 
@@ -605,7 +605,7 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
     if constexpr (KIND == kHidden) {
         if (!e.last) {
             __syncthreads();
-            float* sum = e.sum + n0 + wn * 64;
+            float* sum = e.sum + part_of_k * e.part_stride + n0 + wn * 64;
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 store_block<float>(lds + wave * kBlockBytes, acc[i], 1.f, 1.f, rows_b - n0 - wn * 64, rows_b % 4 == 0, [&](int r) -> float* {
@@ -857,13 +857,41 @@ __global__ __launch_bounds__(256) void ce_store_weight(const Header* header, con
         if (i + k < all) to[i + k] = (Out)(v[k] * down * (of_bias ? 1.f : down_x));
 }
 
+// grad_hidden where its sums over the classes were formed in ranges: joined, scales off, back to the frames.  A workgroup has 256 values, a quarter of the
+// ranges for each wave.
+template <typename Out>
+__global__ __launch_bounds__(256) void ce_store_hidden(const Header* header, const BackHeader* back, const float* part, int splits, int64_t split_stride, const int* row_frame,
+                                                       const int* row_target, int F, int D, Out* out) {
+    __shared__ float sums[4][256];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const float down = ldexpf(1.f, -scale_exponent(back->most_g)), down_w = ldexpf(1.f, -scale_exponent(header->most_w));
+    const int64_t first = (int64_t)blockIdx.x * 256, all = (int64_t)header->rows * D;
+    if (first >= all) return;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const int64_t i = first + k * 64 + lane;
+        float v = 0.f;
+        if (i < all) {
+#pragma unroll 8
+            for (int s = wave; s < splits; s += 4) v += part[s * split_stride + i];
+        }
+        sums[wave][k * 64 + lane] = v;
+    }
+    __syncthreads();
+    const int64_t i = first + threadIdx.x;
+    if (i >= all) return;
+    const int row = (int)(i / D), d = (int)(i - (int64_t)row * D), t = threadIdx.x;
+    const float v = ((sums[0][t] + sums[1][t]) + (sums[2][t] + sums[3][t])) * down * down_w;
+    out[(int64_t)row_frame[row] * D + d] = (Out)(row_target[row] >= F ? __builtin_nanf("") : v);
+}
+
 // ------------------------------------------------------------------------------------------------------------- host
 
 constexpr size_t kPieceBytes = (size_t)512 << 20;      // of G: the caches in front of the memory hold 256 MB
 
 // Where things are in the workspaces.
 struct Layout {
-    int S, Kp, row_tiles, class_tiles, piece, splits;
+    int S, Kp, row_tiles, class_tiles, piece, splits, hidden_splits;
     int64_t rows, rows_p, weights_p;
     size_t header, offsets, row_frame, row_target, target_logit, lse, x, w, part, x_bytes, w_bytes, forward;
     size_t back, row_scale, g, dx, dw, db, g_bytes, backward;
@@ -911,7 +939,12 @@ int layout(const i6train_ce_problem& p, Layout& l) {
     l.row_scale = take(4 * l.rows_p);
     l.g_bytes = (size_t)l.rows_p * l.S * l.piece * 2;
     l.g = take(l.g_bytes);
-    l.dx = take(l.piece < p.F ? 4 * (size_t)l.rows_p * p.D : 0);
+    // Few rows: the sums over the classes are formed in ranges, or a handful of workgroups would go through the whole vocabulary (100 frames, F = 8346, D = 64, float: 88 us
+    // a training step, 528 us in one range).  Ranges are of 256 classes at least, of 512 where there are many tiles, whose join costs more than shorter ranges win (4000 frames,
+    // F = 1000, D = 1024, bfloat16: 117 us in one range, 135 us in three of 334).
+    const int64_t hidden_tiles = ceil_div(l.rows, (int64_t)kM) * ceil_div(p.D, 256), room = p.F / (hidden_tiles < 32 ? 256 : 512), ranges = room < 256 / hidden_tiles ? room : 256 / hidden_tiles;
+    l.hidden_splits = l.piece >= p.F && ranges > 1 ? (int)ranges : 1;
+    l.dx = take(l.piece < p.F || l.hidden_splits > 1 ? 4 * (size_t)l.hidden_splits * l.rows_p * p.D : 0);
     l.dw = take(4 * (size_t)l.splits * l.piece * p.D);
     l.db = take(4 * (size_t)l.splits * l.piece);
     l.backward = at;
@@ -980,11 +1013,15 @@ int backward(const i6train_ce_problem& p, const Layout& l, const float* grad_los
             d.a = {g, g_stride, l.piece, (int64_t)l.g_bytes, 0, &header->rows};
             d.b = piece_w;
             d.b.rows = p.D;
-            d.K = round_up(classes, kK); d.splits = 1;
+            d.K = round_up(classes, kK); d.splits = l.hidden_splits;
             EpilogueArgs o{};
+            o.part_stride = (int64_t)l.rows_p * p.D;
             o.header = header; o.back = back; o.row_target = row_target; o.row_frame = (const int*)(fw + l.row_frame); o.classes = p.F;
-            o.sum = dx; o.sum_stride = p.D; o.add = first > 0; o.last = first + l.piece >= p.F; o.out = grad_hidden;
+            o.sum = dx; o.sum_stride = p.D; o.add = first > 0; o.last = first + l.piece >= p.F && l.hidden_splits == 1; o.out = grad_hidden;
             launch_product<In, kHidden, 4>(d, o, l.rows, p.D, s);
+            if (l.hidden_splits > 1)
+                ce_store_hidden<In><<<dim3((unsigned)ceil_div(l.rows * p.D, (int64_t)256)), dim3(256), 0, s>>>(header, back, dx, l.hidden_splits, o.part_stride, o.row_frame, row_target, p.F,
+                                                                                                              p.D, (In*)grad_hidden);
         }
         if (grad_weight || grad_bias) {
             ProductArgs d{};

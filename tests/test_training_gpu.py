@@ -732,3 +732,12 @@ def test_adamw_large_steps(bits):
     adamw_step(*([x] for x in big), step=1, lr=1e-2, scales=big_scales)
     for a, b in zip([p, m, v] + (list(scales[0]) if scales else []), [big[0], big[2], big[3]] + (list(big_scales[0]) if scales else [])):
         assert torch.equal(repeated(a).view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,F,D", [(1, 1, 4099, 31), (2, 37, 2500, 64), (3, 300, 1030, 520)])
+def test_cross_entropy_of_few_rows_over_many_classes(B, T, F, D, dtype):
+    """The gradient of the features is summed over ranges of the classes."""
+    problem = ce_problem(B, T, F, D, dtype, seed=F)
+    problem[3][0, 0] = -1
+    ce_check(problem)
