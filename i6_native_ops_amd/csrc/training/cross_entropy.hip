@@ -427,7 +427,7 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
     static_assert(KIND != kGradient || (kCols == kN && kN * kGStride <= kStages * kStageBytes), "G goes through the stages' LDS");
     __shared__ alignas(16) char lds[kStages * kStageBytes];
     __shared__ float bias[kLogits ? kM : 1];
-    __shared__ float join[kLogits ? 4 : 1][kM];
+    __shared__ float join[KIND == kStatistics ? 4 : 1][kCols];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), wm = wave & 1, wn = wave >> 1;
     const int rows_a = p.a.n_rows ? *p.a.n_rows : p.a.rows, rows_b = p.b.n_rows ? *p.b.n_rows : p.b.rows;
@@ -927,7 +927,8 @@ int layout(const i6train_ce_problem& p, Layout& l) {
 
     at = 0;
     int64_t piece = (int64_t)(kPieceBytes / (2 * (size_t)l.S * l.rows_p)) / kM * kM;
-    const int64_t classes = (int64_t)l.class_tiles * kM;
+    const int64_t classes = (int64_t)l.class_tiles * kM, most_piece = ((int64_t)1 << 31) / (2 * l.S * l.Kp) / kM * kM;      // (offsets within its weights have 32 bits)
+    piece = piece > most_piece ? most_piece : piece;
     piece = piece < kM ? kM : (piece > classes ? classes : piece);
     l.piece = (int)round_up(ceil_div(classes, ceil_div(classes, piece)), kM);      // pieces of one size
     const int64_t tiles = (int64_t)l.piece / kM * ceil_div(p.D, 256);
@@ -964,6 +965,7 @@ template <typename In, int KIND, int NW> void launch_product(const ProductArgs& 
 
 template <typename In>
 int forward(const i6train_ce_problem& p, const Layout& l, float* loss, char* ws, hipStream_t s) {
+    constexpr int S = sizeof(In) == 4 ? 2 : 1;
     const Frames f = frames_of(p, l);
     const Weights w{p.weight, p.weight_stride_f, p.bias};
     Header* header = (Header*)(ws + l.header);
@@ -977,7 +979,9 @@ int forward(const i6train_ce_problem& p, const Layout& l, float* loss, char* ws,
     q.K = l.Kp; q.splits = 1;
     EpilogueArgs e{};
     e.bias = p.bias; e.header = header; e.part = (float2*)(ws + l.part); e.rows_p = l.rows_p;
-    launch_product<In, kStatistics, 2>(q, e, p.F, l.rows, s);
+    // the three parts of 32-bit operands make a long loop, which larger tiles feed with fewer bytes (subword units: 669 us, 727 us with small ones); else two
+    // workgroups on a compute unit, so that one has products while the other has exponentials (headline layer: 369 us, 376 us with large ones)
+    launch_product<In, kStatistics, S == 2 ? 4 : 2>(q, e, p.F, l.rows, s);
     ce_finish<<<dim3(ceil_div(l.rows, (int64_t)64)), dim3(64), 0, s>>>(header, e.part, l.class_tiles, l.rows_p, o.row_frame, o.row_target, o.target_logit, p.T, p.F,
                                                                          (float*)(ws + l.lse), loss, status_slot());
     return launched();

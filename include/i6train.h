@@ -60,6 +60,7 @@ int i6train_poll_status(int* code, int* seq);
  * 22 bits) before it is multiplied.
  * grad_loss is float [B, T] with strides; grad_hidden [B, T, D], grad_weight [F, D] and grad_bias [F] are of `dtype`,
  * contiguous, and written completely; each of them may be null.
+ * Sizes: B T and F up to 2^22, D up to 2^14.
  */
 typedef struct {
     int B, T, F, D, dtype;

@@ -741,3 +741,12 @@ def test_cross_entropy_of_few_rows_over_many_classes(B, T, F, D, dtype):
     problem = ce_problem(B, T, F, D, dtype, seed=F)
     problem[3][0, 0] = -1
     ce_check(problem)
+
+
+def test_cross_entropy_wide_features():
+    """As many features as are taken, in a batch of few frames; one more is refused."""
+    from i6_native_ops_amd.training import linear_cross_entropy
+    problem = ce_problem(1, 9, 300, 1 << 14, torch.bfloat16)
+    ce_check(problem)
+    with pytest.raises(RuntimeError, match="larger than"):
+        linear_cross_entropy(torch.zeros(1, 9, (1 << 14) + 1, device="cuda"), torch.zeros(600, (1 << 14) + 1, device="cuda"), problem[3], problem[4])
