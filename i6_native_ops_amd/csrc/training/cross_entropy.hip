@@ -416,18 +416,25 @@ __device__ __forceinline__ void store_block(char* lds, const acc_t (&c)[2], floa
 // In           type of the user's tensors: two halves where it has 32 bits
 // KIND         what becomes of a tile
 // NW           pairs of waves: a tile has 64 NW columns
+// index        of the workgroup among those of this product
+template <typename In, int KIND, int NW> struct Shape {
+    static constexpr int kWaves = 2 * NW, kCols = 64 * NW, kStages = NW == 2 ? 3 : 4;
+    static constexpr int kStageBytes = (kM + kCols) * kK * 2;
+    static constexpr bool kLogits = KIND == kStatistics || KIND == kGradient;
+    static constexpr int kBytes = kStages * kStageBytes + (kLogits ? kM * 4 : 0) + (KIND == kStatistics ? 4 * kCols * 4 : 0);
+};
+
 template <typename In, int KIND, int NW>
-__global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueArgs e) {
+__device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueArgs& e, char* lds, int index) {
 #if __HIP_DEVICE_COMPILE__
     constexpr int S = sizeof(In) == 4 ? 2 : 1;
     constexpr bool kAk = KIND != kWeight, kBk = KIND == kStatistics || KIND == kGradient;      // consecutive k
-    constexpr int kWaves = 2 * NW, kCols = 64 * NW, kStages = NW == 2 ? 3 : 4;
-    constexpr int kStageBytes = (kM + kCols) * kK * 2;
-    constexpr bool kLogits = KIND == kStatistics || KIND == kGradient;
+    using Sh = Shape<In, KIND, NW>;
+    constexpr int kWaves = Sh::kWaves, kCols = Sh::kCols, kStages = Sh::kStages, kStageBytes = Sh::kStageBytes;
+    constexpr bool kLogits = Sh::kLogits;
     static_assert(KIND != kGradient || (kCols == kN && kN * kGStride <= kStages * kStageBytes), "G goes through the stages' LDS");
-    __shared__ alignas(16) char lds[kStages * kStageBytes];
-    __shared__ float bias[kLogits ? kM : 1];
-    __shared__ float join[KIND == kStatistics ? 4 : 1][kCols];
+    float* bias = reinterpret_cast<float*>(lds + kStages * kStageBytes);
+    float (*join)[kCols] = reinterpret_cast<float (*)[kCols]>(lds + kStages * kStageBytes + kM * 4);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), wm = wave & 1, wn = wave >> 1;
     const int rows_a = p.a.n_rows ? *p.a.n_rows : p.a.rows, rows_b = p.b.n_rows ? *p.b.n_rows : p.b.rows;
@@ -436,8 +443,8 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
     // the 64 tiles that a die works on at a time have 8 + 8 operand tiles among them, not 64 + 1.
     const int tiles_m = ceil_div(rows_a, kM), tiles_n = ceil_div(rows_b, kCols), tiles = tiles_m * tiles_n * p.splits;
     const int each = ceil_div(tiles, 8);
-    int tile = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= each || tile >= tiles) return;
+    int tile = (index & 7) * each + (index >> 3);
+    if ((index >> 3) >= each || tile >= tiles) return;
     const int part_of_k = tile / (tiles_m * tiles_n);
     tile -= part_of_k * tiles_m * tiles_n;
     const int group = tile / (8 * tiles_n), in_group = min(8, tiles_m - group * 8);
@@ -758,6 +765,26 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
 #endif
 }
 
+template <typename In, int KIND, int NW>
+__global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueArgs e) {
+    __shared__ alignas(16) char lds[Shape<In, KIND, NW>::kBytes];
+    product_of<In, KIND, NW>(p, e, lds, blockIdx.x);
+}
+
+// dh and dW of a piece in one launch, the first `hidden` workgroups (a multiple of eight) for dh: neither needs the other, and where dh leaves compute
+// units idle, dW runs beside it (monophones: 24 us, 39 us one after the other).
+struct BothArgs {
+    ProductArgs p;
+    EpilogueArgs e;
+};
+template <typename In>
+__global__ __launch_bounds__(512, 2) void products_back(BothArgs h, BothArgs w, int hidden) {
+    static_assert(Shape<In, kHidden, 4>::kBytes == Shape<In, kWeight, 4>::kBytes);
+    __shared__ alignas(16) char lds[Shape<In, kHidden, 4>::kBytes];
+    if ((int)blockIdx.x < hidden) product_of<In, kHidden, 4>(h.p, h.e, lds, blockIdx.x);
+    else product_of<In, kWeight, 4>(w.p, w.e, lds, blockIdx.x - hidden);
+}
+
 // ---------------------------------------------------------------------------------------------------------- the rest
 
 // Statistics of the tiles joined: loss and log sum of a row.
@@ -958,9 +985,13 @@ Frames frames_of(const i6train_ce_problem& p, const Layout& l) {
     return {p.hidden, p.hidden_stride_b, p.hidden_stride_t, p.seq_lens, p.targets, p.targets_stride_b, p.targets_stride_t, p.B, p.T, p.F, p.D, l.Kp};
 }
 
+// Workgroups for a product: a multiple of the dies.
+template <int NW> unsigned groups_of(const ProductArgs& q, int64_t rows_a, int64_t rows_b) {
+    return (unsigned)round_up(ceil_div(rows_a, (int64_t)kM) * ceil_div(rows_b, (int64_t)(64 * NW)) * q.splits, 8);
+}
+
 template <typename In, int KIND, int NW> void launch_product(const ProductArgs& q, const EpilogueArgs& e, int64_t rows_a, int64_t rows_b, hipStream_t s) {
-    const int64_t tiles = ceil_div(rows_a, (int64_t)kM) * ceil_div(rows_b, (int64_t)(64 * NW)) * q.splits;
-    product<In, KIND, NW><<<dim3((unsigned)round_up(tiles, 8)), dim3(128 * NW), 0, s>>>(q, e);
+    product<In, KIND, NW><<<dim3(groups_of<NW>(q, rows_a, rows_b)), dim3(128 * NW), 0, s>>>(q, e);
 }
 
 template <typename In>
@@ -1012,32 +1043,38 @@ int backward(const i6train_ce_problem& p, const Layout& l, const float* grad_los
         e.row_target = row_target; e.target_logit = (const float*)(fw + l.target_logit); e.lse = (const float*)(fw + l.lse); e.row_scale = row_scale;
         e.g = g; e.g_stride = g_stride; e.g_half = l.piece;
         launch_product<In, kGradient, 2>(q, e, classes, l.rows, s);
+        BothArgs h{}, v{};
+        unsigned of_hidden = 0, of_weight = 0;
         if (grad_hidden) {
-            ProductArgs d{};
-            d.a = {g, g_stride, l.piece, (int64_t)l.g_bytes, 0, &header->rows};
-            d.b = piece_w;
-            d.b.rows = p.D;
-            d.K = round_up(classes, kK); d.splits = l.hidden_splits;
-            EpilogueArgs o{};
-            o.part_stride = (int64_t)l.rows_p * p.D;
-            o.header = header; o.back = back; o.row_target = row_target; o.row_frame = (const int*)(fw + l.row_frame); o.classes = p.F;
-            o.sum = dx; o.sum_stride = p.D; o.add = first > 0; o.last = first + l.piece >= p.F && l.hidden_splits == 1; o.out = grad_hidden;
-            launch_product<In, kHidden, 4>(d, o, l.rows, p.D, s);
-            if (l.hidden_splits > 1)
-                ce_store_hidden<In><<<dim3((unsigned)ceil_div(l.rows * p.D, (int64_t)256)), dim3(256), 0, s>>>(header, back, dx, l.hidden_splits, o.part_stride, o.row_frame, row_target, p.F,
-                                                                                                              p.D, (In*)grad_hidden);
+            h.p.a = {g, g_stride, l.piece, (int64_t)l.g_bytes, 0, &header->rows};
+            h.p.b = piece_w;
+            h.p.b.rows = p.D;
+            h.p.K = round_up(classes, kK); h.p.splits = l.hidden_splits;
+            h.e.header = header; h.e.back = back; h.e.row_target = row_target; h.e.row_frame = (const int*)(fw + l.row_frame); h.e.classes = p.F;
+            h.e.sum = dx; h.e.sum_stride = p.D; h.e.part_stride = (int64_t)l.rows_p * p.D; h.e.add = first > 0; h.e.last = first + l.piece >= p.F && l.hidden_splits == 1;
+            h.e.out = grad_hidden;
+            of_hidden = groups_of<4>(h.p, l.rows, p.D);
         }
         if (grad_weight || grad_bias) {
-            ProductArgs d{};
-            d.a = {g, g_stride, l.piece, (int64_t)l.g_bytes, classes, nullptr};
-            d.b = {x, row_size, l.Kp, (int64_t)l.x_bytes, p.D, nullptr};
-            d.n_k = &header->rows; d.splits = l.splits;
-            EpilogueArgs o{};
-            o.part_out = dw; o.part_stride = (int64_t)l.piece * p.D; o.bias_out = db; o.bias_stride = l.piece;
-            launch_product<In, kWeight, 4>(d, o, classes, p.D, s);
+            v.p.a = {g, g_stride, l.piece, (int64_t)l.g_bytes, classes, nullptr};
+            v.p.b = {x, row_size, l.Kp, (int64_t)l.x_bytes, p.D, nullptr};
+            v.p.n_k = &header->rows; v.p.splits = l.splits;
+            v.e.part_out = dw; v.e.part_stride = (int64_t)l.piece * p.D; v.e.bias_out = db; v.e.bias_stride = l.piece;
+            of_weight = groups_of<4>(v.p, classes, p.D);
+        }
+        // dh that fills the compute units more than once leaves idle ones at its end alone, which long workgroups of dW do not fill (subword units in 32 bits: 771 us
+        // apart, 786 us together)
+        const bool apart = of_hidden > 256 && of_weight;
+        if (apart) products_back<In><<<dim3(of_hidden), dim3(512), 0, s>>>(h, v, (int)of_hidden);
+        const unsigned with = apart ? 0 : of_hidden;
+        if (with + of_weight) products_back<In><<<dim3(with + of_weight), dim3(512), 0, s>>>(h, v, (int)with);
+        if (of_hidden && l.hidden_splits > 1)
+            ce_store_hidden<In><<<dim3((unsigned)ceil_div(l.rows * p.D, (int64_t)256)), dim3(256), 0, s>>>(header, back, dx, l.hidden_splits, h.e.part_stride, h.e.row_frame, row_target, p.F,
+                                                                                                          p.D, (In*)grad_hidden);
+        if (of_weight) {
             const int64_t n = (int64_t)classes * p.D;
             ce_store_weight<In><<<dim3((unsigned)(ceil_div(n, (int64_t)256) + ceil_div(classes, 256))), dim3(256), 0, s>>>(
-                header, back, dw, l.splits, o.part_stride, n, grad_weight ? (In*)grad_weight + (int64_t)first * p.D : nullptr, db, o.bias_stride, classes,
+                header, back, dw, l.splits, v.e.part_stride, n, grad_weight ? (In*)grad_weight + (int64_t)first * p.D : nullptr, db, v.e.bias_stride, classes,
                 grad_bias ? (In*)grad_bias + first : nullptr);
         }
     }
