@@ -29,7 +29,6 @@ namespace {
 
 constexpr int kM = 256;              // rows of a workgroup's tile of C, and, per two waves of 128 x 64 each, 64 columns
 constexpr int kN = 128;              // its columns where the tile's logits are worked on
-constexpr int kK = 32;               // k of one stage
 constexpr int kThreads = 256;
 constexpr int kParts = 256;          // partial maxima of a tensor
 constexpr int kLookThreads = 1024;   // every wave waits for lengths, targets and rows in turn: many waves, few rows each
@@ -266,8 +265,8 @@ struct Operand {
 };
 struct ProductArgs {
     Operand a, b;
-    int K;                    // of one half; a multiple of kK
-    const int* n_k;           // K = *n_k rounded up to kK, where it is known on the device alone
+    int K;                    // of one half; a multiple of kPad
+    const int* n_k;           // K = *n_k rounded up to kPad, where it is known on the device alone
     int splits;               // ranges of k, one tile of C each
 };
 
@@ -324,10 +323,10 @@ __device__ __forceinline__ void load_to_lds(descriptor d, uint32_t to, uint32_t 
 
 // One operand's part of a stage: R rows of the tile by kK.  LDS is filled by loads that bypass the registers and write 64 lanes x 16 bytes in
 // order; which 16 bytes a lane asks for is free, and places them so that reading has no bank conflicts.
-//   consecutive k:   row r has 4 chunks of 8 k; chunk c lies at place c ^ ((r >> 2) & 3) of the row.  A fragment is one read of 16 bytes.
+//   consecutive k:   row r has kK / 8 chunks of 8 k; chunk c lies at place c ^ turn(r) of the row, other ones in 16 rows (256 bytes: 64 banks).  A fragment is one read of 16 bytes.
 //   consecutive m:   k has R / 8 chunks of 8 m; chunk c lies at place c ^ ((k & 3) << 2).  A fragment is two reads that
 //                    transpose 4 k x 16 m within 16 lanes.
-template <int R, bool kConsecutiveK, int kWaves> struct Side {
+template <int R, bool kConsecutiveK, int kWaves, int kK> struct Side {
     static constexpr int kLoads = R * kK * 2 / 1024 / kWaves;      // per wave and stage
     static constexpr int kBytes = R * kK * 2;
     descriptor source;
@@ -336,6 +335,7 @@ template <int R, bool kConsecutiveK, int kWaves> struct Side {
     uint32_t to;                 // this wave's place in a stage
     int read[4];                 // byte offsets of this lane's fragments
 
+    static __device__ __forceinline__ int turn(int r) { return kK == 32 ? (r >> 2) & 3 : (r >> 1) & 7; }
     __device__ __forceinline__ void set(const Operand& o, int rows, int first, int k0, int base_row) {
         const int lane = threadIdx.x & 63, wave = wave_index();
         const int64_t origin = kConsecutiveK ? first * o.row_stride + k0 : k0 * o.row_stride + first;
@@ -347,7 +347,7 @@ template <int R, bool kConsecutiveK, int kWaves> struct Side {
         for (int i = 0; i < kLoads; i++) {
             const int slot = (i * kWaves + wave) * 64 + lane;
             if (kConsecutiveK) {
-                const int r = slot >> 2, c = (slot & 3) ^ ((r >> 2) & 3);
+                const int r = slot / (kK / 8), c = (slot % (kK / 8)) ^ turn(r);
                 from[i] = (uint32_t)(min(r, rows - 1 - first) * o.row_stride * 2 + c * 16);      // rows behind the last are the last again
             } else {
                 const int k = slot / (R / 8), c = (slot % (R / 8)) ^ ((k & 3) << 2);
@@ -356,9 +356,9 @@ template <int R, bool kConsecutiveK, int kWaves> struct Side {
             }
         }
         if (kConsecutiveK) {
-            const int r = base_row + (lane & 31), x = (r >> 2) & 3;
-            read[0] = r * 64 + (((lane >> 5) ^ x) * 16);
-            read[1] = r * 64 + (((2 + (lane >> 5)) ^ x) * 16);
+            const int r = base_row + (lane & 31);
+#pragma unroll
+            for (int kk = 0; kk < kK / 16; kk++) read[kk] = r * kK * 2 + ((kk * 2 + (lane >> 5)) ^ turn(r)) * 16;
         } else {
             const int k = (lane >> 5) * 8 + ((lane & 15) >> 2), m = base_row / 8 + ((lane >> 4) & 1) * 2;
 #pragma unroll
@@ -371,7 +371,7 @@ template <int R, bool kConsecutiveK, int kWaves> struct Side {
     // block b of 32 rows, k of kk * 16 .. + 15
     __device__ __forceinline__ f16x8 fragment(const char* lds, int b, int kk) const {
         if constexpr (kConsecutiveK) {
-            return *reinterpret_cast<const f16x8*>(lds + read[kk] + b * 32 * 64);
+            return *reinterpret_cast<const f16x8*>(lds + read[kk] + b * 32 * kK * 2);
         } else {
             const char* at = lds + read[b] + kk * 16 * (R * 2);
             using P = __attribute__((address_space(3))) s16x4*;
@@ -418,7 +418,7 @@ __device__ __forceinline__ void store_block(char* lds, const acc_t (&c)[2], floa
 // NW           pairs of waves: a tile has 64 NW columns
 // index        of the workgroup among those of this product
 template <typename In, int KIND, int NW> struct Shape {
-    static constexpr int kWaves = 2 * NW, kCols = 64 * NW, kStages = NW == 2 ? 3 : 4;
+    static constexpr int kWaves = 2 * NW, kCols = 64 * NW, kStages = NW == 2 ? 3 : 2, kK = NW == 2 ? 32 : 64;
     static constexpr int kStageBytes = (kM + kCols) * kK * 2;
     static constexpr bool kLogits = KIND == kStatistics || KIND == kGradient;
     static constexpr int kBytes = kStages * kStageBytes + (kLogits ? kM * 4 : 0) + (KIND == kStatistics ? 4 * kCols * 4 : 0);
@@ -430,7 +430,7 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
     constexpr int S = sizeof(In) == 4 ? 2 : 1;
     constexpr bool kAk = KIND != kWeight, kBk = KIND == kStatistics || KIND == kGradient;      // consecutive k
     using Sh = Shape<In, KIND, NW>;
-    constexpr int kWaves = Sh::kWaves, kCols = Sh::kCols, kStages = Sh::kStages, kStageBytes = Sh::kStageBytes;
+    constexpr int kWaves = Sh::kWaves, kCols = Sh::kCols, kStages = Sh::kStages, kStageBytes = Sh::kStageBytes, kK = Sh::kK;
     constexpr bool kLogits = Sh::kLogits;
     static_assert(KIND != kGradient || (kCols == kN && kN * kGStride <= kStages * kStageBytes), "G goes through the stages' LDS");
     float* bias = reinterpret_cast<float*>(lds + kStages * kStageBytes);
@@ -452,7 +452,7 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
     const int tile_m = group * 8 + tile % in_group, tile_n = tile / in_group;
     const int m0 = tile_m * kM, n0 = tile_n * kCols;
 
-    int K = p.n_k ? round_up(*p.n_k, kK) : p.K;
+    int K = p.n_k ? round_up(*p.n_k, kPad) : p.K;
     int k0 = 0;
     if (p.splits > 1) {
         const int range = ceil_div(ceil_div(K, kK), p.splits) * kK;
@@ -464,8 +464,8 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
     int up = 0, down = 0;      // what the tensors' scales come to
     if constexpr (kLogits) down = scale_exponent(e.header->most_x) + scale_exponent(e.header->most_w);
     if constexpr (KIND == kGradient) up = scale_exponent(e.back->most_g);
-    Side<kM, kAk, kWaves> A;
-    Side<kCols, kBk, kWaves> B;
+    Side<kM, kAk, kWaves, kK> A;
+    Side<kCols, kBk, kWaves, kK> B;
     A.set(p.a, rows_a, m0, k0, wm * 128);
     B.set(p.b, rows_b, n0, k0, wn * 64);
     if constexpr (kLogits) {
@@ -505,7 +505,7 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
     }
 
     const uint32_t stages = lds_address(lds);
-    constexpr int kLoadsA = Side<kM, kAk, kWaves>::kLoads, kPerStage = kLoadsA + Side<kCols, kBk, kWaves>::kLoads;
+    constexpr int kLoadsA = Side<kM, kAk, kWaves, kK>::kLoads, kPerStage = kLoadsA + Side<kCols, kBk, kWaves, kK>::kLoads;
     uint32_t next_a = 0, next_b = 0;           // offsets of the stage that is fetched next
     const auto place_of = [&](int it) {
         if constexpr (S == 2) {
@@ -523,8 +523,8 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
     };
     f16x8 fa[2][4], fb[2][2];
     const auto read = [&](int i, int at, int kk) {      // fragment i of a half stage
-        if (i < 2) fb[kk][i] = B.fragment(lds + at + A.kBytes, i, kk);
-        else fa[kk][i - 2] = A.fragment(lds + at, i - 2, kk);
+        if (i < 2) fb[kk & 1][i] = B.fragment(lds + at + A.kBytes, i, kk);
+        else fa[kk & 1][i - 2] = A.fragment(lds + at, i - 2, kk);
     };
     // kWeight: the fragments of A are G with the rows along k; the gradient of the bias is their sum
     const bool with_bias = KIND == kWeight && e.bias_out && tile_n == 0 && wn == 0;
@@ -537,9 +537,8 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
                 for (int r = 0; r < 8; r++) bias_sum[i] += (float)fa[kk][i][r];
         }
     };
-    // Stages of LDS and two sets of fragments: while the first half of a stage is multiplied its second half is read, and while that is
-    // multiplied the first half of the next stage.  In between the waves meet: this stage is in registers and its LDS free for another one, and the
-    // next stage has come in.  Reads and loads are spread over the products: issued all at once, the loads of eight waves fill the queue
+    // Stages of LDS and two sets of fragments of 16 k: while one is multiplied the next one is read, from the next stage while the last one is. Before that
+    // the waves meet: this stage is in registers and its LDS free for another one, and the next stage has come in.  Reads and loads are spread over the products: issued all at once, the loads of eight waves fill the queue
     // of the compute unit, and no product starts until they have gone through.
     if (all > 0) {
 #pragma unroll
@@ -564,26 +563,27 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
 #pragma unroll
                 for (int i = 0; i < 4; i++) bias_sum[i] *= kLow;
             }
-            if (S == 1 || it >= steps) add_up(0);
+            int free = 0;
+            bool more = false;
 #pragma unroll
-            for (int n = 0; n < 8; n++) {
-                acc[n >> 1][n & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][n >> 1], fb[0][n & 1], acc[n >> 1][n & 1], 0, 0, 0);
-                if (n < 6) read(n, at, 1);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            if (it + kStages - 1 < all) wait_and_meet<(kStages - 2) * kPerStage>();
-            else wait_and_meet<0>();
-            const int free = at;
-            const bool more = it + kStages < all;
-            if (more) place_of(it + kStages);
-            at = at == (kStages - 1) * kStageBytes ? 0 : at + kStageBytes;
-            if (S == 1 || it >= steps) add_up(1);
+            for (int h = 0; h < kK / 16; h++) {
+                const bool last = h == kK / 16 - 1;
+                if (last) {
+                    if (it + kStages - 1 < all) wait_and_meet<(kStages - 2) * kPerStage>();
+                    else wait_and_meet<0>();
+                    free = at;
+                    more = it + kStages < all;
+                    if (more) place_of(it + kStages);
+                    at = at == (kStages - 1) * kStageBytes ? 0 : at + kStageBytes;
+                }
+                if (S == 1 || it >= steps) add_up(h & 1);
 #pragma unroll
-            for (int n = 0; n < 8; n++) {
-                acc[n >> 1][n & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[1][n >> 1], fb[1][n & 1], acc[n >> 1][n & 1], 0, 0, 0);
-                if (n < 6) read(n, at, 0);         // behind the last stage: what is there, and not used
-                if (more && n >= 1 && n - 1 < kPerStage) fetch(n - 1, free);
-                __builtin_amdgcn_sched_barrier(0);
+                for (int n = 0; n < 8; n++) {
+                    acc[n >> 1][n & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[h & 1][n >> 1], fb[h & 1][n & 1], acc[n >> 1][n & 1], 0, 0, 0);
+                    if (n < 6) read(n, at, last ? 0 : h + 1);         // behind the last stage: what is there, and not used
+                    if (last && more && n >= 8 - kPerStage) fetch(n - (8 - kPerStage), free);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
         }
         __builtin_amdgcn_s_setprio(0);
@@ -1049,7 +1049,7 @@ int backward(const i6train_ce_problem& p, const Layout& l, const float* grad_los
             h.p.a = {g, g_stride, l.piece, (int64_t)l.g_bytes, 0, &header->rows};
             h.p.b = piece_w;
             h.p.b.rows = p.D;
-            h.p.K = round_up(classes, kK); h.p.splits = l.hidden_splits;
+            h.p.K = round_up(classes, kPad); h.p.splits = l.hidden_splits;
             h.e.header = header; h.e.back = back; h.e.row_target = row_target; h.e.row_frame = (const int*)(fw + l.row_frame); h.e.classes = p.F;
             h.e.sum = dx; h.e.sum_stride = p.D; h.e.part_stride = (int64_t)l.rows_p * p.D; h.e.add = first > 0; h.e.last = first + l.piece >= p.F && l.hidden_splits == 1;
             h.e.out = grad_hidden;
