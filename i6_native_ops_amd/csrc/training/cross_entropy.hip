@@ -21,6 +21,7 @@
 //
 // Logits are in units of log 2 from the accumulators on: exponentials and logarithms are single instructions.
 #include <cmath>
+#include <type_traits>
 
 #include "train_common.h"
 
@@ -39,7 +40,7 @@ using f16x2 = f16 __attribute__((ext_vector_type(2)));
 using f16x4 = f16 __attribute__((ext_vector_type(4)));
 using f16x8 = f16 __attribute__((ext_vector_type(8)));
 using s16x4 = short __attribute__((ext_vector_type(4)));
-using acc_t = float __attribute__((ext_vector_type(16)));
+using acc_t = float __attribute__((ext_vector_type(4)));
 using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
 
 template <typename N, typename M> __host__ __device__ constexpr N round_up(N n, M to) { return (n + (N)to - 1) / (N)to * (N)to; }
@@ -324,8 +325,9 @@ __device__ __forceinline__ void load_to_lds(descriptor d, uint32_t to, uint32_t 
 // One operand's part of a stage: R rows of the tile by kK.  LDS is filled by loads that bypass the registers and write 64 lanes x 16 bytes in
 // order; which 16 bytes a lane asks for is free, and places them so that reading has no bank conflicts.
 //   consecutive k:   row r has kK / 8 chunks of 8 k; chunk c lies at place c ^ turn(r) of the row, other ones in 16 rows (256 bytes: 64 banks).  A fragment is one read of 16 bytes.
-//   consecutive m:   k has R / 8 chunks of 8 m; chunk c lies at place c ^ ((k & 3) << 2).  A fragment is two reads that
-//                    transpose 4 k x 16 m within 16 lanes.
+//   consecutive m:   k has R / 8 chunks of 8 m; chunk c lies at place c ^ turn(k): pairs of chunks (16 m) stay together, and 8 k lie in other 32 bytes.  A fragment is two
+//                    reads that transpose 4 k x 16 m within 16 lanes.
+// A fragment: 16 rows by 32 k, lane l has row l & 15 and 8 k from 8 (l >> 4) on.
 template <int R, bool kConsecutiveK, int kWaves, int kK> struct Side {
     static constexpr int kLoads = R * kK * 2 / 1024 / kWaves;      // per wave and stage
     static constexpr int kBytes = R * kK * 2;
@@ -333,9 +335,13 @@ template <int R, bool kConsecutiveK, int kWaves, int kK> struct Side {
     uint32_t from[kLoads];       // byte offsets of this lane's chunks at k = 0
     uint32_t step, half;         // bytes from stage to stage, and to the second halves
     uint32_t to;                 // this wave's place in a stage
-    int read[4];                 // byte offsets of this lane's fragments
+    int read[kK / 32];           // consecutive k: byte offsets of this lane's fragments of the first 16 rows
+    int base, row, x;            // consecutive m: those of its k, the first row's, and what its places are turned by
 
-    static __device__ __forceinline__ int turn(int r) { return kK == 32 ? (r >> 2) & 3 : (r >> 1) & 7; }
+    static __device__ __forceinline__ int turn(int i) {
+        if (!kConsecutiveK) return ((i & 3) << 1) | (i & 8);
+        return kK == 32 ? (i >> 2) & 3 : (i >> 1) & 7;
+    }
     __device__ __forceinline__ void set(const Operand& o, int rows, int first, int k0, int base_row) {
         const int lane = threadIdx.x & 63, wave = wave_index();
         const int64_t origin = kConsecutiveK ? first * o.row_stride + k0 : k0 * o.row_stride + first;
@@ -350,30 +356,31 @@ template <int R, bool kConsecutiveK, int kWaves, int kK> struct Side {
                 const int r = slot / (kK / 8), c = (slot % (kK / 8)) ^ turn(r);
                 from[i] = (uint32_t)(min(r, rows - 1 - first) * o.row_stride * 2 + c * 16);      // rows behind the last are the last again
             } else {
-                const int k = slot / (R / 8), c = (slot % (R / 8)) ^ ((k & 3) << 2);
+                const int k = slot / (R / 8), c = (slot % (R / 8)) ^ turn(k);
                 const int last = (int)((o.row_stride - first) / 8 - 1);                          // columns behind the row's end as well
                 from[i] = (uint32_t)(k * o.row_stride * 2 + min(c, last) * 16);
             }
         }
         if (kConsecutiveK) {
-            const int r = base_row + (lane & 31);
+            const int r = base_row + (lane & 15);
 #pragma unroll
-            for (int kk = 0; kk < kK / 16; kk++) read[kk] = r * kK * 2 + ((kk * 2 + (lane >> 5)) ^ turn(r)) * 16;
+            for (int h = 0; h < kK / 32; h++) read[h] = r * kK * 2 + ((h * 4 + (lane >> 4)) ^ turn(r)) * 16;
         } else {
-            const int k = (lane >> 5) * 8 + ((lane & 15) >> 2), m = base_row / 8 + ((lane >> 4) & 1) * 2;
-#pragma unroll
-            for (int i = 0; i < 4; i++) read[i] = k * (R * 2) + (((m + i * 4) ^ ((k & 3) << 2)) + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
+            const int k = (lane >> 4) * 8 + ((lane & 15) >> 2);
+            base = k * (R * 2) + ((lane & 3) >> 1) * 16 + (lane & 1) * 8;
+            row = base_row * 2;
+            x = turn(k) * 16;
         }
     }
     __device__ __forceinline__ void fetch(int i, uint32_t lds, uint32_t offset) const {
         load_to_lds(source, lds + to + i * kWaves * 1024, from[i], offset);
     }
-    // block b of 32 rows, k of kk * 16 .. + 15
-    __device__ __forceinline__ f16x8 fragment(const char* lds, int b, int kk) const {
+    // rows 16 b .. + 15, k of 32 h .. + 31
+    __device__ __forceinline__ f16x8 fragment(const char* lds, int b, int h) const {
         if constexpr (kConsecutiveK) {
-            return *reinterpret_cast<const f16x8*>(lds + read[kk] + b * 32 * kK * 2);
+            return *reinterpret_cast<const f16x8*>(lds + read[h] + b * 16 * kK * 2);
         } else {
-            const char* at = lds + read[b] + kk * 16 * (R * 2);
+            const char* at = lds + base + ((row + b * 32) ^ x) + h * 32 * (R * 2);
             using P = __attribute__((address_space(3))) s16x4*;
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(at + 4 * (R * 2)));
             return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -383,22 +390,22 @@ template <int R, bool kConsecutiveK, int kWaves, int kK> struct Side {
 
 constexpr int kGStride = kM * 2 + 16;      // bytes of a row of G in LDS
 
-// A wave's block of 32 x 64 of C to memory, times two powers of two, through LDS of the wave's own: rows of 64 values in accesses of 16 bytes instead of one
+// A wave's block of 16 x 64 of C to memory, times two powers of two, through LDS of the wave's own: rows of 64 values in accesses of 16 bytes instead of one
 // value a lane.  row(r) is where row r begins, or null; `cols` of the columns are there; `whole`: every 16 bytes of a row are aligned.
-constexpr int kBlockBytes = 32 * (64 * 4 + 16);
+constexpr int kBlockBytes = 16 * (64 * 4 + 16);
 template <typename Out, typename Row>
-__device__ __forceinline__ void store_block(char* lds, const acc_t (&c)[2], float by, float by_too, int cols, bool whole, Row row) {
+__device__ __forceinline__ void store_block(char* lds, const acc_t (&c)[4], float by, float by_too, int cols, bool whole, Row row) {
     constexpr int kStride = 64 * sizeof(Out) + 16, kPer = 16 / sizeof(Out), kLanes = 64 / kPer, kRows = 64 / kLanes;
     const int lane = threadIdx.x & 63;
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int j = 0; j < 2; j++)
+    for (int j = 0; j < 4; j++)
 #pragma unroll
-        for (int r = 0; r < 16; r++)
-            *reinterpret_cast<Out*>(lds + (4 * (lane >> 5) + (r & 3) + 8 * (r >> 2)) * kStride + (j * 32 + (lane & 31)) * sizeof(Out)) = (Out)(c[j][r] * by * by_too);
+        for (int r = 0; r < 4; r++)
+            *reinterpret_cast<Out*>(lds + (4 * (lane >> 4) + r) * kStride + (j * 16 + (lane & 15)) * sizeof(Out)) = (Out)(c[j][r] * by * by_too);
     __builtin_amdgcn_wave_barrier();        // the wave's reads of LDS follow its writes
 #pragma unroll
-    for (int k = 0; k < 32 / kRows; k++) {
+    for (int k = 0; k < 16 / kRows; k++) {
         const int r = k * kRows + lane / kLanes, n = lane % kLanes * kPer;
         const u32x4 v = *reinterpret_cast<const u32x4*>(lds + r * kStride + n * sizeof(Out));
         Out* to = row(r);
@@ -468,28 +475,26 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
     Side<kCols, kBk, kWaves, kK> B;
     A.set(p.a, rows_a, m0, k0, wm * 128);
     B.set(p.b, rows_b, n0, k0, wn * 64);
-    if constexpr (kLogits) {
-        if (tid < kM) {
+    if (kLogits && tid < kM) {
         const int m = m0 + tid;       // classes behind the last: -inf, no probability
         float v = m < rows_a ? 0.f : -INFINITY;
         if (e.bias && m < rows_a) v = (float)static_cast<const In*>(e.bias)[e.first_class + m] * kLog2e;
         bias[tid] = v;
-        }
     }
 
-    // register r of a 32 x 32 block: row (r & 3) + 8 (r >> 2) + 4 (lane >> 5), column lane & 31
-    const int row_in = wm * 128 + 4 * (lane >> 5), col_in = wn * 64 + (lane & 31);
-    acc_t acc[4][2];
+    // register r of a 16 x 16 block: row 4 (lane >> 4) + r, column lane & 15
+    const int row_in = wm * 128 + 4 * (lane >> 4), col_in = wn * 64 + (lane & 15);
+    acc_t acc[8][4];
     if (KIND == kHidden && e.add) {
         const float* sum = e.sum + (int64_t)m0 * e.sum_stride + n0;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < 8; i++)
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int n = min(col_in + j * 32, rows_b - n0 - 1);
+            for (int j = 0; j < 4; j++) {
+                const int n = min(col_in + j * 16, rows_b - n0 - 1);
 #pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int m = min(row_in + i * 32 + (r & 3) + 8 * (r >> 2), rows_a - m0 - 1);
+                for (int r = 0; r < 4; r++) {
+                    const int m = min(row_in + i * 16 + r, rows_a - m0 - 1);
                     acc[i][j][r] = sum[(int64_t)m * e.sum_stride + n] * (S == 2 ? 1.f / kLow : 1.f);       // scaled on the way, below
                 }
             }
@@ -497,11 +502,9 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
         __builtin_amdgcn_s_waitcnt(0x0f70);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < 8; i++)
 #pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
+            for (int j = 0; j < 4; j++) acc[i][j] = 0.f;
     }
 
     const uint32_t stages = lds_address(lds);
@@ -521,25 +524,60 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
         if (i < kLoadsA) A.fetch(i, stages + at, next_a);
         else B.fetch(i - kLoadsA, stages + at + A.kBytes, next_b);
     };
-    f16x8 fa[2][4], fb[2][2];
-    const auto read = [&](int i, int at, int kk) {      // fragment i of a half stage
-        if (i < 2) fb[kk & 1][i] = B.fragment(lds + at + A.kBytes, i, kk);
-        else fa[kk & 1][i - 2] = A.fragment(lds + at, i - 2, kk);
+    f16x8 fa[2][8], fb[2][4];
+    const auto read = [&](auto set, int i, int at, int h) {      // fragment i of 32 k
+        if (i < 4) fb[set.value][i] = B.fragment(lds + at + A.kBytes, i, h);
+        else fa[set.value][i - 4] = A.fragment(lds + at, i - 4, h);
     };
     // kWeight: the fragments of A are G with the rows along k; the gradient of the bias is their sum
     const bool with_bias = KIND == kWeight && e.bias_out && tile_n == 0 && wn == 0;
-    float bias_sum[4] = {};
-    const auto add_up = [&](int kk) {
-        if (KIND == kWeight && with_bias) {
+    float bias_sum[8] = {};
+    int it = 0, at = 0;                                          // stage, and where in LDS it is
+    // 32 k of a stage: the products of one set of fragments, while the other set is read: the next 32 k of the stage, or the first of the next one.  Before
+    // those are read the waves meet: this stage is in registers and its LDS free for another one, and the next stage has come in.
+    // Reads and loads are spread over the products: issued all at once, the loads of eight waves fill the queue of the compute unit, and no product starts
+    // until they have gone through.  A fragment of A is read when the one two before it has been used: registers for ten, not sixteen.
+    const auto part_of_stage = [&](auto set, auto last) {
+        constexpr int kSet = set.value;
+        constexpr bool kLast = last.value;
+        const std::integral_constant<int, 1 - kSet> other{};
+        int free = 0;
+        bool more = false;
+        if (kLast) {
+            if (it + kStages - 1 < all) wait_and_meet<(kStages - 2) * kPerStage>();
+            else wait_and_meet<0>();
+            free = at;
+            more = it + kStages < all;
+            if (more) place_of(it + kStages);
+            at = at == (kStages - 1) * kStageBytes ? 0 : at + kStageBytes;
+        }
+        if (KIND == kWeight && with_bias && (S == 1 || it >= steps)) {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < 8; i++)
 #pragma unroll
-                for (int r = 0; r < 8; r++) bias_sum[i] += (float)fa[kk][i][r];
+                for (int r = 0; r < 8; r++) bias_sum[i] += (float)fa[kSet][i][r];
+        }
+        constexpr int kReadAt[12] = {0, 2, 4, 6, 8, 10, 12, 14, 16, 18, 20, 24};
+#pragma unroll
+        for (int n = 0; n < 32; n++) {
+            acc[n >> 2][n & 3] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[kSet][n >> 2], fb[kSet][n & 3], acc[n >> 2][n & 3], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 12; i++)
+                if (kReadAt[i] == n) read(other, i, at, kLast ? 0 : 1);         // behind the last stage: what is there, and not used
+            if (kLast && more && n % 4 == 1 && n / 4 < kPerStage) fetch(n / 4, free);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // Stages of LDS and two sets of fragments of 16 k: while one is multiplied the next one is read, from the next stage while the last one is. Before that
-    // the waves meet: this stage is in registers and its LDS free for another one, and the next stage has come in.  Reads and loads are spread over the products: issued all at once, the loads of eight waves fill the queue
-    // of the compute unit, and no product starts until they have gone through.
+    const auto scale = [&] {                                     // between the second and the third part of 32-bit operands
+        if (S == 2 && it == 2 * steps) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[i][j] *= kLow;
+                bias_sum[i] *= kLow;
+            }
+        }
+    };
     if (all > 0) {
 #pragma unroll
         for (int n = 0; n < kStages; n++) {
@@ -550,41 +588,19 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
         }
         if (all >= kStages) wait_and_meet<(kStages - 1) * kPerStage>();
         else wait_and_meet<0>();
+        constexpr std::integral_constant<int, 0> first{};
+        constexpr std::integral_constant<int, 1> second{};
 #pragma unroll
-        for (int i = 0; i < 6; i++) read(i, 0, 0);
-        int at = 0;
+        for (int i = 0; i < 12; i++) read(first, i, 0, 0);
         __builtin_amdgcn_s_setprio(1);
-        for (int it = 0; it < all; it++) {
-            if (S == 2 && it == 2 * steps) {
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++) acc[i][j] *= kLow;
-#pragma unroll
-                for (int i = 0; i < 4; i++) bias_sum[i] *= kLow;
+        for (; it < all; it++) {
+            scale();
+            part_of_stage(first, std::bool_constant<kK == 32>{});
+            if constexpr (kK == 32) {
+                if (++it == all) break;
+                scale();
             }
-            int free = 0;
-            bool more = false;
-#pragma unroll
-            for (int h = 0; h < kK / 16; h++) {
-                const bool last = h == kK / 16 - 1;
-                if (last) {
-                    if (it + kStages - 1 < all) wait_and_meet<(kStages - 2) * kPerStage>();
-                    else wait_and_meet<0>();
-                    free = at;
-                    more = it + kStages < all;
-                    if (more) place_of(it + kStages);
-                    at = at == (kStages - 1) * kStageBytes ? 0 : at + kStageBytes;
-                }
-                if (S == 1 || it >= steps) add_up(h & 1);
-#pragma unroll
-                for (int n = 0; n < 8; n++) {
-                    acc[n >> 1][n & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[h & 1][n >> 1], fb[h & 1][n & 1], acc[n >> 1][n & 1], 0, 0, 0);
-                    if (n < 6) read(n, at, last ? 0 : h + 1);         // behind the last stage: what is there, and not used
-                    if (last && more && n >= 8 - kPerStage) fetch(n - (8 - kPerStage), free);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            }
+            part_of_stage(second, std::true_type{});
         }
         __builtin_amdgcn_s_setprio(0);
     }
@@ -593,17 +609,18 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
         __syncthreads();
         float* out = e.part_out + part_of_k * e.part_stride + n0 + wn * 64;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < 8; i++)
             store_block<float>(lds + wave * kBlockBytes, acc[i], 1.f, 1.f, rows_b - n0 - wn * 64, rows_b % 4 == 0, [&](int r) -> float* {
-                const int m = m0 + wm * 128 + i * 32 + r;
+                const int m = m0 + wm * 128 + i * 16 + r;
                 return m < rows_a ? out + (int64_t)m * rows_b : nullptr;
             });
         if (with_bias) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float v = bias_sum[i] + __shfl_xor(bias_sum[i], 32);
-                const int m = m0 + wm * 128 + i * 32 + lane;
-                if (lane < 32 && m < rows_a) e.bias_out[part_of_k * e.bias_stride + m] = v;
+            for (int i = 0; i < 8; i++) {
+                float v = bias_sum[i] + __shfl_xor(bias_sum[i], 16);
+                v += __shfl_xor(v, 32);
+                const int m = m0 + wm * 128 + i * 16 + lane;
+                if (lane < 16 && m < rows_a) e.bias_out[part_of_k * e.bias_stride + m] = v;
             }
         }
         return;
@@ -614,9 +631,9 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
             __syncthreads();
             float* sum = e.sum + part_of_k * e.part_stride + n0 + wn * 64;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < 8; i++)
                 store_block<float>(lds + wave * kBlockBytes, acc[i], 1.f, 1.f, rows_b - n0 - wn * 64, rows_b % 4 == 0, [&](int r) -> float* {
-                    const int m = m0 + wm * 128 + i * 32 + r;
+                    const int m = m0 + wm * 128 + i * 16 + r;
                     return m < rows_a ? sum + (int64_t)m * e.sum_stride : nullptr;
                 });
             return;
@@ -633,12 +650,12 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
         In* out = static_cast<In*>(e.out) + n0 + wn * 64;
         const bool whole = rows_b % (16 / (int)sizeof(In)) == 0;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < 8; i++) {
 #pragma unroll
-            for (int r = 0; r < 16; r++)
-                if (frames[row_in + i * 32 + (r & 3) + 8 * (r >> 2)] < 0) acc[i][0][r] = acc[i][1][r] = __builtin_nanf("");
+            for (int r = 0; r < 4; r++)
+                if (frames[row_in + i * 16 + r] < 0) acc[i][0][r] = acc[i][1][r] = acc[i][2][r] = acc[i][3][r] = __builtin_nanf("");
             store_block<In>(lds + wave * kBlockBytes, acc[i], unscale, unscale_w, rows_b - n0 - wn * 64, whole, [&](int r) -> In* {
-                const int m = wm * 128 + i * 32 + r, frame = frames[m];
+                const int m = wm * 128 + i * 16 + r, frame = frames[m];
                 return m0 + m < rows_a ? out + (int64_t)(frame < 0 ? ~frame : frame) * rows_b : nullptr;
             });
         }
@@ -649,38 +666,38 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
     __syncthreads();
     // logits in units of log 2
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+    for (int i = 0; i < 8; i++) {
+        const float4 b = *reinterpret_cast<const float4*>(&bias[row_in + i * 16]);
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const float4 b = *reinterpret_cast<const float4*>(&bias[row_in + i * 32 + 8 * q]);
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                acc[i][j][4 * q] = fmaf(acc[i][j][4 * q], per, b.x);
-                acc[i][j][4 * q + 1] = fmaf(acc[i][j][4 * q + 1], per, b.y);
-                acc[i][j][4 * q + 2] = fmaf(acc[i][j][4 * q + 2], per, b.z);
-                acc[i][j][4 * q + 3] = fmaf(acc[i][j][4 * q + 3], per, b.w);
-            }
+        for (int j = 0; j < 4; j++) {
+            acc[i][j][0] = fmaf(acc[i][j][0], per, b.x);
+            acc[i][j][1] = fmaf(acc[i][j][1], per, b.y);
+            acc[i][j][2] = fmaf(acc[i][j][2], per, b.z);
+            acc[i][j][3] = fmaf(acc[i][j][3], per, b.w);
         }
+    }
 
     if constexpr (KIND == kStatistics) {
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
+        for (int j = 0; j < 4; j++) {
             float most = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < 8; i++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) most = fmaxf(most, acc[i][j][r]);
+                for (int r = 0; r < 4; r++) most = fmaxf(most, acc[i][j][r]);
+            most = fmaxf(most, __shfl_xor(most, 16));
             most = fmaxf(most, __shfl_xor(most, 32));
             const float base = most == -INFINITY ? 0.f : most;        // classes that are all ruled out: the sum is 0, not NaN
             float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < 8; i++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) sum += exp2_fast(acc[i][j][r] - base);
+                for (int r = 0; r < 4; r++) sum += exp2_fast(acc[i][j][r] - base);
+            sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
-            if (lane < 32) {
-                join[wm * 2][col_in + j * 32] = most;
-                join[wm * 2 + 1][col_in + j * 32] = sum;
+            if (lane < 16) {
+                join[wm * 2][col_in + j * 16] = most;
+                join[wm * 2 + 1][col_in + j * 16] = sum;
             }
         }
         __syncthreads();
@@ -693,13 +710,13 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
 
     if constexpr (KIND == kGradient) {
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const int n = n0 + col_in + j * 32;
+        for (int j = 0; j < 4; j++) {
+            const int n = n0 + col_in + j * 16;
             const float lse = n < rows_b ? e.lse[n] : INFINITY, scale = n < rows_b ? ldexpf(e.row_scale[n], up) : 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < 8; i++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) {
+                for (int r = 0; r < 4; r++) {
                     const float v = exp2_fast(acc[i][j][r] - lse) * scale;
                     if constexpr (S == 2) {
                         f16x2 halves;      // both in the accumulator's register
@@ -727,25 +744,23 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
         for (int h = 0; h < S; h++) {
             // through LDS, so that whole rows of the tile are written at once
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < 8; i++)
 #pragma unroll
-                for (int j = 0; j < 2; j++)
+                for (int j = 0; j < 4; j++) {
+                    f16x4 v;
+                    if constexpr (S == 2) {
+                        const uint32_t which = h ? 0x07060302u : 0x05040100u;       // upper or lower 16 bits of two registers
+                        uint32_t pair[2];
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        f16x4 v;
-                        if constexpr (S == 2) {
-                            const uint32_t which = h ? 0x07060302u : 0x05040100u;       // upper or lower 16 bits of two registers
-                            uint32_t pair[2];
+                        for (int r = 0; r < 2; r++)
+                            pair[r] = __builtin_amdgcn_perm(__float_as_uint(acc[i][j][2 * r + 1]), __float_as_uint(acc[i][j][2 * r]), which);
+                        v = __builtin_bit_cast(f16x4, pair);
+                    } else {
 #pragma unroll
-                            for (int r = 0; r < 2; r++)
-                                pair[r] = __builtin_amdgcn_perm(__float_as_uint(acc[i][j][4 * q + 2 * r + 1]), __float_as_uint(acc[i][j][4 * q + 2 * r]), which);
-                            v = __builtin_bit_cast(f16x4, pair);
-                        } else {
-#pragma unroll
-                            for (int r = 0; r < 4; r++) v[r] = (f16)acc[i][j][4 * q + r];
-                        }
-                        *reinterpret_cast<f16x4*>(lds + (col_in + j * 32) * kGStride + (row_in + i * 32 + 8 * q) * 2) = v;
+                        for (int r = 0; r < 4; r++) v[r] = (f16)acc[i][j][r];
                     }
+                    *reinterpret_cast<f16x4*>(lds + (col_in + j * 16) * kGStride + (row_in + i * 16) * 2) = v;
+                }
             __syncthreads();
             if (place >= 0) {
                 f16 high, low;
