@@ -340,7 +340,7 @@ template <int R, bool kConsecutiveK, int kWaves, int kK> struct Side {
 
     static __device__ __forceinline__ int turn(int i) {
         if (!kConsecutiveK) return ((i & 3) << 1) | (i & 8);
-        return kK == 32 ? (i >> 2) & 3 : (i >> 1) & 7;
+        return kK == 32 ? ((i >> 1) & 2) ^ ((i >> 3) & 1) * 3 : (i >> 1) & 7;
     }
     __device__ __forceinline__ void set(const Operand& o, int rows, int first, int k0, int base_row) {
         const int lane = threadIdx.x & 63, wave = wave_index();
@@ -792,12 +792,17 @@ struct BothArgs {
     ProductArgs p;
     EpilogueArgs e;
 };
-template <typename In>
-__global__ __launch_bounds__(512, 2) void products_back(BothArgs h, BothArgs w, int hidden) {
-    static_assert(Shape<In, kHidden, 4>::kBytes == Shape<In, kWeight, 4>::kBytes);
-    __shared__ alignas(16) char lds[Shape<In, kHidden, 4>::kBytes];
-    if ((int)blockIdx.x < hidden) product_of<In, kHidden, 4>(h.p, h.e, lds, blockIdx.x);
-    else product_of<In, kWeight, 4>(w.p, w.e, lds, blockIdx.x - hidden);
+template <typename In, int NW>
+__global__ __launch_bounds__(128 * NW, 2) void products_back(BothArgs h, BothArgs w, int hidden) {
+    static_assert(Shape<In, kHidden, NW>::kBytes == Shape<In, kWeight, NW>::kBytes);
+    __shared__ alignas(16) char lds[Shape<In, kHidden, NW>::kBytes];
+    if ((int)blockIdx.x < hidden) product_of<In, kHidden, NW>(h.p, h.e, lds, blockIdx.x);
+    else product_of<In, kWeight, NW>(w.p, w.e, lds, blockIdx.x - hidden);
+}
+template <typename In> void launch_back(bool narrow, unsigned hidden, unsigned groups, const BothArgs& h, const BothArgs& w, hipStream_t s) {
+    if (groups == 0) return;
+    if (narrow) products_back<In, 2><<<dim3(groups), dim3(256), 0, s>>>(h, w, (int)hidden);
+    else products_back<In, 4><<<dim3(groups), dim3(512), 0, s>>>(h, w, (int)hidden);
 }
 
 // ---------------------------------------------------------------------------------------------------------- the rest
@@ -934,6 +939,7 @@ constexpr size_t kPieceBytes = (size_t)512 << 20;      // of G: the caches in fr
 // Where things are in the workspaces.
 struct Layout {
     int S, Kp, row_tiles, class_tiles, piece, splits, hidden_splits;
+    bool narrow;
     int64_t rows, rows_p, weights_p;
     size_t header, offsets, row_frame, row_target, target_logit, lse, x, w, part, x_bytes, w_bytes, forward;
     size_t back, row_scale, g, dx, dw, db, g_bytes, backward;
@@ -973,8 +979,14 @@ int layout(const i6train_ce_problem& p, Layout& l) {
     piece = piece > most_piece ? most_piece : piece;
     piece = piece < kM ? kM : (piece > classes ? classes : piece);
     l.piece = (int)round_up(ceil_div(classes, ceil_div(classes, piece)), kM);      // pieces of one size
-    const int64_t tiles = (int64_t)l.piece / kM * ceil_div(p.D, 256);
-    int64_t splits = 256 / tiles < 1 ? 1 : 256 / tiles;
+    // Few tiles leave compute units idle, which tiles of 128 columns leave less (both gradients of 4000 frames, F = 1000, D = 384: 30 us with tiles of 256 columns, 25 with 128,
+    // in 32 bits 70, 56; 8000 frames, F = 1000, D = 512: 32, 28 and 77, 66); more tiles are faster as large ones (8000 frames, F = 2000, D = 512: 49, 50 and 106, 110), and if
+    // half of each is empty, as fast (28800 frames, F = 12001, D = 128: 602, 626 and 1653, 1554 with G; 8000 frames, F = 5001, D = 128: 55, 44 and 120, 103).
+    const int64_t row_tiles = ceil_div(l.rows, (int64_t)kM), class_tiles = l.piece / kM;
+    l.narrow = row_tiles * ceil_div(p.D, 256) <= 64 && (class_tiles * ceil_div(p.D, 256) <= 8 || p.D <= 128);
+    const int columns = l.narrow ? 128 : 256, at_once = l.narrow ? 512 : 256;      // of a tile, and how many the compute units hold
+    const int64_t tiles = class_tiles * ceil_div(p.D, columns);
+    int64_t splits = at_once / tiles < 1 ? 1 : at_once / tiles;
     const int64_t most = ceil_div(l.rows, (int64_t)512), least = ceil_div((int64_t)l.rows_p * l.S * (l.piece > l.Kp ? l.piece : l.Kp) * 2, (int64_t)1 << 31);
     splits = splits > most ? most : splits;
     l.splits = (int)(splits < least ? least : splits);      // offsets within a range of k have 32 bits
@@ -985,7 +997,8 @@ int layout(const i6train_ce_problem& p, Layout& l) {
     // Few rows: the sums over the classes are formed in ranges, or a handful of workgroups would go through the whole vocabulary (100 frames, F = 8346, D = 64, float: 88 us
     // a training step, 528 us in one range).  Ranges are of 256 classes at least, of 512 where there are many tiles, whose join costs more than shorter ranges win (4000 frames,
     // F = 1000, D = 1024, bfloat16: 117 us in one range, 135 us in three of 334).
-    const int64_t hidden_tiles = ceil_div(l.rows, (int64_t)kM) * ceil_div(p.D, 256), room = p.F / (hidden_tiles < 32 ? 256 : 512), ranges = room < 256 / hidden_tiles ? room : 256 / hidden_tiles;
+    const int64_t hidden_tiles = row_tiles * ceil_div(p.D, columns), room = p.F / (hidden_tiles < 32 ? 256 : 512);
+    const int64_t ranges = room < at_once / hidden_tiles ? room : at_once / hidden_tiles;
     l.hidden_splits = l.piece >= p.F && ranges > 1 ? (int)ranges : 1;
     l.dx = take(l.piece < p.F || l.hidden_splits > 1 ? 4 * (size_t)l.hidden_splits * l.rows_p * p.D : 0);
     l.dw = take(4 * (size_t)l.splits * l.piece * p.D);
@@ -1000,10 +1013,10 @@ Frames frames_of(const i6train_ce_problem& p, const Layout& l) {
     return {p.hidden, p.hidden_stride_b, p.hidden_stride_t, p.seq_lens, p.targets, p.targets_stride_b, p.targets_stride_t, p.B, p.T, p.F, p.D, l.Kp};
 }
 
+template <int NW> int64_t tiles_of(int64_t rows_a, int64_t rows_b) { return ceil_div(rows_a, (int64_t)kM) * ceil_div(rows_b, (int64_t)(64 * NW)); }
+
 // Workgroups for a product: a multiple of the dies.
-template <int NW> unsigned groups_of(const ProductArgs& q, int64_t rows_a, int64_t rows_b) {
-    return (unsigned)round_up(ceil_div(rows_a, (int64_t)kM) * ceil_div(rows_b, (int64_t)(64 * NW)) * q.splits, 8);
-}
+template <int NW> unsigned groups_of(const ProductArgs& q, int64_t rows_a, int64_t rows_b) { return (unsigned)round_up(tiles_of<NW>(rows_a, rows_b) * q.splits, 8); }
 
 template <typename In, int KIND, int NW> void launch_product(const ProductArgs& q, const EpilogueArgs& e, int64_t rows_a, int64_t rows_b, hipStream_t s) {
     product<In, KIND, NW><<<dim3(groups_of<NW>(q, rows_a, rows_b)), dim3(128 * NW), 0, s>>>(q, e);
@@ -1025,9 +1038,12 @@ int forward(const i6train_ce_problem& p, const Layout& l, float* loss, char* ws,
     q.K = l.Kp; q.splits = 1;
     EpilogueArgs e{};
     e.bias = p.bias; e.header = header; e.part = (float2*)(ws + l.part); e.rows_p = l.rows_p;
-    // the three parts of 32-bit operands make a long loop, which larger tiles feed with fewer bytes (subword units: 669 us, 727 us with small ones); else two
-    // workgroups on a compute unit, so that one has products while the other has exponentials (headline layer: 369 us, 376 us with large ones)
-    launch_product<In, kStatistics, S == 2 ? 4 : 2>(q, e, p.F, l.rows, s);
+    // Large tiles need fewer bytes for a product, but one workgroup has the compute unit and nothing runs beside its end.  They are for long loops (bfloat16, 28800 frames,
+    // F = 12001: D = 512 366 us with small tiles, 344 with large ones, D = 128 175, 197) whose tiles go round the compute units more than twice, or once where small ones do
+    // not (D = 512, F = 5001: 2400 frames 37, 34 us; 3200 frames, 260 large tiles, 38, 48 us; in 32 bits 8000 frames 143, 135).
+    const int64_t small = tiles_of<2>(p.F, l.rows), large = tiles_of<4>(p.F, l.rows);
+    if (l.Kp * (S == 2 ? 3 : 1) >= 512 && (large > 512 || (small > 256 && large <= 256))) launch_product<In, kStatistics, 4>(q, e, p.F, l.rows, s);
+    else launch_product<In, kStatistics, 2>(q, e, p.F, l.rows, s);
     ce_finish<<<dim3(ceil_div(l.rows, (int64_t)64)), dim3(64), 0, s>>>(header, e.part, l.class_tiles, l.rows_p, o.row_frame, o.row_target, o.target_logit, p.T, p.F,
                                                                          (float*)(ws + l.lse), loss, status_slot());
     return launched();
@@ -1068,21 +1084,21 @@ int backward(const i6train_ce_problem& p, const Layout& l, const float* grad_los
             h.e.header = header; h.e.back = back; h.e.row_target = row_target; h.e.row_frame = (const int*)(fw + l.row_frame); h.e.classes = p.F;
             h.e.sum = dx; h.e.sum_stride = p.D; h.e.part_stride = (int64_t)l.rows_p * p.D; h.e.add = first > 0; h.e.last = first + l.piece >= p.F && l.hidden_splits == 1;
             h.e.out = grad_hidden;
-            of_hidden = groups_of<4>(h.p, l.rows, p.D);
+            of_hidden = l.narrow ? groups_of<2>(h.p, l.rows, p.D) : groups_of<4>(h.p, l.rows, p.D);
         }
         if (grad_weight || grad_bias) {
             v.p.a = {g, g_stride, l.piece, (int64_t)l.g_bytes, classes, nullptr};
             v.p.b = {x, row_size, l.Kp, (int64_t)l.x_bytes, p.D, nullptr};
             v.p.n_k = &header->rows; v.p.splits = l.splits;
             v.e.part_out = dw; v.e.part_stride = (int64_t)l.piece * p.D; v.e.bias_out = db; v.e.bias_stride = l.piece;
-            of_weight = groups_of<4>(v.p, classes, p.D);
+            of_weight = l.narrow ? groups_of<2>(v.p, classes, p.D) : groups_of<4>(v.p, classes, p.D);
         }
         // dh that fills the compute units more than once leaves idle ones at its end alone, which long workgroups of dW do not fill (subword units in 32 bits: 771 us
         // apart, 786 us together)
-        const bool apart = of_hidden > 256 && of_weight;
-        if (apart) products_back<In><<<dim3(of_hidden), dim3(512), 0, s>>>(h, v, (int)of_hidden);
+        const bool apart = of_hidden > (l.narrow ? 512 : 256) && of_weight;
+        if (apart) launch_back<In>(l.narrow, of_hidden, of_hidden, h, v, s);
         const unsigned with = apart ? 0 : of_hidden;
-        if (with + of_weight) products_back<In><<<dim3(with + of_weight), dim3(512), 0, s>>>(h, v, (int)with);
+        launch_back<In>(l.narrow, with, with + of_weight, h, v, s);
         if (of_hidden && l.hidden_splits > 1)
             ce_store_hidden<In><<<dim3((unsigned)ceil_div(l.rows * p.D, (int64_t)256)), dim3(256), 0, s>>>(header, back, dx, l.hidden_splits, h.e.part_stride, h.e.row_frame, row_target, p.F,
                                                                                                           p.D, (In*)grad_hidden);

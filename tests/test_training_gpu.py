@@ -743,6 +743,14 @@ def test_cross_entropy_of_few_rows_over_many_classes(B, T, F, D, dtype):
     ce_check(problem)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_cross_entropy_of_large_tiles(dtype):
+    """Sizes whose products all take the large tiles, none of them full."""
+    problem = ce_problem(3, 400, 7700, 450, dtype, lens=[400, 377, 330], seed=11)
+    problem[3][1, 5:50] = -1
+    ce_check(problem)
+
+
 def test_cross_entropy_wide_features():
     """As many features as are taken, in a batch of few frames; one more is refused."""
     from i6_native_ops_amd.training import linear_cross_entropy
