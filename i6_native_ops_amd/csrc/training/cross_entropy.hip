@@ -5,7 +5,7 @@
 //   backward   for one piece of the vocabulary after another: z again, G = g (softmax(z) - [f = y]) rounded to the operands'
 //              precision, then  dh += G W  and  dW = G^T h
 //
-// All three products run through one kernel, product(): C[m][n] = sum_k A[m][k] B[n][k] on the matrix units.  An operand lies in memory
+// All three products run through one function, product_of(): C[m][n] = sum_k A[m][k] B[n][k] on the matrix units.  An operand lies in memory
 // with consecutive k (W and h for the logits, G for dh) or with consecutive m or n (W for dh, G and h for dW) and is turned
 // as it is read from LDS, so nothing is transposed or written twice.
 //
@@ -20,6 +20,10 @@
 // is sixteen times that for 32-bit ones.
 //
 // Logits are in units of log 2 from the accumulators on: exponentials and logarithms are single instructions.
+//
+// Large layers are bound by the matrix units and by the power they draw: the chip lowers its clock to 1.9 - 2.1 GHz under them.  28 800 frames, F = 12001, D = 512 in
+// bfloat16 (0.353 TFLOP a product): statistics 379 us (932 TFLOP/s), G 2 x 233 us (758, writing 690 MB), dh and dW 2 x 368 us (960), all that goes over the
+// operands alone 90 us.  44 800 frames, F = 5001, D = 500 in 32 bits: the three parts of the statistics run at 1090 TFLOP/s, of dh and dW at 870.
 #include <cmath>
 #include <type_traits>
 
@@ -787,7 +791,7 @@ __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueAr
 }
 
 // dh and dW of a piece in one launch, the first `hidden` workgroups (a multiple of eight) for dh: neither needs the other, and where dh leaves compute
-// units idle, dW runs beside it (monophones: 24 us, 39 us one after the other).
+// units idle, dW runs beside it (14 400 frames, F = 264, D = 512 in bfloat16: a training step 85 us, 98 us with one after the other).
 struct BothArgs {
     ProductArgs p;
     EpilogueArgs e;
@@ -934,7 +938,9 @@ __global__ __launch_bounds__(256) void ce_store_hidden(const Header* header, con
 
 // ------------------------------------------------------------------------------------------------------------- host
 
-constexpr size_t kPieceBytes = (size_t)512 << 20;      // of G: the caches in front of the memory hold 256 MB
+// Of G.  Memory that a step needs against its time, which a join of dh and more workgroups' ends take (headline layer, 28 800 x 12001 x 512 in bfloat16: 1635 us with 256 MB,
+// 1584 with 512, 1573 with 1 GB, which is all of it).
+constexpr size_t kPieceBytes = (size_t)512 << 20;
 
 // Where things are in the workspaces.
 struct Layout {
@@ -994,9 +1000,9 @@ int layout(const i6train_ce_problem& p, Layout& l) {
     l.row_scale = take(4 * l.rows_p);
     l.g_bytes = (size_t)l.rows_p * l.S * l.piece * 2;
     l.g = take(l.g_bytes);
-    // Few rows: the sums over the classes are formed in ranges, or a handful of workgroups would go through the whole vocabulary (100 frames, F = 8346, D = 64, float: 88 us
-    // a training step, 528 us in one range).  Ranges are of 256 classes at least, of 512 where there are many tiles, whose join costs more than shorter ranges win (4000 frames,
-    // F = 1000, D = 1024, bfloat16: 117 us in one range, 135 us in three of 334).
+    // Few rows: the sums over the classes are formed in ranges, or a handful of workgroups would go through the whole vocabulary (100 frames, F = 8346, D = 64, float: 69 us
+    // a training step, 414 us in one range; 4000 frames, F = 5001, D = 512, float: 355 and 508).  Ranges are of 256 classes at least, of 512 where there are many tiles, whose
+    // join costs more than shorter ranges win (4000 frames, F = 1000, D = 1024, bfloat16: 101 us in one range, 131 in three of 334).
     const int64_t hidden_tiles = row_tiles * ceil_div(p.D, columns), room = p.F / (hidden_tiles < 32 ? 256 : 512);
     const int64_t ranges = room < at_once / hidden_tiles ? room : at_once / hidden_tiles;
     l.hidden_splits = l.piece >= p.F && ranges > 1 ? (int)ranges : 1;
@@ -1093,8 +1099,8 @@ int backward(const i6train_ce_problem& p, const Layout& l, const float* grad_los
             v.e.part_out = dw; v.e.part_stride = (int64_t)l.piece * p.D; v.e.bias_out = db; v.e.bias_stride = l.piece;
             of_weight = l.narrow ? groups_of<2>(v.p, classes, p.D) : groups_of<4>(v.p, classes, p.D);
         }
-        // dh that fills the compute units more than once leaves idle ones at its end alone, which long workgroups of dW do not fill (subword units in 32 bits: 771 us
-        // apart, 786 us together)
+        // dh that fills the compute units more than once leaves idle ones at its end alone, which long workgroups of dW do not fill (subword units, 44 800 x 5001 x 500
+        // in 32 bits: a training step 3.00 ms apart, 3.03 together)
         const bool apart = of_hidden > (l.narrow ? 512 : 256) && of_weight;
         if (apart) launch_back<In>(l.narrow, of_hidden, of_hidden, h, v, s);
         const unsigned with = apart ? 0 : of_hidden;
