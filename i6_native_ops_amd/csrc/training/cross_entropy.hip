@@ -288,8 +288,8 @@ struct EpilogueArgs {
     const float *target_logit, *lse, *row_scale;
     f16* g;  int64_t g_stride, g_half;     // [row][halves][piece]
     // kHidden: m is the row, n the feature
-    float* sum;  int64_t sum_stride;       // [m][n] over the pieces so far, or [range of k][m][n]
-    int add, last;                         // to what is there; the last piece, which goes to `out`
+    float* sum;  int64_t sum_stride;       // [range of k][m][n] over the pieces so far
+    int add, last;                         // to what is there; to `out`: the last piece in one range
     const int* row_frame;
     int classes;
     void* out;
@@ -490,7 +490,8 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
     const int row_in = wm * 128 + 4 * (lane >> 4), col_in = wn * 64 + (lane & 15);
     acc_t acc[8][4];
     if (KIND == kHidden && e.add) {
-        const float* sum = e.sum + (int64_t)m0 * e.sum_stride + n0;
+        const float* sum = e.sum + part_of_k * e.part_stride + (int64_t)m0 * e.sum_stride + n0;
+        const float scaled = S == 2 && all > 0 ? 1.f / kLow : 1.f;       // taken back on the way, below
 #pragma unroll
         for (int i = 0; i < 8; i++)
 #pragma unroll
@@ -499,7 +500,7 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const int m = min(row_in + i * 16 + r, rows_a - m0 - 1);
-                    acc[i][j][r] = sum[(int64_t)m * e.sum_stride + n] * (S == 2 ? 1.f / kLow : 1.f);       // scaled on the way, below
+                    acc[i][j][r] = sum[(int64_t)m * e.sum_stride + n] * scaled;
                 }
             }
         // here, or the compiler waits for all loads before the products of every stage
@@ -1003,9 +1004,10 @@ int layout(const i6train_ce_problem& p, Layout& l) {
     // Few rows: the sums over the classes are formed in ranges, or a handful of workgroups would go through the whole vocabulary (100 frames, F = 8346, D = 64, float: 69 us
     // a training step, 414 us in one range; 4000 frames, F = 5001, D = 512, float: 355 and 508).  Ranges are of 256 classes at least, of 512 where there are many tiles, whose
     // join costs more than shorter ranges win (4000 frames, F = 1000, D = 1024, bfloat16: 101 us in one range, 131 in three of 334).
-    const int64_t hidden_tiles = row_tiles * ceil_div(p.D, columns), room = p.F / (hidden_tiles < 32 ? 256 : 512);
+    // Two ranges win nothing, as dW runs where dh leaves units idle (16000 frames, F = 5001, D = 512, bfloat16: 390 us in one range, 449 in two).
+    const int64_t hidden_tiles = row_tiles * ceil_div(p.D, columns), room = (l.piece < p.F ? l.piece : p.F) / (hidden_tiles < 32 ? 256 : 512);
     const int64_t ranges = room < at_once / hidden_tiles ? room : at_once / hidden_tiles;
-    l.hidden_splits = l.piece >= p.F && ranges > 1 ? (int)ranges : 1;
+    l.hidden_splits = ranges > 2 ? (int)ranges : 1;
     l.dx = take(l.piece < p.F || l.hidden_splits > 1 ? 4 * (size_t)l.hidden_splits * l.rows_p * p.D : 0);
     l.dw = take(4 * (size_t)l.splits * l.piece * p.D);
     l.db = take(4 * (size_t)l.splits * l.piece);
@@ -1105,7 +1107,7 @@ int backward(const i6train_ce_problem& p, const Layout& l, const float* grad_los
         if (apart) launch_back<In>(l.narrow, of_hidden, of_hidden, h, v, s);
         const unsigned with = apart ? 0 : of_hidden;
         launch_back<In>(l.narrow, with, with + of_weight, h, v, s);
-        if (of_hidden && l.hidden_splits > 1)
+        if (of_hidden && l.hidden_splits > 1 && first + l.piece >= p.F)
             ce_store_hidden<In><<<dim3((unsigned)ceil_div(l.rows * p.D, (int64_t)256)), dim3(256), 0, s>>>(header, back, dx, l.hidden_splits, h.e.part_stride, h.e.row_frame, row_target, p.F,
                                                                                                           p.D, (In*)grad_hidden);
         if (of_weight) {

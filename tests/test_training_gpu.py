@@ -751,6 +751,14 @@ def test_cross_entropy_of_large_tiles(dtype):
     ce_check(problem)
 
 
+@pytest.mark.parametrize("B,T,F,D,dtype", [
+    (9, 1000, 30001, 40, torch.bfloat16), (9, 1000, 15001, 40, torch.float32), (33, 1000, 9001, 24, torch.bfloat16), (33, 1000, 4501, 24, torch.float32),
+])
+def test_cross_entropy_of_pieces_with_ranges_of_classes_and_without(B, T, F, D, dtype):
+    """More than one piece of the vocabulary; the gradient of the features is summed over ranges of each, or in one."""
+    ce_check(ce_problem(B, T, F, D, dtype, seed=F, lens=[T] * (B - 1) + [3]))
+
+
 def test_cross_entropy_wide_features():
     """As many features as are taken, in a batch of few frames; one more is refused."""
     from i6_native_ops_amd.training import linear_cross_entropy
