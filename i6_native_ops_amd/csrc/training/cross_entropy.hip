@@ -196,11 +196,10 @@ template <int S> __device__ __forceinline__ void store_operand(f16* out, int Kp,
 struct Packed {
     f16 *x, *w;                      // [row][halves][Kp], zeros behind column D and in rows up to a multiple of kPad
     int *row_frame, *row_target;
-    float* target_logit;             // in units of log 2
     float* loss;
 };
 
-// A wave per row: frames as operands, with the logit of their target in 32 bits; then weights.
+// A wave per row: frames as operands, then weights.
 template <typename In>
 __global__ __launch_bounds__(kThreads) void ce_pack(Frames f, Weights w, const int* offsets, const Header* header, Packed o) {
     constexpr int S = sizeof(In) == 4 ? 2 : 1;
@@ -236,24 +235,15 @@ __global__ __launch_bounds__(kThreads) void ce_pack(Frames f, Weights w, const i
         const int target = f.targets[b * f.tgt_b + t * f.tgt_t];
         const bool used = has_target(target, f.F);      // a frame without a target: zeros, whatever it holds
         const In* x = static_cast<const In*>(f.hidden) + b * f.stride_b + t * f.stride_t;
-        const In* y = static_cast<const In*>(w.p) + (used ? target : 0) * w.stride;
-        const bool aligned = (uintptr_t)x % 16 == 0, aligned_y = (uintptr_t)y % 16 == 0;
-        float dot = 0.f;
+        const bool aligned = (uintptr_t)x % 16 == 0;
         for (int c = lane * 8; c < f.Kp; c += 512) {
-            float v[8], u[8];
-            if (used) {
-                load8(x, c, f.D, aligned, v);
-                load8(y, c, f.D, aligned_y, u);
-#pragma unroll
-                for (int i = 0; i < 8; i++) dot = fmaf(v[i], u[i], dot);
-            }
+            float v[8];
+            if (used) load8(x, c, f.D, aligned, v);
             store_operand<S>(o.x + row * row_size, f.Kp, c, used ? v : none, ex);
         }
-        dot = wave_sum(dot);
         if (lane == 0) {
             o.row_frame[row] = (int)r;
             o.row_target[row] = target;
-            o.target_logit[row] = used ? dot + (w.bias ? (float)static_cast<const In*>(w.bias)[target] : 0.f) : 0.f;
         }
     }
 }
@@ -285,7 +275,8 @@ struct EpilogueArgs {
     const int* row_target;
     float2* part;                          // [tile of classes][rows_p]: maximum, sum
     int64_t rows_p;
-    const float *target_logit, *lse, *row_scale;
+    float* target_logit;                   // in units of log 2, from the accumulators: the same bits as in the sum over the classes
+    const float *lse, *row_scale;
     f16* g;  int64_t g_stride, g_half;     // [row][halves][piece]
     // kHidden: m is the row, n the feature
     float* sum;  int64_t sum_stride;       // [range of k][m][n] over the pieces so far
@@ -432,7 +423,7 @@ template <typename In, int KIND, int NW> struct Shape {
     static constexpr int kWaves = 2 * NW, kCols = 64 * NW, kStages = NW == 2 ? 3 : 2, kK = NW == 2 ? 32 : 64;
     static constexpr int kStageBytes = (kM + kCols) * kK * 2;
     static constexpr bool kLogits = KIND == kStatistics || KIND == kGradient;
-    static constexpr int kBytes = kStages * kStageBytes + (kLogits ? kM * 4 : 0) + (KIND == kStatistics ? 4 * kCols * 4 : 0);
+    static constexpr int kBytes = kStages * kStageBytes + (kLogits ? kM * 4 : 0) + (KIND == kStatistics ? 5 * kCols * 4 : 0);
 };
 
 template <typename In, int KIND, int NW>
@@ -446,6 +437,7 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
     static_assert(KIND != kGradient || (kCols == kN && kN * kGStride <= kStages * kStageBytes), "G goes through the stages' LDS");
     float* bias = reinterpret_cast<float*>(lds + kStages * kStageBytes);
     float (*join)[kCols] = reinterpret_cast<float (*)[kCols]>(lds + kStages * kStageBytes + kM * 4);
+    int* target_of = reinterpret_cast<int*>(join[4]);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), wm = wave & 1, wn = wave >> 1;
     const int rows_a = p.a.n_rows ? *p.a.n_rows : p.a.rows, rows_b = p.b.n_rows ? *p.b.n_rows : p.b.rows;
@@ -484,6 +476,10 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
         float v = m < rows_a ? 0.f : -INFINITY;
         if (e.bias && m < rows_a) v = (float)static_cast<const In*>(e.bias)[e.first_class + m] * kLog2e;
         bias[tid] = v;
+    }
+    if (KIND == kStatistics && tid < kCols) {
+        const int y = n0 + tid < rows_b ? e.row_target[n0 + tid] : -1;
+        target_of[tid] = has_target(y, rows_a) ? y - m0 : -1;
     }
 
     // register r of a 16 x 16 block: row 4 (lane >> 4) + r, column lane & 15
@@ -685,6 +681,17 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
     if constexpr (KIND == kStatistics) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
+            // the wave that holds a target's logit leaves it to the loss, which then is not below 0, and to the gradient
+            const int y = target_of[col_in + j * 16] - wm * 128;
+            const bool here = y >= 0 && y < 128 && ((y >> 2) & 3) == (lane >> 4);
+            if (__ballot(here)) {
+                float logit = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) logit = (y & ~12) == i * 16 + r ? acc[i][j][r] : logit;
+                if (here) e.target_logit[n0 + col_in + j * 16] = logit;
+            }
             float most = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 8; i++)
@@ -742,7 +749,7 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
             const int y = e.row_target[n0 + tid] - e.first_class - m0;
             if (y >= 0 && y < min(kM, rows_a - m0)) {
                 place = y;
-                at_target = (exp2_fast(fmaf(e.target_logit[n0 + tid], kLog2e, -e.lse[n0 + tid])) - 1.f) * ldexpf(e.row_scale[n0 + tid], up);
+                at_target = (exp2_fast(e.target_logit[n0 + tid] - e.lse[n0 + tid]) - 1.f) * ldexpf(e.row_scale[n0 + tid], up);
             }
         }
 #pragma unroll 1
@@ -813,8 +820,9 @@ template <typename In> void launch_back(bool narrow, unsigned hidden, unsigned g
 // ---------------------------------------------------------------------------------------------------------- the rest
 
 // Statistics of the tiles joined: loss and log sum of a row.
+template <typename In>
 __global__ __launch_bounds__(64) void ce_finish(const Header* header, const float2* part, int tiles, int64_t rows_p, const int* row_frame,
-                                                 const int* row_target, const float* target_logit, int T, int F, float* lse, float* loss, int* report) {
+                                                 const int* row_target, const float* target_logit, const void* bias, int T, int F, float* lse, float* loss, int* report) {
     const int row = blockIdx.x * 64 + threadIdx.x;
     if (row >= header->rows) return;
     float most = -INFINITY, sum = 0.f;
@@ -837,7 +845,12 @@ __global__ __launch_bounds__(64) void ce_finish(const Header* header, const floa
     const int y = row_target[row], frame = row_frame[row];
     float v = 0.f;
     if (has_target(y, F)) {
-        v = l * kLn2 - target_logit[row];
+        const float logit = target_logit[row];
+        v = (l - logit) * kLn2;
+        if (logit == -INFINITY && bias) {      // a bias beside which the rest is nothing, and which is too large in units of log 2
+            const float b = static_cast<const In*>(bias)[y];
+            if (b * kLog2e == -INFINITY) v = l * kLn2 - b;
+        }
     } else if (y >= F) {
         v = __builtin_nanf("");
         if (report) {
@@ -1038,7 +1051,7 @@ int forward(const i6train_ce_problem& p, const Layout& l, float* loss, char* ws,
     Header* header = (Header*)(ws + l.header);
     int* offsets = (int*)(ws + l.offsets);
     ce_look<In><<<dim3(1 + 2 * kParts), dim3(kLookThreads), 0, s>>>(f, w, offsets, header);
-    const Packed o{(f16*)(ws + l.x), (f16*)(ws + l.w), (int*)(ws + l.row_frame), (int*)(ws + l.row_target), (float*)(ws + l.target_logit), loss};
+    const Packed o{(f16*)(ws + l.x), (f16*)(ws + l.w), (int*)(ws + l.row_frame), (int*)(ws + l.row_target), loss};
     ce_pack<In><<<dim3(groups_for(l.rows + kPad + l.weights_p)), dim3(kThreads), 0, s>>>(f, w, offsets, header, o);
     ProductArgs q{};
     q.a = {o.w, l.S * (int64_t)l.Kp, l.Kp, (int64_t)l.w_bytes, p.F, nullptr};
@@ -1046,14 +1059,15 @@ int forward(const i6train_ce_problem& p, const Layout& l, float* loss, char* ws,
     q.K = l.Kp; q.splits = 1;
     EpilogueArgs e{};
     e.bias = p.bias; e.header = header; e.part = (float2*)(ws + l.part); e.rows_p = l.rows_p;
+    e.row_target = o.row_target; e.target_logit = (float*)(ws + l.target_logit);
     // Large tiles need fewer bytes for a product, but one workgroup has the compute unit and nothing runs beside its end.  They are for long loops (bfloat16, 28800 frames,
     // F = 12001: D = 512 366 us with small tiles, 344 with large ones, D = 128 175, 197) whose tiles go round the compute units more than twice, or once where small ones do
     // not (D = 512, F = 5001: 2400 frames 37, 34 us; 3200 frames, 260 large tiles, 38, 48 us; in 32 bits 8000 frames 143, 135).
     const int64_t small = tiles_of<2>(p.F, l.rows), large = tiles_of<4>(p.F, l.rows);
     if (l.Kp * (S == 2 ? 3 : 1) >= 512 && (large > 512 || (small > 256 && large <= 256))) launch_product<In, kStatistics, 4>(q, e, p.F, l.rows, s);
     else launch_product<In, kStatistics, 2>(q, e, p.F, l.rows, s);
-    ce_finish<<<dim3(ceil_div(l.rows, (int64_t)64)), dim3(64), 0, s>>>(header, e.part, l.class_tiles, l.rows_p, o.row_frame, o.row_target, o.target_logit, p.T, p.F,
-                                                                         (float*)(ws + l.lse), loss, status_slot());
+    ce_finish<In><<<dim3(ceil_div(l.rows, (int64_t)64)), dim3(64), 0, s>>>(header, e.part, l.class_tiles, l.rows_p, o.row_frame, o.row_target, e.target_logit, p.bias, p.T, p.F,
+                                                                             (float*)(ws + l.lse), loss, status_slot());
     return launched();
 }
 
@@ -1079,7 +1093,7 @@ int backward(const i6train_ce_problem& p, const Layout& l, const float* grad_los
         q.K = l.Kp; q.splits = 1;
         EpilogueArgs e{};
         e.bias = p.bias; e.header = header; e.back = back; e.first_class = first;
-        e.row_target = row_target; e.target_logit = (const float*)(fw + l.target_logit); e.lse = (const float*)(fw + l.lse); e.row_scale = row_scale;
+        e.row_target = row_target; e.target_logit = (float*)(fw + l.target_logit); e.lse = (const float*)(fw + l.lse); e.row_scale = row_scale;
         e.g = g; e.g_stride = g_stride; e.g_half = l.piece;
         launch_product<In, kGradient, 2>(q, e, classes, l.rows, s);
         BothArgs h{}, v{};
