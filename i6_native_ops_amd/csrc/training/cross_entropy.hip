@@ -12,12 +12,21 @@
 // The frames of a batch are packed first: only frames that belong to a sequence are rows of the products, and what the others
 // hold is not read.  How many there are is known on the device alone: workgroups without a tile return at once.
 //
-// Operands.  All products have 16-bit floating-point operands with 11 bits of precision, and sums in 32 bits.  Tensors are scaled by a
-// power of two that brings their largest finite value to 2^14 .. 2^15.  bfloat16 values (8 bits) are then held exactly down to 2^-29 of the
-// largest, and G to 2^-12 of each value instead of the 2^-9 that bfloat16 would leave.  A 32-bit value x is split into x1 = f16(s x) and
-// x2 = f16(2^11 (s x - x1)): 22 bits.  Of (x1 + x2 2^-11)(y1 + y2 2^-11) the last term is below the precision and left out: the k-loop runs
-// over x1 y2 and x2 y1, scales the accumulators by 2^-11, and goes on with x1 y1: three times the work, on units whose rate for 16-bit operands
-// is sixteen times that for 32-bit ones.
+// Operands.  The matrix units take 16 bits fast, so every tensor has a form in 16-bit values, and sums are held in 32 bits.
+//
+//   bfloat16   Logits are formed from the values as they are, in instructions for bfloat16: no product is rounded and no value is too large or too small.  The
+//              gradients' products take 16-bit floating-point values with 11 bits, which hold G to 2^-12 of each value instead of the 2^-9 that bfloat16
+//              would leave, and W and h, times a power of two that brings the tensor's largest value to 2^14 .. 2^15, exactly down to 2^-29 of the largest.
+//   float      x is split into x1 = f16(s x) and x2 = f16(2^11 (s x - x1)), s such a power of two: 22 bits down to 2^-29 of the largest value, an error of 2^-51 of it
+//              below.  Of (x1 + x2 2^-11)(y1 + y2 2^-11) the last term is below the precision and left out: the k-loop runs over x1 y2 and x2 y1, scales the
+//              accumulators by 2^-11, and goes on with x1 y1: three times the work, on units whose rate for 16-bit operands is sixteen times that for 32-bit ones.
+//
+// One scale for a tensor is good where its rows are not too different: every row but those of zeros has a mean magnitude (G: an incoming gradient) that the forms
+// above hold well beside the tensor's largest value (kRows, kShares).  That is looked up on the device.  Where it is not so (frames or
+// classes millions of times larger than others, incoming gradients over many powers of ten), the same kernels take another way, `wide`: for bfloat16 the gradients' products
+// too are formed in bfloat16, with G rounded to it; for float the products are formed from the 32-bit values, in the matrix instructions that take
+// them: a sixteenth of the rate, and as precise as a plain product (a training step of 44 800 frames, F = 5001, D = 500: 3.0 ms, 9.7 where the gradients' products alone are
+// formed so, 15.6 where the logits are too).
 //
 // Logits are in units of log 2 from the accumulators on: exponentials and logarithms are single instructions.
 //
@@ -35,14 +44,22 @@ namespace {
 constexpr int kM = 256;              // rows of a workgroup's tile of C, and, per two waves of 128 x 64 each, 64 columns
 constexpr int kN = 128;              // its columns where the tile's logits are worked on
 constexpr int kThreads = 256;
-constexpr int kParts = 256;          // partial maxima of a tensor
+constexpr int kParts = 256;          // partial results of what looks over a tensor
+constexpr int kShareParts = 64;      // those over the incoming gradients, one for a lane of every wave that joins them
+constexpr int kPackGroups = 4096;    // at most, of ce_pack: in bfloat16 it looks over the tensors as well
 constexpr int kLookThreads = 1024;   // every wave waits for lengths, targets and rows in turn: many waves, few rows each
 constexpr int kPad = 64;             // rows and columns of operands are padded with zeros to multiples of this
 constexpr float kLow = 0x1p-11f;     // weight of the second half of a 32-bit value
+// The least mean magnitude of a row (and the least incoming gradient) that is not 0, over the tensor's largest value, of the fast forms; S: halves of a value.
+// What is below a value's last bit, 2^-51 of the largest (16 bits: 2^-40), is then 2^-25 (2^-20) of the row's mean, 2^-29 (2^-24) of the frame's share.
+template <int S> constexpr float kRows = S == 2 ? 0x1p-26f : 0x1p-20f;
+template <int S> constexpr float kShares = S == 2 ? 0x1p-22f : 0x1p-16f;
 
 using f16x2 = f16 __attribute__((ext_vector_type(2)));
 using f16x4 = f16 __attribute__((ext_vector_type(4)));
 using f16x8 = f16 __attribute__((ext_vector_type(8)));
+using bf16x4 = bf16 __attribute__((ext_vector_type(4)));
+using bf16x8 = bf16 __attribute__((ext_vector_type(8)));
 using s16x4 = short __attribute__((ext_vector_type(4)));
 using acc_t = float __attribute__((ext_vector_type(4)));
 using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
@@ -51,27 +68,50 @@ template <typename N, typename M> __host__ __device__ constexpr N round_up(N n, 
 
 // At the start of the forward workspace.
 struct Header {
-    int rows, unused[3];                                   // frames that belong to a sequence
-    alignas(16) uint32_t most_x[kParts], most_w[kParts];   // largest finite magnitudes, as bit patterns
+    int rows;                        // frames that belong to a sequence
+    int up_x, up_w;                  // in 32 bits: exponents of the scales of frames and weights,
+    int wide;                        // and whether their rows are too different for one
 };
 // At the start of the backward workspace.
 struct BackHeader {
-    alignas(16) uint32_t most_g[kParts];
+    int rows, up_x, up_w, wide_rows; // the same, in bfloat16 too
+    int up_g, wide;                  // of G; how the gradients' products are formed
+    alignas(16) uint32_t most[kShareParts], least[kShareParts];      // incoming gradients: partial results
 };
+// Partial results over a tensor, as bit patterns of magnitudes: the largest finite value, and the least mean of a row that is not 0.
+struct Parts {
+    uint32_t *most_x, *least_x, *most_w, *least_w;
+    int n;                           // of each
+};
+constexpr uint32_t kNone = 0x7f7fffffu;                    // no row
 
 __device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t umin(uint32_t a, uint32_t b) { return a < b ? a : b; }
 __device__ __forceinline__ uint32_t finite_bits(float x) {
     const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
     return b < 0x7f800000u ? b : 0u;
 }
+__device__ __forceinline__ uint32_t wave_min(uint32_t x) { return wave_reduce(x, 0xffffffffu, umin); }
 
-// The exponent of the power of two that brings a tensor's largest value to 2^14 .. 2^15, from its partial maxima: in every lane of a whole wave.
-__device__ __forceinline__ int scale_exponent(const uint32_t* parts) {
-    const u32x4 p = reinterpret_cast<const u32x4*>(parts)[threadIdx.x & 63];
-    const uint32_t most = wave_max(umax(umax(p.x, p.y), umax(p.z, p.w)));
-    if (most == 0) return 0;
-    const int k = 14 - ((int)(most >> 23) - 127);          // (subnormals: as 2^-127)
-    return k > 100 ? 100 : k;
+// The exponent of the power of two that brings a tensor's largest value to 2^14 .. 2^15, and whether that is good for all its rows, from
+// partial results: in every lane of a whole wave.
+struct Scale {
+    int up;
+    bool wide;
+};
+__device__ __forceinline__ Scale scale_of(const uint32_t* most_parts, const uint32_t* least_parts, int n, float range) {
+    uint32_t most = 0, least = kNone;
+#pragma unroll 4
+    for (int i = threadIdx.x & 63; i < n; i += 64) {
+        most = umax(most, most_parts[i]);
+        least = umin(least, least_parts[i]);
+    }
+    most = wave_max(most);
+    least = wave_min(least);
+    if (most == 0) return {0, false};
+    const int up = 14 - ((int)(most >> 23) - 127);
+    if (up > 100) return {100, true};                      // scales and their products are normal numbers
+    return {up, __uint_as_float(least) < __uint_as_float(most) * range};
 }
 
 __device__ __forceinline__ bool has_target(int y, int classes) { return y >= 0 && y < classes; }
@@ -109,13 +149,34 @@ template <typename In> __device__ __forceinline__ void load8(const In* row, int 
     for (int i = 0; i < 8; i++) v[i] = c + i < D ? (float)row[c + i] : 0.f;
 }
 
-// Workgroup 0: offsets[b], the first row of sequence b.  The next kParts: largest magnitudes of the frames with a target; the
-// last kParts: those of the weights.
+// What a wave has seen of a tensor.
+struct Seen {
+    uint32_t most = 0, least = kNone, row_most = 0;
+    float row_sum = 0.f;
+    __device__ __forceinline__ void values(const float (&v)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t b = finite_bits(v[i]);
+            row_most = umax(row_most, b);
+            row_sum += __uint_as_float(b);
+        }
+    }
+    __device__ __forceinline__ void end_row(float per_value) {       // by the whole wave
+        const float mean = wave_sum(row_sum) * per_value;
+        most = umax(most, row_most);
+        if (mean > 0.f) least = umin(least, __float_as_uint(mean));
+        row_most = 0;
+        row_sum = 0.f;
+    }
+};
+
+// Workgroup 0: offsets[b], the first row of sequence b.  In 32 bits also: the next kParts look over the frames with a target, the
+// last kParts over the weights.
 template <typename In>
-__global__ __launch_bounds__(kLookThreads) void ce_look(Frames f, Weights w, int* offsets, Header* header) {
+__global__ __launch_bounds__(kLookThreads) void ce_look(Frames f, Weights w, int* offsets, Header* header, Parts parts) {
     constexpr int kWaves = kLookThreads / kWave;
     __shared__ int sums[kWaves];
-    __shared__ uint32_t most_of[kWaves];
+    __shared__ uint32_t most_of[kWaves], least_of[kWaves];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (blockIdx.x == 0) {
         int carry = 0;
@@ -143,7 +204,8 @@ __global__ __launch_bounds__(kLookThreads) void ce_look(Frames f, Weights w, int
     const int part = (blockIdx.x - 1) % kParts;
     const In* base = static_cast<const In*>(weights ? w.p : f.hidden);
     const int64_t rows = weights ? f.F : (int64_t)f.B * f.T;
-    uint32_t most = 0;
+    const float per_value = 1.f / f.D;
+    Seen seen;
     for (int64_t r = (int64_t)part * kWaves + wave; r < rows; r += kParts * kWaves) {
         const In* row;
         if (weights) {
@@ -157,54 +219,77 @@ __global__ __launch_bounds__(kLookThreads) void ce_look(Frames f, Weights w, int
         for (int c = lane * 8; c < f.D; c += 512) {
             float v[8];
             load8(row, c, f.D, aligned, v);
-#pragma unroll
-            for (int i = 0; i < 8; i++) most = umax(most, finite_bits(v[i]));
+            seen.values(v);
         }
+        seen.end_row(per_value);
     }
-    most = wave_max(most);
-    if (lane == 0) most_of[wave] = most;
+    uint32_t most = wave_max(seen.most), least = seen.least;
+    if (lane == 0) {
+        most_of[wave] = most;
+        least_of[wave] = least;
+    }
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int i = 1; i < kWaves; i++) most = umax(most, most_of[i]);
-        (weights ? header->most_w : header->most_x)[part] = most;
+        for (int i = 1; i < kWaves; i++) {
+            most = umax(most, most_of[i]);
+            least = umin(least, least_of[i]);
+        }
+        (weights ? parts.most_w : parts.most_x)[part] = most;
+        (weights ? parts.least_w : parts.least_x)[part] = least;
     }
 }
 
-// x as one operand or as two halves.
+// A 32-bit value as two halves.
 __device__ __forceinline__ void split(float s, f16& high, f16& low) {
     high = (f16)s;
     low = fabsf(s) < 65504.f ? (f16)((s - (float)high) * 0x1p11f) : (f16)0.f;       // infinities and NaN are in the first half alone
 }
-template <int S> __device__ __forceinline__ void store_operand(f16* out, int Kp, int c, const float (&v)[8], int exponent) {
-    f16x8 high, low;
+template <typename In> __device__ __forceinline__ void store_operand(f16* out, int Kp, int c, const float (&v)[8], int up) {
+    if constexpr (sizeof(In) == 2) {
+        bf16x8 as_they_are;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float s = ldexpf(v[i], exponent);
-        if (S == 2) {
+        for (int i = 0; i < 8; i++) as_they_are[i] = (bf16)v[i];
+        *reinterpret_cast<bf16x8*>(out + c) = as_they_are;
+    } else {
+        f16x8 high, low;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
             f16 h, l;
-            split(s, h, l);
+            split(ldexpf(v[i], up), h, l);
             high[i] = h;
             low[i] = l;
-        } else {
-            high[i] = (f16)s;
         }
+        *reinterpret_cast<f16x8*>(out + c) = high;
+        *reinterpret_cast<f16x8*>(out + Kp + c) = low;
     }
-    *reinterpret_cast<f16x8*>(out + c) = high;
-    if (S == 2) *reinterpret_cast<f16x8*>(out + Kp + c) = low;
 }
 
 struct Packed {
-    f16 *x, *w;                      // [row][halves][Kp], zeros behind column D and in rows up to a multiple of kPad
+    f16 *x, *w;                      // [row][halves][Kp] (bfloat16: its values), zeros behind column D and in rows up to a multiple of kPad; in 32 bits not where `wide`
     int *row_frame, *row_target;
     float* loss;
 };
 
-// A wave per row: frames as operands, then weights.
+// A wave per row: frames as operands, then weights.  In bfloat16 it looks over them as well.
 template <typename In>
-__global__ __launch_bounds__(kThreads) void ce_pack(Frames f, Weights w, const int* offsets, const Header* header, Packed o) {
+__global__ __launch_bounds__(kThreads) void ce_pack(Frames f, Weights w, const int* offsets, Header* header, Parts parts, Packed o) {
     constexpr int S = sizeof(In) == 4 ? 2 : 1;
     const int lane = threadIdx.x & 63;
-    const int ex = scale_exponent(header->most_x), ew = scale_exponent(header->most_w);
+    int up_x = 0, up_w = 0;
+    bool store = true;
+    if constexpr (S == 2) {
+        const Scale x = scale_of(parts.most_x, parts.least_x, parts.n, kRows<S>), y = scale_of(parts.most_w, parts.least_w, parts.n, kRows<S>);
+        up_x = x.up;
+        up_w = y.up;
+        store = !(x.wide || y.wide);
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            header->up_x = up_x;
+            header->up_w = up_w;
+            header->wide = !store;
+        }
+    }
+    Seen frames_seen, weights_seen;
+    const float per_value = 1.f / f.D;
     const int64_t frames = (int64_t)f.B * f.T, n_weights = round_up(f.F, kPad), all = frames + kPad + n_weights;
     const int64_t row_size = S * (int64_t)f.Kp;
     const float none[8] = {};
@@ -213,17 +298,21 @@ __global__ __launch_bounds__(kThreads) void ce_pack(Frames f, Weights w, const i
             const int64_t row = r - frames - kPad;
             const In* x = static_cast<const In*>(w.p) + row * w.stride;
             const bool aligned = (uintptr_t)x % 16 == 0;
-            for (int c = lane * 8; c < f.Kp; c += 512) {
+            for (int c = lane * 8; c < f.Kp && store; c += 512) {
                 float v[8];
-                if (row < f.F) load8(x, c, f.D, aligned, v);
-                store_operand<S>(o.w + row * row_size, f.Kp, c, row < f.F ? v : none, ew);
+                if (row < f.F) {
+                    load8(x, c, f.D, aligned, v);
+                    if (S == 1) weights_seen.values(v);
+                }
+                store_operand<In>(o.w + row * row_size, f.Kp, c, row < f.F ? v : none, up_w);
             }
+            if (S == 1 && row < f.F) weights_seen.end_row(per_value);
             continue;
         }
         if (r >= frames) {
             const int64_t row = header->rows + (r - frames);
             if (row < round_up((int64_t)header->rows, kPad))
-                for (int c = lane * 8; c < f.Kp; c += 512) store_operand<S>(o.x + row * row_size, f.Kp, c, none, 0);
+                for (int c = lane * 8; c < f.Kp && store; c += 512) store_operand<In>(o.x + row * row_size, f.Kp, c, none, 0);
             continue;
         }
         const int b = (int)(r / f.T), t = (int)(r % f.T);
@@ -236,14 +325,31 @@ __global__ __launch_bounds__(kThreads) void ce_pack(Frames f, Weights w, const i
         const bool used = has_target(target, f.F);      // a frame without a target: zeros, whatever it holds
         const In* x = static_cast<const In*>(f.hidden) + b * f.stride_b + t * f.stride_t;
         const bool aligned = (uintptr_t)x % 16 == 0;
-        for (int c = lane * 8; c < f.Kp; c += 512) {
+        for (int c = lane * 8; c < f.Kp && store; c += 512) {
             float v[8];
-            if (used) load8(x, c, f.D, aligned, v);
-            store_operand<S>(o.x + row * row_size, f.Kp, c, used ? v : none, ex);
+            if (used) {
+                load8(x, c, f.D, aligned, v);
+                if (S == 1) frames_seen.values(v);
+            }
+            store_operand<In>(o.x + row * row_size, f.Kp, c, used ? v : none, up_x);
         }
+        if (S == 1 && used) frames_seen.end_row(per_value);
         if (lane == 0) {
             o.row_frame[row] = (int)r;
             o.row_target[row] = target;
+        }
+    }
+    if constexpr (S == 1) {
+        __shared__ uint32_t seen[4][4];
+        const uint32_t mine[4] = {wave_max(frames_seen.most), frames_seen.least, wave_max(weights_seen.most), weights_seen.least};
+        if (lane == 0)
+            for (int i = 0; i < 4; i++) seen[threadIdx.x >> 6][i] = mine[i];
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            parts.most_x[blockIdx.x] = umax(umax(seen[0][0], seen[1][0]), umax(seen[2][0], seen[3][0]));
+            parts.least_x[blockIdx.x] = umin(umin(seen[0][1], seen[1][1]), umin(seen[2][1], seen[3][1]));
+            parts.most_w[blockIdx.x] = umax(umax(seen[0][2], seen[1][2]), umax(seen[2][2], seen[3][2]));
+            parts.least_w[blockIdx.x] = umin(umin(seen[0][3], seen[1][3]), umin(seen[2][3], seen[3][3]));
         }
     }
 }
@@ -252,16 +358,16 @@ __global__ __launch_bounds__(kThreads) void ce_pack(Frames f, Weights w, const i
 
 struct Operand {
     const f16* p;
+    const f16* wide;          // bfloat16: the values as they are, laid out alike
     int64_t row_stride;       // elements between rows; a row has consecutive k, or consecutive m (n)
     int64_t half_stride;      // elements to the second halves
     int64_t bytes;            // of the buffer, from p on
-    int rows;                 // m (n) that there are
-    const int* n_rows;        // if that is known on the device alone
+    int rows;                 // m (n) that there are, or kFrames
 };
+constexpr int kFrames = -1;   // as many as there are frames, which is known on the device alone
 struct ProductArgs {
     Operand a, b;
-    int K;                    // of one half; a multiple of kPad
-    const int* n_k;           // K = *n_k rounded up to kPad, where it is known on the device alone
+    int K;                    // of one half; a multiple of kPad; or kFrames: rounded up to it
     int splits;               // ranges of k, one tile of C each
 };
 
@@ -270,8 +376,8 @@ enum Kind { kStatistics, kGradient, kHidden, kWeight };
 struct EpilogueArgs {
     // kStatistics, kGradient: m is the class, n the row
     const void* bias;
-    const Header* header;  const BackHeader* back;
-    int first_class;                       // of this piece
+    const Header* header;  BackHeader* back;
+    int first_class, piece_classes;        // of this piece
     const int* row_target;
     float2* part;                          // [tile of classes][rows_p]: maximum, sum
     int64_t rows_p;
@@ -284,6 +390,7 @@ struct EpilogueArgs {
     const int* row_frame;
     int classes;
     void* out;
+    Frames f;  Weights w;                  // the caller's tensors, for products of 32-bit values
     // kWeight: m is the class, n the feature; ranges of k one after another
     float* part_out;  int64_t part_stride;      // (the stride for kHidden as well)
     float* bias_out;  int64_t bias_stride; // [range][class], sums of G over the rows
@@ -337,10 +444,10 @@ template <int R, bool kConsecutiveK, int kWaves, int kK> struct Side {
         if (!kConsecutiveK) return ((i & 3) << 1) | (i & 8);
         return kK == 32 ? ((i >> 1) & 2) ^ ((i >> 3) & 1) * 3 : (i >> 1) & 7;
     }
-    __device__ __forceinline__ void set(const Operand& o, int rows, int first, int k0, int base_row) {
+    __device__ __forceinline__ void set(const Operand& o, bool wide, int rows, int first, int k0, int base_row) {
         const int lane = threadIdx.x & 63, wave = wave_index();
         const int64_t origin = kConsecutiveK ? first * o.row_stride + k0 : k0 * o.row_stride + first;
-        source = describe(o.p + origin, o.bytes - origin * 2);
+        source = describe((wide && o.wide ? o.wide : o.p) + origin, o.bytes - origin * 2);
         half = (uint32_t)(o.half_stride * 2);
         to = wave * 1024;
         step = kConsecutiveK ? kK * 2 : (uint32_t)(kK * o.row_stride * 2);
@@ -415,9 +522,69 @@ __device__ __forceinline__ void store_block(char* lds, const acc_t (&c)[4], floa
     }
 }
 
+// A wave's 128 x 64 of a product of 32-bit values, straight from memory: h and W from the caller's tensors, G as floats.  A matrix instruction
+// takes 4 k, one from each 16 lanes; lane l has k = 4 (l >> 4) + i of 16 in the i-th one.  Bound by the units for 32-bit operands.
+template <int KIND>
+__device__ __forceinline__ void product_of_floats(const ProductArgs& p, const EpilogueArgs& e, int rows, int rows_a, int rows_b, int m0, int n0, int k0, int end, bool with_bias,
+                                                  acc_t (&acc)[8][4], float (&bias_sum)[8]) {
+#if __HIP_DEVICE_COMPILE__
+    constexpr bool kLogits = KIND == kStatistics || KIND == kGradient;
+    const int lane = threadIdx.x & 63, k_in = (lane >> 4) * 4;
+    const float* w = static_cast<const float*>(e.w.p) + e.first_class * e.w.stride;
+    // a frame's features, and all bits of `there` off where it has no target: what such frames hold does not count
+    const auto frame_of = [&](int row, uint32_t& there) -> const float* {
+        there = has_target(e.row_target[row], e.f.F) ? there : 0u;
+        const int frame = e.row_frame[row];
+        return static_cast<const float*>(e.f.hidden) + frame / e.f.T * e.f.stride_b + frame % e.f.T * e.f.stride_t;
+    };
+    const float *a_row[8], *b_row[4];
+    uint32_t b_there[4] = {~0u, ~0u, ~0u, ~0u};
+    const auto masked = [](float v, uint32_t there) { return __uint_as_float(__float_as_uint(v) & there); };
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int m = min(m0 + i * 16 + (lane & 15), rows_a - 1);
+        a_row[i] = kLogits ? w + m * e.w.stride : reinterpret_cast<const float*>(p.a.p) + (KIND == kHidden ? m * (p.a.row_stride / 2) : m);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int n = min(n0 + j * 16 + (lane & 15), rows_b - 1);
+        b_row[j] = kLogits ? frame_of(n, b_there[j]) : w + n;
+    }
+    end = min(end, kLogits ? e.f.D : (KIND == kHidden ? e.piece_classes : rows));       // the k that there are
+#pragma unroll 1
+    for (int k = k0; k < end; k += 16) {
+        float a[8][4], b[4][4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            // loads of the last k instead of those behind it, and then zeros
+            const int at = min(k + k_in + c, end - 1);
+            uint32_t there = k + k_in + c < end ? ~0u : 0u;
+            const uint32_t a_there = there;
+            const float* x = KIND == kWeight ? frame_of(at, there) : nullptr;
+#pragma unroll
+            for (int i = 0; i < 8; i++) a[i][c] = masked(a_row[i][KIND == kWeight ? at * (p.a.row_stride / 2) : at], a_there);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float v = kLogits ? b_row[j][at] : (KIND == kHidden ? b_row[j][at * e.w.stride] : x[min(n0 + j * 16 + (lane & 15), rows_b - 1)]);
+                b[j][c] = masked(v, there & b_there[j]);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if (KIND == kWeight && with_bias) bias_sum[i] += a[i][c];
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][c], b[j][c], acc[i][j], 0, 0, 0);
+            }
+    }
+#endif
+}
+
 // In           type of the user's tensors: two halves where it has 32 bits
 // KIND         what becomes of a tile
 // NW           pairs of waves: a tile has 64 NW columns
+// kWide        the product is formed the other way: from 32-bit values, or from bfloat16 ones where it would be 16-bit floating-point ones of 11 bits
 // index        of the workgroup among those of this product
 template <typename In, int KIND, int NW> struct Shape {
     static constexpr int kWaves = 2 * NW, kCols = 64 * NW, kStages = NW == 2 ? 3 : 2, kK = NW == 2 ? 32 : 64;
@@ -426,8 +593,11 @@ template <typename In, int KIND, int NW> struct Shape {
     static constexpr int kBytes = kStages * kStageBytes + (kLogits ? kM * 4 : 0) + (KIND == kStatistics ? 5 * kCols * 4 : 0);
 };
 
-template <typename In, int KIND, int NW>
-__device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueArgs& e, char* lds, int index) {
+// kFloats      G leaves as floats
+// frames       how many there are
+// up, wide     kGradient: the exponent of its scale, and whether what takes it is formed the other way
+template <typename In, int KIND, int NW, bool kWide, bool kFloats = false>
+__device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueArgs& e, char* lds, int index, int frames, int up = 0, bool wide = false) {
 #if __HIP_DEVICE_COMPILE__
     constexpr int S = sizeof(In) == 4 ? 2 : 1;
     constexpr bool kAk = KIND != kWeight, kBk = KIND == kStatistics || KIND == kGradient;      // consecutive k
@@ -440,7 +610,7 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
     int* target_of = reinterpret_cast<int*>(join[4]);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), wm = wave & 1, wn = wave >> 1;
-    const int rows_a = p.a.n_rows ? *p.a.n_rows : p.a.rows, rows_b = p.b.n_rows ? *p.b.n_rows : p.b.rows;
+    const int rows_a = p.a.rows == kFrames ? frames : p.a.rows, rows_b = p.b.rows == kFrames ? frames : p.b.rows;
 
     // Workgroups go round the eight dies; each die has an L2 of its own, so it gets a range of tiles of its own, in groups of eight tiles of A:
     // the 64 tiles that a die works on at a time have 8 + 8 operand tiles among them, not 64 + 1.
@@ -455,7 +625,7 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
     const int tile_m = group * 8 + tile % in_group, tile_n = tile / in_group;
     const int m0 = tile_m * kM, n0 = tile_n * kCols;
 
-    int K = p.n_k ? round_up(*p.n_k, kPad) : p.K;
+    int K = p.K == kFrames ? round_up(frames, kPad) : p.K;
     int k0 = 0;
     if (p.splits > 1) {
         const int range = ceil_div(ceil_div(K, kK), p.splits) * kK;
@@ -464,30 +634,21 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
     }
     const int steps = (K - k0) / kK, all = S == 2 ? 3 * steps : steps;
 
-    int up = 0, down = 0;      // what the tensors' scales come to
-    if constexpr (kLogits) down = scale_exponent(e.header->most_x) + scale_exponent(e.header->most_w);
-    if constexpr (KIND == kGradient) up = scale_exponent(e.back->most_g);
     Side<kM, kAk, kWaves, kK> A;
     Side<kCols, kBk, kWaves, kK> B;
-    A.set(p.a, rows_a, m0, k0, wm * 128);
-    B.set(p.b, rows_b, n0, k0, wn * 64);
-    if (kLogits && tid < kM) {
-        const int m = m0 + tid;       // classes behind the last: -inf, no probability
-        float v = m < rows_a ? 0.f : -INFINITY;
-        if (e.bias && m < rows_a) v = (float)static_cast<const In*>(e.bias)[e.first_class + m] * kLog2e;
-        bias[tid] = v;
-    }
-    if (KIND == kStatistics && tid < kCols) {
-        const int y = n0 + tid < rows_b ? e.row_target[n0 + tid] : -1;
-        target_of[tid] = has_target(y, rows_a) ? y - m0 : -1;
-    }
+    A.set(p.a, kWide, rows_a, m0, k0, wm * 128);
+    B.set(p.b, kWide, rows_b, n0, k0, wn * 64);
+    float bias_in = -INFINITY;        // classes behind the last: -inf, no probability
+    if (kLogits && tid < kM && m0 + tid < rows_a) bias_in = e.bias ? (float)static_cast<const In*>(e.bias)[e.first_class + m0 + tid] : 0.f;
+    int target_in = -1;
+    if (KIND == kStatistics && tid < kCols && n0 + tid < rows_b) target_in = e.row_target[n0 + tid];
 
     // register r of a 16 x 16 block: row 4 (lane >> 4) + r, column lane & 15
     const int row_in = wm * 128 + 4 * (lane >> 4), col_in = wn * 64 + (lane & 15);
     acc_t acc[8][4];
     if (KIND == kHidden && e.add) {
         const float* sum = e.sum + part_of_k * e.part_stride + (int64_t)m0 * e.sum_stride + n0;
-        const float scaled = S == 2 && all > 0 ? 1.f / kLow : 1.f;       // taken back on the way, below
+        const float scaled = S == 2 && all > 0 && !kWide ? 1.f / kLow : 1.f;       // taken back on the way, below
 #pragma unroll
         for (int i = 0; i < 8; i++)
 #pragma unroll
@@ -538,7 +699,7 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
     // those are read the waves meet: this stage is in registers and its LDS free for another one, and the next stage has come in.
     // Reads and loads are spread over the products: issued all at once, the loads of eight waves fill the queue of the compute unit, and no product starts
     // until they have gone through.  A fragment of A is read when the one two before it has been used: registers for ten, not sixteen.
-    const auto part_of_stage = [&](auto set, auto last) {
+    const auto part_of_stage = [&](auto set, auto last, auto in_bf16) {
         constexpr int kSet = set.value;
         constexpr bool kLast = last.value;
         const std::integral_constant<int, 1 - kSet> other{};
@@ -556,12 +717,15 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
 #pragma unroll
             for (int i = 0; i < 8; i++)
 #pragma unroll
-                for (int r = 0; r < 8; r++) bias_sum[i] += (float)fa[kSet][i][r];
+                for (int r = 0; r < 8; r++) bias_sum[i] += in_bf16.value ? (float)__builtin_bit_cast(bf16x8, fa[kSet][i])[r] : (float)fa[kSet][i][r];
         }
         constexpr int kReadAt[12] = {0, 2, 4, 6, 8, 10, 12, 14, 16, 18, 20, 24};
 #pragma unroll
         for (int n = 0; n < 32; n++) {
-            acc[n >> 2][n & 3] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[kSet][n >> 2], fb[kSet][n & 3], acc[n >> 2][n & 3], 0, 0, 0);
+            if constexpr (in_bf16.value)
+                acc[n >> 2][n & 3] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fa[kSet][n >> 2]), __builtin_bit_cast(bf16x8, fb[kSet][n & 3]), acc[n >> 2][n & 3], 0, 0, 0);
+            else
+                acc[n >> 2][n & 3] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[kSet][n >> 2], fb[kSet][n & 3], acc[n >> 2][n & 3], 0, 0, 0);
 #pragma unroll
             for (int i = 0; i < 12; i++)
                 if (kReadAt[i] == n) read(other, i, at, kLast ? 0 : 1);         // behind the last stage: what is there, and not used
@@ -579,7 +743,7 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
             }
         }
     };
-    if (all > 0) {
+    const auto run = [&](auto in_bf16) {
 #pragma unroll
         for (int n = 0; n < kStages; n++) {
             if (n >= all) break;
@@ -596,14 +760,18 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
         __builtin_amdgcn_s_setprio(1);
         for (; it < all; it++) {
             scale();
-            part_of_stage(first, std::bool_constant<kK == 32>{});
+            part_of_stage(first, std::bool_constant<kK == 32>{}, in_bf16);
             if constexpr (kK == 32) {
                 if (++it == all) break;
                 scale();
             }
-            part_of_stage(second, std::true_type{});
+            part_of_stage(second, std::true_type{}, in_bf16);
         }
         __builtin_amdgcn_s_setprio(0);
+    };
+    if (all > 0) {
+        if constexpr (S == 2 && kWide) product_of_floats<KIND>(p, e, frames, rows_a, rows_b, m0 + wm * 128, n0 + wn * 64, k0, K, with_bias, acc, bias_sum);
+        else run(std::bool_constant<S == 1 && (kLogits || kWide)>{});
     }
 
     if constexpr (KIND == kWeight) {
@@ -646,7 +814,7 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
             const int m = m0 + i;
             frames[i] = m < rows_a ? (e.row_target[m] >= e.classes ? ~e.row_frame[m] : e.row_frame[m]) : 0;
         }
-        const float unscale = ldexpf(1.f, -scale_exponent(e.back->most_g)), unscale_w = ldexpf(1.f, -scale_exponent(e.header->most_w));
+        const float unscale = ldexpf(1.f, -e.back->up_g), unscale_w = kWide ? 1.f : ldexpf(1.f, -e.back->up_w);
         __syncthreads();
         In* out = static_cast<In*>(e.out) + n0 + wn * 64;
         const bool whole = rows_b % (16 / (int)sizeof(In)) == 0;
@@ -663,7 +831,9 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
         return;
     }
 
-    const float per = fminf(ldexpf(kLog2e, -down), 0x1p127f);
+    if (tid < kM) bias[tid] = bias_in * kLog2e;
+    if (KIND == kStatistics && tid < kCols) target_of[tid] = has_target(target_in, rows_a) ? target_in - m0 : -1;
+    const float per = S == 1 || kWide ? kLog2e : fminf(ldexpf(kLog2e, -(e.header->up_x + e.header->up_w)), 0x1p127f);
     __syncthreads();
     // logits in units of log 2
 #pragma unroll
@@ -721,6 +891,28 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
     }
 
     if constexpr (KIND == kGradient) {
+        const auto target_of_row = [&](int n) { return (exp2_fast(e.target_logit[n] - e.lse[n]) - 1.f) * ldexpf(e.row_scale[n], up); };
+        if constexpr (kFloats) {
+            // four classes from each lane, a column at a time
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int n = n0 + col_in + j * 16, at = min(n, rows_b - 1);
+                const float lse = n < rows_b ? e.lse[at] : INFINITY, scale = n < rows_b ? e.row_scale[at] : 0.f;
+                const int y = e.row_target[at] - e.first_class - m0 - row_in;
+                const bool there = n < rows_b && y >= 0 && y < rows_a - m0 - row_in;
+                const float value = there ? target_of_row(at) : 0.f;
+                float* g = reinterpret_cast<float*>(e.g) + n * (e.g_stride / 2) + m0 + row_in;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    acc_t v;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) v[r] = there && y == i * 16 + r ? value : exp2_fast(acc[i][j][r] - lse) * scale;
+                    *reinterpret_cast<acc_t*>(g + i * 16) = v;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int n = n0 + col_in + j * 16;
@@ -749,7 +941,7 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
             const int y = e.row_target[n0 + tid] - e.first_class - m0;
             if (y >= 0 && y < min(kM, rows_a - m0)) {
                 place = y;
-                at_target = (exp2_fast(e.target_logit[n0 + tid] - e.lse[n0 + tid]) - 1.f) * ldexpf(e.row_scale[n0 + tid], up);
+                at_target = target_of_row(n0 + tid);
             }
         }
 #pragma unroll 1
@@ -767,6 +959,11 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
                         for (int r = 0; r < 2; r++)
                             pair[r] = __builtin_amdgcn_perm(__float_as_uint(acc[i][j][2 * r + 1]), __float_as_uint(acc[i][j][2 * r]), which);
                         v = __builtin_bit_cast(f16x4, pair);
+                    } else if (wide) {
+                        bf16x4 u;
+#pragma unroll
+                        for (int r = 0; r < 4; r++) u[r] = (bf16)acc[i][j][r];
+                        v = __builtin_bit_cast(f16x4, u);
                     } else {
 #pragma unroll
                         for (int r = 0; r < 4; r++) v[r] = (f16)acc[i][j][r];
@@ -777,6 +974,7 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
             if (place >= 0) {
                 f16 high, low;
                 split(at_target, high, low);
+                if (S == 1 && wide) high = __builtin_bit_cast(f16, (bf16)at_target);
                 *reinterpret_cast<f16*>(lds + tid * kGStride + place * 2) = h == 0 ? high : low;
             }
             __syncthreads();
@@ -795,7 +993,26 @@ __device__ __forceinline__ void product_of(const ProductArgs& p, const EpilogueA
 template <typename In, int KIND, int NW>
 __global__ __launch_bounds__(128 * NW, 2) void product(ProductArgs p, EpilogueArgs e) {
     __shared__ alignas(16) char lds[Shape<In, KIND, NW>::kBytes];
-    product_of<In, KIND, NW>(p, e, lds, blockIdx.x);
+#if __HIP_DEVICE_COMPILE__
+    constexpr bool kHalves = sizeof(In) == 4;
+    const int index = blockIdx.x, frames = e.header->rows, wide_rows = e.header->wide;
+    if constexpr (KIND == kGradient) {
+        const Scale g = scale_of(e.back->most, e.back->least, kShareParts, kShares<kHalves ? 2 : 1>);
+        const bool wide = g.wide || (kHalves ? wide_rows : e.back->wide_rows);
+        const int up = wide ? 0 : g.up;
+        if (index == 0 && threadIdx.x == 0) {
+            e.back->up_g = up;
+            e.back->wide = wide;
+        }
+        if constexpr (!kHalves) product_of<In, KIND, NW, false>(p, e, lds, index, frames, up, wide);
+        else if (wide_rows) product_of<In, KIND, NW, true, true>(p, e, lds, index, frames, up);
+        else if (wide) product_of<In, KIND, NW, false, true>(p, e, lds, index, frames, up);
+        else product_of<In, KIND, NW, false>(p, e, lds, index, frames, up);
+    } else {
+        if (kHalves && wide_rows) product_of<In, KIND, NW, kHalves>(p, e, lds, index, frames);
+        else product_of<In, KIND, NW, false>(p, e, lds, index, frames);
+    }
+#endif
 }
 
 // dh and dW of a piece in one launch, the first `hidden` workgroups (a multiple of eight) for dh: neither needs the other, and where dh leaves compute
@@ -805,25 +1022,47 @@ struct BothArgs {
     EpilogueArgs e;
 };
 template <typename In, int NW>
-__global__ __launch_bounds__(128 * NW, 2) void products_back(BothArgs h, BothArgs w, int hidden) {
+__global__ __launch_bounds__(128 * NW, 2) void products_back(BothArgs h, BothArgs w, int hidden, const BackHeader* back) {
     static_assert(Shape<In, kHidden, NW>::kBytes == Shape<In, kWeight, NW>::kBytes);
     __shared__ alignas(16) char lds[Shape<In, kHidden, NW>::kBytes];
-    if ((int)blockIdx.x < hidden) product_of<In, kHidden, NW>(h.p, h.e, lds, blockIdx.x);
-    else product_of<In, kWeight, NW>(w.p, w.e, lds, blockIdx.x - hidden);
+    const int index = blockIdx.x, frames = back->rows;
+    if (back->wide) {
+        if (index < hidden) product_of<In, kHidden, NW, true>(h.p, h.e, lds, index, frames);
+        else product_of<In, kWeight, NW, true>(w.p, w.e, lds, index - hidden, frames);
+    } else {
+        if (index < hidden) product_of<In, kHidden, NW, false>(h.p, h.e, lds, index, frames);
+        else product_of<In, kWeight, NW, false>(w.p, w.e, lds, index - hidden, frames);
+    }
 }
-template <typename In> void launch_back(bool narrow, unsigned hidden, unsigned groups, const BothArgs& h, const BothArgs& w, hipStream_t s) {
+template <typename In> void launch_back(bool narrow, unsigned hidden, unsigned groups, const BothArgs& h, const BothArgs& w, const BackHeader* back, hipStream_t s) {
     if (groups == 0) return;
-    if (narrow) products_back<In, 2><<<dim3(groups), dim3(256), 0, s>>>(h, w, (int)hidden);
-    else products_back<In, 4><<<dim3(groups), dim3(512), 0, s>>>(h, w, (int)hidden);
+    if (narrow) products_back<In, 2><<<dim3(groups), dim3(256), 0, s>>>(h, w, (int)hidden, back);
+    else products_back<In, 4><<<dim3(groups), dim3(512), 0, s>>>(h, w, (int)hidden, back);
 }
 
 // ---------------------------------------------------------------------------------------------------------- the rest
 
-// Statistics of the tiles joined: loss and log sum of a row.
+// Statistics of the tiles joined: loss and log sum of a row.  In bfloat16 the last workgroups join 256 each of what ce_pack's have seen, for the backward pass.
 template <typename In>
-__global__ __launch_bounds__(64) void ce_finish(const Header* header, const float2* part, int tiles, int64_t rows_p, const int* row_frame,
+__global__ __launch_bounds__(64) void ce_finish(const Header* header, Parts seen, Parts joined, const float2* part, int tiles, int64_t rows_p, const int* row_frame,
                                                  const int* row_target, const float* target_logit, const void* bias, int T, int F, float* lse, float* loss, int* report) {
     const int row = blockIdx.x * 64 + threadIdx.x;
+    const int group = (int)blockIdx.x - (int)(gridDim.x - joined.n);
+    if (group >= 0) {
+        const int i = group * 256 + threadIdx.x * 4;
+        const bool there = i < seen.n;
+        const auto join = [&](const uint32_t* from, uint32_t* to, uint32_t none, auto better, auto of_wave) {
+            u32x4 v = none;
+            if (there) v = *reinterpret_cast<const u32x4*>(from + i);
+            const uint32_t best = of_wave(better(better(v.x, v.y), better(v.z, v.w)));
+            if (threadIdx.x == 0) to[group] = best;
+        };
+        join(seen.most_x, joined.most_x, 0u, umax, [](uint32_t v) { return wave_max(v); });
+        join(seen.least_x, joined.least_x, kNone, umin, [](uint32_t v) { return wave_min(v); });
+        join(seen.most_w, joined.most_w, 0u, umax, [](uint32_t v) { return wave_max(v); });
+        join(seen.least_w, joined.least_w, kNone, umin, [](uint32_t v) { return wave_min(v); });
+        return;
+    }
     if (row >= header->rows) return;
     float most = -INFINITY, sum = 0.f;
     for (int i = 0; i < tiles; i += 8) {
@@ -861,44 +1100,99 @@ __global__ __launch_bounds__(64) void ce_finish(const Header* header, const floa
     loss[frame] = v;
 }
 
-// The first kParts workgroups: the incoming gradient of each row; rows without a target, or with one that is out of range, have none.  The
-// others: zeros in the frames behind the ends.
+// Of bfloat16 values: as 16-bit floating-point values of 11 bits, scaled.  Null: not needed.
+struct Copies {
+    const bf16 *x, *w;
+    f16 *x_out, *w_out;
+    int64_t w_values;
+};
+
+// The first kShareParts workgroups: the incoming gradient of each row; rows without a target, or with one that is out of range, have none.  The
+// next ones: zeros in the frames behind the ends.  The others, in bfloat16: copies of the operands.
 template <typename Out>
 __global__ __launch_bounds__(256) void ce_row_scale(const Header* header, const int* row_frame, const int* row_target, const float* grad_loss, int64_t stride_b,
-                                                    int64_t stride_t, Frames f, float* row_scale, BackHeader* back, Out* grad_hidden) {
+                                                    int64_t stride_t, Frames f, Parts joined, Copies copies, int zeros, float* row_scale, BackHeader* back, Out* grad_hidden) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (blockIdx.x >= kParts) {
+    const int helper = (int)blockIdx.x - kShareParts;
+    if (helper >= 0 && helper < zeros) {
         const int64_t frames = (int64_t)f.B * f.T;
-        for (int64_t r = (int64_t)(blockIdx.x - kParts) * 4 + wave; r < frames; r += (int64_t)(gridDim.x - kParts) * 4) {
+        for (int64_t r = (int64_t)helper * 4 + wave; r < frames; r += (int64_t)zeros * 4) {
             const int b = (int)(r / f.T), t = (int)(r % f.T);
             if (t < f.lens[b]) continue;
             for (int d = lane; d < f.D; d += 64) grad_hidden[r * f.D + d] = (Out)0.f;
         }
         return;
     }
-    __shared__ uint32_t most_of[4];
-    uint32_t most = 0;
-    for (int row = blockIdx.x * 256 + threadIdx.x; row < header->rows; row += kParts * 256) {
+    const bool first_group = blockIdx.x == 0, copier = helper >= 0;
+    const int rows = header->rows;
+    // copies: what a thread reads first is on its way while the scales are looked up
+    const int64_t start = (int64_t)(helper - zeros) * 2048 + threadIdx.x * 8, stride = (int64_t)((int)gridDim.x - kShareParts - zeros) * 2048;
+    const int64_t w_end = copies.w_out ? copies.w_values : 0, x_end = copies.x_out ? round_up((int64_t)rows, kPad) * f.Kp : 0;
+    bf16x8 w_first, x_first;
+    if (copier && start < w_end) w_first = *reinterpret_cast<const bf16x8*>(copies.w + start);
+    if (copier && start < x_end) x_first = *reinterpret_cast<const bf16x8*>(copies.x + start);
+    int up_x = header->up_x, up_w = header->up_w;
+    bool wide = header->wide;
+    if (sizeof(Out) == 2 && (copier || first_group)) {
+        const Scale x = scale_of(joined.most_x, joined.least_x, joined.n, kRows<1>), w = scale_of(joined.most_w, joined.least_w, joined.n, kRows<1>);
+        up_x = x.up;
+        up_w = w.up;
+        wide = x.wide || w.wide;
+    }
+    if (first_group && threadIdx.x == 0) {
+        back->rows = rows;
+        back->up_x = up_x;
+        back->up_w = up_w;
+        back->wide_rows = wide;
+    }
+    if (copier) {
+        const auto copy = [&](const bf16* from, f16* to, int64_t end, bf16x8 v, int up) {
+            for (int64_t i = start; i < end; i += stride) {
+                if (i != start) v = *reinterpret_cast<const bf16x8*>(from + i);
+                f16x8 u;
+#pragma unroll
+                for (int k = 0; k < 8; k++) u[k] = (f16)ldexpf((float)v[k], up);
+                *reinterpret_cast<f16x8*>(to + i) = u;
+            }
+        };
+        if (!wide) {
+            copy(copies.w, copies.w_out, w_end, w_first, up_w);
+            copy(copies.x, copies.x_out, x_end, x_first, up_x);
+        }
+        return;
+    }
+    __shared__ uint32_t most_of[4], least_of[4];
+    uint32_t most = 0, least = kNone;
+    for (int row = blockIdx.x * 256 + threadIdx.x; row < rows; row += kShareParts * 256) {
         float g = 0.f;
         const int frame = row_frame[row];
         if (has_target(row_target[row], f.F)) g = grad_loss[(int64_t)(frame / f.T) * stride_b + (int64_t)(frame % f.T) * stride_t];
         row_scale[row] = g;
-        most = umax(most, finite_bits(g));
+        const uint32_t size = finite_bits(g);
+        most = umax(most, size);
+        if (size) least = umin(least, size);
     }
     most = wave_max(most);
-    if (lane == 0) most_of[wave] = most;
+    least = wave_min(least);
+    if (lane == 0) {
+        most_of[wave] = most;
+        least_of[wave] = least;
+    }
     __syncthreads();
-    if (threadIdx.x == 0) back->most_g[blockIdx.x] = umax(umax(most_of[0], most_of[1]), umax(most_of[2], most_of[3]));
+    if (threadIdx.x == 0) {
+        back->most[blockIdx.x] = umax(umax(most_of[0], most_of[1]), umax(most_of[2], most_of[3]));
+        back->least[blockIdx.x] = umin(umin(least_of[0], least_of[1]), umin(least_of[2], least_of[3]));
+    }
 }
 
 // One piece of grad_weight and grad_bias: the ranges of k joined, scales off.  A workgroup has 256 values, a quarter of the ranges for each wave.
 template <typename Out>
-__global__ __launch_bounds__(256) void ce_store_weight(const Header* header, const BackHeader* back, const float* part, int splits, int64_t split_stride, int64_t n, Out* out,
+__global__ __launch_bounds__(256) void ce_store_weight(const BackHeader* back, const float* part, int splits, int64_t split_stride, int64_t n, Out* out,
                                                        const float* bias_part, int64_t bias_stride, int classes, Out* bias) {
     using V = float __attribute__((ext_vector_type(4)));
     __shared__ V sums[4][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const float down = ldexpf(1.f, -scale_exponent(back->most_g)), down_x = ldexpf(1.f, -scale_exponent(header->most_x));
+    const float down = ldexpf(1.f, -back->up_g), down_x = back->wide ? 1.f : ldexpf(1.f, -back->up_x);
     const int64_t groups = ceil_div(n, (int64_t)256);
     const bool of_bias = blockIdx.x >= groups;            // the last workgroups
     const int64_t i = (of_bias ? blockIdx.x - groups : blockIdx.x) * 256 + lane * 4, all = of_bias ? classes : n, stride = of_bias ? bias_stride : split_stride;
@@ -929,7 +1223,7 @@ __global__ __launch_bounds__(256) void ce_store_hidden(const Header* header, con
                                                        const int* row_target, int F, int D, Out* out) {
     __shared__ float sums[4][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const float down = ldexpf(1.f, -scale_exponent(back->most_g)), down_w = ldexpf(1.f, -scale_exponent(header->most_w));
+    const float down = ldexpf(1.f, -back->up_g), down_w = back->wide ? 1.f : ldexpf(1.f, -back->up_w);
     const int64_t first = (int64_t)blockIdx.x * 256, all = (int64_t)header->rows * D;
     if (first >= all) return;
 #pragma unroll
@@ -961,13 +1255,16 @@ struct Layout {
     int S, Kp, row_tiles, class_tiles, piece, splits, hidden_splits;
     bool narrow;
     int64_t rows, rows_p, weights_p;
-    size_t header, offsets, row_frame, row_target, target_logit, lse, x, w, part, x_bytes, w_bytes, forward;
-    size_t back, row_scale, g, dx, dw, db, g_bytes, backward;
+    size_t header, seen, joined, offsets, row_frame, row_target, target_logit, lse, x, w, part, x_bytes, w_bytes, forward;
+    size_t back, row_scale, x_copy, w_copy, g, dx, dw, db, g_bytes, backward;
+    int pack_groups, parts, joins;
 };
 
 bool valid(const i6train_ce_problem* p) {
     return p && p->B > 0 && p->T > 0 && p->F > 0 && p->D > 0 && valid_dtype(p->dtype) && p->weight && p->targets && p->seq_lens;
 }
+
+int groups_for(int64_t rows) { return (int)(rows < 4 * kPackGroups ? round_up(ceil_div(rows, (int64_t)4), 4) : kPackGroups); }
 
 int layout(const i6train_ce_problem& p, Layout& l) {
     l.rows = (int64_t)p.B * p.T;
@@ -981,6 +1278,11 @@ int layout(const i6train_ce_problem& p, Layout& l) {
     size_t at = 0;
     const auto take = [&](size_t bytes) { const size_t here = at; at += align256(bytes); return here; };
     l.header = take(sizeof(Header));
+    l.pack_groups = groups_for(l.rows + kPad + l.weights_p);
+    l.parts = l.S == 2 ? kParts : round_up(l.pack_groups, 4);
+    l.joins = l.S == 2 ? 0 : ceil_div(l.parts, 256);
+    l.seen = take(4 * sizeof(uint32_t) * l.parts);
+    l.joined = take(4 * sizeof(uint32_t) * kPackGroups / 256);
     l.offsets = take(4 * (size_t)p.B);
     l.row_frame = take(4 * l.rows_p);
     l.row_target = take(4 * l.rows_p);
@@ -1012,6 +1314,8 @@ int layout(const i6train_ce_problem& p, Layout& l) {
     l.splits = (int)(splits < least ? least : splits);      // offsets within a range of k have 32 bits
     l.back = take(sizeof(BackHeader));
     l.row_scale = take(4 * l.rows_p);
+    l.x_copy = take(l.S == 1 ? l.x_bytes : 0);
+    l.w_copy = take(l.S == 1 ? l.w_bytes : 0);
     l.g_bytes = (size_t)l.rows_p * l.S * l.piece * 2;
     l.g = take(l.g_bytes);
     // Few rows: the sums over the classes are formed in ranges, or a handful of workgroups would go through the whole vocabulary (100 frames, F = 8346, D = 64, float: 69 us
@@ -1028,8 +1332,6 @@ int layout(const i6train_ce_problem& p, Layout& l) {
     return I6TRAIN_OK;
 }
 
-int groups_for(int64_t rows) { return (int)(rows < 16384 ? ceil_div(rows, (int64_t)4) : 4096); }
-
 Frames frames_of(const i6train_ce_problem& p, const Layout& l) {
     return {p.hidden, p.hidden_stride_b, p.hidden_stride_t, p.seq_lens, p.targets, p.targets_stride_b, p.targets_stride_t, p.B, p.T, p.F, p.D, l.Kp};
 }
@@ -1043,6 +1345,11 @@ template <typename In, int KIND, int NW> void launch_product(const ProductArgs& 
     product<In, KIND, NW><<<dim3(groups_of<NW>(q, rows_a, rows_b)), dim3(128 * NW), 0, s>>>(q, e);
 }
 
+Parts parts_at(const char* ws, int n, int room) {
+    uint32_t* at = (uint32_t*)ws;
+    return {at, at + room, at + 2 * room, at + 3 * room, n};
+}
+
 template <typename In>
 int forward(const i6train_ce_problem& p, const Layout& l, float* loss, char* ws, hipStream_t s) {
     constexpr int S = sizeof(In) == 4 ? 2 : 1;
@@ -1050,23 +1357,25 @@ int forward(const i6train_ce_problem& p, const Layout& l, float* loss, char* ws,
     const Weights w{p.weight, p.weight_stride_f, p.bias};
     Header* header = (Header*)(ws + l.header);
     int* offsets = (int*)(ws + l.offsets);
-    ce_look<In><<<dim3(1 + 2 * kParts), dim3(kLookThreads), 0, s>>>(f, w, offsets, header);
+    const Parts parts = parts_at(ws + l.seen, l.parts, l.parts), joined = parts_at(ws + l.joined, l.joins, kPackGroups / 256);
+    ce_look<In><<<dim3(S == 2 ? 1 + 2 * kParts : 1), dim3(kLookThreads), 0, s>>>(f, w, offsets, header, parts);
     const Packed o{(f16*)(ws + l.x), (f16*)(ws + l.w), (int*)(ws + l.row_frame), (int*)(ws + l.row_target), loss};
-    ce_pack<In><<<dim3(groups_for(l.rows + kPad + l.weights_p)), dim3(kThreads), 0, s>>>(f, w, offsets, header, o);
+    ce_pack<In><<<dim3(l.pack_groups), dim3(kThreads), 0, s>>>(f, w, offsets, header, parts, o);
     ProductArgs q{};
-    q.a = {o.w, l.S * (int64_t)l.Kp, l.Kp, (int64_t)l.w_bytes, p.F, nullptr};
-    q.b = {o.x, l.S * (int64_t)l.Kp, l.Kp, (int64_t)l.x_bytes, 0, &header->rows};
+    q.a = {o.w, nullptr, l.S * (int64_t)l.Kp, l.Kp, (int64_t)l.w_bytes, p.F};
+    q.b = {o.x, nullptr, l.S * (int64_t)l.Kp, l.Kp, (int64_t)l.x_bytes, kFrames};
     q.K = l.Kp; q.splits = 1;
     EpilogueArgs e{};
     e.bias = p.bias; e.header = header; e.part = (float2*)(ws + l.part); e.rows_p = l.rows_p;
-    e.row_target = o.row_target; e.target_logit = (float*)(ws + l.target_logit);
+    e.row_target = o.row_target; e.row_frame = o.row_frame; e.target_logit = (float*)(ws + l.target_logit);
+    e.f = f; e.w = w;
     // Large tiles need fewer bytes for a product, but one workgroup has the compute unit and nothing runs beside its end.  They are for long loops (bfloat16, 28800 frames,
     // F = 12001: D = 512 366 us with small tiles, 344 with large ones, D = 128 175, 197) whose tiles go round the compute units more than twice, or once where small ones do
     // not (D = 512, F = 5001: 2400 frames 37, 34 us; 3200 frames, 260 large tiles, 38, 48 us; in 32 bits 8000 frames 143, 135).
     const int64_t small = tiles_of<2>(p.F, l.rows), large = tiles_of<4>(p.F, l.rows);
     if (l.Kp * (S == 2 ? 3 : 1) >= 512 && (large > 512 || (small > 256 && large <= 256))) launch_product<In, kStatistics, 4>(q, e, p.F, l.rows, s);
     else launch_product<In, kStatistics, 2>(q, e, p.F, l.rows, s);
-    ce_finish<In><<<dim3(ceil_div(l.rows, (int64_t)64)), dim3(64), 0, s>>>(header, e.part, l.class_tiles, l.rows_p, o.row_frame, o.row_target, e.target_logit, p.bias, p.T, p.F,
+    ce_finish<In><<<dim3(ceil_div(l.rows, (int64_t)64) + l.joins), dim3(64), 0, s>>>(header, parts, joined, e.part, l.class_tiles, l.rows_p, o.row_frame, o.row_target, e.target_logit, p.bias, p.T, p.F,
                                                                              (float*)(ws + l.lse), loss, status_slot());
     return launched();
 }
@@ -1083,51 +1392,65 @@ int backward(const i6train_ce_problem& p, const Layout& l, const float* grad_los
     float *dx = (float*)(ws + l.dx), *dw = (float*)(ws + l.dw), *db = grad_bias ? (float*)(ws + l.db) : nullptr;
     const int64_t row_size = l.S * (int64_t)l.Kp, g_stride = l.S * (int64_t)l.piece;
     const int zeros = grad_hidden ? (int)(l.rows < 4096 ? ceil_div(l.rows, (int64_t)4) : 1024) : 0;
-    ce_row_scale<In><<<dim3(kParts + zeros), dim3(256), 0, s>>>(header, (const int*)(fw + l.row_frame), row_target, grad_loss, gs_b, gs_t, frames_of(p, l), row_scale, back, (In*)grad_hidden);
+    int copiers = 0;
+    if (l.S == 1) {
+        const int64_t need = ceil_div((int64_t)(l.x_bytes > l.w_bytes ? l.x_bytes : l.w_bytes), (int64_t)4096);
+        copiers = (int)(need < 4096 ? need : 4096);
+    }
+    const f16 *x16 = x, *w16 = w;             // of the gradients' products
+    Copies copies{};
+    if (l.S == 1) {
+        x16 = (f16*)(ws + l.x_copy); w16 = (f16*)(ws + l.w_copy);
+        copies = {(const bf16*)x, (const bf16*)w, grad_weight ? (f16*)x16 : nullptr, grad_hidden ? (f16*)w16 : nullptr, (int64_t)(l.w_bytes / 2)};
+    }
+    const Frames f = frames_of(p, l);
+    const Parts joined = parts_at(fw + l.joined, l.joins, kPackGroups / 256);
+    ce_row_scale<In><<<dim3(kShareParts + zeros + copiers), dim3(256), 0, s>>>(header, (const int*)(fw + l.row_frame), row_target, grad_loss, gs_b, gs_t, f, joined, copies, zeros, row_scale, back, (In*)grad_hidden);
     for (int first = 0; first < p.F; first += l.piece) {
         const int classes = p.F - first < l.piece ? p.F - first : l.piece;
-        const Operand piece_w{w + first * row_size, row_size, l.Kp, (int64_t)l.w_bytes - first * row_size * 2, classes, nullptr};
         ProductArgs q{};
-        q.a = piece_w;
-        q.b = {x, row_size, l.Kp, (int64_t)l.x_bytes, 0, &header->rows};
+        q.a = {w + first * row_size, nullptr, row_size, l.Kp, (int64_t)l.w_bytes - first * row_size * 2, classes};
+        q.b = {x, nullptr, row_size, l.Kp, (int64_t)l.x_bytes, kFrames};
         q.K = l.Kp; q.splits = 1;
         EpilogueArgs e{};
-        e.bias = p.bias; e.header = header; e.back = back; e.first_class = first;
+        e.bias = p.bias; e.header = header; e.back = back; e.first_class = first; e.piece_classes = classes;
+        e.f = f; e.w = {p.weight, p.weight_stride_f, p.bias}; e.row_frame = (const int*)(fw + l.row_frame);
         e.row_target = row_target; e.target_logit = (float*)(fw + l.target_logit); e.lse = (const float*)(fw + l.lse); e.row_scale = row_scale;
         e.g = g; e.g_stride = g_stride; e.g_half = l.piece;
         launch_product<In, kGradient, 2>(q, e, classes, l.rows, s);
         BothArgs h{}, v{};
         unsigned of_hidden = 0, of_weight = 0;
         if (grad_hidden) {
-            h.p.a = {g, g_stride, l.piece, (int64_t)l.g_bytes, 0, &header->rows};
-            h.p.b = piece_w;
-            h.p.b.rows = p.D;
+            h.p.a = {g, nullptr, g_stride, l.piece, (int64_t)l.g_bytes, kFrames};
+            h.p.b = {w16 + first * row_size, w + first * row_size, row_size, l.Kp, (int64_t)l.w_bytes - first * row_size * 2, p.D};
             h.p.K = round_up(classes, kPad); h.p.splits = l.hidden_splits;
-            h.e.header = header; h.e.back = back; h.e.row_target = row_target; h.e.row_frame = (const int*)(fw + l.row_frame); h.e.classes = p.F;
+            h.e = e;
+            h.e.classes = p.F;
             h.e.sum = dx; h.e.sum_stride = p.D; h.e.part_stride = (int64_t)l.rows_p * p.D; h.e.add = first > 0; h.e.last = first + l.piece >= p.F && l.hidden_splits == 1;
             h.e.out = grad_hidden;
             of_hidden = l.narrow ? groups_of<2>(h.p, l.rows, p.D) : groups_of<4>(h.p, l.rows, p.D);
         }
         if (grad_weight || grad_bias) {
-            v.p.a = {g, g_stride, l.piece, (int64_t)l.g_bytes, classes, nullptr};
-            v.p.b = {x, row_size, l.Kp, (int64_t)l.x_bytes, p.D, nullptr};
-            v.p.n_k = &header->rows; v.p.splits = l.splits;
+            v.p.a = {g, nullptr, g_stride, l.piece, (int64_t)l.g_bytes, classes};
+            v.p.b = {x16, x, row_size, l.Kp, (int64_t)l.x_bytes, p.D};
+            v.e = e;
+            v.p.K = kFrames; v.p.splits = l.splits;
             v.e.part_out = dw; v.e.part_stride = (int64_t)l.piece * p.D; v.e.bias_out = db; v.e.bias_stride = l.piece;
             of_weight = l.narrow ? groups_of<2>(v.p, classes, p.D) : groups_of<4>(v.p, classes, p.D);
         }
         // dh that fills the compute units more than once leaves idle ones at its end alone, which long workgroups of dW do not fill (subword units, 44 800 x 5001 x 500
         // in 32 bits: a training step 3.00 ms apart, 3.03 together)
         const bool apart = of_hidden > (l.narrow ? 512 : 256) && of_weight;
-        if (apart) launch_back<In>(l.narrow, of_hidden, of_hidden, h, v, s);
+        if (apart) launch_back<In>(l.narrow, of_hidden, of_hidden, h, v, back, s);
         const unsigned with = apart ? 0 : of_hidden;
-        launch_back<In>(l.narrow, with, with + of_weight, h, v, s);
+        launch_back<In>(l.narrow, with, with + of_weight, h, v, back, s);
         if (of_hidden && l.hidden_splits > 1 && first + l.piece >= p.F)
             ce_store_hidden<In><<<dim3((unsigned)ceil_div(l.rows * p.D, (int64_t)256)), dim3(256), 0, s>>>(header, back, dx, l.hidden_splits, h.e.part_stride, h.e.row_frame, row_target, p.F,
                                                                                                           p.D, (In*)grad_hidden);
         if (of_weight) {
             const int64_t n = (int64_t)classes * p.D;
             ce_store_weight<In><<<dim3((unsigned)(ceil_div(n, (int64_t)256) + ceil_div(classes, 256))), dim3(256), 0, s>>>(
-                header, back, dw, l.splits, v.e.part_stride, n, grad_weight ? (In*)grad_weight + (int64_t)first * p.D : nullptr, db, v.e.bias_stride, classes,
+                back, dw, l.splits, v.e.part_stride, n, grad_weight ? (In*)grad_weight + (int64_t)first * p.D : nullptr, db, v.e.bias_stride, classes,
                 grad_bias ? (In*)grad_bias + first : nullptr);
         }
     }
@@ -1182,6 +1505,7 @@ int i6train_ce_backward(const i6train_ce_problem* p, const float* grad_loss, int
     }
     Layout l;
     I6TRAIN_TRY(layout(*p, l));
+    if (!p->hidden) return I6TRAIN_ERR_INVALID_ARGUMENT;
     if (forward_bytes < l.forward || workspace_bytes < l.backward) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
     const auto run = p->dtype == I6TRAIN_F32 ? backward<float> : backward<bf16>;
     return run(*p, l, grad_loss, grad_stride_b, grad_stride_t, grad_hidden, grad_weight, grad_bias, (const char*)forward_workspace, (char*)workspace, (hipStream_t)stream);

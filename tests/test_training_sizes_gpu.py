@@ -1,10 +1,11 @@
-"""Cross entropy of frames, classes and incoming gradients of very different sizes."""
+"""Cross entropy of frames, classes and incoming gradients of very different sizes: a large one changes nothing but what
+it enters.  Bounds are those of tests/test_training_gpu.py, computed without the large one."""
 import math
 
 import pytest
 import torch
 
-from tests.test_training_gpu import DTYPES, ce_expected, ce_problem, ce_run, close
+from tests.test_training_gpu import DTYPES, EPS16, EPS32, EPS_HALVES, ce_expected, ce_problem, ce_run, close, gen
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +62,125 @@ def test_target_with_the_lowest_bias(sizes, dtype):
     want = ce_expected(hidden, weight[keep].contiguous(), bias[keep].contiguous(), renumbered, lens, grad)
     for k in ("loss", "hidden"):
         close(got[k][others], want[k][0][others], want[k][1][others], k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [1e9, 1e12, 1e15, 1e25])
+@pytest.mark.parametrize("elements", [1, 64])
+@pytest.mark.parametrize("sizes", SIZES)
+def test_loss_beside_a_large_frame(sizes, elements, size, dtype):
+    hidden, weight, bias, targets, lens, grad = ce_problem(*sizes, dtype, seed=3, lens=[sizes[1]] * sizes[0])
+    from i6_native_ops_amd.training import linear_cross_entropy
+    ordinary = linear_cross_entropy(hidden, weight, targets, lens, bias=bias)
+    hidden[1, 7, :elements] *= size
+    loss = linear_cross_entropy(hidden, weight, targets, lens, bias=bias)
+    want, bound = ce_expected(hidden, weight, bias, without(targets, (1, 7)), lens, grad)["loss"]
+    others = torch.ones_like(targets, dtype=torch.bool)
+    others[1, 7] = False
+    close(loss[others], want[others], bound[others], "loss")
+    if dtype == torch.bfloat16:
+        assert torch.equal(loss[others], ordinary[others])
+    # the frame itself: between 0 and what its logits can differ by
+    z = hidden[1, 7].double() @ weight.double().T + bias.double()
+    exact = torch.logsumexp(z, 0) - z[targets[1, 7].long()]
+    reach = (hidden[1, 7].double().abs() @ weight.double().abs().T).max()
+    assert loss[1, 7] >= -2.0 ** -20 and abs(float(loss[1, 7]) - float(exact)) <= 2 * float(reach) * (sizes[3] + 4) * EPS_HALVES + 1e-5
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [1e9, 1e12, 1e15, 1e25])
+@pytest.mark.parametrize("elements", [1, 64])
+@pytest.mark.parametrize("sizes", SIZES)
+def test_gradients_beside_a_large_frame(sizes, elements, size, dtype):
+    hidden, weight, bias, targets, lens, grad = ce_problem(*sizes, dtype, seed=4, lens=[sizes[1]] * sizes[0])
+    at = (1, 7)
+    hidden[1, 7, :elements] *= size
+    got = ce_run(hidden, weight, bias, targets, lens, grad)
+    assert all(torch.isfinite(x).all() for x in got.values())
+    want = ce_expected(hidden, weight, bias, without(targets, at), lens, grad)
+    others = torch.ones_like(targets, dtype=torch.bool)
+    others[at] = False
+    close(got["hidden"][others], want["hidden"][0][others], want["hidden"][1][others], "hidden")
+    # classes that the large frame says nothing about: neither its target nor of any probability there
+    z = hidden[at].double() @ weight.double().T + bias.double()
+    free = z < z.max() - 1000 - (hidden[at].double().abs() @ weight.double().abs().T).max() * sizes[3] * EPS_HALVES
+    free[targets[at].long()] = False
+    assert free.sum() > sizes[2] // 2
+    for k in ("weight", "bias"):
+        close(got[k][free], want[k][0][free], want[k][1][free], k)
+    # all of its gradient is in the two classes that it does say something about
+    if float(z.max() - z[targets[at].long()]) > float(z.max() - z[free].max()) / 2:
+        y = int(targets[at])
+        share = -grad[at].double() * hidden[at].double()
+        error = (got["weight"][y].double() - share - want["weight"][0][y]).abs()
+        assert (error <= want["weight"][1][y] + share.abs() * 4 * (EPS16 if dtype == torch.bfloat16 else EPS_HALVES) + (EPS16 if dtype == torch.bfloat16 else 4 * EPS32) * share.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [1e9, 1e12, 1e25])
+@pytest.mark.parametrize("sizes", SIZES)
+def test_loss_and_gradients_beside_a_large_class(sizes, size, dtype):
+    """A class whose weights are far larger than the others': frames that it is improbable for are as they would be without it."""
+    hidden, weight, bias, targets, lens, grad = ce_problem(*sizes, dtype, seed=5, lens=[sizes[1]] * sizes[0])
+    c = 130
+    targets[targets == c] = 0
+    weight[c] = (weight[c].float() * size).to(dtype)
+    z = hidden.double() @ weight[c].double()
+    margin = (hidden.double().abs() @ weight[c].double().abs()) * (sizes[3] + 4) * EPS_HALVES + 1000
+    targets[z > -margin] = -1
+    assert (targets >= 0).float().mean() > 0.3
+    got = ce_run(hidden, weight, bias, targets, lens, grad)
+    keep = torch.arange(sizes[2], device="cuda") != c
+    renumbered = torch.where(targets > c, targets - 1, targets)
+    want = ce_expected(hidden, weight[keep].contiguous(), bias[keep].contiguous(), renumbered, lens, grad)
+    close(got["loss"], *want["loss"], "loss")
+    close(got["hidden"], *want["hidden"], "hidden")
+    for k in ("weight", "bias"):
+        close(got[k][keep], *want[k], k)
+        assert (got[k][c] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes", SIZES)
+def test_gradients_of_very_small_and_very_large_shares(sizes, dtype):
+    """Incoming gradients over thirty powers of ten: every frame's gradient is as precise as it would be alone."""
+    hidden, weight, bias, targets, lens, grad = ce_problem(*sizes, dtype, seed=6)
+    share = torch.exp((torch.rand(targets.shape, generator=gen(7), device="cuda") - 0.5) * 30 * math.log(10.0))
+    got = ce_run(hidden, weight, bias, targets, lens, share * grad.sign())
+    alone, bound = ce_expected(hidden, weight, bias, targets, lens, grad.sign())["hidden"]
+    by = share.double()[:, :, None]
+    close(got["hidden"], alone * by, bound * by, "hidden")
+    want = ce_expected(hidden, weight, bias, targets, lens, share * grad.sign())
+    for k in ("weight", "bias"):
+        close(got[k], *want[k], k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_frames_of_many_sizes(dtype):
+    """Frames over twenty powers of ten."""
+    hidden, weight, bias, targets, lens, grad = ce_problem(3, 250, 300, 128, dtype, seed=8, lens=[250, 250, 99])
+    size = torch.exp(-torch.rand((3, 250, 1), generator=gen(9), device="cuda") * 20 * math.log(10.0))
+    hidden = (hidden.float() * size).to(dtype)
+    got = ce_run(hidden, weight, bias, targets, lens, grad)
+    want = ce_expected(hidden, weight, bias, targets, lens, grad)
+    for k in got:
+        close(got[k], *want[k], k)
+
+
+@pytest.mark.parametrize("B,T,F,D,dtype", [
+    (3, 400, 7700, 450, torch.float32), (3, 400, 7700, 450, torch.bfloat16), (9, 1000, 15001, 40, torch.float32), (33, 1000, 9001, 24, torch.bfloat16),
+    (1, 700, 4099, 31, torch.float32), (20, 300, 130, 500, torch.float32), (8, 2000, 3001, 260, torch.float32),
+])
+def test_frames_and_shares_of_many_sizes_in_large_layers(B, T, F, D, dtype):
+    """Large and small tiles, several pieces of the vocabulary, ranges of frames and of classes."""
+    hidden, weight, bias, targets, lens, grad = ce_problem(B, T, F, D, dtype, seed=F, lens=[T] * (B - 1) + [T - 5])
+    targets[0, 3:9] = -1
+    hidden[0, 3:9] = float("nan")
+    size = torch.exp(-torch.rand((B, T, 1), generator=gen(9), device="cuda") * 12 * math.log(10.0))
+    clean = torch.nan_to_num(hidden.float() * size).to(dtype)
+    got = ce_run((hidden.float() * size).to(dtype), weight, bias, targets, lens, grad * size[:, :, 0].flip(1))
+    want = ce_expected(clean, weight, bias, targets, lens, grad * size[:, :, 0].flip(1))
+    for k in got:
+        close(got[k], *want[k], k)
+    again = ce_run((hidden.float() * size).to(dtype), weight, bias, targets, lens, grad * size[:, :, 0].flip(1))
+    assert all(torch.equal(got[k], again[k]) for k in got)
