@@ -47,7 +47,7 @@ def test_gradients_of_a_large_frame_are_finite(sizes, size, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("sizes", SIZES)
+@pytest.mark.parametrize("sizes", [(2, 50, 10, 64)] + SIZES)
 def test_target_with_the_lowest_bias(sizes, dtype):
     """A class with the type's lowest value as bias costs, as a target, what the bias says; elsewhere it is not there."""
     hidden, weight, bias, targets, lens, grad = ce_problem(*sizes, dtype, seed=10, lens=[sizes[1]] * sizes[0])
@@ -62,6 +62,16 @@ def test_target_with_the_lowest_bias(sizes, dtype):
     want = ce_expected(hidden, weight[keep].contiguous(), bias[keep].contiguous(), renumbered, lens, grad)
     for k in ("loss", "hidden"):
         close(got[k][others], want[k][0][others], want[k][1][others], k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_small_layers_whose_classes_all_have_the_lowest_bias(dtype):
+    """Sums of the lowest value and a logit round to the lowest value: the classes are equal."""
+    hidden, weight, _, targets, lens, grad = ce_problem(2, 50, 10, 64, dtype, seed=10, lens=[50, 50])
+    got = ce_run(hidden, weight, torch.full((10,), torch.finfo(dtype).min, dtype=dtype, device="cuda"), targets, lens, grad)
+    assert (got["loss"] - math.log(10)).abs().max() < 1e-5
+    G = (torch.full((2, 50, 10), 0.1, dtype=torch.float64, device="cuda") - torch.nn.functional.one_hot(targets.long(), 10)) * grad.double()[:, :, None]
+    close(got["hidden"], G @ weight.double(), (G.abs() @ weight.double().abs()) * (2.0 ** -20 + (EPS16 if dtype == torch.bfloat16 else 0)), "hidden")
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
