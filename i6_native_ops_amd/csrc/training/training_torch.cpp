@@ -149,10 +149,10 @@ bool wants_gradient(std::initializer_list<torch::Tensor> inputs) {
     return false;
 }
 
-// Gradients of gradients are refused as they are asked for, not as create_graph is.
-variable_list once(const char* op, const variable_list& incoming, variable_list outgoing) {
+// Gradients of gradients are refused as they are asked for, not as create_graph is.  A gradient depends on the inputs as it does on the incoming one.
+variable_list once(const char* op, const variable_list& incoming, std::initializer_list<torch::Tensor> inputs, variable_list outgoing) {
     if (!at::GradMode::is_enabled()) return outgoing;
-    bool tracked = false;
+    bool tracked = wants_gradient(inputs);
     for (const torch::Tensor& g : incoming) tracked = tracked || (g.defined() && g.requires_grad());
     if (!tracked) return outgoing;
     for (torch::Tensor& g : outgoing)
@@ -174,7 +174,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         variable_list out(5);
         for (int i = 0; i < 3; i++)
             if (got[i]) out[i] = *got[i];
-        return once("linear_cross_entropy", grads, std::move(out));
+        return once("linear_cross_entropy", grads, {saved[0], saved[1], saved[2]}, std::move(out));
     }
 };
 
@@ -260,8 +260,7 @@ std::vector<torch::Tensor> gated_recurrence_backward(const Optional& grad_h, con
 struct GatedRecurrence : torch::autograd::Function<GatedRecurrence> {
     static variable_list forward(AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& gate, const Optional& initial, const Optional& seq_lens) {
         std::vector<Optional> got = gated_recurrence_forward(x, gate, seq_lens, initial, true);
-        ctx->save_for_backward({x, gate, or_none(seq_lens), *got[2]});
-        ctx->saved_data["with_state"] = initial.has_value();
+        ctx->save_for_backward({x, gate, or_none(seq_lens), *got[2], or_none(initial)});
         ctx->set_materialize_grads(false);
         return {*got[0], *got[1]};
     }
@@ -269,7 +268,7 @@ struct GatedRecurrence : torch::autograd::Function<GatedRecurrence> {
         const variable_list saved = ctx->get_saved_variables();
         const Optional grad_h = grads[0].defined() ? Optional(rows(grads[0])) : Optional(), grad_last = grads[1].defined() ? Optional(grads[1].contiguous()) : Optional();
         const std::vector<torch::Tensor> got = gated_recurrence_backward(grad_h, grad_last, saved[0], saved[1], given(saved[2]), saved[3]);
-        return once("gated_recurrence", grads, {got[0], got[1], ctx->saved_data["with_state"].toBool() && ctx->needs_input_grad(2) ? got[2] : torch::Tensor(), torch::Tensor()});
+        return once("gated_recurrence", grads, {saved[0], saved[1], saved[4]}, {got[0], got[1], saved[4].defined() && ctx->needs_input_grad(2) ? got[2] : torch::Tensor(), torch::Tensor()});
     }
 };
 
