@@ -316,7 +316,18 @@ void adamw_step(const std::vector<torch::Tensor>& params, const std::vector<torc
         }
     }
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(device);
-    check("adamw_step", i6train_adamw(table.data(), (int)n, dtype, bits, step, lr, beta1, beta2, eps, weight_decay, (void*)current_stream()));
+    const int rc = i6train_adamw(table.data(), (int)n, dtype, bits, step, lr, beta1, beta2, eps, weight_decay, (void*)current_stream());
+    // what a graph has saved of these tensors is not what it was; tensors made in inference mode are in no graph and have no version
+    const auto changed = [](const torch::Tensor& t) {
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    };
+    for (const auto* list : {&params, &exp_avgs, &exp_avg_sqs})
+        for (const torch::Tensor& t : *list) changed(t);
+    for (const auto& pair : scales) {
+        changed(pair.first);
+        changed(pair.second);
+    }
+    check("adamw_step", rc);
 }
 
 }  // namespace

@@ -43,3 +43,34 @@ def test_a_graph_of_the_gradients_that_is_not_used():
     again = torch.autograd.grad(loss.sum(), leaves, create_graph=True)
     for a, b in zip(plain, again):
         assert torch.equal(a, b.detach())
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_optimiser_steps_are_seen_by_autograd(bits):
+    """A second backward pass over a graph whose weights a step has changed raises, as after torch's own optimisers."""
+    from i6_native_ops_amd.training import AdamW, linear_cross_entropy
+    for sizes in [(2, 5, 7, 8), (2, 300, 400, 64)]:
+        hidden, weight, bias, targets, lens, _ = ce_problem(*sizes, torch.float32)
+        hidden.requires_grad_()
+        weight = torch.nn.Parameter(weight)
+        opt = AdamW([weight], lr=1e-2, state_bits=bits)
+        loss = linear_cross_entropy(hidden, weight, targets, lens, bias=bias).sum()
+        loss.backward(retain_graph=True)
+        opt.step()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+
+def test_steps_count_as_changes_of_all_they_write():
+    from i6_native_ops_amd.training import adamw_step
+    p, g = torch.ones(300, device="cuda"), torch.ones(300, device="cuda")
+    m, v = (torch.zeros(300, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2))
+    scales = (torch.ones(2, device="cuda"), torch.ones(2, device="cuda"))
+    before = [x._version for x in (p, m, v, *scales)]
+    adamw_step([p], [g], [m], [v], step=1, lr=1e-2, scales=[scales])
+    assert all(x._version > b for x, b in zip((p, m, v, *scales), before)) and g._version == 0
+    with torch.inference_mode():                         # tensors without a version
+        p, m, v = (torch.ones(300, device="cuda") for _ in range(3))
+        adamw_step([p], [p.clone()], [m], [v], step=1, lr=1e-2)
+    adamw_step([p], [p.clone()], [m], [v], step=2, lr=1e-2)
+    assert torch.isfinite(p).all()
