@@ -142,6 +142,10 @@ using torch::autograd::variable_list;
 torch::Tensor rows(const torch::Tensor& x) { return x.dim() == 0 || x.stride(-1) == 1 ? x : x.contiguous(); }
 Optional given(const torch::Tensor& x) { return x.defined() ? Optional(x) : Optional(); }
 torch::Tensor or_none(const Optional& x) { return x ? *x : torch::Tensor(); }
+// Tangents would be lost in silence: the kernels know nothing of them.
+void refuse_tangents(const char* op, std::initializer_list<torch::Tensor> inputs) {
+    for (const torch::Tensor& x : inputs) TORCH_CHECK(!x.defined() || !x._fw_grad(/*level=*/0).defined(), op, " has no forward-mode derivative");
+}
 bool wants_gradient(std::initializer_list<torch::Tensor> inputs) {
     if (!at::GradMode::is_enabled()) return false;
     for (const torch::Tensor& x : inputs)
@@ -179,6 +183,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
 };
 
 torch::Tensor linear_cross_entropy(const torch::Tensor& hidden, const torch::Tensor& weight, const torch::Tensor& targets, const torch::Tensor& seq_lens, const Optional& bias) {
+    refuse_tangents("linear_cross_entropy", {hidden, weight, or_none(bias)});
     if (wants_gradient({hidden, weight, or_none(bias)}))
         return LinearCrossEntropy::apply(rows(hidden), rows(weight), bias, targets, seq_lens);
     return std::get<0>(linear_cross_entropy_forward(rows(hidden), rows(weight), targets, seq_lens, bias));
@@ -273,6 +278,7 @@ struct GatedRecurrence : torch::autograd::Function<GatedRecurrence> {
 };
 
 std::tuple<torch::Tensor, torch::Tensor> gated_recurrence(const torch::Tensor& x, const torch::Tensor& gate, const Optional& seq_lens, const Optional& initial) {
+    refuse_tangents("gated_recurrence", {x, gate, or_none(initial)});
     if (wants_gradient({x, gate, or_none(initial)})) {
         const variable_list out = GatedRecurrence::apply(rows(x), rows(gate), initial, seq_lens);
         return {out[0], out[1]};

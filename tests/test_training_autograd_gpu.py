@@ -74,3 +74,20 @@ def test_steps_count_as_changes_of_all_they_write():
         adamw_step([p], [p.clone()], [m], [v], step=1, lr=1e-2)
     adamw_step([p], [p.clone()], [m], [v], step=2, lr=1e-2)
     assert torch.isfinite(p).all()
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_tangents_are_refused(which):
+    import torch.autograd.forward_ad as fwad
+    from i6_native_ops_amd.training import gated_recurrence, linear_cross_entropy
+    hidden, weight, bias, targets, lens, _ = ce_problem(2, 5, 7, 8, torch.float32)
+    x, gate, rec_lens, state, _ = rec_problem(2, 5, 8, torch.float32)
+    with fwad.dual_level():
+        args = [hidden, weight, bias]
+        args[which] = fwad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError, match="linear_cross_entropy has no forward-mode derivative"):
+            linear_cross_entropy(args[0], args[1], targets, lens, bias=args[2])
+        args = [x, gate, state]
+        args[which] = fwad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError, match="gated_recurrence has no forward-mode derivative"):
+            gated_recurrence(args[0], args[1], rec_lens, initial_state=args[2])
