@@ -55,6 +55,8 @@ void check_status() {
     raise_reported("NativeOp: an earlier call reported: ");
 }
 
+bool unit_stride(const torch::Tensor& x) { return x.dim() == 0 || x.stride(-1) == 1 || x.size(-1) == 1; }
+
 torch::Tensor bytes(size_t n, const torch::Tensor& like) {
     return torch::empty({(int64_t)n}, torch::TensorOptions().device(like.device()).dtype(torch::kUInt8));
 }
@@ -85,8 +87,8 @@ std::tuple<torch::Tensor, torch::Tensor> linear_cross_entropy_forward(const torc
     CHECK_CUDA(seq_lens);
     CHECK_CONTIGUOUS(seq_lens);
     CHECK_TYPE(seq_lens, torch::kInt32);
-    TORCH_CHECK(hidden.dim() == 3 && hidden.stride(2) == 1, "hidden must have shape (B, T, D) with unit innermost stride");
-    TORCH_CHECK(weight.dim() == 2 && weight.size(1) == hidden.size(2) && weight.stride(1) == 1, "weight must have shape (F, D) with unit innermost stride");
+    TORCH_CHECK(hidden.dim() == 3 && unit_stride(hidden), "hidden must have shape (B, T, D) with unit innermost stride");
+    TORCH_CHECK(weight.dim() == 2 && weight.size(1) == hidden.size(2) && unit_stride(weight), "weight must have shape (F, D) with unit innermost stride");
     TORCH_CHECK(targets.dim() == 2 && targets.size(0) == hidden.size(0) && targets.size(1) == hidden.size(1), "targets must have shape (B, T)");
     TORCH_CHECK(seq_lens.dim() == 1 && seq_lens.size(0) == hidden.size(0), "seq_lens must have shape (B,)");
     CHECK_DEVICE(weight, hidden);
@@ -139,7 +141,8 @@ std::vector<Optional> linear_cross_entropy_backward(const torch::Tensor& grad_lo
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-torch::Tensor rows(const torch::Tensor& x) { return x.dim() == 0 || x.stride(-1) == 1 ? x : x.contiguous(); }
+// The last dimension with unit stride.  Where it has one value its stride says nothing and may be anything, contiguous() or not.
+torch::Tensor rows(const torch::Tensor& x) { return unit_stride(x) ? x : x.contiguous(); }
 Optional given(const torch::Tensor& x) { return x.defined() ? Optional(x) : Optional(); }
 torch::Tensor or_none(const Optional& x) { return x ? *x : torch::Tensor(); }
 // Tangents would be lost in silence: the kernels know nothing of them.
@@ -198,8 +201,8 @@ i6train_rec_problem rec_problem(const torch::Tensor& x, const torch::Tensor& gat
     CHECK_CUDA(gate);
     CHECK_TYPE(gate, x.dtype());
     CHECK_DEVICE(gate, x);
-    TORCH_CHECK(x.dim() == 3 && x.stride(2) == 1, "x must have shape (B, T, D) with unit innermost stride");
-    TORCH_CHECK(gate.sizes() == x.sizes() && gate.stride(2) == 1, "gate must have the shape of x, with unit innermost stride");
+    TORCH_CHECK(x.dim() == 3 && unit_stride(x), "x must have shape (B, T, D) with unit innermost stride");
+    TORCH_CHECK(gate.sizes() == x.sizes() && unit_stride(gate), "gate must have the shape of x, with unit innermost stride");
     TORCH_CHECK(x.numel() > 0, "NativeOp assertion failed: B > 0, T > 0, D > 0");
     TORCH_CHECK(x.size(0) <= 65535 && x.size(1) <= (1 << 30) && x.size(2) <= (1 << 30), "NativeOp: gated_recurrence: at most 65535 sequences");
     if (seq_lens) {
@@ -248,7 +251,7 @@ std::vector<torch::Tensor> gated_recurrence_backward(const Optional& grad_h, con
                                                      const torch::Tensor& states) {
     const i6train_rec_problem p = rec_problem(x, gate, seq_lens, Optional());
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
-    if (grad_h) TORCH_CHECK(grad_h->sizes() == x.sizes() && grad_h->dtype() == x.dtype() && grad_h->stride(2) == 1 && grad_h->device() == x.device(), "grad_h must match x");
+    if (grad_h) TORCH_CHECK(grad_h->sizes() == x.sizes() && grad_h->dtype() == x.dtype() && unit_stride(*grad_h) && grad_h->device() == x.device(), "grad_h must match x");
     if (grad_last)
         TORCH_CHECK(grad_last->dtype() == torch::kFloat32 && grad_last->is_contiguous() && grad_last->numel() == (int64_t)p.B * p.D && grad_last->device() == x.device(),
                     "grad_last must be a contiguous float32 tensor of shape (B, D)");

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests.test_training_gpu import ce_problem, rec_problem
+from tests.test_training_gpu import DTYPES, ce_problem, rec_problem
 
 pytestmark = pytest.mark.gpu
 
@@ -91,3 +91,25 @@ def test_tangents_are_refused(which):
         args[which] = fwad.make_dual(args[which], torch.ones_like(args[which]))
         with pytest.raises(RuntimeError, match="gated_recurrence has no forward-mode derivative"):
             gated_recurrence(args[0], args[1], rec_lens, initial_state=args[2])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_single_channels_of_any_stride(dtype):
+    """Where the last dimension has one value its stride says nothing, and torch leaves it as it is."""
+    from i6_native_ops_amd.training import gated_recurrence, linear_cross_entropy
+    x, gate, lens, state, _ = rec_problem(2, 30, 1, dtype)
+    want, last = gated_recurrence(x, gate, lens, initial_state=state)
+    odd = [torch.as_strided(v, v.shape, (30, 1, 30)) for v in (x, gate)]
+    leaf = odd[0].detach().requires_grad_()
+    h, again = gated_recurrence(leaf, odd[1], lens, initial_state=state)
+    assert torch.equal(h, want) and torch.equal(again, last)
+    h.sum().backward()
+    assert leaf.grad.shape == x.shape
+    one = torch.ones((1, 1, 1), dtype=dtype, device="cuda").requires_grad_()
+    h, _ = gated_recurrence(one, one.detach())
+    h.sum().backward()                                   # an incoming gradient whose strides are all 0
+    assert abs(float(one.grad) - float(torch.sigmoid(torch.tensor(-1.0)))) < 2.0 ** -8
+    hidden, weight, bias, targets, lens, _ = ce_problem(2, 300, 40, 1, dtype)
+    want = linear_cross_entropy(hidden, weight, targets, lens, bias=bias)
+    got = linear_cross_entropy(torch.as_strided(hidden, hidden.shape, (300, 1, 300)), torch.as_strided(weight, weight.shape, (1, 40)), targets, lens, bias=bias)
+    assert torch.equal(want, got)
