@@ -117,7 +117,24 @@ __device__ __forceinline__ void chunk32(const i6train_adamw_tensor& t, const Fac
 
 __device__ __forceinline__ float scale_of(uint32_t bits) {
     const float s = __uint_as_float(bits) * kPerMax;
-    return s < kLeastScale ? kLeastScale : s;      // (NaN stays)
+    return s < kLeastScale ? kLeastScale : s;
+}
+
+// The scales of a wave's block from its largest magnitudes as bit patterns.  Infinities and NaN are on top of these; they say nothing about
+// the others of their block, so where there are any, the largest of those that are numbers is looked for.
+constexpr uint32_t kInfinity = 0x7f800000u;
+__device__ __forceinline__ float scale_of_block(uint32_t most, f32x4 v) {
+    most = wave_max(most);
+    if (most >= kInfinity) {
+        most = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t b = __float_as_uint(fabsf(v[i]));
+            most = b < kInfinity && b > most ? b : most;
+        }
+        most = wave_max(most);
+    }
+    return scale_of(most);
 }
 
 // Distance of the 8-bit values around y >= 0: 2^(e - 3), e the exponent, -6 at least.
@@ -138,7 +155,7 @@ __device__ __forceinline__ float round_m(float y, float u) {
     const float a = fabsf(y), q = quantum(a);
     float k = floorf(a * per_quantum(a) + u) * q;
     k = k > kE4m3Max ? kE4m3Max : k;
-    return copysignf(k, y);
+    return copysignf(fmaf(a, 0.f, k), y);      // NaN for infinities, which the format does not have
 }
 
 // The root so that its square keeps its mean: up where y^2 - low^2 > u (high^2 - low^2).  The square would otherwise grow by the variance of
@@ -148,8 +165,9 @@ __device__ __forceinline__ float round_root(float y, float u) {
     const float q = quantum(y);
     const float low = floorf(y * per_quantum(y)) * q;
     const bool up = (y * y - low * low > u * (q * (low + low + q))) || (low == 0.f && y > 0.f);
-    const float k = up ? low + q : low;
-    return k > kE4m3Max ? kE4m3Max : k;
+    float k = up ? low + q : low;
+    k = k > kE4m3Max ? kE4m3Max : k;
+    return fmaf(y, 0.f, k);
 }
 
 __device__ __forceinline__ f32x4 from_fp8(uint32_t w) {
@@ -213,8 +231,7 @@ __device__ __forceinline__ void chunk8(const i6train_adamw_tensor& t, const Fact
             most_m = bm > most_m ? bm : most_m;
             most_r = br > most_r ? br : most_r;
         }
-        // as bit patterns: a NaN in a block is not lost
-        const float sm = scale_of(wave_max(most_m)), sr = scale_of(wave_max(most_r));
+        const float sm = scale_of_block(most_m, mv), sr = scale_of_block(most_r, rv);
         const float per_m = 1.f / sm, per_r = 1.f / sr;
 #pragma unroll
         for (int i = 0; i < 4; i++) {

@@ -119,7 +119,8 @@ int i6train_rec_backward(const i6train_rec_problem* p, const void* grad_h, int64
  *
  * state_bits 32: exp_avg and exp_avg_sq are float.  state_bits 8: exp_avg holds m and exp_avg_sq the square root of v,
  * both in the 8-bit floating-point format with 4 exponent and 3 mantissa bits (bias 7, no infinities), each block of
- * I6TRAIN_BLOCK consecutive values with a float scale of its own, largest magnitude / 448 (2^-100 at least).  Values are rounded up
+ * I6TRAIN_BLOCK consecutive values with a float scale of its own, largest finite magnitude / 448 (2^-100 at least).  What is
+ * not finite is held as NaN, and the others of its block are as without it.  Values are rounded up
  * or down so that m and v keep their means over the steps: with the place j in the block and s = step, the two turns
  *   um = ((j PHI + s ROOT) mod 2^32) >> 16,  uv = ((j ROOT + s PHI) mod 2^32) >> 16,  PHI 2654435769, ROOT 1779033703
  * are compared, as fractions of 2^16, with where the value stands between its neighbours.  A root that is not zero does not
