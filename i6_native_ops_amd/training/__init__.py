@@ -92,13 +92,15 @@ def adamw_step(
 
     :param params: contiguous tensors, all float32 or all bfloat16
     :param grads: of the same types and sizes
-    :param step: number of this step, from 1
+    :param step: number of this step, from 1.  It is part of the call: a captured step repeats this number, with its corrections, rate and
+        roundings, at every replay
     """
     core.adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales or [], int(step), lr, betas[0], betas[1], eps, weight_decay)
 
 
 class AdamW(torch.optim.Optimizer):
-    """AdamW on ``adamw_step``: one launch for the tensors of a parameter group.
+    """AdamW on ``adamw_step``: one launch for the tensors of a parameter group.  ``step`` is not for capture into a graph, whose
+    replays would all be the same step, and refuses it.
 
     :param state_bits: 32, or 8: a quarter of the optimiser's memory, and 16 instead of 28 bytes moved for each float32
         parameter in a step
@@ -127,6 +129,8 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW.step cannot be captured: every replay would be the step of this number, with its corrections and roundings")
         loss = None
         if closure is not None:
             with torch.enable_grad():

@@ -37,3 +37,20 @@ def test_one_bad_gradient_in_8_bits_spoils_one_value(dtype, bad):
         assert torch.isnan(runs[0][0][at]) and torch.isnan(runs[0][1][at])
         assert torch.equal(runs[0][3], runs[1][3])
     assert torch.equal(runs[0][4], runs[1][4])
+
+
+def test_optimiser_steps_are_not_captured(monkeypatch):
+    """A replay would repeat the number of the captured step, and with it its corrections and roundings."""
+    from i6_native_ops_amd.training import AdamW
+    p = torch.nn.Parameter(torch.ones(10, device="cuda"))
+    opt = AdamW([p], lr=1e-2)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    held = p.detach().clone()
+    with monkeypatch.context() as patch:
+        patch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="AdamW.step cannot be captured"):
+            opt.step()
+    assert opt.state[p]["step"] == 1 and torch.equal(p.detach(), held)
+    opt.step()
+    assert opt.state[p]["step"] == 2
