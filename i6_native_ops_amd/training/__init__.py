@@ -143,12 +143,13 @@ class AdamW(torch.optim.Optimizer):
                 if p.grad.is_sparse:
                     raise RuntimeError("AdamW does not take sparse gradients")
                 state = self.state[p] or self._start(p, group["state_bits"])
-                state["step"] += 1
-                calls.setdefault((p.device, p.dtype, state["step"]), []).append((p, state))
+                calls.setdefault((p.device, p.dtype, state["step"] + 1), []).append((p, state))
             for (_, _, step), items in calls.items():
                 scales = [(s["exp_avg_scale"], s["exp_avg_sq_scale"]) for _, s in items] if group["state_bits"] == 8 else None
                 adamw_step([p for p, _ in items], [p.grad.contiguous() for p, _ in items], [s["exp_avg"] for _, s in items],
                            [s["exp_avg_sq"] for _, s in items], step, group["lr"], group["betas"], group["eps"], group["weight_decay"], scales)
+                for _, state in items:       # a call that has been refused is no step
+                    state["step"] = step
         return loss
 
     def load_state_dict(self, state_dict):

@@ -54,3 +54,17 @@ def test_optimiser_steps_are_not_captured(monkeypatch):
     assert opt.state[p]["step"] == 1 and torch.equal(p.detach(), held)
     opt.step()
     assert opt.state[p]["step"] == 2
+
+
+def test_steps_that_fail_are_not_counted():
+    from i6_native_ops_amd.training import AdamW
+    p = torch.nn.Parameter(torch.ones(4, 6, device="cuda"))
+    q = torch.nn.Parameter(torch.ones(4, 6, device="cuda").T)          # not contiguous: refused
+    opt = AdamW([p, q], lr=1e-2)
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        opt.step()
+    assert opt.state[p].get("step", 0) == 0
+    q.grad = None
+    opt.step()
+    assert opt.state[p]["step"] == 1
