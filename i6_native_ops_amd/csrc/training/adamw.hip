@@ -284,7 +284,7 @@ extern "C" int i6train_adamw(const i6train_adamw_tensor* tensors, int n_tensors,
         if (t.n == 0) continue;
         if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq) return I6TRAIN_ERR_INVALID_ARGUMENT;
         if (state_bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)) return I6TRAIN_ERR_INVALID_ARGUMENT;
-        if (t.n > ((int64_t)1 << 40)) return I6TRAIN_ERR_TOO_LARGE;
+        if (!launchable(ceil_div(t.n, (int64_t)kChunk), kThreads)) return I6TRAIN_ERR_TOO_LARGE;
         values += t.n;
     }
     const bool stream_past = values * (3 * (int64_t)elem_size(dtype) + (state_bits == 8 ? 4 : 16)) > kStreamBytes;
@@ -297,7 +297,6 @@ extern "C" int i6train_adamw(const i6train_adamw_tensor* tensors, int n_tensors,
     k.eps = (float)eps;
     k.turn_m = (uint32_t)step * kRoot;
     k.turn_v = (uint32_t)step * kPhi;
-    constexpr int64_t kMostGroups = 0x7fffffff;
     Table tab;
     tab.n = 0;
     int64_t wgs = 0;
@@ -312,7 +311,7 @@ extern "C" int i6train_adamw(const i6train_adamw_tensor* tensors, int n_tensors,
     for (int i = 0; i < n_tensors; i++) {
         if (tensors[i].n == 0) continue;
         const int64_t need = ceil_div(tensors[i].n, (int64_t)kChunk);
-        if (tab.n == kMaxTensors || wgs + need > kMostGroups) I6TRAIN_TRY(flush());
+        if (tab.n == kMaxTensors || !launchable(wgs + need, kThreads)) I6TRAIN_TRY(flush());
         tab.t[tab.n] = tensors[i];
         tab.first[tab.n] = (int)wgs;
         tab.n++;

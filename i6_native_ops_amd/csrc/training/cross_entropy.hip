@@ -1269,6 +1269,8 @@ int groups_for(int64_t rows) { return (int)(rows < 4 * kPackGroups ? round_up(ce
 int layout(const i6train_ce_problem& p, Layout& l) {
     l.rows = (int64_t)p.B * p.T;
     if (l.rows > (1 << 22) || p.F > (1 << 22) || p.D > (1 << 14)) return I6TRAIN_ERR_TOO_LARGE;
+    // (the launches with the most workgroups; those of large tiles have half as many of twice the threads)
+    if (!launchable(round_up(ceil_div((int64_t)p.F, (int64_t)kM) * ceil_div(l.rows, (int64_t)kN), 8), kThreads)) return I6TRAIN_ERR_TOO_LARGE;
     l.S = p.dtype == I6TRAIN_F32 ? 2 : 1;
     l.Kp = round_up(p.D, kPad);
     l.row_tiles = (int)ceil_div(l.rows, (int64_t)kN);

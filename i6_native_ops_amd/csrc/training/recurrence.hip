@@ -400,6 +400,11 @@ bool valid(const i6train_rec_problem* p) {
     return p && p->B > 0 && p->T > 0 && p->D > 0 && p->B <= 65535 && valid_dtype(p->dtype) && p->x && p->gate && p->T <= (1 << 30);
 }
 
+int checked(const i6train_rec_problem* p) {
+    if (!valid(p)) return I6TRAIN_ERR_INVALID_ARGUMENT;
+    return launchable(ceil_div(p->D, 64), 512) ? I6TRAIN_OK : I6TRAIN_ERR_TOO_LARGE;
+}
+
 int n_states(const i6train_rec_problem& p) { return ceil_div(p.T, kStateSpan); }
 
 Args args_of(const i6train_rec_problem& p) {
@@ -442,13 +447,15 @@ using namespace i6train;
 extern "C" {
 
 int i6train_rec_states_size(const i6train_rec_problem* p, size_t* bytes) {
-    if (!valid(p) || !bytes) return I6TRAIN_ERR_INVALID_ARGUMENT;
+    I6TRAIN_TRY(checked(p));
+    if (!bytes) return I6TRAIN_ERR_INVALID_ARGUMENT;
     *bytes = sizeof(float) * (size_t)p->B * n_states(*p) * p->D;
     return I6TRAIN_OK;
 }
 
 int i6train_rec_workspace_size(const i6train_rec_problem* p, size_t* bytes) {
-    if (!valid(p) || !bytes) return I6TRAIN_ERR_INVALID_ARGUMENT;
+    I6TRAIN_TRY(checked(p));
+    if (!bytes) return I6TRAIN_ERR_INVALID_ARGUMENT;
     int n, f;
     cut(*p, 1, n, f);                    // single channels: the most groups, hence the fewest segments
     int n2;
@@ -458,7 +465,8 @@ int i6train_rec_workspace_size(const i6train_rec_problem* p, size_t* bytes) {
 }
 
 int i6train_rec_forward(const i6train_rec_problem* p, void* h, float* last, float* states, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!valid(p) || !h || !last) return I6TRAIN_ERR_INVALID_ARGUMENT;
+    I6TRAIN_TRY(checked(p));
+    if (!h || !last) return I6TRAIN_ERR_INVALID_ARGUMENT;
     Args a = args_of(*p);
     a.h = h; a.last = last; a.states = states;
     const int V = vector_width(*p, nullptr, 0, 0);
@@ -476,7 +484,8 @@ int i6train_rec_forward(const i6train_rec_problem* p, void* h, float* last, floa
 int i6train_rec_backward(const i6train_rec_problem* p, const void* grad_h, int64_t grad_stride_b, int64_t grad_stride_t,
                          const float* grad_last, const float* states, void* grad_x, void* grad_gate, float* grad_initial,
                          void* workspace, size_t workspace_bytes, void* stream) {
-    if (!valid(p) || !states || !grad_x || !grad_gate) return I6TRAIN_ERR_INVALID_ARGUMENT;
+    I6TRAIN_TRY(checked(p));
+    if (!states || !grad_x || !grad_gate) return I6TRAIN_ERR_INVALID_ARGUMENT;
     Args a = args_of(*p);
     a.dh = grad_h; a.dh_b = grad_stride_b; a.dh_t = grad_stride_t;
     a.dlast = grad_last; a.states = const_cast<float*>(states);

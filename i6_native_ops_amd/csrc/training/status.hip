@@ -34,7 +34,7 @@ const char* i6train_strerror(int code) {
         case I6TRAIN_ERR_INVALID_ARGUMENT: return "invalid argument";
         case I6TRAIN_ERR_WORKSPACE_TOO_SMALL: return "workspace too small";
         case I6TRAIN_ERR_LAUNCH: return "HIP call failed";
-        case I6TRAIN_ERR_TOO_LARGE: return "the problem is larger than this operator's 32-bit offsets inside a tile allow";
+        case I6TRAIN_ERR_TOO_LARGE: return "the problem is larger than this operator takes";
         case I6TRAIN_ERR_BAD_TARGET: return "target out of range";
         default: return "unknown status";
     }

@@ -45,6 +45,9 @@ inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 template <typename A, typename B> __host__ __device__ inline A ceil_div(A a, B b) { return (a + (A)b - 1) / (A)b; }
 inline bool valid_dtype(int dtype) { return dtype == I6TRAIN_F32 || dtype == I6TRAIN_BF16; }
 
+// A launch has fewer than 2^32 threads in each dimension.
+inline bool launchable(int64_t groups, int threads) { return groups < ((int64_t)1 << 32) / threads; }
+
 // The status of the last launch, as a code of this library.
 inline int launched() { return hipGetLastError() == hipSuccess ? I6TRAIN_OK : I6TRAIN_ERR_LAUNCH; }
 

@@ -66,7 +66,7 @@ int i6train_poll_status(int* code, int* seq);
  * grad_loss is float [B, T] with strides; grad_hidden [B, T, D], grad_weight [F, D] and grad_bias [F] are of `dtype`,
  * contiguous, and written completely; each of them may be null.  Both
  * calls read hidden and weight.
- * Sizes: B T and F up to 2^22, D up to 2^14.
+ * Sizes: B T and F up to 2^22, ceil(B T / 128) ceil(F / 256) below 2^24, D up to 2^14; larger ones are I6TRAIN_ERR_TOO_LARGE.
  */
 typedef struct {
     int B, T, F, D, dtype;
@@ -90,6 +90,7 @@ int i6train_ce_backward(const i6train_ce_problem* p, const float* grad_loss, int
  * h is 0 behind the end of a sequence; last[b] is the state after its last frame (initial[b] if it has none).  The
  * state is held in 32 bits; h is rounded to `dtype` as it is written.  seq_lens null: all sequences have T frames.
  * x, gate [B, T, D] of `dtype` with strides; h [B, T, D] contiguous; initial, last float [B, D] contiguous.
+ * Sizes: B up to 65 535, T up to 2^30, D below 2^29.
  *
  * `states` (may be null) receives what i6train_rec_backward needs: the state in front of every span of frames, float,
  * i6train_rec_states_size bytes.  `workspace` is used where one sequence is worked on by several workgroups.
@@ -134,7 +135,7 @@ typedef struct {
     void* exp_avg_sq;
     float* exp_avg_scale;    /* state_bits 8: ceil(n / I6TRAIN_BLOCK) floats each */
     float* exp_avg_sq_scale;
-    int64_t n;               /* values; 0 is allowed */
+    int64_t n;               /* values, fewer than 2^36; 0 is allowed */
 } i6train_adamw_tensor;
 
 /* `tensors` is a host array. */
