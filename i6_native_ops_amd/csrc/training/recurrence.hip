@@ -370,7 +370,7 @@ __global__ __launch_bounds__(64 * W) void rec_backward(Args a) {
 constexpr int kUnits = 256;             // compute units
 constexpr int kMostSegments = 64, kLeastSegment = 128;
 
-// Channels of a lane.  64 floats are a row of 256 bytes for a wave; of bfloat16, pairs are, unless the workgroups are then fewer than the compute
+// Channels of a lane.  Pairs are for many workgroups, so their sequences are in one piece.  64 floats are a row of 256 bytes for a wave; of bfloat16, pairs are, unless the workgroups are then fewer than the compute
 // units: single channels are twice as many with half the work each (training, 16 x 2000 x 1024: 147 us, pairs 164 us; 1 x 4000 x 512: 42 and 55 us; but
 // 32 x 1000 x 1024: 124 and 110 us).
 int vector_width(const i6train_rec_problem& p, const void* dh, int64_t dh_b, int64_t dh_t) {
@@ -382,8 +382,8 @@ int vector_width(const i6train_rec_problem& p, const void* dh, int64_t dh_b, int
 // Segments of whole state spans: one, unless the (sequence, channel) groups leave compute units idle; then enough for two workgroups on each, of at least
 // kLeastSegment frames, and at least three, as the first launch goes through all of them as well.  (Training, float, 1 x 1000 x 512: 27 us, 38 us with 256 frames at least, 66 us in one
 // piece; 19 x 437 x 321, where there is little to gain: 44 us, and 40 us in one piece.)
-void cut(const i6train_rec_problem& p, int V, int& segments, int& seg_frames) {
-    const int64_t groups = (int64_t)p.B * ceil_div(p.D, 64 * V);
+void cut(const i6train_rec_problem& p, int& segments, int& seg_frames) {
+    const int64_t groups = (int64_t)p.B * ceil_div(p.D, 64);
     int64_t n = 1;
     if (groups < kUnits) {
         n = ceil_div((int64_t)2 * kUnits, groups);
@@ -424,7 +424,8 @@ template <typename T, int V> int forward(Args a, hipStream_t s) {
     } else if (a.T <= 16) {
         rec_forward<T, V, 1, 4, false><<<grid, dim3(64), 0, s>>>(a);
     } else {
-        if (a.segments > 1) rec_forward<T, V, 8, 16, true><<<grid, dim3(512), 0, s>>>(a);
+        if constexpr (V == 1)
+            if (a.segments > 1) rec_forward<T, 1, 8, 16, true><<<grid, dim3(512), 0, s>>>(a);
         rec_forward<T, V, 8, 16, false><<<grid, dim3(512), 0, s>>>(a);
     }
     return launched();
@@ -432,7 +433,8 @@ template <typename T, int V> int forward(Args a, hipStream_t s) {
 
 template <typename T, int V> int backward(Args a, hipStream_t s) {
     const dim3 grid(ceil_div(a.D, 64 * V), a.B, a.segments);
-    if (a.segments > 1) rec_backward<T, V, 8, 8, true><<<grid, dim3(512), 0, s>>>(a);
+    if constexpr (V == 1)
+        if (a.segments > 1) rec_backward<T, 1, 8, 8, true><<<grid, dim3(512), 0, s>>>(a);
     rec_backward<T, V, 8, 8, false><<<grid, dim3(512), 0, s>>>(a);
     return launched();
 }
@@ -457,10 +459,8 @@ int i6train_rec_workspace_size(const i6train_rec_problem* p, size_t* bytes) {
     I6TRAIN_TRY(checked(p));
     if (!bytes) return I6TRAIN_ERR_INVALID_ARGUMENT;
     int n, f;
-    cut(*p, 1, n, f);                    // single channels: the most groups, hence the fewest segments
-    int n2;
-    cut(*p, 2, n2, f);
-    *bytes = n > 1 || n2 > 1 ? 2 * segment_bytes(*p) : 0;
+    cut(*p, n, f);
+    *bytes = n > 1 ? 2 * segment_bytes(*p) : 0;
     return I6TRAIN_OK;
 }
 
@@ -470,7 +470,7 @@ int i6train_rec_forward(const i6train_rec_problem* p, void* h, float* last, floa
     Args a = args_of(*p);
     a.h = h; a.last = last; a.states = states;
     const int V = vector_width(*p, nullptr, 0, 0);
-    cut(*p, V, a.segments, a.seg_frames);
+    cut(*p, a.segments, a.seg_frames);
     if (a.segments > 1) {
         if (!workspace || workspace_bytes < 2 * segment_bytes(*p)) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
         a.seg_a = static_cast<float*>(workspace);
@@ -491,7 +491,7 @@ int i6train_rec_backward(const i6train_rec_problem* p, const void* grad_h, int64
     a.dlast = grad_last; a.states = const_cast<float*>(states);
     a.dx = grad_x; a.dgate = grad_gate; a.dinitial = grad_initial;
     const int V = vector_width(*p, grad_h, grad_stride_b, grad_stride_t);
-    cut(*p, V, a.segments, a.seg_frames);
+    cut(*p, a.segments, a.seg_frames);
     if (a.segments > 1) {
         if (!workspace || workspace_bytes < 2 * segment_bytes(*p)) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
         a.seg_a = static_cast<float*>(workspace);
