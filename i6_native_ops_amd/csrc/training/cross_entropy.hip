@@ -21,9 +21,9 @@
 //              below.  Of (x1 + x2 2^-11)(y1 + y2 2^-11) the last term is below the precision and left out: the k-loop runs over x1 y2 and x2 y1, scales the
 //              accumulators by 2^-11, and goes on with x1 y1: three times the work, on units whose rate for 16-bit operands is sixteen times that for 32-bit ones.
 //
-// One scale for a tensor is good where its rows are not too different: every row but those of zeros has a mean magnitude (G: an incoming gradient) that the forms
-// above hold well beside the tensor's largest value (kRows, kShares).  That is looked up on the device.  Where it is not so (frames or
-// classes millions of times larger than others, incoming gradients over many powers of ten), the same kernels take another way, `wide`: for bfloat16 the gradients' products
+// One scale for a tensor is good where its values are not too different: in every row but those of zeros the values that are not 0 have a geometric mean (G: an incoming
+// gradient) that the forms above hold well beside the tensor's largest value (kRows, kShares).  That is looked up on the device.  Where it is not so (frames,
+// classes or features millions of times larger than others, incoming gradients over many powers of ten), the same kernels take another way, `wide`: for bfloat16 the gradients' products
 // too are formed in bfloat16, with G rounded to it; for float the products are formed from the 32-bit values, in the matrix instructions that take
 // them: a sixteenth of the rate, and as precise as a plain product (a training step of 44 800 frames, F = 5001, D = 500: 3.0 ms, 9.7 where the gradients' products alone are
 // formed so, 15.6 where the logits are too).
@@ -50,10 +50,10 @@ constexpr int kPackGroups = 4096;    // at most, of ce_pack: in bfloat16 it look
 constexpr int kLookThreads = 1024;   // every wave waits for lengths, targets and rows in turn: many waves, few rows each
 constexpr int kPad = 64;             // rows and columns of operands are padded with zeros to multiples of this
 constexpr float kLow = 0x1p-11f;     // weight of the second half of a 32-bit value
-// The least mean magnitude of a row (and the least incoming gradient) that is not 0, over the tensor's largest value, of the fast forms; S: halves of a value.
+// By how many powers of two the mean of a row (and an incoming gradient) may be below the tensor's largest value in the fast forms; S: halves of a value.
 // What is below a value's last bit, 2^-51 of the largest (16 bits: 2^-40), is then 2^-25 (2^-20) of the row's mean, 2^-29 (2^-24) of the frame's share.
-template <int S> constexpr float kRows = S == 2 ? 0x1p-26f : 0x1p-20f;
-template <int S> constexpr float kShares = S == 2 ? 0x1p-22f : 0x1p-16f;
+template <int S> constexpr int kRows = S == 2 ? 26 : 20;
+template <int S> constexpr int kShares = S == 2 ? 22 : 16;
 
 using f16x2 = f16 __attribute__((ext_vector_type(2)));
 using f16x4 = f16 __attribute__((ext_vector_type(4)));
@@ -78,12 +78,12 @@ struct BackHeader {
     int up_g, wide;                  // of G; how the gradients' products are formed
     alignas(16) uint32_t most[kShareParts], least[kShareParts];      // incoming gradients: partial results
 };
-// Partial results over a tensor, as bit patterns of magnitudes: the largest finite value, and the least mean of a row that is not 0.
+// Partial results over a tensor: the largest finite value, as its bit pattern, and the least mean exponent of a row that is not 0.
 struct Parts {
     uint32_t *most_x, *least_x, *most_w, *least_w;
     int n;                           // of each
 };
-constexpr uint32_t kNone = 0x7f7fffffu;                    // no row
+constexpr uint32_t kNone = 255;                            // no row
 
 __device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
 __device__ __forceinline__ uint32_t umin(uint32_t a, uint32_t b) { return a < b ? a : b; }
@@ -99,7 +99,7 @@ struct Scale {
     int up;
     bool wide;
 };
-__device__ __forceinline__ Scale scale_of(const uint32_t* most_parts, const uint32_t* least_parts, int n, float range) {
+__device__ __forceinline__ Scale scale_of(const uint32_t* most_parts, const uint32_t* least_parts, int n, int range) {
     uint32_t most = 0, least = kNone;
 #pragma unroll 4
     for (int i = threadIdx.x & 63; i < n; i += 64) {
@@ -109,9 +109,9 @@ __device__ __forceinline__ Scale scale_of(const uint32_t* most_parts, const uint
     most = wave_max(most);
     least = wave_min(least);
     if (most == 0) return {0, false};
-    const int up = 14 - ((int)(most >> 23) - 127);
+    const int top = (int)(most >> 23), up = 14 - (top - 127);
     if (up > 100) return {100, true};                      // scales and their products are normal numbers
-    return {up, __uint_as_float(least) < __uint_as_float(most) * range};
+    return {up, (int)least < top - range};
 }
 
 __device__ __forceinline__ bool has_target(int y, int classes) { return y >= 0 && y < classes; }
@@ -151,22 +151,21 @@ template <typename In> __device__ __forceinline__ void load8(const In* row, int 
 
 // What a wave has seen of a tensor.
 struct Seen {
-    uint32_t most = 0, least = kNone, row_most = 0;
-    float row_sum = 0.f;
+    uint32_t most = 0, least = kNone;
+    int exponents = 0, values_in = 0;          // of the row: what a lane has seen of it
     __device__ __forceinline__ void values(const float (&v)[8]) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const uint32_t b = finite_bits(v[i]);
-            row_most = umax(row_most, b);
-            row_sum += __uint_as_float(b);
+            most = umax(most, b);
+            exponents += (int)(b >> 23);
+            values_in += b != 0;
         }
     }
-    __device__ __forceinline__ void end_row(float per_value) {       // by the whole wave
-        const float mean = wave_sum(row_sum) * per_value;
-        most = umax(most, row_most);
-        if (mean > 0.f) least = umin(least, __float_as_uint(mean));
-        row_most = 0;
-        row_sum = 0.f;
+    __device__ __forceinline__ void end_row() {               // by the whole wave
+        const float sum = wave_sum((float)exponents), n = wave_sum((float)values_in);
+        if (n > 0.f) least = umin(least, (uint32_t)(sum * rcp_fast(n)));
+        exponents = values_in = 0;
     }
 };
 
@@ -204,7 +203,6 @@ __global__ __launch_bounds__(kLookThreads) void ce_look(Frames f, Weights w, int
     const int part = (blockIdx.x - 1) % kParts;
     const In* base = static_cast<const In*>(weights ? w.p : f.hidden);
     const int64_t rows = weights ? f.F : (int64_t)f.B * f.T;
-    const float per_value = 1.f / f.D;
     Seen seen;
     for (int64_t r = (int64_t)part * kWaves + wave; r < rows; r += kParts * kWaves) {
         const In* row;
@@ -221,7 +219,7 @@ __global__ __launch_bounds__(kLookThreads) void ce_look(Frames f, Weights w, int
             load8(row, c, f.D, aligned, v);
             seen.values(v);
         }
-        seen.end_row(per_value);
+        seen.end_row();
     }
     uint32_t most = wave_max(seen.most), least = seen.least;
     if (lane == 0) {
@@ -289,7 +287,6 @@ __global__ __launch_bounds__(kThreads) void ce_pack(Frames f, Weights w, const i
         }
     }
     Seen frames_seen, weights_seen;
-    const float per_value = 1.f / f.D;
     const int64_t frames = (int64_t)f.B * f.T, n_weights = round_up(f.F, kPad), all = frames + kPad + n_weights;
     const int64_t row_size = S * (int64_t)f.Kp;
     const float none[8] = {};
@@ -306,7 +303,7 @@ __global__ __launch_bounds__(kThreads) void ce_pack(Frames f, Weights w, const i
                 }
                 store_operand<In>(o.w + row * row_size, f.Kp, c, row < f.F ? v : none, up_w);
             }
-            if (S == 1 && row < f.F) weights_seen.end_row(per_value);
+            if (S == 1 && row < f.F) weights_seen.end_row();
             continue;
         }
         if (r >= frames) {
@@ -333,7 +330,7 @@ __global__ __launch_bounds__(kThreads) void ce_pack(Frames f, Weights w, const i
             }
             store_operand<In>(o.x + row * row_size, f.Kp, c, used ? v : none, up_x);
         }
-        if (S == 1 && used) frames_seen.end_row(per_value);
+        if (S == 1 && used) frames_seen.end_row();
         if (lane == 0) {
             o.row_frame[row] = (int)r;
             o.row_target[row] = target;
@@ -1170,7 +1167,7 @@ __global__ __launch_bounds__(256) void ce_row_scale(const Header* header, const 
         row_scale[row] = g;
         const uint32_t size = finite_bits(g);
         most = umax(most, size);
-        if (size) least = umin(least, size);
+        if (size) least = umin(least, size >> 23);
     }
     most = wave_max(most);
     least = wave_min(least);

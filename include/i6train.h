@@ -59,9 +59,9 @@ int i6train_poll_status(int* code, int* seq);
  * bfloat16: logits are formed from the operands as they are.  The gradient with respect to the logits is rounded to 11 bits before
  * it is multiplied, with operands that are exact down to 2^-29 of their tensor's largest value.
  * 32 bits: operands and the gradient with respect to the logits are held in 22 bits, down to 2^-29 of the largest value of a tensor.
- * Where that is too little for a row (of hidden or weight: a mean magnitude below 2^-26 of the tensor's largest value, in bfloat16 2^-20, or an
- * incoming gradient below 2^-22 of the largest, 2^-16), which the device finds out, 32-bit products are formed from the values as they are, and
- * bfloat16 ones with the gradient with respect to the logits rounded to bfloat16.  Rows of zeros do not count.  So what a frame or a class holds changes
+ * Where that is too little for a row (of hidden or weight: a geometric mean of the values other than 0 below 2^-26 of the tensor's largest value, in
+ * bfloat16 2^-20, or an incoming gradient below 2^-22 of the largest, 2^-16), which the device finds out, 32-bit products are formed from the values as they are, and
+ * bfloat16 ones with the gradient with respect to the logits rounded to bfloat16.  Rows of zeros do not count.  So what a frame, a class or a feature holds changes
  * the precision of the others' results, at most within these bounds, and 32-bit calls become up to five times slower.
  * grad_loss is float [B, T] with strides; grad_hidden [B, T, D], grad_weight [F, D] and grad_bias [F] are of `dtype`,
  * contiguous, and written completely; each of them may be null.  Both

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from tests.test_training_gpu import DTYPES, EPS16, EPS32, EPS_HALVES, ce_expected, ce_problem, ce_run, close, gen
+from tests.test_training_gpu import DTYPES, EPS16, EPS32, EPS_HALVES, ce_check, ce_expected, ce_problem, ce_run, close, gen
 
 pytestmark = pytest.mark.gpu
 
@@ -194,3 +194,16 @@ def test_frames_and_shares_of_many_sizes_in_large_layers(B, T, F, D, dtype):
         close(got[k], *want[k], k)
     again = ce_run((hidden.float() * size).to(dtype), weight, bias, targets, lens, grad * size[:, :, 0].flip(1))
     assert all(torch.equal(got[k], again[k]) for k in got)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [1e6, 1e12, 1e20])
+@pytest.mark.parametrize("of", ["hidden", "weight"])
+@pytest.mark.parametrize("sizes", SIZES + [(3, 300, 100, 9)])
+def test_a_large_feature(sizes, of, size, dtype):
+    """One feature of all frames, or of all classes, far larger than the others, where the other operand has zeros: nothing of it is in the logits."""
+    hidden, weight, bias, targets, lens, grad = ce_problem(*sizes, dtype, seed=12, lens=[sizes[1]] * sizes[0])
+    large, zero = (hidden, weight) if of == "hidden" else (weight, hidden)
+    large[..., 5] *= size
+    zero[..., 5] = 0
+    ce_check((hidden, weight, bias, targets, lens, grad))
