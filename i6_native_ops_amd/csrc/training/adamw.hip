@@ -3,8 +3,8 @@
 // Bound by memory: a value in 32 bits moves 28 bytes (parameter and two states both ways, gradient one way), with
 // states in 8 bits 16.06.  The table of tensors travels in the kernel's arguments, so a step is one launch for up to kMaxTensors
 // tensors, copies nothing to the device and can be captured into a graph.  A workgroup takes kChunk consecutive values of one
-// tensor; which tensor, it finds by bisection over the first workgroup of each.  38 tensors of 37 M values in 32 bits: 175 us (1.05 GB, 6.0 TB/s); 74 tensors of
-// 226 M values with states in 8 bits: 640 us (3.63 GB, 5.7 TB/s).
+// tensor; which tensor, it finds by bisection over the first workgroup of each.  38 tensors of 37 M values in 32 bits: 187 us (1.05 GB, 5.6 TB/s); 74 tensors of
+// 226 M values with states in 8 bits: 650 us (3.63 GB, 5.6 TB/s).
 #include <cmath>
 
 #include "train_common.h"

@@ -31,8 +31,8 @@
 // Logits are in units of log 2 from the accumulators on: exponentials and logarithms are single instructions.
 //
 // Large layers are bound by the matrix units and by the power they draw: the chip lowers its clock to 1.9 - 2.1 GHz under them.  28 800 frames, F = 12001, D = 512 in
-// bfloat16 (0.353 TFLOP a product): statistics 379 us (932 TFLOP/s), G 2 x 233 us (758, writing 690 MB), dh and dW 2 x 368 us (960), all that goes over the
-// operands alone 90 us.  44 800 frames, F = 5001, D = 500 in 32 bits: the three parts of the statistics run at 1090 TFLOP/s, of dh and dW at 870.
+// bfloat16 (0.353 TFLOP a product): on several cards statistics 357 - 367 us (960 - 990 TFLOP/s), G 2 x 232 - 238 us (740 - 760, writing 690 MB), dh and dW
+// 2 x 354 - 360 us (980 - 1000), all that goes over the operands alone 80 us.  44 800 frames, F = 5001, D = 500 in 32 bits: the three parts of the statistics run at 1090 TFLOP/s, of dh and dW at 870.
 #include <cmath>
 #include <type_traits>
 

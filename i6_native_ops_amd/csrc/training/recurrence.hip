@@ -59,7 +59,9 @@ template <typename T, int V> __device__ __forceinline__ void put(T* at, const fl
     }
 }
 
-// f and 1 - f, neither by subtraction: both keep their relative precision where the gate is large.
+// f and 1 - f, neither by subtraction: both keep their relative precision where the gate is large.  From the instructions for 2^x and 1 / x, each right to an ulp of 32
+// bits: f is off by some ulp, which the sums over the frames leave as it is (19 x 437 x 321, all outputs: 2.7e-7 from 64 bits, 4.3e-7 with elementary operations), and a
+// correctly rounded exponential and quotient would take several times as many instructions.
 __device__ __forceinline__ void sigmoid2(float g, float& f, float& rest) {
     const float q = exp2_fast(-fabsf(g) * kLog2e), r = rcp_fast(1.f + q), s = q * r;
     f = g >= 0.f ? r : s;
