@@ -207,3 +207,28 @@ def test_a_large_feature(sizes, of, size, dtype):
     large[..., 5] *= size
     zero[..., 5] = 0
     ce_check((hidden, weight, bias, targets, lens, grad))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [1e4, 1e6, 1e12])
+def test_a_large_frame_in_a_large_layer(size, dtype):
+    """The statistics have other tiles here than the gradient of the logits, whose exponentials have to fit them bit for bit."""
+    hidden, weight, bias, targets, lens, grad = ce_problem(3, 400, 7700, 450, dtype, seed=13, lens=[400, 400, 390])
+    hidden[1, 5:80:7] *= size
+    got = ce_run(hidden, weight, bias, targets, lens, grad)
+    assert all(torch.isfinite(x).all() for x in got.values()) and (got["loss"] >= -2.0 ** -20).all()
+    others = torch.ones_like(targets, dtype=torch.bool)
+    others[1, 5:80:7] = False
+    want = ce_expected(hidden, weight, bias, torch.where(others, targets, -1), lens, grad)
+    for k in ("loss", "hidden"):
+        close(got[k][others], want[k][0][others], want[k][1][others], k)
+    # a large frame's probabilities are 0 and 1: its gradient is the difference of two rows of the weights, or nothing
+    z = hidden[1, 5:80:7].double() @ weight.double().T + bias.double()
+    two = z.topk(2).values
+    sure = two[:, 0] - two[:, 1] > (hidden[1, 5:80:7].double().abs() @ weight.double().abs().T).amax(1) * 460 * EPS_HALVES + 100
+    rows = weight.double()[z.argmax(1)] - weight.double()[targets[1, 5:80:7].long()]
+    exact = rows * grad[1, 5:80:7].double()[:, None]
+    error = (got["hidden"][1, 5:80:7].double() - exact).abs()
+    allowed = (rows.abs() + 2 * weight.double().abs().max()) * grad[1, 5:80:7].double().abs()[:, None] * (4 * EPS16 if dtype == torch.bfloat16 else 8 * EPS_HALVES) + 1e-30
+    assert (error <= allowed)[sure].all()
+    assert sure.any() or size < 1e5
