@@ -10,7 +10,7 @@ import sysconfig
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 TRAINING = os.path.join(CSRC, "training")
-TRAINING_SOURCES = ("cross_entropy.hip", "recurrence.hip", "adamw.hip", "status.hip")
+TRAINING_SOURCES = ("cross_entropy.hip", "delta.hip", "logp.hip", "orth.hip", "recurrence.hip", "adamw.hip", "status.hip")
 OUT = os.path.join(PKG, "fbw")
 LIB = os.path.join(OUT, "libi6fbw.so")
 EXT = os.path.join(OUT, "fbw_core" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
@@ -24,6 +24,20 @@ HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
 def _run(cmd):
     print(" ".join(cmd), flush=True)
     subprocess.check_call(cmd)
+
+
+def _compile(cmd):
+    """Runs a compiler that reports on its kernels, and returns its remarks; what else it says is printed."""
+    import re
+    print(" ".join(cmd), flush=True)
+    done = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    other = [l for l in done.stdout.splitlines()
+             if "-Rpass-analysis=kernel-resource-usage" not in l and not re.match(r"^\s*(\d+ )?\|", l)]     # (and the source lines quoted with them)
+    if other:
+        print("\n".join(other), flush=True)
+    if done.returncode != 0:
+        raise subprocess.CalledProcessError(done.returncode, cmd)
+    return done.stdout
 
 
 def kernel_resources(remarks):
@@ -64,17 +78,17 @@ def build_lib(out_root=PKG, sub="fbw", name="libi6fbw.so", folder=CSRC, sources=
     import json
     lib = os.path.join(out_root, sub, name)
     os.makedirs(os.path.dirname(lib), exist_ok=True)
-    cmd = [HIPCC, *HIP_FLAGS, "-shared", "-Rpass-analysis=kernel-resource-usage", *(os.path.join(folder, s) for s in sources), "-o", lib]
-    print(" ".join(cmd), flush=True)
-    done = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    remarks = done.stdout
-    import re
-    other = [l for l in remarks.splitlines()
-             if "-Rpass-analysis=kernel-resource-usage" not in l and not re.match(r"^\s*(\d+ )?\|", l)]     # (and the source lines quoted with them)
-    if other:
-        print("\n".join(other), flush=True)
-    if done.returncode != 0:
-        raise subprocess.CalledProcessError(done.returncode, cmd)
+    flags = [*HIP_FLAGS, "-Rpass-analysis=kernel-resource-usage"]
+    if len(sources) == 1:
+        remarks = _compile([HIPCC, *flags, "-shared", os.path.join(folder, sources[0]), "-o", lib])
+    else:       # every source by itself, side by side
+        import tempfile
+        from concurrent.futures import ThreadPoolExecutor
+        with tempfile.TemporaryDirectory() as made, ThreadPoolExecutor(min(8, len(sources))) as pool:
+            objects = [os.path.join(made, os.path.splitext(s)[0] + ".o") for s in sources]
+            commands = [[HIPCC, *flags, "-c", os.path.join(folder, s), "-o", o] for s, o in zip(sources, objects)]
+            remarks = "\n".join(pool.map(_compile, commands))
+            _run([HIPCC, *HIP_FLAGS, "-shared", *objects, "-o", lib])
     record = kernel_resources(remarks)
     record["_sources_sha256"] = sources_digest(folder)
     with open(os.path.join(out_root, sub, "kernel_resources.json"), "w") as f:

@@ -1,0 +1,1042 @@
+// Gated delta rule over the frames of a batch (include/i6delta.h):  S' = f S,  S = S' + k (w (v - S'^T k))^T,  o = S^T q.
+//
+// Chunks of C frames.  With c_i the sum of log f up to frame i of a chunk, D_ij = exp(c_i - c_j) and S0 the state in front of it, the rows
+// u_i = w_i (v_i - S'_i^T k_i) that are written solve a triangular system, and all else are products:
+//   (1 + A) U = R,  R = w (V - exp(c) K S0),  A_ij = w_i D_ij k_i.k_j (j < i)
+//   O = exp(c) Q S0 + P U,  P_ij = D_ij q_i.k_j (j <= i);   S1 = exp(c_C) S0 + (exp(c_C - c) K)^T U
+// Backward, with G1 the gradient of S1, from the last chunk to the first:
+//   dU = P^T dO + exp(c_C - c) K G1,  (1 + A)^T dR = dU,  dV = w dR,  G0 = exp(c_C) G1 + (exp(c) Q)^T dO - (w exp(c) K)^T dR
+// and from S0, G1, U and dR of a chunk all gradients of its q, k, gates, for all chunks at once (delta_gradients).
+//
+// Every column of the state goes its own way: a wave has columns of its own, their states in registers as they come out of the matrix
+// instructions, which is also how these take them for their second operand (with the order of k that both operands share), so states, R, U, O and their
+// gradients never leave the wave; K, Q, A and P go through LDS.
+#include <cmath>
+
+#include "train_common.h"
+#include "../../../include/i6delta.h"
+
+namespace i6train {
+namespace {
+
+using acc_t = float __attribute__((ext_vector_type(4)));
+using bf16x8 = bf16 __attribute__((ext_vector_type(8)));
+
+constexpr float kNormEps = 1e-6f;
+constexpr int kThreads = 256;
+constexpr int kC = 32;                   // frames of a chunk
+
+struct Rows {                            // of the chunks' frames, [B][H][chunks C]
+    float c, c_rest;                     // sum of log f within the chunk, as two floats
+    float w, rk, rq, pad0, pad1, pad2;   // share, 1 / length of key and query
+};
+
+struct Args {
+    const void *q, *k, *v, *gate, *beta;
+    int64_t q_b, q_t, q_g, k_b, k_t, k_g, v_b, v_t, v_h, gate_b, gate_t, gate_h, beta_b, beta_t, beta_h;
+    const int32_t* lens;
+    const float* initial;
+    int B, T, H, G, K, V, chunks;
+    void* o;
+    float* last;
+    Rows* rows;                          // null: not for training
+    float *states, *u;                   // [B][H][chunks][K][V], [B][H][chunks C][V]
+    // backward
+    const void* d_o;
+    int64_t do_b, do_t, do_h;
+    const float* d_last;
+    float *ends, *dr, *d_initial;        // gradients of the states behind the chunks, of R
+    void *d_q, *d_k, *d_v, *d_gate, *d_beta;
+    float *d_q_head, *d_k_head;          // [B][T][H][K], where heads share keys
+};
+
+__device__ __forceinline__ float exp_fast(float x) { return exp2_fast(x * kLog2e); }
+__device__ __forceinline__ int len_of(const Args& a, int b) {
+    if (!a.lens) return a.T;
+    const int n = a.lens[b];
+    return n < 0 ? 0 : (n > a.T ? a.T : n);
+}
+__device__ __forceinline__ float log_sigmoid(float x) { return fminf(x, 0.f) - log1pf(expf(-fabsf(x))); }
+__device__ __forceinline__ float sigmoid(float x) {
+    const float e = expf(-fabsf(x));
+    return (x >= 0.f ? 1.f : e) / (1.f + e);
+}
+
+// 16 bytes of a row of `n` values from value `at` on; zeros behind them.
+template <typename T> struct Piece {
+    static constexpr int kN = 16 / sizeof(T);
+    using type = T __attribute__((ext_vector_type(kN)));
+};
+template <typename T> __device__ __forceinline__ typename Piece<T>::type load_piece(const T* row, int at, int n, bool whole) {
+    using P = typename Piece<T>::type;
+    if (whole && at + Piece<T>::kN <= n) return *reinterpret_cast<const P*>(row + at);
+    P p;
+#pragma unroll
+    for (int i = 0; i < Piece<T>::kN; i++) p[i] = at + i < n ? row[at + i] : (T)0.f;
+    return p;
+}
+
+// -------------------------------------------------------------------------------------------------- products of 16 x 16 x 16
+// An accumulator: lane l has column l & 15 and rows 4 (l >> 4) .. + 3.  Of the second operand a lane has k = 4 (l >> 4) .. + 3 of its column:
+// an accumulator is one as it is.  Of the first operand it has the same k of row l & 15.
+__device__ __forceinline__ acc_t product(acc_t a, acc_t b, acc_t c) {
+#if __HIP_DEVICE_COMPILE__
+#pragma unroll
+    for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+#endif
+    return c;
+}
+
+// A matrix in LDS, rows of kStride floats.
+template <int kStride> struct Tile {
+    float* p;
+    // first operand: rows 16 m .., k 16 n ..
+    __device__ __forceinline__ acc_t rows(int m, int n) const {
+        const int lane = threadIdx.x & 63;
+        return *reinterpret_cast<const acc_t*>(p + (16 * m + (lane & 15)) * kStride + 16 * n + 4 * (lane >> 4));
+    }
+    // the transpose as first operand: its rows are columns 16 m .., its k are rows 16 n ..
+    __device__ __forceinline__ acc_t columns(int m, int n) const {
+        const int lane = threadIdx.x & 63;
+        const float* at = p + (16 * n + 4 * (lane >> 4)) * kStride + 16 * m + (lane & 15);
+        acc_t v;
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = at[i * kStride];
+        return v;
+    }
+    __device__ __forceinline__ void put(int m, int n, acc_t v) const {
+        const int lane = threadIdx.x & 63;
+        float* at = p + (16 * m + 4 * (lane >> 4)) * kStride + 16 * n + (lane & 15);
+#pragma unroll
+        for (int i = 0; i < 4; i++) at[i * kStride] = v[i];
+    }
+};
+
+// What stands behind is not moved in front: loads and their addresses would otherwise fill the registers.
+__device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }
+
+__device__ __forceinline__ acc_t four(const float* p) { return *reinterpret_cast<const acc_t*>(p); }
+
+// ------------------------------------------------------------------------------------------------------ a chunk's matrices
+
+// What a chunk's workgroup holds of keys, queries and decays in LDS.
+template <int KP> struct Chunk {
+    static constexpr int kStride = KP + 4, kSquare = kC + 4;
+    float k[kC * kStride], q[kC * kStride];
+    float a[kC * kSquare], p[kC * kSquare], inverse[kC * 20];
+    float c[kC], c_rest[kC], w[kC], rk[kC], rq[kC];
+    float from_start[kC], to_end[kC];    // exp(c), exp(c_C - c)
+};
+
+// Keys and queries of a chunk, loaded ahead: kPer pieces of each for a thread.
+template <typename T, int KP> struct Ahead {
+    static constexpr int kPieces = KP / Piece<T>::kN, kThreadsPerRow = kThreads / kC, kPer = (kPieces + kThreadsPerRow - 1) / kThreadsPerRow;
+    typename Piece<T>::type k[kPer], q[kPer];
+    float gate, beta;
+    __device__ __forceinline__ void fetch(const Args& a, int b, int h, int first, int len, bool whole) {
+        const int row = threadIdx.x / kThreadsPerRow, j = threadIdx.x % kThreadsPerRow, t = first + row;
+        const int g = h / (a.H / a.G);
+        const T* kr = static_cast<const T*>(a.k) + b * a.k_b + t * a.k_t + g * a.k_g;
+        const T* qr = static_cast<const T*>(a.q) + b * a.q_b + t * a.q_t + g * a.q_g;
+        const typename Piece<T>::type none = {};
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int at = (i * kThreadsPerRow + j) * Piece<T>::kN;
+            const bool there = t < len && at < a.K;
+            k[i] = there ? load_piece(kr, at, a.K, whole) : none;
+            q[i] = there ? load_piece(qr, at, a.K, whole) : none;
+        }
+        if (threadIdx.x < kC) {
+            const int tt = first + threadIdx.x;
+            const bool there = tt < len;
+            gate = there ? (float)static_cast<const T*>(a.gate)[b * a.gate_b + tt * a.gate_t + h * a.gate_h] : 0.f;
+            beta = there ? (float)static_cast<const T*>(a.beta)[b * a.beta_b + tt * a.beta_t + h * a.beta_h] : 0.f;
+        }
+    }
+    // to LDS, with lengths, shares and decays.  The sum of log f is taken in 64 bits: differences of it are what counts, and it may be far larger.
+    __device__ __forceinline__ void store(Chunk<KP>& s, int first, int len) {
+        const int row = threadIdx.x / kThreadsPerRow, j = threadIdx.x % kThreadsPerRow;
+        float kk = 0.f, qq = 0.f;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int at = (i * kThreadsPerRow + j) * Piece<T>::kN;
+#pragma unroll
+            for (int e = 0; e < Piece<T>::kN; e++) {
+                kk = fmaf((float)k[i][e], (float)k[i][e], kk);
+                qq = fmaf((float)q[i][e], (float)q[i][e], qq);
+            }
+            if (at < KP) {
+#pragma unroll
+                for (int e = 0; e < Piece<T>::kN; e++) {
+                    s.k[row * Chunk<KP>::kStride + at + e] = (float)k[i][e];
+                    s.q[row * Chunk<KP>::kStride + at + e] = (float)q[i][e];
+                }
+            }
+        }
+#pragma unroll
+        for (int m = 1; m < kThreadsPerRow; m *= 2) {
+            kk += __shfl_xor(kk, m);
+            qq += __shfl_xor(qq, m);
+        }
+        if (j == 0) {
+            s.rk[row] = 1.f / sqrtf(kk + kNormEps);
+            s.rq[row] = 1.f / sqrtf(qq + kNormEps);
+        }
+        if (threadIdx.x < kWave) {
+            const int i = threadIdx.x;
+            const bool there = i < kC && first + i < len;
+            // a gate of -inf: a factor that is 0, and sums that stay numbers
+            double c = there ? (double)fmaxf(log_sigmoid(gate), -1e6f) : 0.0;
+#pragma unroll
+            for (int m = 1; m < kC; m *= 2) {
+                const double before = __shfl_up(c, m);
+                if (i >= m) c += before;
+            }
+            const double end = __shfl(c, kC - 1);
+            if (i < kC) {
+                const float hi = (float)c;
+                s.c[i] = hi;
+                s.c_rest[i] = (float)(c - (double)hi);
+                s.w[i] = there ? sigmoid(beta) : 0.f;
+                s.from_start[i] = exp_fast(hi);
+                s.to_end[i] = exp_fast((float)(end - c));
+            }
+        }
+    }
+};
+
+// Row of the n-th block of a lower triangle.
+__device__ __forceinline__ int block_row(int n) {
+    int i = 0;
+    while ((i + 1) * (i + 2) / 2 <= n) i++;
+    return i;
+}
+
+// A (strictly lower) and P (lower) of the chunk into LDS, without the blocks above the diagonal.
+template <int KP> __device__ __forceinline__ void squares(Chunk<KP>& s) {
+    constexpr int M = kC / 16;
+    const Tile<Chunk<KP>::kStride> k{s.k};
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll 1
+    for (int n = wave; n < M * (M + 1); n += 4) {       // lower blocks, of A and P in turn
+        const int which = n & 1, i = block_row(n >> 1), j = (n >> 1) - i * (i + 1) / 2;
+        const Tile<Chunk<KP>::kStride> left{which ? s.q : s.k};
+        acc_t v = 0.f;
+#pragma unroll
+        for (int x = 0; x < KP / 16; x++) v = product(left.rows(i, x), k.rows(j, x), v);
+        const int col = 16 * j + (lane & 15), row = 16 * i + 4 * (lane >> 4);
+        const float c = s.c[col], c_rest = s.c_rest[col], r = s.rk[col];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int at = row + e;
+            const float d = exp_fast((s.c[at] - c) + (s.c_rest[at] - c_rest));
+            const float by = which ? s.rq[at] : s.rk[at] * s.w[at];
+            v[e] = (which ? col <= at : col < at) ? v[e] * r * d * by : 0.f;
+        }
+        Tile<Chunk<KP>::kSquare>{which ? s.p : s.a}.put(i, j, v);
+    }
+}
+
+// The inverses of 1 + A's blocks on the diagonal, a block for a wave, by substitution: sixteen lanes have four rows, which they solve among themselves, and what
+// these rows take from those below is a product.  (The product of 1 + A's powers would need fewer steps, but with keys that are alike its terms are thousands of times
+// larger than the result.)
+template <int KP> __device__ __forceinline__ void invert(Chunk<KP>& s) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, group = lane >> 4, col = lane & 15;
+    if (wave >= kC / 16) return;
+    const acc_t row = -Tile<Chunk<KP>::kSquare>{s.a}.rows(wave, wave);
+    const float* block = s.a + (16 * wave + 4 * group) * Chunk<KP>::kSquare + 16 * wave + 4 * group;
+    const acc_t l1 = four(block + Chunk<KP>::kSquare), l2 = four(block + 2 * Chunk<KP>::kSquare), l3 = four(block + 3 * Chunk<KP>::kSquare);
+    acc_t t = 0.f, left;
+#pragma unroll
+    for (int i = 0; i < 4; i++) left[i] = 4 * group + i == col ? 1.f : 0.f;
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+        acc_t x = left;
+        x[1] = fmaf(-l1[0], x[0], x[1]);
+        x[2] = fmaf(-l2[1], x[1], fmaf(-l2[0], x[0], x[2]));
+        x[3] = fmaf(-l3[2], x[2], fmaf(-l3[1], x[1], fmaf(-l3[0], x[0], x[3])));
+        const acc_t none = 0.f;
+        x = group == g ? x : none;
+        t += x;
+        if (g < 3) left = product(row, x, left);
+    }
+    Tile<20>{s.inverse}.put(wave, 0, t);
+}
+
+// Columns of a wave: NT for each lane, next to each other.
+template <int NT> struct Columns {
+    int first;                           // this lane's
+    __device__ __forceinline__ explicit Columns(int block) : first((block * 4 + (int)(threadIdx.x >> 6)) * 16 * NT + (int)(threadIdx.x & 15) * NT) {}
+};
+
+// Values of `T` at rows 16 m + 4 (lane >> 4) + r of a matrix, as accumulators.
+template <typename T, int NT, int M>
+__device__ __forceinline__ void load_columns(acc_t (&v)[M][NT], const T* p, int64_t stride, int rows, int col, int cols) {
+    const int at = 4 * ((threadIdx.x & 63) >> 4);
+    p += at * stride + col;
+    asm volatile("" : "+v"(p));       // rows' addresses are formed here, or the compiler keeps them all from chunk to chunk
+#pragma unroll
+    for (int m = 0; m < M; m++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const bool there = 16 * m + at + e < rows;
+#pragma unroll
+            for (int j = 0; j < NT; j++) v[m][j][e] = there && col + j < cols ? (float)p[j] : 0.f;
+            p += stride;
+        }
+        p += 12 * stride;
+    }
+}
+template <typename T, int NT, int M>
+__device__ __forceinline__ void store_columns(const acc_t (&v)[M][NT], T* p, int64_t stride, int rows, int col, int cols) {
+    const int at = 4 * ((threadIdx.x & 63) >> 4);
+    p += at * stride + col;
+    asm volatile("" : "+v"(p));       // rows' addresses are formed here, or the compiler keeps them all from chunk to chunk
+#pragma unroll
+    for (int m = 0; m < M; m++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const bool there = 16 * m + at + e < rows;
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+                if (there && col + j < cols) p[j] = (T)v[m][j][e];
+            p += stride;
+        }
+        p += 12 * stride;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------- forward
+
+template <typename T, int KP, int NT>
+__global__ __launch_bounds__(kThreads, 2) void delta_forward(Args a, bool whole) {
+    constexpr int M = kC / 16, KT = KP / 16;
+    __shared__ __align__(16) Chunk<KP> s;
+    const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 63, at = 4 * (lane >> 4);
+    const int col = Columns<NT>(blockIdx.x).first;
+    const int len = len_of(a, b), chunks = ceil_div(len, kC);
+    const int64_t head = (int64_t)b * a.H + h;
+    const Tile<Chunk<KP>::kStride> k{s.k}, q{s.q};
+    const Tile<Chunk<KP>::kSquare> ta{s.a}, tp{s.p};
+    const Tile<20> inverse{s.inverse};
+
+    acc_t state[KT][NT];
+    if (a.initial) {
+        load_columns<float, NT, KT>(state, a.initial + head * a.K * a.V, a.V, a.K, col, a.V);
+    } else {
+#pragma unroll
+        for (int i = 0; i < KT; i++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) state[i][j] = 0.f;
+    }
+    Ahead<T, KP> next;
+    acc_t v_next[M][NT];
+    const T* v = static_cast<const T*>(a.v) + b * a.v_b + h * a.v_h;
+    if (chunks) {
+        next.fetch(a, b, h, 0, len, whole);
+        load_columns<T, NT, M>(v_next, v, a.v_t, len, col, a.V);
+    }
+    for (int n = 0; n < chunks; n++) {
+        const int first = n * kC, rows = min(kC, len - first);
+        next.store(s, first, len);
+        acc_t r[M][NT];
+#pragma unroll
+        for (int m = 0; m < M; m++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) r[m][j] = v_next[m][j];
+        if (a.states) store_columns<float, NT, KT>(state, a.states + (head * a.chunks + n) * a.K * a.V, a.V, a.K, col, a.V);
+        __syncthreads();
+        if (n + 1 < chunks) {
+            next.fetch(a, b, h, first + kC, len, whole);
+            load_columns<T, NT, M>(v_next, v + (first + kC) * a.v_t, a.v_t, len - first - kC, col, a.V);
+        }
+        phase();
+        squares(s);
+        if (a.rows && blockIdx.x == 0 && threadIdx.x < kC) {
+            const int i = threadIdx.x;
+            a.rows[head * a.chunks * kC + first + i] = Rows{s.c[i], s.c_rest[i], s.w[i], s.rk[i], s.rq[i], 0.f, 0.f, 0.f};
+        }
+        __syncthreads();
+        invert(s);
+        phase();
+        // R = w (V - exp(c) K S0)
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+            acc_t ks[NT] = {};
+#pragma unroll
+            for (int x = 0; x < KT; x++) {
+                const acc_t row = k.rows(m, x);
+#pragma unroll
+                for (int j = 0; j < NT; j++) ks[j] = product(row, state[x][j], ks[j]);
+            }
+            const acc_t by = four(s.from_start + 16 * m + at) * four(s.rk + 16 * m + at), w = four(s.w + 16 * m + at);
+#pragma unroll
+            for (int j = 0; j < NT; j++) r[m][j] = w * (r[m][j] - by * ks[j]);
+        }
+        __syncthreads();
+        // U, sixteen frames after sixteen
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+#pragma unroll
+            for (int x = 0; x < m; x++) {
+                const acc_t row = -ta.rows(m, x);
+#pragma unroll
+                for (int j = 0; j < NT; j++) r[m][j] = product(row, r[x][j], r[m][j]);
+            }
+            const acc_t row = inverse.rows(m, 0);
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                const acc_t none = 0.f;
+                r[m][j] = product(row, r[m][j], none);
+            }
+        }
+        if (a.u) store_columns<float, NT, M>(r, a.u + (head * a.chunks * kC + first) * a.V, a.V, kC, col, a.V);
+        acc_t o[M][NT];
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+#pragma unroll
+            for (int j = 0; j < NT; j++) o[m][j] = 0.f;
+#pragma unroll
+            for (int x = 0; x < KT; x++) {
+                const acc_t row = q.rows(m, x);
+#pragma unroll
+                for (int j = 0; j < NT; j++) o[m][j] = product(row, state[x][j], o[m][j]);
+            }
+            const acc_t by = four(s.from_start + 16 * m + at) * four(s.rq + 16 * m + at);
+#pragma unroll
+            for (int j = 0; j < NT; j++) o[m][j] *= by;
+#pragma unroll
+            for (int x = 0; x <= m; x++) {
+                const acc_t row = tp.rows(m, x);
+#pragma unroll
+                for (int j = 0; j < NT; j++) o[m][j] = product(row, r[x][j], o[m][j]);
+            }
+        }
+        store_columns<T, NT, M>(o, static_cast<T*>(a.o) + (((int64_t)b * a.T + first) * a.H + h) * a.V, (int64_t)a.H * a.V, rows, col, a.V);
+        // the state behind the chunk
+        const float decay = s.from_start[kC - 1];
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+            const acc_t by = four(s.to_end + 16 * m + at) * four(s.rk + 16 * m + at);
+#pragma unroll
+            for (int j = 0; j < NT; j++) r[m][j] *= by;
+        }
+#pragma unroll
+        for (int i = 0; i < KT; i++) {
+#pragma unroll
+            for (int j = 0; j < NT; j++) state[i][j] *= decay;
+#pragma unroll
+            for (int m = 0; m < M; m++) {
+                const acc_t row = k.columns(i, m);
+#pragma unroll
+                for (int j = 0; j < NT; j++) state[i][j] = product(row, r[m][j], state[i][j]);
+            }
+        }
+        __syncthreads();
+    }
+    store_columns<float, NT, KT>(state, a.last + head * a.K * a.V, a.V, a.K, col, a.V);
+    for (int t = len + (int)(threadIdx.x >> 6); t < a.T; t += 4) {
+        T* o = static_cast<T*>(a.o) + (((int64_t)b * a.T + t) * a.H + h) * a.V;
+        for (int c = blockIdx.x * 64 * NT + lane; c < min(a.V, (int)(blockIdx.x + 1) * 64 * NT); c += 64) o[c] = (T)0.f;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------ frame by frame
+
+// Few frames, no training: 64 columns of a head, KP / 4 rows of the state in the registers of each of four waves.  The state is read and written once; with
+// x = S^T k and y = S^T q of the state in front of a frame,  u = w (v - f x),  o = f y + (k.q) u.
+template <typename T, int KP>
+__global__ __launch_bounds__(kThreads) void delta_frames(Args a) {
+    constexpr int R = KP / 4;
+    __shared__ __align__(16) float key[KP], query[KP], sums[4][2][64], dots[2][3];
+    const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
+    const int len = len_of(a, b), g = h / (a.H / a.G);
+    const int64_t head = (int64_t)b * a.H + h;
+    const bool mine = col < a.V;
+    float state[R];
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        const int row = wave * R + i;
+        state[i] = a.initial && mine && row < a.K ? a.initial[(head * a.K + row) * a.V + col] : 0.f;
+    }
+    for (int t = 0; t < a.T; t++) {
+        T* o = static_cast<T*>(a.o) + (((int64_t)b * a.T + t) * a.H + h) * a.V;
+        if (t >= len) {
+            if (wave == 0 && mine) o[col] = (T)0.f;
+            continue;
+        }
+        const T* kr = static_cast<const T*>(a.k) + b * a.k_b + t * a.k_t + g * a.k_g;
+        const T* qr = static_cast<const T*>(a.q) + b * a.q_b + t * a.q_t + g * a.q_g;
+        const float v = mine ? (float)static_cast<const T*>(a.v)[b * a.v_b + t * a.v_t + h * a.v_h + col] : 0.f;
+        const float gate = (float)static_cast<const T*>(a.gate)[b * a.gate_b + t * a.gate_t + h * a.gate_h];
+        const float beta = (float)static_cast<const T*>(a.beta)[b * a.beta_b + t * a.beta_t + h * a.beta_h];
+        if (wave < 2) {                  // KP <= 128: two values a lane
+            const int i = wave * 64 + lane;
+            const float kv = i < a.K ? (float)kr[i] : 0.f, qv = i < a.K ? (float)qr[i] : 0.f;
+            if (i < KP) {
+                key[i] = kv;
+                query[i] = qv;
+            }
+            const float kk = wave_sum(kv * kv), qq = wave_sum(qv * qv), kq = wave_sum(kv * qv);
+            if (lane == 0) {
+                dots[wave][0] = kk;
+                dots[wave][1] = qq;
+                dots[wave][2] = kq;
+            }
+        }
+        __syncthreads();
+        const float rk = 1.f / sqrtf(dots[0][0] + dots[1][0] + kNormEps), rq = 1.f / sqrtf(dots[0][1] + dots[1][1] + kNormEps);
+        const float kq = (dots[0][2] + dots[1][2]) * rk * rq, f = expf(log_sigmoid(gate)), w = sigmoid(beta);
+        float x = 0.f, y = 0.f, kv[R];
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            kv[i] = key[wave * R + i];
+            x = fmaf(state[i], kv[i], x);
+            y = fmaf(state[i], query[wave * R + i], y);
+        }
+        sums[wave][0][lane] = x;
+        sums[wave][1][lane] = y;
+        __syncthreads();
+        x = ((sums[0][0][lane] + sums[1][0][lane]) + (sums[2][0][lane] + sums[3][0][lane])) * rk;
+        y = ((sums[0][1][lane] + sums[1][1][lane]) + (sums[2][1][lane] + sums[3][1][lane])) * rq;
+        const float u = w * (v - f * x);
+        if (wave == 0 && mine) o[col] = (T)fmaf(kq, u, f * y);
+        const float uk = u * rk;
+#pragma unroll
+        for (int i = 0; i < R; i++) state[i] = fmaf(kv[i], uk, f * state[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        const int row = wave * R + i;
+        if (mine && row < a.K) a.last[(head * a.K + row) * a.V + col] = state[i];
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------ backward
+
+// From the last chunk to the first: gradients of the states behind the chunks, of R and of v.
+template <typename T, int KP, int NT>
+__global__ __launch_bounds__(kThreads, 2) void delta_backward(Args a, bool whole) {
+    constexpr int M = kC / 16, KT = KP / 16;
+    __shared__ __align__(16) Chunk<KP> s;
+    const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 63, at = 4 * (lane >> 4);
+    const int col = Columns<NT>(blockIdx.x).first;
+    const int len = len_of(a, b), chunks = ceil_div(len, kC);
+    const int64_t head = (int64_t)b * a.H + h;
+    const Tile<Chunk<KP>::kStride> k{s.k}, q{s.q};
+    const Tile<Chunk<KP>::kSquare> ta{s.a}, tp{s.p};
+    const Tile<20> inverse{s.inverse};
+
+    acc_t d[KT][NT];
+    if (a.d_last) {
+        load_columns<float, NT, KT>(d, a.d_last + head * a.K * a.V, a.V, a.K, col, a.V);
+    } else {
+#pragma unroll
+        for (int i = 0; i < KT; i++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) d[i][j] = 0.f;
+    }
+    Ahead<T, KP> next;
+    acc_t o_next[M][NT] = {};
+    const T* d_o = static_cast<const T*>(a.d_o) + b * a.do_b + h * a.do_h;
+    const auto fetch = [&](int first) {
+        next.fetch(a, b, h, first, len, whole);
+        if (a.d_o) load_columns<T, NT, M>(o_next, d_o + first * a.do_t, a.do_t, len - first, col, a.V);
+    };
+    if (chunks) fetch((chunks - 1) * kC);
+    for (int n = chunks - 1; n >= 0; n--) {
+        const int first = n * kC, rows = min(kC, len - first);
+        next.store(s, first, len);
+        acc_t o[M][NT], r[M][NT];
+#pragma unroll
+        for (int m = 0; m < M; m++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) o[m][j] = o_next[m][j];
+        store_columns<float, NT, KT>(d, a.ends + (head * a.chunks + n) * a.K * a.V, a.V, a.K, col, a.V);
+        __syncthreads();
+        if (n) fetch(first - kC);
+        phase();
+        squares(s);
+        __syncthreads();
+        invert(s);
+        phase();
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+#pragma unroll
+            for (int j = 0; j < NT; j++) r[m][j] = 0.f;
+#pragma unroll
+            for (int x = 0; x < KT; x++) {
+                const acc_t row = k.rows(m, x);
+#pragma unroll
+                for (int j = 0; j < NT; j++) r[m][j] = product(row, d[x][j], r[m][j]);
+            }
+            const acc_t by = four(s.to_end + 16 * m + at) * four(s.rk + 16 * m + at);
+#pragma unroll
+            for (int j = 0; j < NT; j++) r[m][j] *= by;
+#pragma unroll
+            for (int x = m; x < M; x++) {
+                const acc_t row = tp.columns(m, x);
+#pragma unroll
+                for (int j = 0; j < NT; j++) r[m][j] = product(row, o[x][j], r[m][j]);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int m = M - 1; m >= 0; m--) {
+#pragma unroll
+            for (int x = m + 1; x < M; x++) {
+                const acc_t row = -ta.columns(m, x);
+#pragma unroll
+                for (int j = 0; j < NT; j++) r[m][j] = product(row, r[x][j], r[m][j]);
+            }
+            const acc_t row = inverse.columns(0, m);
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                const acc_t none = 0.f;
+                r[m][j] = product(row, r[m][j], none);
+            }
+        }
+        store_columns<float, NT, M>(r, a.dr + (head * a.chunks * kC + first) * a.V, a.V, kC, col, a.V);
+        acc_t dv[M][NT];
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+            const acc_t w = four(s.w + 16 * m + at), start = four(s.from_start + 16 * m + at);
+            const acc_t by_q = start * four(s.rq + 16 * m + at), by_k = -start * four(s.rk + 16 * m + at);
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                dv[m][j] = r[m][j] * w;
+                o[m][j] *= by_q;
+                r[m][j] = dv[m][j] * by_k;
+            }
+        }
+        store_columns<T, NT, M>(dv, static_cast<T*>(a.d_v) + (((int64_t)b * a.T + first) * a.H + h) * a.V, (int64_t)a.H * a.V, rows, col, a.V);
+        phase();
+        const float decay = s.from_start[kC - 1];
+#pragma unroll
+        for (int i = 0; i < KT; i++) {
+#pragma unroll
+            for (int j = 0; j < NT; j++) d[i][j] *= decay;
+#pragma unroll
+            for (int m = 0; m < M; m++) {
+                const acc_t row_q = q.columns(i, m), row_k = k.columns(i, m);
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    d[i][j] = product(row_q, o[m][j], d[i][j]);
+                    d[i][j] = product(row_k, r[m][j], d[i][j]);
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (a.d_initial) store_columns<float, NT, KT>(d, a.d_initial + head * a.K * a.V, a.V, a.K, col, a.V);
+    for (int t = len + (int)(threadIdx.x >> 6); t < a.T; t += 4) {
+        T* dv = static_cast<T*>(a.d_v) + (((int64_t)b * a.T + t) * a.H + h) * a.V;
+        for (int c = blockIdx.x * 64 * NT + lane; c < min(a.V, (int)(blockIdx.x + 1) * 64 * NT); c += 64) dv[c] = (T)0.f;
+    }
+}
+
+// Four values of a row of a float matrix with V columns; zeros behind them.
+__device__ __forceinline__ acc_t load_four(const float* row, int at, int n, bool whole) {
+    if (whole) return at < n ? *reinterpret_cast<const acc_t*>(row + at) : acc_t{0.f, 0.f, 0.f, 0.f};
+    acc_t v;
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = at + i < n ? row[at + i] : 0.f;
+    return v;
+}
+
+// All other gradients of a chunk, from the state in front of it, the gradient of that behind it, U and dR:
+//   dq^ = exp(c) dO S0^T + Z K^,   dk^ = exp(c_C - c) U G1^T - w exp(c) dR S0^T + Z^T Q^ + (E + E^T) K^,   Z = D (dO U^T),  E = - w D (dR U^T)
+// (lower triangles, E's without its diagonal).  What decays with c_i is a row's dot product with its query's gradient and the part of its key's that stands on
+// the left; what decays with - c_j that with the other part; so the gradient of c needs no products of its own, nor A and P.
+template <typename T, int KP>
+__global__ __launch_bounds__(kThreads, 2) void delta_gradients(Args a) {
+    constexpr int M = kC / 16, N = KP == 128 ? 2 : 1, kV = 128 + 4, kSquare = kC + 4;
+    __shared__ __align__(16) float s_o[kC * kV], s_u[kC * kV], s_r[kC * kV], s_z[kC * kSquare], s_e[kC * kSquare];
+    __shared__ __align__(16) float s_c[kC], s_rest[kC], s_w[kC], s_rk[kC], s_rq[kC], s_start[kC], s_end[kC], s_dots[4][kC][4], s_whole[4], s_gate[kC];
+    const int b = blockIdx.z, h = blockIdx.y, n = blockIdx.x, first = n * kC;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = 4 * (lane >> 4);
+    const int len = len_of(a, b), live = min(kC, len - first), rows = min(kC, a.T - first), g = h / (a.H / a.G);
+    const int64_t head = (int64_t)b * a.H + h, frame = (int64_t)b * a.T + first;
+    const int col = wave * 16 * N + (lane & 15) * N;
+    T* dq = static_cast<T*>(a.d_q) + (frame * a.G + g) * a.K;
+    T* dk = static_cast<T*>(a.d_k) + (frame * a.G + g) * a.K;
+    float* dq_head = a.d_q_head + (frame * a.H + h) * a.K;
+    float* dk_head = a.d_k_head + (frame * a.H + h) * a.K;
+    const auto store = [&](const acc_t (&v)[M][N], bool keys) {
+        if (a.d_q_head) store_columns<float, N, M>(v, keys ? dk_head : dq_head, (int64_t)a.H * a.K, rows, col, a.K);
+        else store_columns<T, N, M>(v, keys ? dk : dq, (int64_t)a.G * a.K, rows, col, a.K);
+    };
+    T* d_gate = static_cast<T*>(a.d_gate) + frame * a.H + h;
+    T* d_beta = static_cast<T*>(a.d_beta) + frame * a.H + h;
+    if (live <= 0) {
+        acc_t none[M][N] = {};
+        if (col < KP) {
+            store(none, false);
+            store(none, true);
+        }
+        if ((int)threadIdx.x < rows) {
+            d_gate[threadIdx.x * a.H] = (T)0.f;
+            d_beta[threadIdx.x * a.H] = (T)0.f;
+        }
+        return;
+    }
+
+    const bool whole = a.V % 4 == 0;
+    const int cols = (a.V + 15) / 16 * 16;
+    {
+        constexpr int kPerRow = kThreads / kC;
+        const int row = threadIdx.x / kPerRow, j = threadIdx.x % kPerRow;
+        const float* u = a.u + (head * a.chunks * kC + first + row) * a.V;
+        const float* r = a.dr + (head * a.chunks * kC + first + row) * a.V;
+        const T* d_o = static_cast<const T*>(a.d_o) + b * a.do_b + (first + row) * a.do_t + h * a.do_h;
+        float ru = 0.f;
+        for (int c = j * 4; c < cols; c += kPerRow * 4) {
+            const acc_t uv = load_four(u, c, a.V, whole), rv = load_four(r, c, a.V, whole);
+            acc_t ov;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                ov[i] = a.d_o && row < live && c + i < a.V ? (float)d_o[c + i] : 0.f;
+                ru = fmaf(uv[i], rv[i], ru);
+            }
+            *reinterpret_cast<acc_t*>(s_u + row * kV + c) = uv;
+            *reinterpret_cast<acc_t*>(s_r + row * kV + c) = rv;
+            *reinterpret_cast<acc_t*>(s_o + row * kV + c) = ov;
+        }
+#pragma unroll
+        for (int m = 1; m < kPerRow; m *= 2) ru += __shfl_xor(ru, m);
+        // u = w (v - ...), so dw = dR.u / w, times w (1 - w)
+        if (j == 0 && row < rows) {
+            const float beta = row < live ? (float)static_cast<const T*>(a.beta)[b * a.beta_b + (first + row) * a.beta_t + h * a.beta_h] : 0.f;
+            d_beta[row * a.H] = (T)(row < live ? ru * sigmoid(-beta) : 0.f);
+        }
+        if (threadIdx.x < kC) {
+            const int i = threadIdx.x;
+            const Rows x = a.rows[head * a.chunks * kC + first + i], end = a.rows[head * a.chunks * kC + first + kC - 1];
+            s_c[i] = x.c; s_rest[i] = x.c_rest; s_w[i] = x.w; s_rk[i] = x.rk; s_rq[i] = x.rq;
+            s_start[i] = exp_fast(x.c);
+            s_end[i] = exp_fast((end.c - x.c) + (end.c_rest - x.c_rest));
+        }
+    }
+    __syncthreads();
+    const Tile<kV> to{s_o}, tu{s_u}, tr{s_r};
+    const Tile<kSquare> tz{s_z}, te{s_e};
+    const int blocks = cols / 16;
+    acc_t yq[M][N] = {}, yp[M][N] = {}, ym[M][N] = {};
+    float crossed = 0.f;                 // <S1, G1>, what decays with c_C
+    if (col < KP) {
+        const float* states = a.states + (head * a.chunks + n) * a.K * a.V;
+        const float* ends = a.ends + (head * a.chunks + n) * a.K * a.V;
+#pragma unroll 1
+        for (int x = 0; x < blocks; x++) {
+            acc_t sv[N], gv[N];
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                const bool there = col + j < a.K;
+                sv[j] = there ? load_four(states + (int64_t)(col + j) * a.V, 16 * x + at, a.V, whole) : acc_t{0.f, 0.f, 0.f, 0.f};
+                gv[j] = there ? load_four(ends + (int64_t)(col + j) * a.V, 16 * x + at, a.V, whole) : acc_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < 4; i++) crossed = fmaf(sv[j][i], gv[j][i], crossed);
+            }
+#pragma unroll
+            for (int m = 0; m < M; m++) {
+                const acc_t o = to.rows(m, x), r = tr.rows(m, x), u = tu.rows(m, x);
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    yq[m][j] = product(o, sv[j], yq[m][j]);
+                    yp[m][j] = product(r, sv[j], yp[m][j]);
+                    ym[m][j] = product(u, gv[j], ym[m][j]);
+                }
+            }
+        }
+        crossed *= s_start[kC - 1];
+    }
+    {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < M; i++)
+#pragma unroll
+            for (int j = 0; j <= i; j++)
+#pragma unroll
+                for (int which = 0; which < 2; which++) {
+                    if ((c++ & 3) != wave) continue;
+                    acc_t v = 0.f;
+#pragma unroll 1
+                    for (int x = 0; x < blocks; x++) v = product(which ? tr.rows(i, x) : to.rows(i, x), tu.rows(j, x), v);
+                    const int column = 16 * j + (lane & 15), row = 16 * i + at;
+                    const float cc = s_c[column], rest = s_rest[column], rk = s_rk[column];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int t = row + e;
+                        const float decay = exp_fast((s_c[t] - cc) + (s_rest[t] - rest));
+                        const float by = which ? -s_w[t] * s_rk[t] : s_rq[t];
+                        v[e] = (which ? column < t : column <= t) ? v[e] * decay * rk * by : 0.f;
+                    }
+                    (which ? te : tz).put(i, j, v);
+                }
+    }
+    __syncthreads();
+    acc_t kv[M][N], qv[M][N];
+    if (col < KP) {
+        load_columns<T, N, M>(kv, static_cast<const T*>(a.k) + b * a.k_b + first * a.k_t + g * a.k_g, a.k_t, live, col, a.K);
+        load_columns<T, N, M>(qv, static_cast<const T*>(a.q) + b * a.q_b + first * a.q_t + g * a.q_g, a.q_t, live, col, a.K);
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+            const acc_t start = four(s_start + 16 * m + at), rk = four(s_rk + 16 * m + at);
+            const acc_t by_q = start * four(s_rq + 16 * m + at), by_p = -start * rk * four(s_w + 16 * m + at), by_m = four(s_end + 16 * m + at) * rk;
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                yq[m][j] *= by_q;
+                yp[m][j] *= by_p;
+                ym[m][j] *= by_m;
+#pragma unroll
+                for (int e = 0; e < 4; e++) crossed = fmaf(ym[m][j][e], kv[m][j][e], crossed);
+            }
+#pragma unroll
+            for (int x = 0; x <= m; x++) {
+                const acc_t z = tz.rows(m, x), e = te.rows(m, x);
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    yq[m][j] = product(z, kv[x][j], yq[m][j]);
+                    yp[m][j] = product(e, kv[x][j], yp[m][j]);
+                }
+            }
+#pragma unroll
+            for (int x = m; x < M; x++) {
+                const acc_t z = tz.columns(m, x), e = te.columns(m, x);
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    ym[m][j] = product(z, qv[x][j], ym[m][j]);
+                    ym[m][j] = product(e, kv[x][j], ym[m][j]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                float dots[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    dots[0] = fmaf(qv[m][j][e], yq[m][j][e], dots[0]);
+                    dots[1] = fmaf(kv[m][j][e], yp[m][j][e], dots[1]);
+                    dots[2] = fmaf(kv[m][j][e], ym[m][j][e], dots[2]);
+                }
+#pragma unroll
+                for (int i = 0; i < 3; i++) {
+#pragma unroll
+                    for (int x = 1; x < 16; x *= 2) dots[i] += __shfl_xor(dots[i], x);
+                    if ((lane & 15) == 0) s_dots[wave][16 * m + at + e][i] = dots[i];
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int m = 0; m < M; m++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int i = 0; i < 3; i++)
+                    if ((lane & 15) == 0) s_dots[wave][16 * m + at + e][i] = 0.f;
+    }
+    crossed = wave_sum(crossed);
+    if (lane == 0) s_whole[wave] = crossed;
+    __syncthreads();
+    const auto dot = [&](int row, int i) { return (s_dots[0][row][i] + s_dots[1][row][i]) + (s_dots[2][row][i] + s_dots[3][row][i]); };
+    if (col < KP) {
+#pragma unroll
+        for (int m = 0; m < M; m++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int row = 16 * m + at + e;
+                const float rq = s_rq[row], rk = s_rk[row];
+                const float q_off = rq * rq * dot(row, 0), k_off = rk * rk * (dot(row, 1) + dot(row, 2));
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    yq[m][j][e] = yq[m][j][e] - qv[m][j][e] * q_off;
+                    yp[m][j][e] = (yp[m][j][e] + ym[m][j][e]) - kv[m][j][e] * k_off;
+                }
+            }
+        store(yq, false);
+        store(yp, true);
+    }
+    if (wave == 0) {
+        // of log f: what decays over the frame, a sum over the frames from it to the chunk's end
+        float d = 0.f;
+        if (lane < kC) {
+            d = (dot(lane, 0) + dot(lane, 1)) - dot(lane, 2);
+            if (lane == kC - 1) d += (s_whole[0] + s_whole[1]) + (s_whole[2] + s_whole[3]);
+        }
+#pragma unroll
+        for (int m = 1; m < kC; m *= 2) {
+            const float behind = __shfl_down(d, m);
+            if (lane + m < kC) d += behind;
+        }
+        if (lane < rows) {
+            const float gate = lane < live ? (float)static_cast<const T*>(a.gate)[b * a.gate_b + (first + lane) * a.gate_t + h * a.gate_h] : 0.f;
+            d_gate[lane * a.H] = (T)(lane < live ? d * sigmoid(-gate) : 0.f);
+        }
+    }
+}
+
+// Gradients of keys and queries that heads share: the sum over these.
+template <typename T> __global__ __launch_bounds__(kThreads) void delta_shared(Args a) {
+    const int64_t n = (int64_t)a.B * a.T * a.G * a.K;
+    const int each = a.H / a.G;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
+        const int64_t row = i / a.K;
+        const float* q = a.d_q_head + (row * each) * a.K + i % a.K;
+        const float* k = a.d_k_head + (row * each) * a.K + i % a.K;
+        float sq = 0.f, sk = 0.f;
+        for (int j = 0; j < each; j++) {
+            sq += q[(int64_t)j * a.K];
+            sk += k[(int64_t)j * a.K];
+        }
+        static_cast<T*>(a.d_q)[i] = (T)sq;
+        static_cast<T*>(a.d_k)[i] = (T)sk;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- host
+
+constexpr int kMostFrames = 16;          // frame by frame up to this many
+
+int checked(const i6delta_problem* p) {
+    if (!p || p->B <= 0 || p->T <= 0 || p->H <= 0 || p->G <= 0 || p->K <= 0 || p->V <= 0 || p->H % p->G || !valid_dtype(p->dtype) || !p->q || !p->k || !p->v || !p->gate ||
+        !p->beta)
+        return I6TRAIN_ERR_INVALID_ARGUMENT;
+    if (p->B > 65535 || p->H > 65535 || p->K > 128 || p->V > 128 || p->T > (1 << 30) || (int64_t)p->B * p->H * ceil_div(p->T, kC) >= (1 << 24)) return I6TRAIN_ERR_TOO_LARGE;
+    return I6TRAIN_OK;
+}
+
+Args args_of(const i6delta_problem& p) {
+    Args a{};
+    a.q = p.q; a.k = p.k; a.v = p.v; a.gate = p.gate; a.beta = p.beta;
+    a.q_b = p.q_stride_b; a.q_t = p.q_stride_t; a.q_g = p.q_stride_g;
+    a.k_b = p.k_stride_b; a.k_t = p.k_stride_t; a.k_g = p.k_stride_g;
+    a.v_b = p.v_stride_b; a.v_t = p.v_stride_t; a.v_h = p.v_stride_h;
+    a.gate_b = p.gate_stride_b; a.gate_t = p.gate_stride_t; a.gate_h = p.gate_stride_h;
+    a.beta_b = p.beta_stride_b; a.beta_t = p.beta_stride_t; a.beta_h = p.beta_stride_h;
+    a.lens = p.seq_lens; a.initial = p.initial;
+    a.B = p.B; a.T = p.T; a.H = p.H; a.G = p.G; a.K = p.K; a.V = p.V;
+    a.chunks = ceil_div(p.T, kC);
+    return a;
+}
+
+// Whether keys and queries can be read in pieces of 16 bytes.
+bool whole_pieces(const i6delta_problem& p) {
+    const size_t n = elem_size(p.dtype);
+    const auto whole = [&](const void* x, int64_t s0, int64_t s1, int64_t s2) {
+        return (uintptr_t)x % 16 == 0 && (s0 * (int64_t)n) % 16 == 0 && (s1 * (int64_t)n) % 16 == 0 && (s2 * (int64_t)n) % 16 == 0;
+    };
+    return whole(p.q, p.q_stride_b, p.q_stride_t, p.q_stride_g) && whole(p.k, p.k_stride_b, p.k_stride_t, p.k_stride_g);
+}
+
+struct Sizes {
+    size_t rows, states, u, heads;
+    explicit Sizes(const i6delta_problem& p) {
+        const size_t n = (size_t)p.B * p.H * ceil_div(p.T, kC);
+        rows = align256(n * kC * sizeof(Rows));
+        states = align256(n * p.K * p.V * sizeof(float));
+        u = align256(n * kC * p.V * sizeof(float));
+        heads = p.H > p.G ? align256((size_t)p.B * p.T * p.H * p.K * sizeof(float)) : 0;
+    }
+    size_t kept() const { return rows + states + u; }
+    size_t back() const { return states + u + 2 * heads; }
+};
+
+template <typename T, int KP, int NT> void run_forward(const Args& a, bool whole, hipStream_t s) {
+    delta_forward<T, KP, NT><<<dim3(ceil_div(a.V, 64 * NT), a.H, a.B), dim3(kThreads), 0, s>>>(a, whole);
+}
+template <typename T, int KP, int NT> void run_backward(const Args& a, bool whole, hipStream_t s) {
+    delta_backward<T, KP, NT><<<dim3(ceil_div(a.V, 64 * NT), a.H, a.B), dim3(kThreads), 0, s>>>(a, whole);
+}
+
+template <typename T, int KP> int forward(const Args& a, bool whole, hipStream_t s) {
+    if (!a.rows && a.T <= kMostFrames) {
+        delta_frames<T, KP><<<dim3(ceil_div(a.V, 64), a.H, a.B), dim3(kThreads), 0, s>>>(a);
+    } else if (a.V > 64) {
+        run_forward<T, KP, 2>(a, whole, s);
+    } else {
+        run_forward<T, KP, 1>(a, whole, s);
+    }
+    return launched();
+}
+
+template <typename T, int KP> int backward(const Args& a, bool whole, hipStream_t s) {
+    if (a.V > 64) run_backward<T, KP, 2>(a, whole, s); else run_backward<T, KP, 1>(a, whole, s);
+    I6TRAIN_TRY(launched());
+    delta_gradients<T, KP><<<dim3(a.chunks, a.H, a.B), dim3(kThreads), 0, s>>>(a);
+    I6TRAIN_TRY(launched());
+    if (a.d_q_head) {
+        const int64_t n = (int64_t)a.B * a.T * a.G * a.K, groups = ceil_div(n, (int64_t)kThreads);
+        delta_shared<T><<<dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(kThreads), 0, s>>>(a);
+    }
+    return launched();
+}
+
+template <typename T> int forward_of(const Args& a, bool whole, hipStream_t s) {
+    return a.K <= 32 ? forward<T, 32>(a, whole, s) : (a.K <= 64 ? forward<T, 64>(a, whole, s) : forward<T, 128>(a, whole, s));
+}
+template <typename T> int backward_of(const Args& a, bool whole, hipStream_t s) {
+    return a.K <= 32 ? backward<T, 32>(a, whole, s) : (a.K <= 64 ? backward<T, 64>(a, whole, s) : backward<T, 128>(a, whole, s));
+}
+
+}  // namespace
+}  // namespace i6train
+
+using namespace i6train;
+
+extern "C" {
+
+int i6delta_sizes(const i6delta_problem* p, int train, size_t* kept_bytes, size_t* forward_bytes, size_t* backward_bytes) {
+    I6TRAIN_TRY(checked(p));
+    if (!kept_bytes || !forward_bytes || !backward_bytes) return I6TRAIN_ERR_INVALID_ARGUMENT;
+    const Sizes n(*p);
+    *kept_bytes = train ? n.kept() : 0;
+    *forward_bytes = 0;
+    *backward_bytes = train ? n.back() : 0;
+    return I6TRAIN_OK;
+}
+
+int i6delta_forward(const i6delta_problem* p, void* o, float* last, void* kept, size_t kept_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+    I6TRAIN_TRY(checked(p));
+    if (!o || !last) return I6TRAIN_ERR_INVALID_ARGUMENT;
+    Args a = args_of(*p);
+    a.o = o; a.last = last;
+    if (kept) {
+        const Sizes n(*p);
+        if (kept_bytes < n.kept()) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
+        char* at = static_cast<char*>(kept);
+        a.rows = reinterpret_cast<Rows*>(at);
+        a.states = reinterpret_cast<float*>(at + n.rows);
+        a.u = reinterpret_cast<float*>(at + n.rows + n.states);
+    }
+    (void)workspace; (void)workspace_bytes;
+    const bool whole = whole_pieces(*p);
+    return p->dtype == I6TRAIN_F32 ? forward_of<float>(a, whole, (hipStream_t)stream) : forward_of<bf16>(a, whole, (hipStream_t)stream);
+}
+
+int i6delta_backward(const i6delta_problem* p, const void* grad_o, int64_t grad_stride_b, int64_t grad_stride_t, int64_t grad_stride_h, const float* grad_last, const void* kept,
+                     size_t kept_bytes, void* grad_q, void* grad_k, void* grad_v, void* grad_gate, void* grad_beta, float* grad_initial, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+    I6TRAIN_TRY(checked(p));
+    if (!kept || !workspace || !grad_q || !grad_k || !grad_v || !grad_gate || !grad_beta) return I6TRAIN_ERR_INVALID_ARGUMENT;
+    const Sizes n(*p);
+    if (kept_bytes < n.kept() || workspace_bytes < n.back()) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
+    Args a = args_of(*p);
+    char* at = static_cast<char*>(const_cast<void*>(kept));
+    a.rows = reinterpret_cast<Rows*>(at);
+    a.states = reinterpret_cast<float*>(at + n.rows);
+    a.u = reinterpret_cast<float*>(at + n.rows + n.states);
+    a.d_o = grad_o; a.do_b = grad_stride_b; a.do_t = grad_stride_t; a.do_h = grad_stride_h;
+    a.d_last = grad_last;
+    a.d_q = grad_q; a.d_k = grad_k; a.d_v = grad_v; a.d_gate = grad_gate; a.d_beta = grad_beta; a.d_initial = grad_initial;
+    at = static_cast<char*>(workspace);
+    a.ends = reinterpret_cast<float*>(at);
+    a.dr = reinterpret_cast<float*>(at + n.states);
+    if (n.heads) {
+        a.d_q_head = reinterpret_cast<float*>(at + n.states + n.u);
+        a.d_k_head = reinterpret_cast<float*>(at + n.states + n.u + n.heads);
+    }
+    const bool whole = whole_pieces(*p);
+    return p->dtype == I6TRAIN_F32 ? backward_of<float>(a, whole, (hipStream_t)stream) : backward_of<bf16>(a, whole, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -2,6 +2,7 @@
 // stream and the autograd graph; all arithmetic is behind the C ABI declared in include/i6train.h.  The graph's nodes
 // are C++: the smallest training steps take as long as their host work, of which nodes in Python would be the larger part.
 #include <optional>
+#include <string>
 #include <tuple>
 #include <vector>
 
@@ -11,6 +12,9 @@
 #include <torch/extension.h>
 
 #include "../../../include/i6fbw.h"
+#include "../../../include/i6delta.h"
+#include "../../../include/i6logp.h"
+#include "../../../include/i6orth.h"
 #include "../../../include/i6train.h"
 
 namespace {
@@ -41,13 +45,13 @@ void raise_reported(const char* prefix) {
 }
 
 // As the status mode of the other modules says: not at all, by waiting, or by a later call.
-void report(hipStream_t stream) {
+void report(hipStream_t stream, const char* op = "linear_cross_entropy") {
     const int mode = i6fbw_get_status_mode();
     if (mode == 0) return;
     hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing(stream, &capture) != hipSuccess || capture != hipStreamCaptureStatusNone) return;
     if (mode == 1) TORCH_CHECK(hipStreamSynchronize(stream) == hipSuccess, "NativeOp: HIP call failed");
-    raise_reported(mode == 1 ? "NativeOp: linear_cross_entropy: " : "NativeOp: an earlier call reported: ");
+    raise_reported(mode == 1 ? (std::string("NativeOp: ") + op + ": ").c_str() : "NativeOp: an earlier call reported: ");
 }
 
 void check_status() {
@@ -339,11 +343,17 @@ void adamw_step(const std::vector<torch::Tensor>& params, const std::vector<torc
     check("adamw_step", rc);
 }
 
+#include "more_torch.inc"
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("linear_cross_entropy", &linear_cross_entropy, "loss (B, T)");
     m.def("gated_recurrence", &gated_recurrence, "h (B, T, D), last (B, D)");
     m.def("adamw_step", &adamw_step, "One AdamW step over lists of tensors, in place");
+    m.def("target_log_probs", &target_log_probs, "log_prob (B, T), entropy (B, T), top_log_probs (B, T, k), top_classes (B, T, k)");
+    m.def("gated_delta_rule", &gated_delta_rule, "o (B, T, H, V), last (B, H, K, V)");
+    m.def("orthogonalize", &orthogonalize, "The orthogonal factors of matrices");
+    m.def("muon_step", &muon_step, "One step on the orthogonal factors of the averaged gradients, in place");
     m.def("check_status", &check_status, "Waits for the device and raises the first problem that kernels of earlier calls reported");
 }
