@@ -367,14 +367,13 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_backward
     // the row is in memory before single classes of it are written again
     __threadfence();
     G::meet();
-    if (thread < k + 1) {
-        const int32_t* best = a.top_class + frame * k;
-        const int c = thread < k ? best[thread] : y;
+    const int32_t* best = a.top_class + frame * k;
+    for (int i = thread; i <= k; i += kThreads) {
+        const int c = i < k ? best[i] : y;
         bool there = c >= 0 && c < a.F;
-        float more = thread < k ? mine : gl;
-        if (thread < k && c == y) more += gl;
-        if (thread == k)
-            for (int i = 0; i < k; i++) there = there && best[i] != y;      // the alternative's thread has it
+        float more = i < k ? (a.g_top ? a.g_top[frame * k + i] : 0.f) + (c == y ? gl : 0.f) : gl;
+        if (i == k)
+            for (int j = 0; j < k; j++) there = there && best[j] != y;      // the alternative's thread has it
         if (there) to[c] = (T)(share((float)from[c]) + more);
     }
 }

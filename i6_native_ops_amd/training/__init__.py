@@ -151,6 +151,16 @@ def adamw_step(
     core.adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales or [], int(step), lr, betas[0], betas[1], eps, weight_decay)
 
 
+def _load_states(optimizer: torch.optim.Optimizer, state_dict: dict) -> None:
+    """The states keep their own types, which the base class would turn into those of the parameters."""
+    torch.optim.Optimizer.load_state_dict(optimizer, state_dict)
+    names = [i for g in state_dict["param_groups"] for i in g["params"]]
+    params = [p for g in optimizer.param_groups for p in g["params"]]
+    for name, p in zip(names, params):
+        if name in state_dict["state"]:
+            optimizer.state[p] = {k: v.detach().clone().to(p.device) if torch.is_tensor(v) else v for k, v in state_dict["state"][name].items()}
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW on ``adamw_step``: one launch for the tensors of a parameter group.  ``step`` is not for capture into a graph, whose
     replays would all be the same step, and refuses it.
@@ -206,13 +216,7 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """The states keep their own types, which the base class would turn into those of the parameters."""
-        super().load_state_dict(state_dict)
-        names = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
-        for name, p in zip(names, params):
-            if name in state_dict["state"]:
-                self.state[p] = {k: v.detach().clone().to(p.device) if torch.is_tensor(v) else v for k, v in state_dict["state"][name].items()}
+        _load_states(self, state_dict)
 
 
 def orthogonalize(updates: Sequence[torch.Tensor], steps: int = 5) -> List[torch.Tensor]:
@@ -293,4 +297,5 @@ class Muon(torch.optim.Optimizer):
                           group["weight_decay"], group["steps"], group["adjust_lr"])
         return loss
 
-    load_state_dict = AdamW.load_state_dict
+    def load_state_dict(self, state_dict):
+        _load_states(self, state_dict)

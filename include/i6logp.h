@@ -15,7 +15,8 @@
  *
  * Gradient, for the incoming gl of log_prob, ge of entropy and gt of top (float, contiguous; each may be null):
  *   grad_logits_f = gl [f = y] + sum_j gt_j [f = top_class_j] - p_f (gl + sum_j gt_j + ge (log p_f + entropy))
- * written completely, contiguous, of `dtype`, zeros behind the end, NaN where y >= F.  Sums and statistics are held in 32 bits.
+ * written completely, contiguous, of `dtype`, zeros behind the end, NaN where y >= F.  Sums and statistics are held in 32 bits; shares below 2^-126 of a
+ * frame's largest are 0.
  * Sizes: F up to 2^28; B T below 2^22, below 2^26 where F is 512 or less; larger ones are I6TRAIN_ERR_TOO_LARGE.
  */
 #ifndef I6LOGP_H
