@@ -893,6 +893,8 @@ template <typename T> __global__ __launch_bounds__(kThreads) void delta_shared(A
     }
 }
 
+#include "delta_16.inc"
+
 // ---------------------------------------------------------------------------------------------------------------- host
 
 constexpr int kMostFrames = 16;          // frame by frame up to this many
@@ -915,7 +917,7 @@ Args args_of(const i6delta_problem& p) {
     a.beta_b = p.beta_stride_b; a.beta_t = p.beta_stride_t; a.beta_h = p.beta_stride_h;
     a.lens = p.seq_lens; a.initial = p.initial;
     a.B = p.B; a.T = p.T; a.H = p.H; a.G = p.G; a.K = p.K; a.V = p.V;
-    a.chunks = ceil_div(p.T, kC);
+    a.chunks = ceil_div(p.T, p.dtype == I6TRAIN_BF16 ? kC16 : kC);
     return a;
 }
 
@@ -928,41 +930,73 @@ bool whole_pieces(const i6delta_problem& p) {
     return whole(p.q, p.q_stride_b, p.q_stride_t, p.q_stride_g) && whole(p.k, p.k_stride_b, p.k_stride_t, p.k_stride_g);
 }
 
-struct Sizes {
-    size_t rows, states, u, heads;
-    explicit Sizes(const i6delta_problem& p) {
-        const size_t n = (size_t)p.B * p.H * ceil_div(p.T, kC);
-        rows = align256(n * kC * sizeof(Rows));
-        states = align256(n * p.K * p.V * sizeof(float));
-        u = align256(n * kC * p.V * sizeof(float));
-        heads = p.H > p.G ? align256((size_t)p.B * p.T * p.H * p.K * sizeof(float)) : 0;
+int padded_keys(int K) { return K <= 32 ? 32 : (K <= 64 ? 64 : 128); }
+
+// Where the parts of a call's memory are.
+struct Places {
+    size_t rows, states, states_factor, u, u_factor, kept;           // kept
+    size_t ends, ends_factor, dr, dr_factor, d_q, d_k, back;         // the backward workspace
+    int pairs;
+    explicit Places(const i6delta_problem& p) {
+        const bool x16 = p.dtype == I6TRAIN_BF16;
+        const int C = x16 ? kC16 : kC, KP = padded_keys(p.K);
+        const size_t n = (size_t)p.B * p.H * ceil_div(p.T, C);
+        pairs = p.V > 64 ? 4 : 2;
+        const size_t s = align256(x16 ? n * KP * pairs * 32 * sizeof(f16) : n * p.K * p.V * sizeof(float)), f = x16 ? align256(n * 2 * pairs * sizeof(float)) : 0;
+        const size_t r = align256(x16 ? n * C * pairs * 32 * sizeof(f16) : n * C * p.V * sizeof(float));
+        const size_t heads = p.H > p.G ? align256((size_t)p.B * p.T * p.H * p.K * sizeof(float)) : 0;
+        rows = 0;
+        states = align256(n * C * sizeof(Rows));
+        states_factor = states + s;
+        u = states_factor + f;
+        u_factor = u + r;
+        kept = u_factor + f;
+        ends = 0;
+        ends_factor = s;
+        dr = ends_factor + f;
+        dr_factor = dr + r;
+        d_q = dr_factor + f;
+        d_k = d_q + heads;
+        back = d_k + heads;
     }
-    size_t kept() const { return rows + states + u; }
-    size_t back() const { return states + u + 2 * heads; }
 };
 
-template <typename T, int KP, int NT> void run_forward(const Args& a, bool whole, hipStream_t s) {
-    delta_forward<T, KP, NT><<<dim3(ceil_div(a.V, 64 * NT), a.H, a.B), dim3(kThreads), 0, s>>>(a, whole);
+struct Call {
+    Args a;
+    Args16 k16;
+    bool whole;
+};
+
+template <int KP> void run_forward(const Call& c, hipStream_t s, float) {
+    const Args& a = c.a;
+    if (a.V > 64) delta_forward<float, KP, 2><<<dim3(ceil_div(a.V, 128), a.H, a.B), dim3(kThreads), 0, s>>>(a, c.whole);
+    else delta_forward<float, KP, 1><<<dim3(1, a.H, a.B), dim3(kThreads), 0, s>>>(a, c.whole);
 }
-template <typename T, int KP, int NT> void run_backward(const Args& a, bool whole, hipStream_t s) {
-    delta_backward<T, KP, NT><<<dim3(ceil_div(a.V, 64 * NT), a.H, a.B), dim3(kThreads), 0, s>>>(a, whole);
+template <int KP> void run_forward(const Call& c, hipStream_t s, bf16) {
+    delta_forward16<KP><<<dim3(ceil_div(c.a.V, 64), c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.k16, c.whole);
+}
+template <int KP> void run_backward(const Call& c, hipStream_t s, float) {
+    const Args& a = c.a;
+    if (a.V > 64) delta_backward<float, KP, 2><<<dim3(ceil_div(a.V, 128), a.H, a.B), dim3(kThreads), 0, s>>>(a, c.whole);
+    else delta_backward<float, KP, 1><<<dim3(1, a.H, a.B), dim3(kThreads), 0, s>>>(a, c.whole);
+    delta_gradients<float, KP><<<dim3(a.chunks, a.H, a.B), dim3(kThreads), 0, s>>>(a);
+}
+template <int KP> void run_backward(const Call& c, hipStream_t s, bf16) {
+    delta_backward16<KP><<<dim3(ceil_div(c.a.V, 64), c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.k16, c.whole);
+    if (c.k16.pairs == 4) delta_gradients16<KP, 4><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(512), 0, s>>>(c.a, c.k16, c.whole);
+    else delta_gradients16<KP, 2><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(512), 0, s>>>(c.a, c.k16, c.whole);
 }
 
-template <typename T, int KP> int forward(const Args& a, bool whole, hipStream_t s) {
-    if (!a.rows && a.T <= kMostFrames) {
-        delta_frames<T, KP><<<dim3(ceil_div(a.V, 64), a.H, a.B), dim3(kThreads), 0, s>>>(a);
-    } else if (a.V > 64) {
-        run_forward<T, KP, 2>(a, whole, s);
-    } else {
-        run_forward<T, KP, 1>(a, whole, s);
-    }
+template <typename T, int KP> int forward(const Call& c, hipStream_t s) {
+    const Args& a = c.a;
+    if (!a.rows && a.T <= kMostFrames) delta_frames<T, KP><<<dim3(ceil_div(a.V, 64), a.H, a.B), dim3(kThreads), 0, s>>>(a);
+    else run_forward<KP>(c, s, T());
     return launched();
 }
 
-template <typename T, int KP> int backward(const Args& a, bool whole, hipStream_t s) {
-    if (a.V > 64) run_backward<T, KP, 2>(a, whole, s); else run_backward<T, KP, 1>(a, whole, s);
-    I6TRAIN_TRY(launched());
-    delta_gradients<T, KP><<<dim3(a.chunks, a.H, a.B), dim3(kThreads), 0, s>>>(a);
+template <typename T, int KP> int backward(const Call& c, hipStream_t s) {
+    const Args& a = c.a;
+    run_backward<KP>(c, s, T());
     I6TRAIN_TRY(launched());
     if (a.d_q_head) {
         const int64_t n = (int64_t)a.B * a.T * a.G * a.K, groups = ceil_div(n, (int64_t)kThreads);
@@ -971,11 +1005,35 @@ template <typename T, int KP> int backward(const Args& a, bool whole, hipStream_
     return launched();
 }
 
-template <typename T> int forward_of(const Args& a, bool whole, hipStream_t s) {
-    return a.K <= 32 ? forward<T, 32>(a, whole, s) : (a.K <= 64 ? forward<T, 64>(a, whole, s) : forward<T, 128>(a, whole, s));
+template <typename T> int forward_of(const Call& c, hipStream_t s) {
+    switch (padded_keys(c.a.K)) {
+        case 32: return forward<T, 32>(c, s);
+        case 64: return forward<T, 64>(c, s);
+        default: return forward<T, 128>(c, s);
+    }
 }
-template <typename T> int backward_of(const Args& a, bool whole, hipStream_t s) {
-    return a.K <= 32 ? backward<T, 32>(a, whole, s) : (a.K <= 64 ? backward<T, 64>(a, whole, s) : backward<T, 128>(a, whole, s));
+template <typename T> int backward_of(const Call& c, hipStream_t s) {
+    switch (padded_keys(c.a.K)) {
+        case 32: return backward<T, 32>(c, s);
+        case 64: return backward<T, 64>(c, s);
+        default: return backward<T, 128>(c, s);
+    }
+}
+
+Call call_of(const i6delta_problem& p, const Places& at, void* kept) {
+    Call c{};
+    c.a = args_of(p);
+    c.whole = whole_pieces(p);
+    c.k16.pairs = at.pairs;
+    if (kept) {
+        char* base = static_cast<char*>(kept);
+        c.a.rows = reinterpret_cast<Rows*>(base + at.rows);
+        c.a.states = reinterpret_cast<float*>(base + at.states);
+        c.a.u = reinterpret_cast<float*>(base + at.u);
+        c.k16.states = {reinterpret_cast<f16*>(base + at.states), reinterpret_cast<float*>(base + at.states_factor)};
+        c.k16.u = {reinterpret_cast<f16*>(base + at.u), reinterpret_cast<float*>(base + at.u_factor)};
+    }
+    return c;
 }
 
 }  // namespace
@@ -988,29 +1046,22 @@ extern "C" {
 int i6delta_sizes(const i6delta_problem* p, int train, size_t* kept_bytes, size_t* forward_bytes, size_t* backward_bytes) {
     I6TRAIN_TRY(checked(p));
     if (!kept_bytes || !forward_bytes || !backward_bytes) return I6TRAIN_ERR_INVALID_ARGUMENT;
-    const Sizes n(*p);
-    *kept_bytes = train ? n.kept() : 0;
+    const Places at(*p);
+    *kept_bytes = train ? at.kept : 0;
     *forward_bytes = 0;
-    *backward_bytes = train ? n.back() : 0;
+    *backward_bytes = train ? at.back : 0;
     return I6TRAIN_OK;
 }
 
 int i6delta_forward(const i6delta_problem* p, void* o, float* last, void* kept, size_t kept_bytes, void* workspace, size_t workspace_bytes, void* stream) {
     I6TRAIN_TRY(checked(p));
     if (!o || !last) return I6TRAIN_ERR_INVALID_ARGUMENT;
-    Args a = args_of(*p);
-    a.o = o; a.last = last;
-    if (kept) {
-        const Sizes n(*p);
-        if (kept_bytes < n.kept()) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
-        char* at = static_cast<char*>(kept);
-        a.rows = reinterpret_cast<Rows*>(at);
-        a.states = reinterpret_cast<float*>(at + n.rows);
-        a.u = reinterpret_cast<float*>(at + n.rows + n.states);
-    }
+    const Places at(*p);
+    if (kept && kept_bytes < at.kept) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
     (void)workspace; (void)workspace_bytes;
-    const bool whole = whole_pieces(*p);
-    return p->dtype == I6TRAIN_F32 ? forward_of<float>(a, whole, (hipStream_t)stream) : forward_of<bf16>(a, whole, (hipStream_t)stream);
+    Call c = call_of(*p, at, kept);
+    c.a.o = o; c.a.last = last;
+    return p->dtype == I6TRAIN_F32 ? forward_of<float>(c, (hipStream_t)stream) : forward_of<bf16>(c, (hipStream_t)stream);
 }
 
 int i6delta_backward(const i6delta_problem* p, const void* grad_o, int64_t grad_stride_b, int64_t grad_stride_t, int64_t grad_stride_h, const float* grad_last, const void* kept,
@@ -1018,25 +1069,23 @@ int i6delta_backward(const i6delta_problem* p, const void* grad_o, int64_t grad_
                      size_t workspace_bytes, void* stream) {
     I6TRAIN_TRY(checked(p));
     if (!kept || !workspace || !grad_q || !grad_k || !grad_v || !grad_gate || !grad_beta) return I6TRAIN_ERR_INVALID_ARGUMENT;
-    const Sizes n(*p);
-    if (kept_bytes < n.kept() || workspace_bytes < n.back()) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
-    Args a = args_of(*p);
-    char* at = static_cast<char*>(const_cast<void*>(kept));
-    a.rows = reinterpret_cast<Rows*>(at);
-    a.states = reinterpret_cast<float*>(at + n.rows);
-    a.u = reinterpret_cast<float*>(at + n.rows + n.states);
+    const Places at(*p);
+    if (kept_bytes < at.kept || workspace_bytes < at.back) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
+    Call c = call_of(*p, at, const_cast<void*>(kept));
+    Args& a = c.a;
     a.d_o = grad_o; a.do_b = grad_stride_b; a.do_t = grad_stride_t; a.do_h = grad_stride_h;
     a.d_last = grad_last;
     a.d_q = grad_q; a.d_k = grad_k; a.d_v = grad_v; a.d_gate = grad_gate; a.d_beta = grad_beta; a.d_initial = grad_initial;
-    at = static_cast<char*>(workspace);
-    a.ends = reinterpret_cast<float*>(at);
-    a.dr = reinterpret_cast<float*>(at + n.states);
-    if (n.heads) {
-        a.d_q_head = reinterpret_cast<float*>(at + n.states + n.u);
-        a.d_k_head = reinterpret_cast<float*>(at + n.states + n.u + n.heads);
+    char* base = static_cast<char*>(workspace);
+    a.ends = reinterpret_cast<float*>(base + at.ends);
+    a.dr = reinterpret_cast<float*>(base + at.dr);
+    c.k16.ends = {reinterpret_cast<f16*>(base + at.ends), reinterpret_cast<float*>(base + at.ends_factor)};
+    c.k16.dr = {reinterpret_cast<f16*>(base + at.dr), reinterpret_cast<float*>(base + at.dr_factor)};
+    if (p->H > p->G) {
+        a.d_q_head = reinterpret_cast<float*>(base + at.d_q);
+        a.d_k_head = reinterpret_cast<float*>(base + at.d_k);
     }
-    const bool whole = whole_pieces(*p);
-    return p->dtype == I6TRAIN_F32 ? backward_of<float>(a, whole, (hipStream_t)stream) : backward_of<bf16>(a, whole, (hipStream_t)stream);
+    return p->dtype == I6TRAIN_F32 ? backward_of<float>(c, (hipStream_t)stream) : backward_of<bf16>(c, (hipStream_t)stream);
 }
 
 }  // extern "C"

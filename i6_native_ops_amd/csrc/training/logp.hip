@@ -16,6 +16,7 @@ namespace i6train {
 namespace {
 
 constexpr int kCandidates = 256;
+#define I6_INLINE __attribute__((always_inline))
 
 struct Args {
     const void* logits;
@@ -93,7 +94,7 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_forward(
     const int64_t frame = (int64_t)blockIdx.x * kTeams + team;
     if (frame >= (int64_t)a.B * a.T) return;
     const int thread = G::thread(), lane = threadIdx.x & 63, wave = kWaves == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int b = (int)(frame / a.T), t = (int)(frame % a.T), k = a.k;
+    const int b = (int)((uint32_t)frame / (uint32_t)a.T), t = (int)((uint32_t)frame % (uint32_t)a.T), k = a.k;
     if (t >= a.lens[b]) {
         if (thread == 0) {
             a.log_prob[frame] = 0.f;
@@ -124,35 +125,49 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_forward(
     const int y = a.targets[b * a.t_b + t * a.t_t];
     const float picked = thread == 0 && y >= 0 && y < a.F ? (float)row.p[y] : 0.f;
 
-    // f(score, index) for all scores of this thread; those that fill up are -inf, with indexes of F or more
-    const auto each = [&](auto f) {
+    // f(piece, index of its first score) for all pieces of this thread, those behind the row's end with index F and -inf; then the single score.  All lanes of a
+    // wave together
+    const auto read_pieces = [&](auto f) I6_INLINE {
+        for (int first = 0; first < row.pieces; first += kThreads) {
+            const int at = first + thread;
+            Vector<T> v;
+#pragma unroll
+            for (int e = 0; e < P; e++) v[e] = (T)-INFINITY;
+            if (at < row.pieces) v = row.piece(at);
+            f(v, at < row.pieces ? row.head + at * P : a.F);
+        }
+    };
+    const auto pieces = [&](auto f) I6_INLINE {
         if constexpr (kHeld > 0) {
 #pragma unroll
             for (int i = 0; i < kHeld; i++) {
-                const int at = i * kThreads + thread, first = at < row.pieces ? row.head + at * P : a.F;
-                asm volatile("" : "+v"(held[i]));              // what one pass makes of the scores is not kept for the next
-#pragma unroll
-                for (int e = 0; e < P; e++) f((float)held[i][e], first + e);
+                const int at = i * kThreads + thread;
+                f(held[i], at < row.pieces ? row.head + at * P : a.F);
+                __builtin_amdgcn_sched_barrier(0);             // a few registers besides those of the row
             }
         } else {
-            for (int at = thread; at < row.pieces; at += kThreads) {
-                const Vector<T> v = row.piece(at);
-#pragma unroll
-                for (int e = 0; e < P; e++) f((float)v[e], row.head + at * P + e);
-            }
+            read_pieces(f);
         }
-        f(single, single_at >= 0 ? single_at : a.F);
     };
+    // what one pass makes of the scores is not kept for the next
+    const auto forget = [&] {
+        if constexpr (kHeld > 0) {
+#pragma unroll
+            for (int i = 0; i < kHeld; i++) asm volatile("" : "+v"(held[i]));
+        }
+    };
+    float most = single;                                       // (NaN is seen by the sums)
+    pieces([&](const Vector<T>& v, int) I6_INLINE {
+#pragma unroll
+        for (int e = 0; e < P; e += 2) most = fmaxf(fmaxf((float)v[e], (float)v[e + 1]), most);
+    });
 
-    float most = -INFINITY;
-    each([&](float z, int) { most = fmaxf(most, z); });      // (NaN is seen by the sums)
-
-    // a bound that k scores reach: the k-th largest of the lanes' largest, to 22 bits
+    // a bound that k scores reach: the k-th largest of the lanes' largest, to 16 bits
     uint32_t bound = 0;
     if (k > 0) {
         const uint32_t key = key_of(most);
 #pragma unroll
-        for (int bit = 31; bit >= 10; bit--) {
+        for (int bit = 31; bit >= 16; bit--) {
             const uint32_t more = bound | (1u << bit);
             if (__builtin_popcountll(__ballot(key >= more)) >= k) bound = more;
         }
@@ -175,18 +190,31 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_forward(
         s.count = 0;
     }
 
-    float rest = 0.f, moment = 0.f;
+    // sums over the scores but the largest, and how many of those there are
+    float rest = 0.f, more = 0.f, moment = 0.f, more_moment = 0.f;
     int n = 0;
-    each([&](float z, int) {
-        const float d = z - m, e = exp2_fast(d * kLog2e);
+    const auto add = [&](float z, float& sum, float& sum_moment) I6_INLINE {
+        const float d = z - m;
         const bool largest = z == m;
-        n += largest;
-        rest += largest ? 0.f : e;
-        moment = fmaf(largest ? 0.f : e, fmaxf(d, -1e30f), moment);      // (0 times -inf)
+        n += __builtin_popcountll(__ballot(largest));
+        const float e = largest ? 0.f : exp2_fast(d * kLog2e);
+        sum += e;
+        sum_moment = fmaf(e, fmaxf(d, -1e30f), sum_moment);      // (0 times -inf)
+    };
+    forget();
+    pieces([&](const Vector<T>& v, int) I6_INLINE {
+#pragma unroll
+        for (int e = 0; e < P; e += 2) {
+            add((float)v[e], rest, moment);
+            add((float)v[e + 1], more, more_moment);
+        }
     });
+    add(single, rest, moment);
+    rest += more;
+    moment += more_moment;
     rest = wave_sum(rest);
     moment = wave_sum(moment);
-    float equal = wave_sum((float)n);                          // (exact up to 2^24 a wave, that is, for all rows there are)
+    float equal = (float)n;                                    // (exact up to 2^24 a wave, that is, for all rows there are)
     if (kWaves > 1) {
         // part[0] is read by all before the waves meet below, and these are other places
         if (lane == 0) {
@@ -202,19 +230,31 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_forward(
             moment += s.part[2][w];
         }
     }
-    // candidates
+    // Candidates, whichever lanes of a wave have one.
+    const auto keep = [&](float z, int at, bool is) I6_INLINE {
+        const uint64_t mask = __ballot(is);
+        if (!mask) return;
+        uint32_t slot = 0;
+        if (lane == 0) slot = atomicAdd(&s.count, (uint32_t)__builtin_popcountll(mask));
+        slot = __builtin_amdgcn_readfirstlane(slot) + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+        if (is && slot < (uint32_t)kCandidates) {
+            s.value[slot] = z;
+            s.index[slot] = at;
+        }
+    };
+    forget();
     if (k > 0) {
         const float least = of_key(bound < 0x007fffffu ? 0x007fffffu : bound);      // -inf at least
         if (kWaves == 1) G::meet();
-        each([&](float z, int at) {
-            if (z >= least && at < a.F) {
-                const uint32_t slot = atomicAdd(&s.count, 1u);
-                if (slot < (uint32_t)kCandidates) {
-                    s.value[slot] = z;
-                    s.index[slot] = at;
-                }
-            }
+        pieces([&](const Vector<T>& v, int at) I6_INLINE {
+            float best = fmaxf((float)v[0], (float)v[1]);
+#pragma unroll
+            for (int e = 2; e < P; e += 2) best = fmaxf(fmaxf((float)v[e], (float)v[e + 1]), best);
+            if (!__any(best >= least)) return;
+#pragma unroll
+            for (int e = 0; e < P; e++) keep((float)v[e], at + e, (float)v[e] >= least && at < a.F);
         });
+        keep(single, single_at, single >= least && single_at >= 0);
     }
     G::meet();
     if (kWaves > 1) {
@@ -228,7 +268,7 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_forward(
     if (m == INFINITY || rest != rest) state = kBad;
     const float ratio = rest / equal, log_total = log2_fast(equal) * kLn2 + log1pf(ratio), total = equal + rest;
     const float entropy = state == kFine ? log_total - moment / total : (state == kEmpty ? 0.f : __builtin_nanf(""));
-    const auto log_p = [&](float z) { return state == kFine ? (z - m) - log_total : (state == kEmpty ? -INFINITY : __builtin_nanf("")); };
+    const auto log_p = [&](float z) I6_INLINE { return state == kFine ? (z - m) - log_total : (state == kEmpty ? -INFINITY : __builtin_nanf("")); };
     if (thread == 0) {
         float v = y < 0 ? 0.f : log_p(picked);
         if (y >= a.F) {
@@ -255,10 +295,17 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_forward(
     }
     int count = (int)s.count;
     if (count > kCandidates) {
-        const auto counted = [&](auto f) {                     // of the row's scores, those with f
-            int c = 0;
-            each([&](float z, int at) { c += at < a.F && f(z, at); });
-            uint32_t sum = wave_reduce((uint32_t)c, 0, [](uint32_t x, uint32_t y) { return x + y; });
+        // from memory, all scores: rows of this kind are few, and with what this needs the others would not keep theirs in registers
+        const auto each = [&](auto f) I6_INLINE {
+            read_pieces([&](const Vector<T>& v, int at) I6_INLINE {
+#pragma unroll
+                for (int e = 0; e < P; e++) f((float)v[e], at + e);
+            });
+            f(single, single_at >= 0 ? single_at : a.F);
+        };
+        const auto counted = [&](auto f) I6_INLINE {                     // of the row's scores, those with f
+            uint32_t sum = 0;
+            each([&](float z, int at) I6_INLINE { sum += __builtin_popcountll(__ballot(at < a.F && f(z, at))); });
             if (kWaves > 1) {
                 __syncthreads();
                 if (lane == 0) s.bound[wave] = sum;
@@ -269,30 +316,30 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_forward(
             }
             return (int)sum;
         };
-        uint32_t kth = 0;
-        for (int bit = 31; bit >= 0; bit--) {
-            const uint32_t more = kth | (1u << bit);
-            if (counted([&](float z, int) { return key_of(z) >= more; }) >= k) kth = more;
+        // between the bound and the largest score; with fewer than k scores above -inf it is that
+        const uint32_t lowest = 0x007fffffu, top = key_of(m);
+        uint32_t kth = lowest;
+        if (bound > lowest || counted([&](float z, int) I6_INLINE { return key_of(z) > lowest; }) >= k) {
+            const int same = bound == top ? 0 : 32 - __builtin_clz(bound ^ top);      // bits in which the two differ, and those behind
+            kth = same == 32 ? 0 : bound >> same << same;
+            for (int bit = same - 1; bit >= 0; bit--) {
+                const uint32_t next = kth | (1u << bit);
+                if (counted([&](float z, int) I6_INLINE { return key_of(z) >= next; }) >= k) kth = next;
+            }
         }
         // the scores that are larger, and equal ones up to the index `last`
-        const int ties = k - counted([&](float z, int) { return key_of(z) > kth; });
+        const int ties = k - counted([&](float z, int) I6_INLINE { return key_of(z) > kth; });
         int last = 0;
-        for (int bit = 30; bit >= 0; bit--) {
-            const int more = last + (1 << bit);
-            if (more < a.F && counted([&](float z, int at) { return key_of(z) == kth && at < more; }) < ties) last = more;
+        for (int bit = 31 - __builtin_clz(a.F); bit >= 0; bit--) {
+            const int next = last + (1 << bit);
+            if (next < a.F && counted([&](float z, int at) I6_INLINE { return key_of(z) == kth && at < next; }) < ties) last = next;
         }
         G::meet();
         if (thread == 0) s.count = 0;
         G::meet();
-        each([&](float z, int at) {
+        each([&](float z, int at) I6_INLINE {
             const uint32_t key = key_of(z);
-            if (at < a.F && (key > kth || (key == kth && at <= last))) {
-                const uint32_t slot = atomicAdd(&s.count, 1u);
-                if (slot < (uint32_t)kCandidates) {
-                    s.value[slot] = z;
-                    s.index[slot] = at;
-                }
-            }
+            keep(z, at, at < a.F && (key > kth || (key == kth && at <= last)));
         });
         G::meet();
         count = min((int)s.count, kCandidates);
@@ -301,6 +348,7 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_forward(
         const float z = s.value[c];
         const int at = s.index[c];
         int place = 0;
+#pragma unroll 8
         for (int i = 0; i < count; i++) {
             const float other = s.value[i];
             place += other > z || (other == z && s.index[i] < at);
@@ -314,15 +362,23 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_forward(
 
 // ------------------------------------------------------------------------------------------------------------ backward
 
-// All classes as if none were a target or an alternative; then those that are again, each by one thread.
+// A target and alternatives are found by the pieces they are in: a bit for each piece, modulo kMarks, and those whose bit is set look through the list.
+constexpr int kMarks = 2048;
+
 template <typename T, int kThreads>
 __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_backward(Args a) {
     using G = Team<kThreads>;
-    constexpr int kTeams = G::kWaves == 1 ? 4 : 1, P = kPiece<T>;
+    constexpr int kTeams = G::kWaves == 1 ? 4 : 1, P = kPiece<T>, kList = I6LOGP_MOST_ALTERNATIVES + 1;
+    __shared__ uint32_t all_marks[kTeams][kMarks / 32];
+    __shared__ int all_class[kTeams][kList];
+    __shared__ float all_more[kTeams][kList];
     const int team = kTeams == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t frame = (int64_t)blockIdx.x * kTeams + team;
     if (frame >= (int64_t)a.B * a.T) return;
-    const int thread = G::thread(), b = (int)(frame / a.T), t = (int)(frame % a.T), k = a.k;
+    uint32_t* marks = all_marks[team];
+    int* classes = all_class[team];
+    float* mores = all_more[team];
+    const int thread = G::thread(), b = (int)((uint32_t)frame / (uint32_t)a.T), t = (int)((uint32_t)frame % (uint32_t)a.T), k = a.k;
     T* to = static_cast<T*>(a.grad) + frame * a.F;
     const Row<T> out(to, a.F);
     const int single = out.single(thread);
@@ -340,41 +396,57 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_backward
     if (state == kEmpty && y < a.F) return fill(0.f);
     if (state != kFine || y >= a.F) return fill(__builtin_nanf(""));
     const float gl = a.g_log_prob && y >= 0 ? a.g_log_prob[frame] : 0.f, ge = a.g_entropy ? a.g_entropy[frame] : 0.f;
-    float gt = 0.f;
     const int lane = threadIdx.x & 63;
-    const float mine = a.g_top && lane < k ? a.g_top[frame * k + lane] : 0.f;
-    gt = wave_sum(mine);
-    const float sum = gl + gt;
+    const float gt = a.g_top && lane < k ? a.g_top[frame * k + lane] : 0.f, sum = gl + wave_sum(gt);
+    for (int i = thread; i < kMarks / 32; i += kThreads) marks[i] = 0;
+    G::meet();
+    // number of the piece of a class; the single ones in front and behind have numbers of their own
+    const auto piece_of = [&](int c) { return (uint32_t)(c - out.head + P) / P; };
+    const auto list = [&](int i, int c, float more) {
+        classes[i] = c;
+        mores[i] = more;
+        if (c >= 0) atomicOr(&marks[piece_of(c) / 32 % (kMarks / 32)], 1u << (piece_of(c) & 31));
+    };
+    if (thread < k) list(thread, a.top_class[frame * k + thread], gt);
+    if (thread == 0) list(k, y, gl);
+    G::meet();
+    const auto marked = [&](int c) { return marks[piece_of(c) / 32 % (kMarks / 32)] >> (piece_of(c) & 31) & 1; };
+    const auto listed = [&](int c) {
+        float more = 0.f;
+        for (int i = 0; i <= k; i++) more += classes[i] == c ? mores[i] : 0.f;
+        return more;
+    };
     // - p (gl + sum gt + ge (log p + entropy))
     const auto share = [&](float z) {
         const float log_p = (z - m) - log_total, p = exp2_fast(log_p * kLog2e);
         return -p * fmaf(ge, fmaxf(log_p, -1e30f) + entropy, sum);
     };
     const T* from = static_cast<const T*>(a.logits) + b * a.l_b + t * a.l_t;
+    const auto one = [&](int i) {
+        float g = share((float)from[i]);
+        if (marked(i)) g += listed(i);
+        to[i] = (T)g;
+    };
     if ((((uintptr_t)from ^ (uintptr_t)to) & 15) == 0) {
+#pragma unroll 4
         for (int i = thread; i < out.pieces; i += kThreads) {
-            const int64_t at = out.head + (int64_t)i * P;
+            const int at = out.head + i * P;
             const Vector<T> z = *reinterpret_cast<const Vector<T>*>(from + at);
-            Vector<T> g;
+            float g[P];
 #pragma unroll
-            for (int e = 0; e < P; e++) g[e] = (T)share((float)z[e]);
-            *reinterpret_cast<Vector<T>*>(to + at) = g;
+            for (int e = 0; e < P; e++) g[e] = share((float)z[e]);
+            if (marked(at)) {
+#pragma unroll
+                for (int e = 0; e < P; e++) g[e] += listed(at + e);
+            }
+            Vector<T> v;
+#pragma unroll
+            for (int e = 0; e < P; e++) v[e] = (T)g[e];
+            *reinterpret_cast<Vector<T>*>(to + at) = v;
         }
-        if (single >= 0) to[single] = (T)share((float)from[single]);
+        if (single >= 0) one(single);
     } else {
-        for (int i = thread; i < a.F; i += kThreads) to[i] = (T)share((float)from[i]);
-    }
-    // the row is in memory before single classes of it are written again
-    __threadfence();
-    G::meet();
-    const int32_t* best = a.top_class + frame * k;
-    for (int i = thread; i <= k; i += kThreads) {
-        const int c = i < k ? best[i] : y;
-        bool there = c >= 0 && c < a.F;
-        float more = i < k ? (a.g_top ? a.g_top[frame * k + i] : 0.f) + (c == y ? gl : 0.f) : gl;
-        if (i == k)
-            for (int j = 0; j < k; j++) there = there && best[j] != y;      // the alternative's thread has it
-        if (there) to[c] = (T)(share((float)from[c]) + more);
+        for (int i = thread; i < a.F; i += kThreads) one(i);
     }
 }
 
