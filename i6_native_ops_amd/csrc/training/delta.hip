@@ -28,7 +28,8 @@ constexpr int kC = 32;                   // frames of a chunk
 
 struct Rows {                            // of the chunks' frames, [B][H][chunks C]
     float c, c_rest;                     // sum of log f within the chunk, as two floats
-    float w, rk, rq, pad0, pad1, pad2;   // share, 1 / length of key and query
+    float w, rk, rq;                     // share, 1 / length of key and query
+    float start, end, pad;               // exp(c), exp(c_C - c)
 };
 
 struct Args {
@@ -897,7 +898,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void delta_shared(A
 
 // ---------------------------------------------------------------------------------------------------------------- host
 
-constexpr int kMostFrames = 16;          // frame by frame up to this many
+constexpr int kMostFrames = 16;          // frame by frame up to this many, without training
 
 int checked(const i6delta_problem* p) {
     if (!p || p->B <= 0 || p->T <= 0 || p->H <= 0 || p->G <= 0 || p->K <= 0 || p->V <= 0 || p->H % p->G || !valid_dtype(p->dtype) || !p->q || !p->k || !p->v || !p->gate ||
@@ -930,14 +931,19 @@ bool whole_pieces(const i6delta_problem& p) {
     return whole(p.q, p.q_stride_b, p.q_stride_t, p.q_stride_g) && whole(p.k, p.k_stride_b, p.k_stride_t, p.k_stride_g);
 }
 
+// bfloat16: whether they are copied first.
+bool packs(const i6delta_problem& p) { return p.K % 8 || !whole_pieces(p); }
+int packed_row(int K) { return ceil_div(K, 8) * 8; }
+
 int padded_keys(int K) { return K <= 32 ? 32 : (K <= 64 ? 64 : 128); }
 
 // Where the parts of a call's memory are.
 struct Places {
-    size_t rows, states, states_factor, u, u_factor, kept;           // kept
-    size_t ends, ends_factor, dr, dr_factor, d_q, d_k, back;         // the backward workspace
+    size_t rows, states, states_factor, u, u_factor, kept;           // kept; rows are in the forward workspace where nothing is
+    size_t blocks, packed, forward;                                  // the forward workspace
+    size_t ends, ends_factor, dr, dr_factor, d_q, d_k, back_blocks, back_packed, back;      // the backward workspace
     int pairs;
-    explicit Places(const i6delta_problem& p) {
+    Places(const i6delta_problem& p, bool train) {
         const bool x16 = p.dtype == I6TRAIN_BF16;
         const int C = x16 ? kC16 : kC, KP = padded_keys(p.K);
         const size_t n = (size_t)p.B * p.H * ceil_div(p.T, C);
@@ -957,14 +963,23 @@ struct Places {
         dr_factor = dr + r;
         d_q = dr_factor + f;
         d_k = d_q + heads;
-        back = d_k + heads;
+        const size_t copy = !packs(p) ? 0 : align256((size_t)2 * p.B * p.T * p.G * packed_row(p.K) * sizeof(bf16));
+        back_blocks = d_k + heads;
+        back_packed = back_blocks + (x16 ? align256(n * kChunkBlocks<true> * sizeof(bf16)) : 0);
+        back = back_packed + (x16 ? copy : 0);
+        // frame by frame nothing is needed
+        const bool chunked = x16 && (train || p.T > kMostFrames);
+        blocks = chunked && !train ? states : 0;
+        packed = chunked ? blocks + align256(n * kChunkBlocks<false> * sizeof(bf16)) : 0;
+        forward = chunked ? packed + copy : 0;
     }
 };
 
 struct Call {
     Args a;
     Args16 k16;
-    bool whole;
+    bool whole, train;
+    bf16* blocks;
 };
 
 template <int KP> void run_forward(const Call& c, hipStream_t s, float) {
@@ -973,7 +988,8 @@ template <int KP> void run_forward(const Call& c, hipStream_t s, float) {
     else delta_forward<float, KP, 1><<<dim3(1, a.H, a.B), dim3(kThreads), 0, s>>>(a, c.whole);
 }
 template <int KP> void run_forward(const Call& c, hipStream_t s, bf16) {
-    delta_forward16<KP><<<dim3(ceil_div(c.a.V, 64), c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.k16, c.whole);
+    delta_prepare16<KP, false><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.blocks);
+    delta_forward16<KP><<<dim3(ceil_div(c.a.V, 64), c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.k16, c.blocks);
 }
 template <int KP> void run_backward(const Call& c, hipStream_t s, float) {
     const Args& a = c.a;
@@ -982,14 +998,15 @@ template <int KP> void run_backward(const Call& c, hipStream_t s, float) {
     delta_gradients<float, KP><<<dim3(a.chunks, a.H, a.B), dim3(kThreads), 0, s>>>(a);
 }
 template <int KP> void run_backward(const Call& c, hipStream_t s, bf16) {
-    delta_backward16<KP><<<dim3(ceil_div(c.a.V, 64), c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.k16, c.whole);
-    if (c.k16.pairs == 4) delta_gradients16<KP, 4><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(512), 0, s>>>(c.a, c.k16, c.whole);
-    else delta_gradients16<KP, 2><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(512), 0, s>>>(c.a, c.k16, c.whole);
+    delta_prepare16<KP, true><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.blocks);
+    delta_backward16<KP><<<dim3(ceil_div(c.a.V, 64), c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.k16, c.blocks);
+    if (c.k16.pairs == 4) delta_gradients16<KP, 4><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(512), 0, s>>>(c.a, c.k16);
+    else delta_gradients16<KP, 2><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(512), 0, s>>>(c.a, c.k16);
 }
 
 template <typename T, int KP> int forward(const Call& c, hipStream_t s) {
     const Args& a = c.a;
-    if (!a.rows && a.T <= kMostFrames) delta_frames<T, KP><<<dim3(ceil_div(a.V, 64), a.H, a.B), dim3(kThreads), 0, s>>>(a);
+    if (!c.train && a.T <= kMostFrames) delta_frames<T, KP><<<dim3(ceil_div(a.V, 64), a.H, a.B), dim3(kThreads), 0, s>>>(a);
     else run_forward<KP>(c, s, T());
     return launched();
 }
@@ -1020,11 +1037,27 @@ template <typename T> int backward_of(const Call& c, hipStream_t s) {
     }
 }
 
+// Takes the call to a copy of keys and queries, if that is needed.
+int pack(Call& c, const i6delta_problem& p, bf16* to, hipStream_t s) {
+    if (!packs(p)) return I6TRAIN_OK;
+    Args& a = c.a;
+    const int row = packed_row(p.K);
+    const int64_t rows = (int64_t)p.B * p.T * p.G, groups = ceil_div(rows * (row / 8), (int64_t)kThreads);
+    bf16* q = to + rows * row;
+    delta_pack16<<<dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(kThreads), 0, s>>>(a, to, q, row);
+    a.k = to; a.q = q;
+    a.k_g = a.q_g = row;
+    a.k_t = a.q_t = (int64_t)p.G * row;
+    a.k_b = a.q_b = (int64_t)p.T * p.G * row;
+    return launched();
+}
+
 Call call_of(const i6delta_problem& p, const Places& at, void* kept) {
     Call c{};
     c.a = args_of(p);
     c.whole = whole_pieces(p);
     c.k16.pairs = at.pairs;
+    c.train = kept;
     if (kept) {
         char* base = static_cast<char*>(kept);
         c.a.rows = reinterpret_cast<Rows*>(base + at.rows);
@@ -1046,9 +1079,9 @@ extern "C" {
 int i6delta_sizes(const i6delta_problem* p, int train, size_t* kept_bytes, size_t* forward_bytes, size_t* backward_bytes) {
     I6TRAIN_TRY(checked(p));
     if (!kept_bytes || !forward_bytes || !backward_bytes) return I6TRAIN_ERR_INVALID_ARGUMENT;
-    const Places at(*p);
+    const Places at(*p, train);
     *kept_bytes = train ? at.kept : 0;
-    *forward_bytes = 0;
+    *forward_bytes = at.forward;
     *backward_bytes = train ? at.back : 0;
     return I6TRAIN_OK;
 }
@@ -1056,11 +1089,15 @@ int i6delta_sizes(const i6delta_problem* p, int train, size_t* kept_bytes, size_
 int i6delta_forward(const i6delta_problem* p, void* o, float* last, void* kept, size_t kept_bytes, void* workspace, size_t workspace_bytes, void* stream) {
     I6TRAIN_TRY(checked(p));
     if (!o || !last) return I6TRAIN_ERR_INVALID_ARGUMENT;
-    const Places at(*p);
-    if (kept && kept_bytes < at.kept) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
-    (void)workspace; (void)workspace_bytes;
+    const Places at(*p, kept);
+    if ((kept && kept_bytes < at.kept) || (at.forward && (!workspace || workspace_bytes < at.forward))) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
     Call c = call_of(*p, at, kept);
     c.a.o = o; c.a.last = last;
+    if (at.forward) {
+        c.blocks = reinterpret_cast<bf16*>(static_cast<char*>(workspace) + at.blocks);
+        if (!kept) c.a.rows = static_cast<Rows*>(workspace);
+        I6TRAIN_TRY(pack(c, *p, reinterpret_cast<bf16*>(static_cast<char*>(workspace) + at.packed), (hipStream_t)stream));
+    }
     return p->dtype == I6TRAIN_F32 ? forward_of<float>(c, (hipStream_t)stream) : forward_of<bf16>(c, (hipStream_t)stream);
 }
 
@@ -1069,7 +1106,7 @@ int i6delta_backward(const i6delta_problem* p, const void* grad_o, int64_t grad_
                      size_t workspace_bytes, void* stream) {
     I6TRAIN_TRY(checked(p));
     if (!kept || !workspace || !grad_q || !grad_k || !grad_v || !grad_gate || !grad_beta) return I6TRAIN_ERR_INVALID_ARGUMENT;
-    const Places at(*p);
+    const Places at(*p, true);
     if (kept_bytes < at.kept || workspace_bytes < at.back) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
     Call c = call_of(*p, at, const_cast<void*>(kept));
     Args& a = c.a;
@@ -1081,6 +1118,8 @@ int i6delta_backward(const i6delta_problem* p, const void* grad_o, int64_t grad_
     a.dr = reinterpret_cast<float*>(base + at.dr);
     c.k16.ends = {reinterpret_cast<f16*>(base + at.ends), reinterpret_cast<float*>(base + at.ends_factor)};
     c.k16.dr = {reinterpret_cast<f16*>(base + at.dr), reinterpret_cast<float*>(base + at.dr_factor)};
+    c.blocks = reinterpret_cast<bf16*>(base + at.back_blocks);
+    if (p->dtype == I6TRAIN_BF16) I6TRAIN_TRY(pack(c, *p, reinterpret_cast<bf16*>(base + at.back_packed), (hipStream_t)stream));
     if (p->H > p->G) {
         a.d_q_head = reinterpret_cast<float*>(base + at.d_q);
         a.d_k_head = reinterpret_cast<float*>(base + at.d_k);

@@ -191,6 +191,15 @@ def test_keys_that_are_alike_and_keys_of_nothing(dtype):
     check(p, run(p), expected(p))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,K,V", [(49, 20, 64), (64, 64, 64), (64, 100, 30), (200, 128, 128), (300, 32, 100)])
+def test_frames_that_reach_far(T, K, V, dtype):
+    """States that last for a thousand frames: every block of a chunk's matrices counts, the farthest ones too."""
+    p = problem(2, T, 2, 1, K, V, dtype, lens="all")
+    p["gate"][:] = 7.0
+    check(p, run(p), expected(p))
+
+
 def test_a_strong_gate_among_weak_ones():
     """Sums of log f of thousands in front of differences of less than one."""
     p = problem(1, 64, 1, 1, 16, 16, torch.float32, lens="all")
