@@ -931,9 +931,10 @@ bool whole_pieces(const i6delta_problem& p) {
     return whole(p.q, p.q_stride_b, p.q_stride_t, p.q_stride_g) && whole(p.k, p.k_stride_b, p.k_stride_t, p.k_stride_g);
 }
 
-// bfloat16: whether they are copied first.
-bool packs(const i6delta_problem& p) { return p.K % 8 || !whole_pieces(p); }
-int packed_row(int K) { return ceil_div(K, 8) * 8; }
+// bfloat16: whether rows of `cols` values can be read in pieces of 16 bytes; otherwise they are copied first, each in so many values.
+bool whole_rows(const void* x, int64_t s0, int64_t s1, int64_t s2, int cols) { return (uintptr_t)x % 16 == 0 && s0 % 8 == 0 && s1 % 8 == 0 && s2 % 8 == 0 && cols % 8 == 0; }
+int packed_row(int cols) { return ceil_div(cols, 8) * 8; }
+size_t packed_bytes(const i6delta_problem& p, int heads, int cols) { return align256((size_t)p.B * p.T * heads * packed_row(cols) * sizeof(bf16)); }
 
 int padded_keys(int K) { return K <= 32 ? 32 : (K <= 64 ? 64 : 128); }
 
@@ -963,15 +964,18 @@ struct Places {
         dr_factor = dr + r;
         d_q = dr_factor + f;
         d_k = d_q + heads;
-        const size_t copy = !packs(p) ? 0 : align256((size_t)2 * p.B * p.T * p.G * packed_row(p.K) * sizeof(bf16));
+        // whatever their strides are: those of the incoming gradient are not known before it is there
+        const size_t k = packed_bytes(p, p.G, p.K), v = packed_bytes(p, p.H, p.V);
+        const size_t copy_k = whole_rows(p.k, p.k_stride_b, p.k_stride_t, p.k_stride_g, p.K) ? 0 : k, copy_q = whole_rows(p.q, p.q_stride_b, p.q_stride_t, p.q_stride_g, p.K) ? 0 : k;
+        const size_t copy_v = whole_rows(p.v, p.v_stride_b, p.v_stride_t, p.v_stride_h, p.V) ? 0 : v;
         back_blocks = d_k + heads;
         back_packed = back_blocks + (x16 ? align256(n * kChunkBlocks<true> * sizeof(bf16)) : 0);
-        back = back_packed + (x16 ? copy : 0);
+        back = back_packed + (x16 ? copy_k + copy_q + v : 0);
         // frame by frame nothing is needed
         const bool chunked = x16 && (train || p.T > kMostFrames);
         blocks = chunked && !train ? states : 0;
         packed = chunked ? blocks + align256(n * kChunkBlocks<false> * sizeof(bf16)) : 0;
-        forward = chunked ? packed + copy : 0;
+        forward = chunked ? packed + copy_k + copy_q + copy_v : 0;
     }
 };
 
@@ -989,7 +993,8 @@ template <int KP> void run_forward(const Call& c, hipStream_t s, float) {
 }
 template <int KP> void run_forward(const Call& c, hipStream_t s, bf16) {
     delta_prepare16<KP, false><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.blocks);
-    delta_forward16<KP><<<dim3(ceil_div(c.a.V, 64), c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.k16, c.blocks);
+    if (c.a.V > 64) delta_forward16<KP, 8><<<dim3(c.a.H, c.a.B), dim3(512), 0, s>>>(c.a, c.k16, c.blocks);
+    else delta_forward16<KP, 4><<<dim3(c.a.H, c.a.B), dim3(256), 0, s>>>(c.a, c.k16, c.blocks);
 }
 template <int KP> void run_backward(const Call& c, hipStream_t s, float) {
     const Args& a = c.a;
@@ -999,7 +1004,8 @@ template <int KP> void run_backward(const Call& c, hipStream_t s, float) {
 }
 template <int KP> void run_backward(const Call& c, hipStream_t s, bf16) {
     delta_prepare16<KP, true><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.blocks);
-    delta_backward16<KP><<<dim3(ceil_div(c.a.V, 64), c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.k16, c.blocks);
+    if (c.a.V > 64) delta_backward16<KP, 8><<<dim3(c.a.H, c.a.B), dim3(512), 0, s>>>(c.a, c.k16, c.blocks);
+    else delta_backward16<KP, 4><<<dim3(c.a.H, c.a.B), dim3(256), 0, s>>>(c.a, c.k16, c.blocks);
     if (c.k16.pairs == 4) delta_gradients16<KP, 4><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(512), 0, s>>>(c.a, c.k16);
     else delta_gradients16<KP, 2><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(512), 0, s>>>(c.a, c.k16);
 }
@@ -1037,18 +1043,17 @@ template <typename T> int backward_of(const Call& c, hipStream_t s) {
     }
 }
 
-// Takes the call to a copy of keys and queries, if that is needed.
-int pack(Call& c, const i6delta_problem& p, bf16* to, hipStream_t s) {
-    if (!packs(p)) return I6TRAIN_OK;
-    Args& a = c.a;
-    const int row = packed_row(p.K);
-    const int64_t rows = (int64_t)p.B * p.T * p.G, groups = ceil_div(rows * (row / 8), (int64_t)kThreads);
-    bf16* q = to + rows * row;
-    delta_pack16<<<dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(kThreads), 0, s>>>(a, to, q, row);
-    a.k = to; a.q = q;
-    a.k_g = a.q_g = row;
-    a.k_t = a.q_t = (int64_t)p.G * row;
-    a.k_b = a.q_b = (int64_t)p.T * p.G * row;
+// Takes the call to a copy of one of its tensors, if that is needed.
+int pack(const Args& a, char*& to, const void*& x, int64_t& s0, int64_t& s1, int64_t& s2, int heads, int cols, hipStream_t s) {
+    if (whole_rows(x, s0, s1, s2, cols)) return I6TRAIN_OK;
+    const int row = packed_row(cols);
+    const int64_t rows = (int64_t)a.B * a.T * heads, groups = ceil_div(rows * (row / 8), (int64_t)kThreads);
+    delta_pack16<<<dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(kThreads), 0, s>>>(a, Strided{static_cast<const bf16*>(x), s0, s1, s2, heads, cols}, reinterpret_cast<bf16*>(to), row);
+    x = to;
+    s2 = row;
+    s1 = (int64_t)heads * row;
+    s0 = (int64_t)a.T * heads * row;
+    to += align256((size_t)rows * row * sizeof(bf16));
     return launched();
 }
 
@@ -1096,7 +1101,11 @@ int i6delta_forward(const i6delta_problem* p, void* o, float* last, void* kept, 
     if (at.forward) {
         c.blocks = reinterpret_cast<bf16*>(static_cast<char*>(workspace) + at.blocks);
         if (!kept) c.a.rows = static_cast<Rows*>(workspace);
-        I6TRAIN_TRY(pack(c, *p, reinterpret_cast<bf16*>(static_cast<char*>(workspace) + at.packed), (hipStream_t)stream));
+        Args& a = c.a;
+        char* to = static_cast<char*>(workspace) + at.packed;
+        I6TRAIN_TRY(pack(a, to, a.k, a.k_b, a.k_t, a.k_g, a.G, a.K, (hipStream_t)stream));
+        I6TRAIN_TRY(pack(a, to, a.q, a.q_b, a.q_t, a.q_g, a.G, a.K, (hipStream_t)stream));
+        I6TRAIN_TRY(pack(a, to, a.v, a.v_b, a.v_t, a.v_h, a.H, a.V, (hipStream_t)stream));
     }
     return p->dtype == I6TRAIN_F32 ? forward_of<float>(c, (hipStream_t)stream) : forward_of<bf16>(c, (hipStream_t)stream);
 }
@@ -1119,7 +1128,12 @@ int i6delta_backward(const i6delta_problem* p, const void* grad_o, int64_t grad_
     c.k16.ends = {reinterpret_cast<f16*>(base + at.ends), reinterpret_cast<float*>(base + at.ends_factor)};
     c.k16.dr = {reinterpret_cast<f16*>(base + at.dr), reinterpret_cast<float*>(base + at.dr_factor)};
     c.blocks = reinterpret_cast<bf16*>(base + at.back_blocks);
-    if (p->dtype == I6TRAIN_BF16) I6TRAIN_TRY(pack(c, *p, reinterpret_cast<bf16*>(base + at.back_packed), (hipStream_t)stream));
+    if (p->dtype == I6TRAIN_BF16) {
+        char* to = base + at.back_packed;
+        I6TRAIN_TRY(pack(a, to, a.k, a.k_b, a.k_t, a.k_g, a.G, a.K, (hipStream_t)stream));
+        I6TRAIN_TRY(pack(a, to, a.q, a.q_b, a.q_t, a.q_g, a.G, a.K, (hipStream_t)stream));
+        if (a.d_o) I6TRAIN_TRY(pack(a, to, a.d_o, a.do_b, a.do_t, a.do_h, a.H, a.V, (hipStream_t)stream));
+    }
     if (p->H > p->G) {
         a.d_q_head = reinterpret_cast<float*>(base + at.d_q);
         a.d_k_head = reinterpret_cast<float*>(base + at.d_k);
