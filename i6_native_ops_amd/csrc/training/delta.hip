@@ -11,6 +11,7 @@
 // Every column of the state goes its own way: a wave has columns of its own, their states in registers as they come out of the matrix
 // instructions, which is also how these take them for their second operand (with the order of k that both operands share), so states, R, U, O and their
 // gradients never leave the wave; K, Q, A and P go through LDS.
+#include <algorithm>
 #include <cmath>
 
 #include "train_common.h"
@@ -899,6 +900,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void delta_shared(A
 // ---------------------------------------------------------------------------------------------------------------- host
 
 constexpr int kMostFrames = 16;          // frame by frame up to this many, without training
+constexpr int kCus = 256;
 
 int checked(const i6delta_problem* p) {
     if (!p || p->B <= 0 || p->T <= 0 || p->H <= 0 || p->G <= 0 || p->K <= 0 || p->V <= 0 || p->H % p->G || !valid_dtype(p->dtype) || !p->q || !p->k || !p->v || !p->gate ||
@@ -943,7 +945,9 @@ struct Places {
     size_t rows, states, states_factor, u, u_factor, kept;           // kept; rows are in the forward workspace where nothing is
     size_t blocks, packed, forward;                                  // the forward workspace
     size_t ends, ends_factor, dr, dr_factor, d_q, d_k, back_blocks, back_packed, back;      // the backward workspace
-    int pairs;
+    size_t split, turns;                                             // of the forward workspace, and turns behind split
+    size_t back_split;
+    int pairs, segments = 1, per;
     Places(const i6delta_problem& p, bool train) {
         const bool x16 = p.dtype == I6TRAIN_BF16;
         const int C = x16 ? kC16 : kC, KP = padded_keys(p.K);
@@ -970,12 +974,30 @@ struct Places {
         const size_t copy_v = whole_rows(p.v, p.v_stride_b, p.v_stride_t, p.v_stride_h, p.V) ? 0 : v;
         back_blocks = d_k + heads;
         back_packed = back_blocks + (x16 ? align256(n * kChunkBlocks<true> * sizeof(bf16)) : 0);
-        back = back_packed + (x16 ? copy_k + copy_q + v : 0);
+        back_split = back_packed + (x16 ? copy_k + copy_q + v : 0);
+        // Segments: as many as fill the card, and no more than pay for going along them one after the other; below three the second pass costs what the first one saves, and
+        // a short sequence does not pay for the launches.  Without and with them, heads of 64 (128): 8 of 2048 frames 142 -> 54 us (225 -> 87), of 512 45 -> 37 (66 -> 52),
+        // of 256 28.5 -> 29 (40.6 -> 41.6); 64 of 2048 frames 164 -> 108 (254 -> 208), of 1024 89 -> 67 (136 -> 134), of 512 53 -> 49 (76 -> 91).
+        const int chunks = ceil_div(p.T, C);
+        const int64_t heads_at_once = (int64_t)p.B * p.H;
+        per = chunks;
+        if (x16 && chunks >= (heads_at_once > 32 ? 16 : 8)) {
+            const int most = (int)std::min<int64_t>(kCus / heads_at_once, (int64_t)sqrt(5.0 * chunks));
+            if (most >= 3) {
+                per = ceil_div(chunks, most);
+                segments = ceil_div(chunks, per);
+            }
+        }
+        const size_t slots = (size_t)p.B * p.H * (segments - 1);
+        turns = align256(slots * p.K * p.V * sizeof(float));
+        const size_t split_bytes = turns + align256(slots * KP * KP * sizeof(float));
+        back = back_split + split_bytes;
         // frame by frame nothing is needed
         const bool chunked = x16 && (train || p.T > kMostFrames);
         blocks = chunked && !train ? states : 0;
         packed = chunked ? blocks + align256(n * kChunkBlocks<false> * sizeof(bf16)) : 0;
-        forward = chunked ? packed + copy_k + copy_q + copy_v : 0;
+        split = chunked ? packed + copy_k + copy_q + copy_v : 0;
+        forward = chunked ? split + split_bytes : 0;
     }
 };
 
@@ -993,8 +1015,15 @@ template <int KP> void run_forward(const Call& c, hipStream_t s, float) {
 }
 template <int KP> void run_forward(const Call& c, hipStream_t s, bf16) {
     delta_prepare16<KP, false><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.blocks);
-    if (c.a.V > 64) delta_forward16<KP, 8><<<dim3(c.a.H, c.a.B), dim3(512), 0, s>>>(c.a, c.k16, c.blocks);
-    else delta_forward16<KP, 4><<<dim3(c.a.H, c.a.B), dim3(256), 0, s>>>(c.a, c.k16, c.blocks);
+    const Args16& k = c.k16;
+    const int groups = ceil_div(32 * k.pairs + KP, 128);
+    if (k.segments > 1) {
+        delta_forward16<KP, 8, true><<<dim3(c.a.H * groups, c.a.B, k.segments - 1), dim3(512), 0, s>>>(c.a, k, c.blocks);
+        delta_join16<KP><<<dim3(ceil_div(c.a.V, 16), c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, k, false);
+    }
+    const dim3 grid(c.a.H, c.a.B, k.segments);
+    if (c.a.V > 64) delta_forward16<KP, 8, false><<<grid, dim3(512), 0, s>>>(c.a, k, c.blocks);
+    else delta_forward16<KP, 4, false><<<grid, dim3(256), 0, s>>>(c.a, k, c.blocks);
 }
 template <int KP> void run_backward(const Call& c, hipStream_t s, float) {
     const Args& a = c.a;
@@ -1004,8 +1033,15 @@ template <int KP> void run_backward(const Call& c, hipStream_t s, float) {
 }
 template <int KP> void run_backward(const Call& c, hipStream_t s, bf16) {
     delta_prepare16<KP, true><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.blocks);
-    if (c.a.V > 64) delta_backward16<KP, 8><<<dim3(c.a.H, c.a.B), dim3(512), 0, s>>>(c.a, c.k16, c.blocks);
-    else delta_backward16<KP, 4><<<dim3(c.a.H, c.a.B), dim3(256), 0, s>>>(c.a, c.k16, c.blocks);
+    const Args16& k = c.k16;
+    const int groups = ceil_div(32 * k.pairs + KP, 128);
+    if (k.segments > 1) {
+        delta_backward16<KP, 8, true><<<dim3(c.a.H * groups, c.a.B, k.segments - 1), dim3(512), 0, s>>>(c.a, k, c.blocks);
+        delta_join16<KP><<<dim3(ceil_div(c.a.V, 16), c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, k, true);
+    }
+    const dim3 grid(c.a.H, c.a.B, k.segments);
+    if (c.a.V > 64) delta_backward16<KP, 8, false><<<grid, dim3(512), 0, s>>>(c.a, k, c.blocks);
+    else delta_backward16<KP, 4, false><<<grid, dim3(256), 0, s>>>(c.a, k, c.blocks);
     if (c.k16.pairs == 4) delta_gradients16<KP, 4><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(512), 0, s>>>(c.a, c.k16);
     else delta_gradients16<KP, 2><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(512), 0, s>>>(c.a, c.k16);
 }
@@ -1062,6 +1098,8 @@ Call call_of(const i6delta_problem& p, const Places& at, void* kept) {
     c.a = args_of(p);
     c.whole = whole_pieces(p);
     c.k16.pairs = at.pairs;
+    c.k16.segments = at.segments;
+    c.k16.per = at.per;
     c.train = kept;
     if (kept) {
         char* base = static_cast<char*>(kept);
@@ -1101,6 +1139,8 @@ int i6delta_forward(const i6delta_problem* p, void* o, float* last, void* kept, 
     if (at.forward) {
         c.blocks = reinterpret_cast<bf16*>(static_cast<char*>(workspace) + at.blocks);
         if (!kept) c.a.rows = static_cast<Rows*>(workspace);
+        c.k16.ends = reinterpret_cast<float*>(static_cast<char*>(workspace) + at.split);
+        c.k16.turns = reinterpret_cast<float*>(static_cast<char*>(workspace) + at.split + at.turns);
         Args& a = c.a;
         char* to = static_cast<char*>(workspace) + at.packed;
         I6TRAIN_TRY(pack(a, to, a.k, a.k_b, a.k_t, a.k_g, a.G, a.K, (hipStream_t)stream));
@@ -1125,9 +1165,11 @@ int i6delta_backward(const i6delta_problem* p, const void* grad_o, int64_t grad_
     char* base = static_cast<char*>(workspace);
     a.ends = reinterpret_cast<float*>(base + at.ends);
     a.dr = reinterpret_cast<float*>(base + at.dr);
-    c.k16.ends = {reinterpret_cast<f16*>(base + at.ends), reinterpret_cast<float*>(base + at.ends_factor)};
+    c.k16.left = {reinterpret_cast<f16*>(base + at.ends), reinterpret_cast<float*>(base + at.ends_factor)};
     c.k16.dr = {reinterpret_cast<f16*>(base + at.dr), reinterpret_cast<float*>(base + at.dr_factor)};
     c.blocks = reinterpret_cast<bf16*>(base + at.back_blocks);
+    c.k16.ends = reinterpret_cast<float*>(base + at.back_split);
+    c.k16.turns = reinterpret_cast<float*>(base + at.back_split + at.turns);
     if (p->dtype == I6TRAIN_BF16) {
         char* to = base + at.back_packed;
         I6TRAIN_TRY(pack(a, to, a.k, a.k_b, a.k_t, a.k_g, a.G, a.K, (hipStream_t)stream));
