@@ -9,6 +9,7 @@
 // left singular vectors of all sizes, and the small ones grow 3.4 times in each iteration, 485 times in five.
 #include <cmath>
 
+#include "lds_loads.h"
 #include "train_common.h"
 #include "../../../include/i6orth.h"
 
@@ -24,7 +25,8 @@ constexpr double kLeastNorm = 1e-7;
 constexpr float kScaleX = 0x1p15f, kScaleA = 0x1p15f, kScaleB = 0x1p14f;
 constexpr int kMaxTensors = 40;          // x 96 bytes: the arguments of a kernel may have 4 KB
 constexpr int kThreads = 256;
-constexpr int kTile = 128, kStep = 32, kRowPad = 32;
+constexpr int kRowPad = 64;               // of columns: what the products run over
+constexpr double kLargeTiles = 1.6;      // a round of large tiles to one of small ones, measured
 constexpr int kParts = 256;              // partial sums of squares of a matrix
 
 struct Matrix {
@@ -41,7 +43,7 @@ struct Matrix {
 static_assert(sizeof(Matrix) <= 112, "kernel arguments");
 struct Table {
     Matrix t[kMaxTensors - 6];
-    int count;
+    int count, groups;
     float mu;
     int nesterov;
 };
@@ -56,6 +58,10 @@ __device__ __forceinline__ const Matrix& find(const Table& tab, int wg) {
     return tab.t[lo];
 }
 
+// Where a value's first half is in a matrix of `stride` columns; the second one is 32 places behind.  32 first and 32 second halves in turn are 128 bytes, what a stage
+// takes of a row.
+__device__ __forceinline__ int64_t place(int row, int col, int stride) { return (int64_t)row * 2 * stride + (col >> 5) * 64 + (col & 31); }
+
 __device__ __forceinline__ void halves(float v, f16& hi, f16& lo) {
     hi = (f16)v;
     lo = (f16)(v - (float)hi);
@@ -63,201 +69,489 @@ __device__ __forceinline__ void halves(float v, f16& hi, f16& lo) {
 
 // ------------------------------------------------------------------------------------------------------ norms, operands
 
-// Momentum, and sums of squares.
-template <typename T> __global__ __launch_bounds__(kThreads) void orth_norms(Table tab) {
-    const Matrix& t = find(tab, blockIdx.x);
-    const int part = blockIdx.x - t.first;
-    const int64_t n = (int64_t)t.rows * t.cols;
-    const T* g = static_cast<const T*>(t.update);
-    double sum = 0.0;
-    for (int64_t i = (int64_t)part * kThreads + threadIdx.x; i < n; i += (int64_t)t.parts_n * kThreads) {
-        float u = (float)g[i];
-        if (t.momentum) {
-            const float m = fmaf(tab.mu, t.momentum[i], (1.f - tab.mu) * u);
-            t.momentum[i] = m;
-            u = tab.nesterov ? fmaf(tab.mu, m, (1.f - tab.mu) * u) : m;
-        }
-        sum += (double)u * (double)u;
-    }
-    __shared__ double waves[kThreads / kWave];
+// The sum over a workgroup, in all its threads; `waves` is room in LDS.
+template <int N> __device__ __forceinline__ double sum_of_all(double sum, double* waves) {
 #pragma unroll
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) t.parts[part] = (waves[0] + waves[1]) + (waves[2] + waves[3]);
+    sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < N / kWave; i++) sum += waves[i];
+    return sum;
 }
 
-// X and its transpose, tiles of 64 x 64 of the update.
-template <typename T> __global__ __launch_bounds__(kThreads) void orth_operands(Table tab) {
-    const Matrix& t = find(tab, blockIdx.x);
-    const int tiles_c = ceil_div(t.cols, 64), tile = blockIdx.x - t.first, r0 = tile / tiles_c * 64, c0 = tile % tiles_c * 64;
-    __shared__ float values[64][65];
-    __shared__ double total[kThreads / kWave];
-    double sum = 0.0;
-    for (int i = threadIdx.x; i < t.parts_n; i += kThreads) sum += t.parts[i];
+// N values of a row side by side, in one load if `whole`; zeros behind the last.
+template <typename T, int N> __device__ __forceinline__ void load_some(float (&v)[N], const T* p, int64_t left, bool whole) {
+    using P = T __attribute__((ext_vector_type(N)));
+    if (whole && left >= N) {
+        const P x = *reinterpret_cast<const P*>(p);
 #pragma unroll
-    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-    if ((threadIdx.x & 63) == 0) total[threadIdx.x >> 6] = sum;
-    __syncthreads();
-    const double norm = sqrt((total[0] + total[1]) + (total[2] + total[3]));
+        for (int e = 0; e < N; e++) v[e] = (float)x[e];
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < N; e++) v[e] = e < left ? (float)p[e] : 0.f;
+}
+
+// Momentum, and the sum of the squares of a thread's share: pieces of 8 values from `first` on.
+template <typename T> __device__ __forceinline__ double squares_of(const Matrix& t, float mu, bool nesterov, int64_t first, int64_t step) {
+    const int64_t n = (int64_t)t.rows * t.cols;
+    const T* g = static_cast<const T*>(t.update);
+    const bool whole = (uintptr_t)g % 16 == 0, whole_m = (uintptr_t)t.momentum % 16 == 0;
+    double sum = 0.0;
+    for (int64_t i = first * 8; i < n; i += step * 8) {
+        float u[8], m[8];
+        load_some(u, g + i, n - i, whole);
+        if (t.momentum) {
+            load_some(m, t.momentum + i, n - i, whole_m);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                m[e] = fmaf(mu, m[e], (1.f - mu) * u[e]);
+                u[e] = nesterov ? fmaf(mu, m[e], (1.f - mu) * u[e]) : m[e];
+            }
+            if (whole_m && n - i >= 8) {
+                *reinterpret_cast<acc_t*>(t.momentum + i) = acc_t{m[0], m[1], m[2], m[3]};
+                *reinterpret_cast<acc_t*>(t.momentum + i + 4) = acc_t{m[4], m[5], m[6], m[7]};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (e < n - i) t.momentum[i + e] = m[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) sum += (double)u[e] * (double)u[e];
+    }
+    return sum;
+}
+
+template <typename T> __global__ __launch_bounds__(kThreads) void orth_norms(Table tab) {
+    const Matrix& t = find(tab, blockIdx.x);
+    __shared__ double waves[kThreads / kWave];
+    const int part = blockIdx.x - t.first;
+    const double sum = sum_of_all<kThreads>(squares_of<T>(t, tab.mu, tab.nesterov, (int64_t)part * kThreads + threadIdx.x, (int64_t)t.parts_n * kThreads), waves);
+    if (threadIdx.x == 0) t.parts[part] = sum;
+}
+
+// X and its transpose: a tile of 64 x 64 of the update, from row r0 and column c0 on.
+using Turned = float[64][65];
+template <typename T> __device__ __forceinline__ void operands_of(const Matrix& t, float mu, bool nesterov, double sum, int r0, int c0, Turned& values) {
+    const double norm = sqrt(sum);
     const float scale = (float)((double)kScaleX / (norm < kLeastNorm ? kLeastNorm : norm));
     const T* g = static_cast<const T*>(t.update);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int r = wave; r < 64; r += 4) {
-        const int row = r0 + r, col = c0 + lane;
-        float u = 0.f;
-        if (row < t.rows && col < t.cols) {
-            const int64_t i = (int64_t)row * t.cols + col;
-            u = (float)g[i];
-            if (t.momentum) u = tab.nesterov ? fmaf(tab.mu, t.momentum[i], (1.f - tab.mu) * u) : t.momentum[i];
+    const bool whole = (uintptr_t)g % 16 == 0 && t.cols % 8 == 0, whole_m = (uintptr_t)t.momentum % 16 == 0 && t.cols % 8 == 0;
+    for (int i = threadIdx.x; i < 64 * 8; i += kThreads) {
+        const int r = i >> 3, c = (i & 7) * 8, row = r0 + r, col = c0 + c;
+        const int64_t at = (int64_t)row * t.cols + col, left = row < t.rows ? t.cols - col : 0;
+        float u[8], m[8];
+        load_some(u, g + (left > 0 ? at : 0), left, whole);
+        if (t.momentum) {
+            load_some(m, t.momentum + (left > 0 ? at : 0), left, whole_m);
+#pragma unroll
+            for (int e = 0; e < 8; e++) u[e] = nesterov ? fmaf(mu, m[e], (1.f - mu) * u[e]) : m[e];
         }
-        values[r][lane] = u * scale;
+#pragma unroll
+        for (int e = 0; e < 8; e++) values[r][c + e] = u[e] * scale;
     }
     __syncthreads();
-    // the matrix as it lies is X, or its transpose
+    // the matrix as it lies is X, or its transpose; behind the last column there are zeros
     const bool wide = t.rows <= t.cols;
-    const auto store = [&](f16* to, int row, int col, int rows, int stride, int64_t half, float v) {
-        if (row >= rows || col >= stride) return;
-        f16 hi, lo;
-        halves(v, hi, lo);
-        to[(int64_t)row * stride + col] = hi;
-        to[half + (int64_t)row * stride + col] = lo;
-    };
-    const int64_t half_x = (int64_t)t.n * t.mp, half_xt = (int64_t)t.m * t.np;
-    for (int r = wave; r < 64; r += 4) {
-        if (wide) {
-            store(t.x, r0 + r, c0 + lane, t.n, t.mp, half_x, values[r][lane]);
-            store(t.xt, c0 + r, r0 + lane, t.m, t.np, half_xt, values[lane][r]);
-        } else {
-            store(t.xt, r0 + r, c0 + lane, t.m, t.np, half_xt, values[r][lane]);
-            store(t.x, c0 + r, r0 + lane, t.n, t.mp, half_x, values[lane][r]);
+    const auto store = [&](f16* to, int rows, int stride, int row0, int col0, bool turned) {
+        for (int i = threadIdx.x; i < 64 * 8; i += kThreads) {
+            const int r = i >> 3, c = (i & 7) * 8, row = row0 + r, col = col0 + c;
+            if (row >= rows || col >= stride) continue;
+            f16x8 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                f16 h, l;
+                halves(turned ? values[c + e][r] : values[r][c + e], h, l);
+                hi[e] = h;
+                lo[e] = l;
+            }
+            f16* at = to + place(row, col, stride);
+            *reinterpret_cast<f16x8*>(at) = hi;
+            *reinterpret_cast<f16x8*>(at + 32) = lo;
         }
-    }
+    };
+    store(wide ? t.x : t.xt, t.rows, wide ? t.mp : t.np, r0, c0, false);
+    store(wide ? t.xt : t.x, t.cols, wide ? t.np : t.mp, c0, r0, true);
+}
+
+template <typename T> __global__ __launch_bounds__(kThreads) void orth_operands(Table tab) {
+    const Matrix& t = find(tab, blockIdx.x);
+    const int tiles_c = ceil_div(t.cols, 64), tile = blockIdx.x - t.first;
+    __shared__ Turned values;
+    __shared__ double waves[kThreads / kWave];
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < t.parts_n; i += kThreads) sum += t.parts[i];
+    operands_of<T>(t, tab.mu, tab.nesterov, sum_of_all<kThreads>(sum, waves), tile / tiles_c * 64, tile % tiles_c * 64, values);
 }
 
 // ------------------------------------------------------------------------------------------------------------ products
 
 enum Kind { kGram, kFactor, kUpdate, kLast };
 
-// C[i][j] = sum_k P[i][k] Q[j][k]: P = Q = X, P = Q = A, and P = B, Q = X^T.
-template <typename T, int KIND> __global__ __launch_bounds__(kThreads, 2) void orth_product(Table tab) {
-    constexpr int kStride = kStep + 8;
-    const Matrix& t = find(tab, blockIdx.x);
+// The packed halves of a value, and four of them side by side.
+__device__ __forceinline__ uint32_t packed(float v) {
+    f16 hi, lo;
+    halves(v, hi, lo);
+    return (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
+}
+
+// C[i][j] = sum_k P[i][k] Q[j][k]: P = Q = X, P = Q = A, and P = B, Q = X^T.  Tiles of 32 S x 32 S, four waves with 16 S x 16 S each.  A stage has of every row 128 bytes:
+// 32 k, first and second halves (kHalves = 2), or the first halves of 64 k.  In LDS a row's eight pieces of 16 bytes are turned by the row, so that eight lanes that read
+// eight rows' pieces reach all banks; the loads, which write LDS in order, take them from the turned places.
+template <typename T, int KIND, int S, int kHalves> __device__ __forceinline__ void product_of(const Matrix& t, int ti, int tj, char* lds) {
+    constexpr int kTile = 32 * S, kSide = kTile * 128, kStage = 2 * kSide, kLoads = S;       // per wave, stage and operand
     constexpr bool kSymmetric = KIND == kGram || KIND == kFactor;
+    constexpr int kStep = kHalves == 2 ? 32 : 64;
     const f16* p = KIND == kGram ? t.x : (KIND == kFactor ? t.a : t.b);
     const f16* q = KIND == kGram ? t.x : (KIND == kFactor ? t.a : t.xt);
-    const int rows_p = t.n, rows_q = kSymmetric ? t.n : t.m, k_all = KIND == kGram ? t.mp : t.np;
-    const int64_t half_p = (int64_t)rows_p * k_all, half_q = (int64_t)rows_q * k_all;
-    int tile = blockIdx.x - t.first, ti = 0, tj = 0;
-    if (kSymmetric) {
-        while ((ti + 1) * (ti + 2) / 2 <= tile) ti++;
-        tj = tile - ti * (ti + 1) / 2;
-    } else {
-        const int tiles_j = ceil_div(rows_q, kTile);
-        ti = tile / tiles_j;
-        tj = tile % tiles_j;
-    }
+    const int rows_q = kSymmetric ? t.n : t.m, k_all = KIND == kGram ? t.mp : t.np;
     const int i0 = ti * kTile, j0 = tj * kTile;
-    __shared__ __align__(16) f16 sp[2][kTile * kStride], sq[2][kTile * kStride];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave & 1, wj = wave >> 1;
-    // a thread loads 16 halves of a row
-    const int row = threadIdx.x >> 1, at = (threadIdx.x & 1) * 16;
-    const f16* from_p = p + (int64_t)min(i0 + row, rows_p - 1) * k_all + at;
-    const f16* from_q = q + (int64_t)min(j0 + row, rows_q - 1) * k_all + at;
-    f16x8 in[8];
-    const auto fetch = [&](int k) {
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                in[h * 4 + c] = *reinterpret_cast<const f16x8*>(from_p + h * half_p + k + c * 8);
-                in[h * 4 + 2 + c] = *reinterpret_cast<const f16x8*>(from_q + h * half_q + k + c * 8);
-            }
+    const int lane = threadIdx.x & 63, wave = wave_index(), wi = wave & 1, wj = wave >> 1;
+
+    const int64_t row_bytes = (int64_t)k_all * 4;
+    const descriptor from_p = describe(reinterpret_cast<const char*>(p) + i0 * row_bytes, min(t.n - i0, kTile) * row_bytes);
+    const descriptor from_q = describe(reinterpret_cast<const char*>(q) + j0 * row_bytes, min(rows_q - j0, kTile) * row_bytes);
+    uint32_t from;                       // of the lane's piece: 8 rows a load
+    {
+        const int row = wave * kLoads * 8 + (lane >> 3), piece = (lane & 7) ^ (lane >> 3);
+        from = (uint32_t)(row * row_bytes) + (kHalves == 2 ? piece * 16 : (piece >> 2) * 128 + (piece & 3) * 16);
+    }
+    const uint32_t lds0 = lds_address(lds) + wave * kLoads * 1024, eight_rows = (uint32_t)(8 * row_bytes);
+    const auto fetch = [&](int i, int stage, uint32_t offset) {
+        const uint32_t to = lds0 + stage * kStage + (i & 1) * kSide + (i >> 1) * 1024;
+        load_to_lds(i & 1 ? from_q : from_p, to, from + (i >> 1) * eight_rows, offset);
     };
-    acc_t acc[4][4];
+    constexpr uint32_t kStepBytes = kHalves == 2 ? 128 : 256;
+    acc_t acc[S][S];
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+    for (int i = 0; i < S; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = 0.f;
-    fetch(0);
-    for (int k = 0; k < k_all; k += kStep) {
-        __syncthreads();
+        for (int j = 0; j < S; j++) acc[i][j] = 0.f;
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+    for (int i = 0; i < 2 * kLoads; i++) fetch(i, 0, 0);
+    const int steps = k_all / kStep;
+    // fragments: the lane's row, and pieces 0 .. 3 and 4 .. 7
+    const uint32_t read0 = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) * 16), read1 = read0 ^ 64;
+    for (int k = 0; k < steps; k++) {
+        wait_and_meet<0>();
+        const char* sp = lds + (k & 1) * kStage + wi * (16 * S * 128);
+        const char* sq = lds + (k & 1) * kStage + kSide + wj * (16 * S * 128);
+        f16x8 fq[2][S], fp[2][2];
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                *reinterpret_cast<f16x8*>(&sp[h][row * kStride + at + c * 8]) = in[h * 4 + c];
-                *reinterpret_cast<f16x8*>(&sq[h][row * kStride + at + c * 8]) = in[h * 4 + 2 + c];
+        for (int j = 0; j < S; j++) {
+            fq[0][j] = *reinterpret_cast<const f16x8*>(sq + read0 + j * 2048);
+            fq[1][j] = *reinterpret_cast<const f16x8*>(sq + read1 + j * 2048);
+        }
+        fp[0][0] = *reinterpret_cast<const f16x8*>(sp + read0);
+        fp[0][1] = *reinterpret_cast<const f16x8*>(sp + read1);
+        const uint32_t offset = (uint32_t)(k + 1) * kStepBytes;
+        const bool more = k + 1 < steps;
+#pragma unroll
+        for (int i = 0; i < S; i++) {
+            if (i + 1 < S) {
+                fp[(i + 1) & 1][0] = *reinterpret_cast<const f16x8*>(sp + read0 + (i + 1) * 2048);
+                fp[(i + 1) & 1][1] = *reinterpret_cast<const f16x8*>(sp + read1 + (i + 1) * 2048);
             }
-        __syncthreads();
-        if (k + kStep < k_all) fetch(k + kStep);
-        f16x8 fq[2][4];
-        const int from = (lane & 15) * kStride + (lane >> 4) * 8;
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) fq[h][j] = *reinterpret_cast<const f16x8*>(&sq[h][(wj * 64 + j * 16) * kStride + from]);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const f16x8 hi = *reinterpret_cast<const f16x8*>(&sp[0][(wi * 64 + i * 16) * kStride + from]);
-            const f16x8 lo = *reinterpret_cast<const f16x8*>(&sp[1][(wi * 64 + i * 16) * kStride + from]);
+            if (more) {
+                fetch(2 * i, (k + 1) & 1, offset);
+                fetch(2 * i + 1, (k + 1) & 1, offset);
+            }
+            const f16x8 p0 = fp[i & 1][0], p1 = fp[i & 1][1];
 #if __HIP_DEVICE_COMPILE__
+            if (kHalves == 2) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, fq[1][j], acc[i][j], 0, 0, 0);
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, fq[0][j], acc[i][j], 0, 0, 0);
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, fq[0][j], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < S; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p0, fq[1][j], acc[i][j], 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < S; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p1, fq[0][j], acc[i][j], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int j = 0; j < S; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p1, fq[1][j], acc[i][j], 0, 0, 0);
             }
+#pragma unroll
+            for (int j = 0; j < S; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p0, fq[0][j], acc[i][j], 0, 0, 0);
 #endif
         }
     }
-    // what becomes of a tile
+    // What becomes of a tile.  A lane has four values of a column of C, which stand side by side in C's transpose; rows go through LDS, where a wave has room for 64 of them.
+    const int at = 4 * (lane >> 4), ci0 = i0 + wi * 16 * S, cj0 = j0 + wj * 16 * S;
+    const bool wide = t.rows <= t.cols, whole = t.cols % 4 == 0 && (uintptr_t)t.result % (4 * sizeof(T)) == 0;
+    constexpr int kWidth = 16 * S;
+    uint32_t* mine = reinterpret_cast<uint32_t*>(lds) + wave * 64 * kWidth;
+    wait_and_meet<0>();
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+    for (int strip = 0; strip < S / 4; strip++) {
 #pragma unroll
-        for (int j = 0; j < 4; j++)
+        for (int i4 = 0; i4 < 4; i4++) {
+            const int i = strip * 4 + i4, ci = ci0 + i * 16 + at;
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int ci = i0 + wi * 64 + i * 16 + 4 * (lane >> 4) + r, cj = j0 + wj * 64 + j * 16 + (lane & 15);
-                const float c = acc[i][j][r];
-                if (ci >= t.n) continue;
-                f16 hi, lo;
-                if (kSymmetric) {
-                    if (cj > ci) continue;
-                    const int64_t half = (int64_t)t.n * t.np, here = (int64_t)ci * t.np + cj, there = (int64_t)cj * t.np + ci;
-                    f16* to = KIND == kGram ? t.a : t.b;
-                    float v;
-                    if (KIND == kGram) {
-                        v = c * (kScaleA / (kScaleX * kScaleX));
-                    } else {
-                        const float a = (float)t.a[here] + (float)t.a[half + here];
-                        v = fmaf(kC * (kScaleB / (kScaleA * kScaleA)), c, kB * (kScaleB / kScaleA) * a);
+            for (int j = 0; j < S; j++) {
+                const int cj = cj0 + j * 16 + (lane & 15);
+                const bool there = cj < rows_q && ci < t.np;
+                acc_t v = acc[i][j];
+                if (KIND == kGram) v *= kScaleA / (kScaleX * kScaleX);
+                else {
+                    const f16* own = (KIND == kFactor ? t.a : t.xt) + place(there ? cj : 0, there ? ci : 0, t.np);
+                    const acc_t x = __builtin_convertvector(*reinterpret_cast<const f16x4*>(own), acc_t) + __builtin_convertvector(*reinterpret_cast<const f16x4*>(own + 32), acc_t);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        v[e] = KIND == kFactor ? fmaf(kC * (kScaleB / (kScaleA * kScaleA)), v[e], kB * (kScaleB / kScaleA) * x[e]) : fmaf(v[e], 1.f / kScaleB, kA * x[e]);
+                }
+                uint32_t words[4];
+                if (KIND == kLast) {
+                    const acc_t o = v * (1.f / kScaleX);
+                    if (!wide && whole) {        // the result's rows are C's columns
+                        if (cj < t.m && ci < t.cols) {
+                            using T4 = T __attribute__((ext_vector_type(4)));
+                            T4* to = reinterpret_cast<T4*>(static_cast<T*>(t.result) + (int64_t)cj * t.cols + ci);
+                            T4 r = __builtin_convertvector(o, T4);
+                            if (t.momentum) {
+                                const acc_t was = __builtin_convertvector(*to, acc_t);
+#pragma unroll
+                                for (int e = 0; e < 4; e++) r[e] = (T)fmaf(-t.rate, o[e], was[e] * t.keep);
+                            }
+                            *to = r;
+                        }
+                        continue;
                     }
-                    halves(v, hi, lo);
-                    to[here] = hi;
-                    to[half + here] = lo;
-                    to[there] = hi;
-                    to[half + there] = lo;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) words[e] = __float_as_uint(o[e]);
                 } else {
-                    if (cj >= t.m) continue;
-                    const int64_t half_x = (int64_t)t.n * t.mp, here = (int64_t)ci * t.mp + cj;
-                    const float x = (float)t.x[here] + (float)t.x[half_x + here];
-                    const float v = fmaf(kA, x, c * (1.f / kScaleB));
-                    if (KIND == kUpdate) {
-                        const int64_t half_xt = (int64_t)t.m * t.np, there = (int64_t)cj * t.np + ci;
-                        halves(v, hi, lo);
-                        t.x[here] = hi;
-                        t.x[half_x + here] = lo;
-                        t.xt_next[there] = hi;
-                        t.xt_next[half_xt + there] = lo;
-                    } else {
-                        const int64_t out = t.rows <= t.cols ? (int64_t)ci * t.cols + cj : (int64_t)cj * t.cols + ci;
-                        T* to = static_cast<T*>(t.result) + out;
-                        const float o = v * (1.f / kScaleX);
-                        *to = t.momentum ? (T)fmaf(-t.rate, o, (float)*to * t.keep) : (T)o;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) words[e] = there && ci + e < t.n ? packed(v[e]) : 0;
+                    if (there && (!kSymmetric || ti != tj)) {
+                        f16* to = (KIND == kGram ? t.a : (KIND == kFactor ? t.b : t.xt_next)) + place(cj, ci, t.np);
+                        *reinterpret_cast<uint2*>(to) = make_uint2(__builtin_amdgcn_perm(words[1], words[0], 0x05040100), __builtin_amdgcn_perm(words[3], words[2], 0x05040100));
+                        *reinterpret_cast<uint2*>(to + 32) = make_uint2(__builtin_amdgcn_perm(words[1], words[0], 0x07060302), __builtin_amdgcn_perm(words[3], words[2], 0x07060302));
                     }
                 }
+#pragma unroll
+                for (int e = 0; e < 4; e++) mine[(i4 * 16 + at + e) * kWidth + ((j * 16 + (lane & 15)) ^ (at << 2))] = words[e];
             }
+            if (S == 8) __builtin_amdgcn_sched_barrier(0);       // or what all 16 x 16 tiles load is loaded first
+        }
+        asm volatile("" ::: "memory");   // a wave's own part of LDS, which it reads in the order of its writes
+        if (KIND == kLast) {
+            const auto put = [&](int r, int c) {
+                const int ci = ci0 + strip * 64 + r, cj = cj0 + c;
+                if (ci >= t.n || cj >= t.m) return;
+                const float o = __uint_as_float(mine[r * kWidth + (c ^ ((r & 12) << 2))]);
+                T* to = static_cast<T*>(t.result) + (wide ? (int64_t)ci * t.cols + cj : (int64_t)cj * t.cols + ci);
+                *to = t.momentum ? (T)fmaf(-t.rate, o, (float)*to * t.keep) : (T)o;
+            };
+            if (wide) {
+                for (int x = lane; x < 64 * kWidth; x += 64) put(x / kWidth, x % kWidth);
+            } else if (!whole) {
+                for (int c = 0; c < kWidth; c++) put(lane, c);
+            }
+            continue;
+        }
+        const int stride = kSymmetric ? t.np : t.mp;
+        f16* out = KIND == kGram ? t.a : (KIND == kFactor ? t.b : t.x);
+#pragma unroll 4
+        for (int x = lane; x < 64 * (kWidth / 8); x += 64) {
+            const int r = x / (kWidth / 8), c = x % (kWidth / 8) * 8, ci = ci0 + strip * 64 + r, cj = cj0 + c;
+            if (ci >= t.n || cj >= stride) continue;
+            const uint4* w = reinterpret_cast<const uint4*>(mine + r * kWidth + (c ^ ((r & 12) << 2)));
+            const uint4 u = w[0], v = w[1];
+            f16* to = out + place(ci, cj, stride);
+            *reinterpret_cast<uint4*>(to) = make_uint4(__builtin_amdgcn_perm(u.y, u.x, 0x05040100), __builtin_amdgcn_perm(u.w, u.z, 0x05040100), __builtin_amdgcn_perm(v.y, v.x, 0x05040100),
+                                                       __builtin_amdgcn_perm(v.w, v.z, 0x05040100));
+            *reinterpret_cast<uint4*>(to + 32) = make_uint4(__builtin_amdgcn_perm(u.y, u.x, 0x07060302), __builtin_amdgcn_perm(u.w, u.z, 0x07060302),
+                                                            __builtin_amdgcn_perm(v.y, v.x, 0x07060302), __builtin_amdgcn_perm(v.w, v.z, 0x07060302));
+        }
+        asm volatile("" ::: "memory");
+    }
+}
+
+constexpr int stages_bytes(int S) { return 2 * 2 * 32 * S * 128; }
+template <typename T, int KIND, int S, int kHalves> __global__ __launch_bounds__(kThreads, S == 8 ? 1 : 2) void orth_product(Table tab) {
+    constexpr int kTile = 32 * S;
+    __shared__ __align__(128) char lds[stages_bytes(S)];
+    // neighbours in the order of the tiles go to the same eighth of the card, which has a cache of its own
+    const int per = ceil_div(tab.groups, 8), wg = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+    if (wg >= tab.groups) return;
+    const Matrix& t = find(tab, wg);
+    int tile = wg - t.first, ti = 0, tj = 0;
+    if (KIND == kGram || KIND == kFactor) {
+        while ((ti + 1) * (ti + 2) / 2 <= tile) ti++;
+        tj = tile - ti * (ti + 1) / 2;
+    } else {                             // four rows of tiles side by side
+        const int tiles_i = ceil_div(t.n, kTile), tiles_j = ceil_div(t.m, kTile), four_rows = tile / (4 * tiles_j), high = min(4, tiles_i - 4 * four_rows);
+        tile -= four_rows * 4 * tiles_j;
+        ti = 4 * four_rows + tile % high;
+        tj = tile / high;
+    }
+    product_of<T, KIND, S, kHalves>(t, ti, tj, lds);
+}
+
+// Small matrices: a workgroup does all of it for one, X and A (then B) in LDS.  A wave has sixteen rows of X, or a part of their columns, in 32 bits in its registers.
+// What bounds it are the waits of a chain of products that has 15 links: two matrices of 128 x 64 take %%SMALL%%.
+constexpr int kSmallThreads = 512, kSmallBytes = 140 * 1024, kSmallTiles = 8;
+__host__ __device__ constexpr int small_parts(int n) { return n <= 16 ? 8 : (n <= 32 ? 4 : (n <= 64 ? 2 : 1)); }     // waves of sixteen rows
+__host__ __device__ constexpr int up32(int n) { return (n + 31) / 32 * 32; }
+constexpr bool is_small(int n, int m) {
+    return n <= 128 && (m + 15) / 16 <= kSmallTiles * small_parts(n) && (int64_t)up32(n) * (up32(m) + 8 + up32(n) + 8) * 4 <= kSmallBytes;
+}
+
+// Operands of sixteen rows and 32 k, first or second halves: a lane has k = 4 (lane >> 4) .. + 3 and 16 more.
+__device__ __forceinline__ f16x8 two(f16x4 a, f16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+__device__ __forceinline__ f16x8 rows_of(const f16* p, int stride, int row0, int k0, int lane) {
+    const f16* at = p + (row0 + (lane & 15)) * stride + k0 + 4 * (lane >> 4);
+    return two(*reinterpret_cast<const f16x4*>(at), *reinterpret_cast<const f16x4*>(at + 16));
+}
+__device__ __forceinline__ f16x8 columns_of(const f16* p, int stride, int col0, int k0, int lane) {     // reads that turn 4 rows x 16 columns within 16 lanes
+    f16x8 r = {};
+#if __HIP_DEVICE_COMPILE__
+    using s16x4 = short __attribute__((ext_vector_type(4)));
+    using P = __attribute__((address_space(3))) s16x4*;
+    const f16* at = p + (k0 + 4 * (lane >> 4) + ((lane & 15) >> 2)) * stride + col0 + 4 * (lane & 3);
+    r = two(__builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)at)), __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(at + 16 * stride))));
+#endif
+    return r;
+}
+// The lane, of which the compiler does not know that it is the same as before: addresses are formed where they are used, or those of all tiles fill the registers.
+__device__ __forceinline__ int this_lane() {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+__device__ __forceinline__ acc_t multiplied(f16x8 a, f16x8 b, acc_t c) {
+#if __HIP_DEVICE_COMPILE__
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+#endif
+    return c;
+}
+
+template <typename T> __global__ __launch_bounds__(kSmallThreads) void orth_small(Table tab, int iterations) {
+    __shared__ __align__(16) f16 room[kSmallBytes / 2];
+    __shared__ double waves[kSmallThreads / kWave];
+    const Matrix& t = tab.t[blockIdx.x];
+    const int n32 = up32(t.n), m32 = up32(t.m), sx = m32 + 8, sa = n32 + 8, plane_x = n32 * sx, plane_a = n32 * sa;
+    f16* x = room;
+    f16* a = room + 2 * plane_x;
+    for (int i = threadIdx.x; i < (plane_x + plane_a) / 4; i += kSmallThreads) reinterpret_cast<uint4*>(room)[i] = make_uint4(0, 0, 0, 0);
+    const double norm = sqrt(sum_of_all<kSmallThreads>(squares_of<T>(t, tab.mu, tab.nesterov, threadIdx.x, kSmallThreads), waves));
+    const float scale = (float)((double)kScaleX / (norm < kLeastNorm ? kLeastNorm : norm));
+    const bool wide = t.rows <= t.cols;
+    const T* g = static_cast<const T*>(t.update);
+    for (int i = threadIdx.x; i < t.rows * t.cols; i += kSmallThreads) {
+        const int r = i / t.cols, c = i - r * t.cols, at = wide ? r * sx + c : c * sx + r;
+        float u = (float)g[i];
+        if (t.momentum) u = tab.nesterov ? fmaf(tab.mu, t.momentum[i], (1.f - tab.mu) * u) : t.momentum[i];
+        halves(u * scale, x[at], x[plane_x + at]);
+    }
+    __syncthreads();
+    const int wave = wave_index();
+    int lane = this_lane(), at = 4 * (lane >> 4), own = lane & 15;
+    const int parts = small_parts(t.n), row0 = wave / parts * 16, part = wave % parts, tiles_n = ceil_div(t.n, 16), tiles_m = ceil_div(t.m, 16);
+    const bool mine = row0 < t.n;
+    constexpr int kA16 = 8;
+    acc_t xr[kSmallTiles], ar[kA16];
+    const acc_t none = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSmallTiles; i++) {
+        xr[i] = none;
+        const int j = part + parts * i;
+        if (mine && j < tiles_m) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const f16* from = x + (row0 + at + e) * sx + 16 * j + own;
+                xr[i][e] = (float)from[0] + (float)from[plane_x];
+            }
+        }
+    }
+    // X X^T or A A: rows by rows
+    const auto square = [&](const f16* p, int stride, int plane, int k_all, auto take) {
+        acc_t hi[kA16], lo[kA16];
+#pragma unroll
+        for (int i = 0; i < kA16; i++) hi[i] = lo[i] = none;
+        if (mine)
+            for (int k = 0; k < k_all; k += 32) {
+                const int lane = this_lane();
+                const f16x8 p0 = rows_of(p, stride, row0, k, lane), p1 = rows_of(p + plane, stride, row0, k, lane);
+#pragma unroll
+                for (int i = 0; i < kA16; i++) {
+                    const int j = part + parts * i;
+                    if (j >= tiles_n) continue;
+                    const f16x8 q0 = rows_of(p, stride, 16 * j, k, lane), q1 = rows_of(p + plane, stride, 16 * j, k, lane);
+                    hi[i] = multiplied(p0, q0, hi[i]);
+                    lo[i] = multiplied(p1, q0, multiplied(p0, q1, lo[i]));
+                }
+            }
+#pragma unroll
+        for (int i = 0; i < kA16; i++) ar[i] = take(hi[i] + lo[i], ar[i]);
+    };
+    const auto store_square = [&]() {    // both are symmetric: a lane's four rows of a column are four columns of a row
+        if (!mine) return;
+        const int lane = this_lane(), at = 4 * (lane >> 4), own = lane & 15;
+#pragma unroll
+        for (int i = 0; i < kA16; i++) {
+            const int j = part + parts * i;
+            if (j >= tiles_n) continue;
+            f16x4 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                f16 h, l;
+                halves(ar[i][e], h, l);
+                hi[e] = h;
+                lo[e] = l;
+            }
+            f16* to = a + (16 * j + own) * sa + row0 + at;
+            *reinterpret_cast<f16x4*>(to) = hi;
+            *reinterpret_cast<f16x4*>(to + plane_a) = lo;
+        }
+    };
+    for (int it = 0; it < iterations; it++) {
+        square(x, sx, plane_x, m32, [&](acc_t v, acc_t) { return v * (kScaleA / (kScaleX * kScaleX)); });
+        store_square();
+        __syncthreads();
+        square(a, sa, plane_a, n32, [&](acc_t v, acc_t was) { return v * (kC * (kScaleB / (kScaleA * kScaleA))) + was * (kB * (kScaleB / kScaleA)); });
+        __syncthreads();
+        store_square();
+        __syncthreads();
+        acc_t v[kSmallTiles];
+#pragma unroll
+        for (int i = 0; i < kSmallTiles; i++) v[i] = none;
+        if (mine)
+            for (int k = 0; k < n32; k += 32) {
+                const int lane = this_lane();
+                const f16x8 p0 = rows_of(a, sa, row0, k, lane), p1 = rows_of(a + plane_a, sa, row0, k, lane);
+#pragma unroll
+                for (int i = 0; i < kSmallTiles; i++) {
+                    const int j = part + parts * i;
+                    if (j >= tiles_m) continue;
+                    const f16x8 q0 = columns_of(x, sx, 16 * j, k, lane), q1 = columns_of(x + plane_x, sx, 16 * j, k, lane);
+                    v[i] = multiplied(p0, q0, multiplied(p1, q0, multiplied(p0, q1, v[i])));
+                }
+            }
+        __syncthreads();
+        const bool last = it + 1 == iterations;
+        lane = this_lane();
+        at = 4 * (lane >> 4);
+        own = lane & 15;
+#pragma unroll
+        for (int i = 0; i < kSmallTiles; i++) {
+            const int j = part + parts * i, cj = 16 * j + own;
+            if (!mine || j >= tiles_m) continue;
+            xr[i] = xr[i] * kA + v[i] * (1.f / kScaleB);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int ci = row0 + at + e;
+                if (!last) {
+                    f16* to = x + ci * sx + cj;
+                    halves(xr[i][e], to[0], to[plane_x]);
+                } else if (ci < t.n && cj < t.m) {
+                    const float o = xr[i][e] * (1.f / kScaleX);
+                    T* to = static_cast<T*>(t.result) + (wide ? ci * t.cols + cj : cj * t.cols + ci);
+                    *to = t.momentum ? (T)fmaf(-t.rate, o, (float)*to * t.keep) : (T)o;
+                }
+            }
+        }
+        __syncthreads();
+    }
 }
 
 // No iterations: X itself.
@@ -266,26 +560,10 @@ template <typename T> __global__ __launch_bounds__(kThreads) void orth_copy(Tabl
     const int64_t n = (int64_t)t.rows * t.cols, i = (int64_t)(blockIdx.x - t.first) * kThreads + threadIdx.x;
     if (i >= n) return;
     const int r = (int)(i / t.cols), c = (int)(i % t.cols);
-    const int64_t at = t.rows <= t.cols ? (int64_t)r * t.mp + c : (int64_t)c * t.mp + r;
-    const float o = ((float)t.x[at] + (float)t.x[(int64_t)t.n * t.mp + at]) * (1.f / kScaleX);
+    const f16* x = t.rows <= t.cols ? t.x + place(r, c, t.mp) : t.x + place(c, r, t.mp);
+    const float o = ((float)x[0] + (float)x[32]) * (1.f / kScaleX);
     T* to = static_cast<T*>(t.result) + i;
     *to = t.momentum ? (T)fmaf(-t.rate, o, (float)*to * t.keep) : (T)o;
-}
-
-// Columns behind the last, which the products run over: zeros.
-__global__ __launch_bounds__(kThreads) void orth_pads(Table tab) {
-    const Matrix& t = find(tab, blockIdx.x);
-    const int row = (blockIdx.x - t.first) * kThreads + threadIdx.x;
-    const auto clear = [&](f16* p, int rows, int cols, int stride) {
-        if (row >= rows) return;
-        for (int h = 0; h < 2; h++)
-            for (int c = cols; c < stride; c++) p[(int64_t)h * rows * stride + (int64_t)row * stride + c] = (f16)0.f;
-    };
-    clear(t.x, t.n, t.m, t.mp);
-    clear(t.xt, t.m, t.n, t.np);
-    clear(t.xt_next, t.m, t.n, t.np);
-    clear(t.a, t.n, t.n, t.np);
-    clear(t.b, t.n, t.n, t.np);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
@@ -337,21 +615,45 @@ template <typename Groups, typename Launch> int over(Table& tab, Groups groups, 
     return launched();
 }
 
-template <typename T> int run(Table& tab, int iterations, hipStream_t s) {
+// A product over all matrices.  Tiles of 256 x 256 keep the matrix units busier, one workgroup a unit; tiles of 128 x 128, two a unit, waste less of small matrices and of the
+// last round.
+template <typename T, int KIND, int kHalves> int multiply(Table& tab, hipStream_t s) {
+    constexpr bool kSymmetric = KIND == kGram || KIND == kFactor;
+    const auto tiles = [](const Matrix& t, int side) {
+        const int64_t i = ceil_div(t.n, side);
+        return kSymmetric ? i * (i + 1) / 2 : i * ceil_div(t.m, side);
+    };
+    const auto in_all = [&](int side) {
+        int64_t all = 0;
+        for (int i = 0; i < tab.count; i++) all += tiles(tab.t[i], side);
+        return all;
+    };
+    const bool large = kLargeTiles * (double)ceil_div(in_all(256), (int64_t)256) <= (double)ceil_div(in_all(128), (int64_t)512);
+    return over(tab, [&](const Matrix& t) { return tiles(t, large ? 256 : 128); }, [&](dim3 g) {
+        tab.groups = (int)g.x;
+        const dim3 grid(ceil_div(g.x, 8u) * 8);
+        if (large) orth_product<T, KIND, 8, kHalves><<<grid, dim3(kThreads), 0, s>>>(tab);
+        else orth_product<T, KIND, 4, kHalves><<<grid, dim3(kThreads), 0, s>>>(tab);
+    });
+}
+
+template <typename T> int run(Table& tab, bool small, int iterations, hipStream_t s) {
     const dim3 threads(kThreads);
-    const auto tiles = [](int n) { return ceil_div(n, kTile); };
-    const auto triangle = [&](const Matrix& t) { return (int64_t)tiles(t.n) * (tiles(t.n) + 1) / 2; };
-    const auto all_tiles = [&](const Matrix& t) { return (int64_t)tiles(t.n) * tiles(t.m); };
+    if (small) {
+        orth_small<T><<<dim3(tab.count), dim3(kSmallThreads), 0, s>>>(tab, iterations);
+        return launched();
+    }
     I6TRAIN_TRY(over(tab, [](const Matrix& t) { return (int64_t)t.parts_n; }, [&](dim3 g) { orth_norms<T><<<g, threads, 0, s>>>(tab); }));
-    I6TRAIN_TRY(over(tab, [](const Matrix& t) { return (int64_t)ceil_div(t.m, kThreads); }, [&](dim3 g) { orth_pads<<<g, threads, 0, s>>>(tab); }));
     I6TRAIN_TRY(over(tab, [](const Matrix& t) { return (int64_t)ceil_div(t.rows, 64) * ceil_div(t.cols, 64); }, [&](dim3 g) { orth_operands<T><<<g, threads, 0, s>>>(tab); }));
     if (iterations == 0)
         return over(tab, [](const Matrix& t) { return ceil_div((int64_t)t.rows * t.cols, (int64_t)kThreads); }, [&](dim3 g) { orth_copy<T><<<g, threads, 0, s>>>(tab); });
     for (int i = 0; i < iterations; i++) {
-        I6TRAIN_TRY(over(tab, triangle, [&](dim3 g) { orth_product<T, kGram><<<g, threads, 0, s>>>(tab); }));
-        I6TRAIN_TRY(over(tab, triangle, [&](dim3 g) { orth_product<T, kFactor><<<g, threads, 0, s>>>(tab); }));
-        if (i + 1 < iterations) I6TRAIN_TRY(over(tab, all_tiles, [&](dim3 g) { orth_product<T, kUpdate><<<g, threads, 0, s>>>(tab); }));
-        else I6TRAIN_TRY(over(tab, all_tiles, [&](dim3 g) { orth_product<T, kLast><<<g, threads, 0, s>>>(tab); }));
+        I6TRAIN_TRY((multiply<T, kGram, 2>(tab, s)));
+        I6TRAIN_TRY((multiply<T, kFactor, 2>(tab, s)));
+        // 16-bit results: nothing follows in which an error of the last product grows.  Half the bits, 2^-12 of B's and X's values, add 0.1 to what the rounding of the result
+        // is off by (relative 2-norm 1.66e-3 -> 1.85e-3) and make it 1.5 times as fast.
+        if (i + 1 < iterations) I6TRAIN_TRY((multiply<T, kUpdate, 2>(tab, s)));
+        else I6TRAIN_TRY((multiply<T, kLast, sizeof(T) == 2 ? 1 : 2>(tab, s)));
         for (int j = 0; j < tab.count; j++) {
             f16* xt = tab.t[j].xt;
             tab.t[j].xt = tab.t[j].xt_next;
@@ -384,32 +686,38 @@ int i6orth_step(const i6orth_tensor* tensors, int n_tensors, int dtype, int iter
     if (iterations < 0 || !(mu >= 0 && mu < 1)) return I6TRAIN_ERR_INVALID_ARGUMENT;
     if (need == 0) return I6TRAIN_OK;
     if (!workspace || workspace_bytes < need) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
-    char* at = static_cast<char*>(workspace);
     Table tab;
     tab.count = 0;
     tab.mu = (float)mu;
     tab.nesterov = nesterov;
-    const auto flush = [&]() {
-        if (tab.count == 0) return I6TRAIN_OK;
-        const int rc = dtype == I6TRAIN_BF16 ? run<bf16>(tab, iterations, (hipStream_t)stream) : run<float>(tab, iterations, (hipStream_t)stream);
-        tab.count = 0;
-        return rc;
-    };
-    for (int i = 0; i < n_tensors; i++) {
-        const i6orth_tensor& t = tensors[i];
-        if (t.rows == 0 || t.cols == 0) continue;
-        if (tab.count == (int)(sizeof(tab.t) / sizeof(tab.t[0]))) I6TRAIN_TRY(flush());
-        const Places p(t);
-        Matrix& m = tab.t[tab.count++];
-        m.update = t.update; m.result = t.result; m.momentum = t.momentum;
-        m.x = reinterpret_cast<f16*>(at + p.x); m.xt = reinterpret_cast<f16*>(at + p.xt); m.xt_next = reinterpret_cast<f16*>(at + p.xt_next);
-        m.a = reinterpret_cast<f16*>(at + p.a); m.b = reinterpret_cast<f16*>(at + p.b);
-        m.parts = reinterpret_cast<double*>(at + p.parts);
-        m.rows = t.rows; m.cols = t.cols; m.n = p.n; m.m = p.m; m.np = p.np; m.mp = p.mp;
-        m.keep = t.keep; m.rate = t.rate; m.parts_n = p.parts_n;
-        at += p.all;
+    // which way a matrix goes depends on it alone, and so does its result
+    for (const bool small : {true, false}) {
+        const auto flush = [&]() {
+            if (tab.count == 0) return I6TRAIN_OK;
+            const int rc = dtype == I6TRAIN_BF16 ? run<bf16>(tab, small, iterations, (hipStream_t)stream) : run<float>(tab, small, iterations, (hipStream_t)stream);
+            tab.count = 0;
+            return rc;
+        };
+        char* at = static_cast<char*>(workspace);
+        for (int i = 0; i < n_tensors; i++) {
+            const i6orth_tensor& t = tensors[i];
+            if (t.rows == 0 || t.cols == 0) continue;
+            const Places p(t);
+            if (small == (iterations > 0 && is_small(p.n, p.m))) {
+                if (tab.count == (int)(sizeof(tab.t) / sizeof(tab.t[0]))) I6TRAIN_TRY(flush());
+                Matrix& m = tab.t[tab.count++];
+                m.update = t.update; m.result = t.result; m.momentum = t.momentum;
+                m.x = reinterpret_cast<f16*>(at + p.x); m.xt = reinterpret_cast<f16*>(at + p.xt); m.xt_next = reinterpret_cast<f16*>(at + p.xt_next);
+                m.a = reinterpret_cast<f16*>(at + p.a); m.b = reinterpret_cast<f16*>(at + p.b);
+                m.parts = reinterpret_cast<double*>(at + p.parts);
+                m.rows = t.rows; m.cols = t.cols; m.n = p.n; m.m = p.m; m.np = p.np; m.mp = p.mp;
+                m.keep = t.keep; m.rate = t.rate; m.parts_n = p.parts_n;
+            }
+            at += p.all;
+        }
+        I6TRAIN_TRY(flush());
     }
-    return flush();
+    return I6TRAIN_OK;
 }
 
 }  // extern "C"
