@@ -388,6 +388,7 @@ template <typename T, int KIND, int S, int kHalves> __global__ __launch_bounds__
 }
 
 // Small matrices: a workgroup does all of it for one, X and A (then B) in LDS.  A wave has sixteen rows of X, or a part of their columns, in 32 bits in its registers.
+// All four products of the halves: short sums have little error of their own beside that of the last one, and matrix instructions are not what is waited for.
 // What bounds it are the waits of a chain of products that has 15 links: two matrices of 128 x 64 take %%SMALL%%.
 constexpr int kSmallThreads = 512, kSmallBytes = 140 * 1024, kSmallTiles = 8;
 __host__ __device__ constexpr int small_parts(int n) { return n <= 16 ? 8 : (n <= 32 ? 4 : (n <= 64 ? 2 : 1)); }     // waves of sixteen rows
@@ -478,7 +479,7 @@ template <typename T> __global__ __launch_bounds__(kSmallThreads) void orth_smal
                     if (j >= tiles_n) continue;
                     const f16x8 q0 = rows_of(p, stride, 16 * j, k, lane), q1 = rows_of(p + plane, stride, 16 * j, k, lane);
                     hi[i] = multiplied(p0, q0, hi[i]);
-                    lo[i] = multiplied(p1, q0, multiplied(p0, q1, lo[i]));
+                    lo[i] = multiplied(p1, q0, multiplied(p0, q1, multiplied(p1, q1, lo[i])));
                 }
             }
 #pragma unroll
@@ -524,7 +525,7 @@ template <typename T> __global__ __launch_bounds__(kSmallThreads) void orth_smal
                     const int j = part + parts * i;
                     if (j >= tiles_m) continue;
                     const f16x8 q0 = columns_of(x, sx, 16 * j, k, lane), q1 = columns_of(x + plane_x, sx, 16 * j, k, lane);
-                    v[i] = multiplied(p0, q0, multiplied(p1, q0, multiplied(p0, q1, v[i])));
+                    v[i] = multiplied(p0, q0, multiplied(p1, q0, multiplied(p0, q1, multiplied(p1, q1, v[i]))));
                 }
             }
         __syncthreads();
