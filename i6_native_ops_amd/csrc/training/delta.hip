@@ -265,12 +265,6 @@ template <int KP> __device__ __forceinline__ void invert(Chunk<KP>& s) {
     Tile<20>{s.inverse}.put(wave, 0, t);
 }
 
-// Columns of a wave: NT for each lane, next to each other.
-template <int NT> struct Columns {
-    int first;                           // this lane's
-    __device__ __forceinline__ explicit Columns(int block) : first((block * 4 + (int)(threadIdx.x >> 6)) * 16 * NT + (int)(threadIdx.x & 15) * NT) {}
-};
-
 // Values of `T` at rows 16 m + 4 (lane >> 4) + r of a matrix, as accumulators.
 template <typename T, int NT, int M>
 __device__ __forceinline__ void load_columns(acc_t (&v)[M][NT], const T* p, int64_t stride, int rows, int col, int cols) {
@@ -305,141 +299,6 @@ __device__ __forceinline__ void store_columns(const acc_t (&v)[M][NT], T* p, int
             p += stride;
         }
         p += 12 * stride;
-    }
-}
-
-// ------------------------------------------------------------------------------------------------------------- forward
-
-template <typename T, int KP, int NT>
-__global__ __launch_bounds__(kThreads, 2) void delta_forward(Args a, bool whole) {
-    constexpr int M = kC / 16, KT = KP / 16;
-    __shared__ __align__(16) Chunk<KP> s;
-    const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 63, at = 4 * (lane >> 4);
-    const int col = Columns<NT>(blockIdx.x).first;
-    const int len = len_of(a, b), chunks = ceil_div(len, kC);
-    const int64_t head = (int64_t)b * a.H + h;
-    const Tile<Chunk<KP>::kStride> k{s.k}, q{s.q};
-    const Tile<Chunk<KP>::kSquare> ta{s.a}, tp{s.p};
-    const Tile<20> inverse{s.inverse};
-
-    acc_t state[KT][NT];
-    if (a.initial) {
-        load_columns<float, NT, KT>(state, a.initial + head * a.K * a.V, a.V, a.K, col, a.V);
-    } else {
-#pragma unroll
-        for (int i = 0; i < KT; i++)
-#pragma unroll
-            for (int j = 0; j < NT; j++) state[i][j] = 0.f;
-    }
-    Ahead<T, KP> next;
-    acc_t v_next[M][NT];
-    const T* v = static_cast<const T*>(a.v) + b * a.v_b + h * a.v_h;
-    if (chunks) {
-        next.fetch(a, b, h, 0, len, whole);
-        load_columns<T, NT, M>(v_next, v, a.v_t, len, col, a.V);
-    }
-    for (int n = 0; n < chunks; n++) {
-        const int first = n * kC, rows = min(kC, len - first);
-        next.store(s, first, len);
-        acc_t r[M][NT];
-#pragma unroll
-        for (int m = 0; m < M; m++)
-#pragma unroll
-            for (int j = 0; j < NT; j++) r[m][j] = v_next[m][j];
-        if (a.states) store_columns<float, NT, KT>(state, a.states + (head * a.chunks + n) * a.K * a.V, a.V, a.K, col, a.V);
-        __syncthreads();
-        if (n + 1 < chunks) {
-            next.fetch(a, b, h, first + kC, len, whole);
-            load_columns<T, NT, M>(v_next, v + (first + kC) * a.v_t, a.v_t, len - first - kC, col, a.V);
-        }
-        phase();
-        squares(s);
-        if (a.rows && blockIdx.x == 0 && threadIdx.x < kC) {
-            const int i = threadIdx.x;
-            a.rows[head * a.chunks * kC + first + i] = Rows{s.c[i], s.c_rest[i], s.w[i], s.rk[i], s.rq[i], 0.f, 0.f, 0.f};
-        }
-        __syncthreads();
-        invert(s);
-        phase();
-        // R = w (V - exp(c) K S0)
-#pragma unroll
-        for (int m = 0; m < M; m++) {
-            acc_t ks[NT] = {};
-#pragma unroll
-            for (int x = 0; x < KT; x++) {
-                const acc_t row = k.rows(m, x);
-#pragma unroll
-                for (int j = 0; j < NT; j++) ks[j] = product(row, state[x][j], ks[j]);
-            }
-            const acc_t by = four(s.from_start + 16 * m + at) * four(s.rk + 16 * m + at), w = four(s.w + 16 * m + at);
-#pragma unroll
-            for (int j = 0; j < NT; j++) r[m][j] = w * (r[m][j] - by * ks[j]);
-        }
-        __syncthreads();
-        // U, sixteen frames after sixteen
-#pragma unroll
-        for (int m = 0; m < M; m++) {
-#pragma unroll
-            for (int x = 0; x < m; x++) {
-                const acc_t row = -ta.rows(m, x);
-#pragma unroll
-                for (int j = 0; j < NT; j++) r[m][j] = product(row, r[x][j], r[m][j]);
-            }
-            const acc_t row = inverse.rows(m, 0);
-#pragma unroll
-            for (int j = 0; j < NT; j++) {
-                const acc_t none = 0.f;
-                r[m][j] = product(row, r[m][j], none);
-            }
-        }
-        if (a.u) store_columns<float, NT, M>(r, a.u + (head * a.chunks * kC + first) * a.V, a.V, kC, col, a.V);
-        acc_t o[M][NT];
-#pragma unroll
-        for (int m = 0; m < M; m++) {
-#pragma unroll
-            for (int j = 0; j < NT; j++) o[m][j] = 0.f;
-#pragma unroll
-            for (int x = 0; x < KT; x++) {
-                const acc_t row = q.rows(m, x);
-#pragma unroll
-                for (int j = 0; j < NT; j++) o[m][j] = product(row, state[x][j], o[m][j]);
-            }
-            const acc_t by = four(s.from_start + 16 * m + at) * four(s.rq + 16 * m + at);
-#pragma unroll
-            for (int j = 0; j < NT; j++) o[m][j] *= by;
-#pragma unroll
-            for (int x = 0; x <= m; x++) {
-                const acc_t row = tp.rows(m, x);
-#pragma unroll
-                for (int j = 0; j < NT; j++) o[m][j] = product(row, r[x][j], o[m][j]);
-            }
-        }
-        store_columns<T, NT, M>(o, static_cast<T*>(a.o) + (((int64_t)b * a.T + first) * a.H + h) * a.V, (int64_t)a.H * a.V, rows, col, a.V);
-        // the state behind the chunk
-        const float decay = s.from_start[kC - 1];
-#pragma unroll
-        for (int m = 0; m < M; m++) {
-            const acc_t by = four(s.to_end + 16 * m + at) * four(s.rk + 16 * m + at);
-#pragma unroll
-            for (int j = 0; j < NT; j++) r[m][j] *= by;
-        }
-#pragma unroll
-        for (int i = 0; i < KT; i++) {
-#pragma unroll
-            for (int j = 0; j < NT; j++) state[i][j] *= decay;
-#pragma unroll
-            for (int m = 0; m < M; m++) {
-                const acc_t row = k.columns(i, m);
-#pragma unroll
-                for (int j = 0; j < NT; j++) state[i][j] = product(row, r[m][j], state[i][j]);
-            }
-        }
-        __syncthreads();
-    }
-    store_columns<float, NT, KT>(state, a.last + head * a.K * a.V, a.V, a.K, col, a.V);
-    for (int t = len + (int)(threadIdx.x >> 6); t < a.T; t += 4) {
-        T* o = static_cast<T*>(a.o) + (((int64_t)b * a.T + t) * a.H + h) * a.V;
-        for (int c = blockIdx.x * 64 * NT + lane; c < min(a.V, (int)(blockIdx.x + 1) * 64 * NT); c += 64) o[c] = (T)0.f;
     }
 }
 
@@ -515,127 +374,6 @@ __global__ __launch_bounds__(kThreads) void delta_frames(Args a) {
 }
 
 // ------------------------------------------------------------------------------------------------------------ backward
-
-// From the last chunk to the first: gradients of the states behind the chunks, of R and of v.
-template <typename T, int KP, int NT>
-__global__ __launch_bounds__(kThreads, 2) void delta_backward(Args a, bool whole) {
-    constexpr int M = kC / 16, KT = KP / 16;
-    __shared__ __align__(16) Chunk<KP> s;
-    const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 63, at = 4 * (lane >> 4);
-    const int col = Columns<NT>(blockIdx.x).first;
-    const int len = len_of(a, b), chunks = ceil_div(len, kC);
-    const int64_t head = (int64_t)b * a.H + h;
-    const Tile<Chunk<KP>::kStride> k{s.k}, q{s.q};
-    const Tile<Chunk<KP>::kSquare> ta{s.a}, tp{s.p};
-    const Tile<20> inverse{s.inverse};
-
-    acc_t d[KT][NT];
-    if (a.d_last) {
-        load_columns<float, NT, KT>(d, a.d_last + head * a.K * a.V, a.V, a.K, col, a.V);
-    } else {
-#pragma unroll
-        for (int i = 0; i < KT; i++)
-#pragma unroll
-            for (int j = 0; j < NT; j++) d[i][j] = 0.f;
-    }
-    Ahead<T, KP> next;
-    acc_t o_next[M][NT] = {};
-    const T* d_o = static_cast<const T*>(a.d_o) + b * a.do_b + h * a.do_h;
-    const auto fetch = [&](int first) {
-        next.fetch(a, b, h, first, len, whole);
-        if (a.d_o) load_columns<T, NT, M>(o_next, d_o + first * a.do_t, a.do_t, len - first, col, a.V);
-    };
-    if (chunks) fetch((chunks - 1) * kC);
-    for (int n = chunks - 1; n >= 0; n--) {
-        const int first = n * kC, rows = min(kC, len - first);
-        next.store(s, first, len);
-        acc_t o[M][NT], r[M][NT];
-#pragma unroll
-        for (int m = 0; m < M; m++)
-#pragma unroll
-            for (int j = 0; j < NT; j++) o[m][j] = o_next[m][j];
-        store_columns<float, NT, KT>(d, a.ends + (head * a.chunks + n) * a.K * a.V, a.V, a.K, col, a.V);
-        __syncthreads();
-        if (n) fetch(first - kC);
-        phase();
-        squares(s);
-        __syncthreads();
-        invert(s);
-        phase();
-#pragma unroll
-        for (int m = 0; m < M; m++) {
-#pragma unroll
-            for (int j = 0; j < NT; j++) r[m][j] = 0.f;
-#pragma unroll
-            for (int x = 0; x < KT; x++) {
-                const acc_t row = k.rows(m, x);
-#pragma unroll
-                for (int j = 0; j < NT; j++) r[m][j] = product(row, d[x][j], r[m][j]);
-            }
-            const acc_t by = four(s.to_end + 16 * m + at) * four(s.rk + 16 * m + at);
-#pragma unroll
-            for (int j = 0; j < NT; j++) r[m][j] *= by;
-#pragma unroll
-            for (int x = m; x < M; x++) {
-                const acc_t row = tp.columns(m, x);
-#pragma unroll
-                for (int j = 0; j < NT; j++) r[m][j] = product(row, o[x][j], r[m][j]);
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int m = M - 1; m >= 0; m--) {
-#pragma unroll
-            for (int x = m + 1; x < M; x++) {
-                const acc_t row = -ta.columns(m, x);
-#pragma unroll
-                for (int j = 0; j < NT; j++) r[m][j] = product(row, r[x][j], r[m][j]);
-            }
-            const acc_t row = inverse.columns(0, m);
-#pragma unroll
-            for (int j = 0; j < NT; j++) {
-                const acc_t none = 0.f;
-                r[m][j] = product(row, r[m][j], none);
-            }
-        }
-        store_columns<float, NT, M>(r, a.dr + (head * a.chunks * kC + first) * a.V, a.V, kC, col, a.V);
-        acc_t dv[M][NT];
-#pragma unroll
-        for (int m = 0; m < M; m++) {
-            const acc_t w = four(s.w + 16 * m + at), start = four(s.from_start + 16 * m + at);
-            const acc_t by_q = start * four(s.rq + 16 * m + at), by_k = -start * four(s.rk + 16 * m + at);
-#pragma unroll
-            for (int j = 0; j < NT; j++) {
-                dv[m][j] = r[m][j] * w;
-                o[m][j] *= by_q;
-                r[m][j] = dv[m][j] * by_k;
-            }
-        }
-        store_columns<T, NT, M>(dv, static_cast<T*>(a.d_v) + (((int64_t)b * a.T + first) * a.H + h) * a.V, (int64_t)a.H * a.V, rows, col, a.V);
-        phase();
-        const float decay = s.from_start[kC - 1];
-#pragma unroll
-        for (int i = 0; i < KT; i++) {
-#pragma unroll
-            for (int j = 0; j < NT; j++) d[i][j] *= decay;
-#pragma unroll
-            for (int m = 0; m < M; m++) {
-                const acc_t row_q = q.columns(i, m), row_k = k.columns(i, m);
-#pragma unroll
-                for (int j = 0; j < NT; j++) {
-                    d[i][j] = product(row_q, o[m][j], d[i][j]);
-                    d[i][j] = product(row_k, r[m][j], d[i][j]);
-                }
-            }
-        }
-        __syncthreads();
-    }
-    if (a.d_initial) store_columns<float, NT, KT>(d, a.d_initial + head * a.K * a.V, a.V, a.K, col, a.V);
-    for (int t = len + (int)(threadIdx.x >> 6); t < a.T; t += 4) {
-        T* dv = static_cast<T*>(a.d_v) + (((int64_t)b * a.T + t) * a.H + h) * a.V;
-        for (int c = blockIdx.x * 64 * NT + lane; c < min(a.V, (int)(blockIdx.x + 1) * 64 * NT); c += 64) dv[c] = (T)0.f;
-    }
-}
 
 // Four values of a row of a float matrix with V columns; zeros behind them.
 __device__ __forceinline__ acc_t load_four(const float* row, int at, int n, bool whole) {
@@ -896,6 +634,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void delta_shared(A
 }
 
 #include "delta_16.inc"
+#include "delta_32.inc"
 
 // ---------------------------------------------------------------------------------------------------------------- host
 
@@ -924,14 +663,8 @@ Args args_of(const i6delta_problem& p) {
     return a;
 }
 
-// Whether keys and queries can be read in pieces of 16 bytes.
-bool whole_pieces(const i6delta_problem& p) {
-    const size_t n = elem_size(p.dtype);
-    const auto whole = [&](const void* x, int64_t s0, int64_t s1, int64_t s2) {
-        return (uintptr_t)x % 16 == 0 && (s0 * (int64_t)n) % 16 == 0 && (s1 * (int64_t)n) % 16 == 0 && (s2 * (int64_t)n) % 16 == 0;
-    };
-    return whole(p.q, p.q_stride_b, p.q_stride_t, p.q_stride_g) && whole(p.k, p.k_stride_b, p.k_stride_t, p.k_stride_g);
-}
+// 32 bits: whether rows begin where they can be read in pieces of 16 bytes.
+bool whole_floats(const void* x, int64_t s0, int64_t s1, int64_t s2) { return (uintptr_t)x % 16 == 0 && s0 % 4 == 0 && s1 % 4 == 0 && s2 % 4 == 0; }
 
 // bfloat16: whether rows of `cols` values can be read in pieces of 16 bytes; otherwise they are copied first, each in so many values.
 bool whole_rows(const void* x, int64_t s0, int64_t s1, int64_t s2, int cols) { return (uintptr_t)x % 16 == 0 && s0 % 8 == 0 && s1 % 8 == 0 && s2 % 8 == 0 && cols % 8 == 0; }
@@ -973,7 +706,7 @@ struct Places {
         const size_t copy_k = whole_rows(p.k, p.k_stride_b, p.k_stride_t, p.k_stride_g, p.K) ? 0 : k, copy_q = whole_rows(p.q, p.q_stride_b, p.q_stride_t, p.q_stride_g, p.K) ? 0 : k;
         const size_t copy_v = whole_rows(p.v, p.v_stride_b, p.v_stride_t, p.v_stride_h, p.V) ? 0 : v;
         back_blocks = d_k + heads;
-        back_packed = back_blocks + (x16 ? align256(n * kChunkBlocks<true> * sizeof(bf16)) : 0);
+        back_packed = back_blocks + align256(x16 ? n * kChunkBlocks<true> * sizeof(bf16) : n * kBlocks32 * 256 * sizeof(float));
         back_split = back_packed + (x16 ? copy_k + copy_q + v : 0);
         // Segments: as many as fill the card, and no more than pay for going along them one after the other; below three the second pass costs what the first one saves, and
         // a short sequence does not pay for the launches.  Without and with them, heads of 64 (128): 8 of 2048 frames 142 -> 54 us (225 -> 87), of 512 45 -> 37 (66 -> 52),
@@ -981,7 +714,7 @@ struct Places {
         const int chunks = ceil_div(p.T, C);
         const int64_t heads_at_once = (int64_t)p.B * p.H;
         per = chunks;
-        if (x16 && chunks >= (heads_at_once > 32 ? 16 : 8)) {
+        if (chunks >= (heads_at_once > 32 ? 16 : 8)) {
             const int most = (int)std::min<int64_t>(kCus / heads_at_once, (int64_t)sqrt(5.0 * chunks));
             if (most >= 3) {
                 per = ceil_div(chunks, most);
@@ -993,10 +726,10 @@ struct Places {
         const size_t split_bytes = turns + align256(slots * KP * KP * sizeof(float));
         back = back_split + split_bytes;
         // frame by frame nothing is needed
-        const bool chunked = x16 && (train || p.T > kMostFrames);
+        const bool chunked = train || p.T > kMostFrames;
         blocks = chunked && !train ? states : 0;
-        packed = chunked ? blocks + align256(n * kChunkBlocks<false> * sizeof(bf16)) : 0;
-        split = chunked ? packed + copy_k + copy_q + copy_v : 0;
+        packed = chunked ? blocks + align256(x16 ? n * kChunkBlocks<false> * sizeof(bf16) : n * kBlocks32 * 256 * sizeof(float)) : 0;
+        split = chunked ? packed + (x16 ? copy_k + copy_q + copy_v : 0) : 0;
         forward = chunked ? split + split_bytes : 0;
     }
 };
@@ -1004,14 +737,24 @@ struct Places {
 struct Call {
     Args a;
     Args16 k16;
-    bool whole, train;
+    bool whole, whole_v, train;
     bf16* blocks;
 };
 
+// Whether a workgroup has all of a head's more than 64 columns: its waves share a unit two by two.  With half the card's units or fewer a head's columns are two workgroups'.
+bool wide(const Call& c) { return c.a.V > 64 && (int64_t)c.a.B * c.a.H * c.k16.segments * 2 > kCus; }
+
 template <int KP> void run_forward(const Call& c, hipStream_t s, float) {
-    const Args& a = c.a;
-    if (a.V > 64) delta_forward<float, KP, 2><<<dim3(ceil_div(a.V, 128), a.H, a.B), dim3(kThreads), 0, s>>>(a, c.whole);
-    else delta_forward<float, KP, 1><<<dim3(1, a.H, a.B), dim3(kThreads), 0, s>>>(a, c.whole);
+    const Args16& k = c.k16;
+    float* blocks = reinterpret_cast<float*>(c.blocks);
+    delta_prepare32<KP, false><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, blocks, c.whole);
+    const int groups = ceil_div(32 * k.pairs + KP, 128);
+    if (k.segments > 1) {
+        delta_forward32<KP, 8, true><<<dim3(c.a.H * groups, c.a.B, k.segments - 1), dim3(512), 0, s>>>(c.a, k, blocks, c.whole, c.whole_v);
+        delta_join16<KP, kC><<<dim3(ceil_div(c.a.V, 16), c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, k, false);
+    }
+    if (wide(c)) delta_forward32<KP, 8, false><<<dim3(c.a.H, c.a.B, k.segments), dim3(512), 0, s>>>(c.a, k, blocks, c.whole, c.whole_v);
+    else delta_forward32<KP, 4, false><<<dim3(c.a.H * ceil_div(c.a.V, 64), c.a.B, k.segments), dim3(256), 0, s>>>(c.a, k, blocks, c.whole, c.whole_v);
 }
 template <int KP> void run_forward(const Call& c, hipStream_t s, bf16) {
     delta_prepare16<KP, false><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.blocks);
@@ -1019,17 +762,23 @@ template <int KP> void run_forward(const Call& c, hipStream_t s, bf16) {
     const int groups = ceil_div(32 * k.pairs + KP, 128);
     if (k.segments > 1) {
         delta_forward16<KP, 8, true><<<dim3(c.a.H * groups, c.a.B, k.segments - 1), dim3(512), 0, s>>>(c.a, k, c.blocks);
-        delta_join16<KP><<<dim3(ceil_div(c.a.V, 16), c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, k, false);
+        delta_join16<KP, kC16><<<dim3(ceil_div(c.a.V, 16), c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, k, false);
     }
-    const dim3 grid(c.a.H, c.a.B, k.segments);
-    if (c.a.V > 64) delta_forward16<KP, 8, false><<<grid, dim3(512), 0, s>>>(c.a, k, c.blocks);
-    else delta_forward16<KP, 4, false><<<grid, dim3(256), 0, s>>>(c.a, k, c.blocks);
+    if (wide(c)) delta_forward16<KP, 8, false><<<dim3(c.a.H, c.a.B, k.segments), dim3(512), 0, s>>>(c.a, k, c.blocks);
+    else delta_forward16<KP, 4, false><<<dim3(c.a.H * ceil_div(c.a.V, 64), c.a.B, k.segments), dim3(256), 0, s>>>(c.a, k, c.blocks);
 }
 template <int KP> void run_backward(const Call& c, hipStream_t s, float) {
-    const Args& a = c.a;
-    if (a.V > 64) delta_backward<float, KP, 2><<<dim3(ceil_div(a.V, 128), a.H, a.B), dim3(kThreads), 0, s>>>(a, c.whole);
-    else delta_backward<float, KP, 1><<<dim3(1, a.H, a.B), dim3(kThreads), 0, s>>>(a, c.whole);
-    delta_gradients<float, KP><<<dim3(a.chunks, a.H, a.B), dim3(kThreads), 0, s>>>(a);
+    const Args16& k = c.k16;
+    float* blocks = reinterpret_cast<float*>(c.blocks);
+    delta_prepare32<KP, true><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, blocks, c.whole);
+    const int groups = ceil_div(32 * k.pairs + KP, 128);
+    if (k.segments > 1) {
+        delta_backward32<KP, 8, true><<<dim3(c.a.H * groups, c.a.B, k.segments - 1), dim3(512), 0, s>>>(c.a, k, blocks, c.whole, c.whole_v);
+        delta_join16<KP, kC><<<dim3(ceil_div(c.a.V, 16), c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, k, true);
+    }
+    if (wide(c)) delta_backward32<KP, 8, false><<<dim3(c.a.H, c.a.B, k.segments), dim3(512), 0, s>>>(c.a, k, blocks, c.whole, c.whole_v);
+    else delta_backward32<KP, 4, false><<<dim3(c.a.H * ceil_div(c.a.V, 64), c.a.B, k.segments), dim3(256), 0, s>>>(c.a, k, blocks, c.whole, c.whole_v);
+    delta_gradients<float, KP><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a);
 }
 template <int KP> void run_backward(const Call& c, hipStream_t s, bf16) {
     delta_prepare16<KP, true><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.blocks);
@@ -1037,11 +786,10 @@ template <int KP> void run_backward(const Call& c, hipStream_t s, bf16) {
     const int groups = ceil_div(32 * k.pairs + KP, 128);
     if (k.segments > 1) {
         delta_backward16<KP, 8, true><<<dim3(c.a.H * groups, c.a.B, k.segments - 1), dim3(512), 0, s>>>(c.a, k, c.blocks);
-        delta_join16<KP><<<dim3(ceil_div(c.a.V, 16), c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, k, true);
+        delta_join16<KP, kC16><<<dim3(ceil_div(c.a.V, 16), c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, k, true);
     }
-    const dim3 grid(c.a.H, c.a.B, k.segments);
-    if (c.a.V > 64) delta_backward16<KP, 8, false><<<grid, dim3(512), 0, s>>>(c.a, k, c.blocks);
-    else delta_backward16<KP, 4, false><<<grid, dim3(256), 0, s>>>(c.a, k, c.blocks);
+    if (wide(c)) delta_backward16<KP, 8, false><<<dim3(c.a.H, c.a.B, k.segments), dim3(512), 0, s>>>(c.a, k, c.blocks);
+    else delta_backward16<KP, 4, false><<<dim3(c.a.H * ceil_div(c.a.V, 64), c.a.B, k.segments), dim3(256), 0, s>>>(c.a, k, c.blocks);
     if (c.k16.pairs == 4) delta_gradients16<KP, 4><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(512), 0, s>>>(c.a, c.k16);
     else delta_gradients16<KP, 2><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(512), 0, s>>>(c.a, c.k16);
 }
@@ -1096,7 +844,8 @@ int pack(const Args& a, char*& to, const void*& x, int64_t& s0, int64_t& s1, int
 Call call_of(const i6delta_problem& p, const Places& at, void* kept) {
     Call c{};
     c.a = args_of(p);
-    c.whole = whole_pieces(p);
+    c.whole = whole_floats(p.q, p.q_stride_b, p.q_stride_t, p.q_stride_g) && whole_floats(p.k, p.k_stride_b, p.k_stride_t, p.k_stride_g);
+    c.whole_v = whole_floats(p.v, p.v_stride_b, p.v_stride_t, p.v_stride_h);
     c.k16.pairs = at.pairs;
     c.k16.segments = at.segments;
     c.k16.per = at.per;
@@ -1141,11 +890,13 @@ int i6delta_forward(const i6delta_problem* p, void* o, float* last, void* kept, 
         if (!kept) c.a.rows = static_cast<Rows*>(workspace);
         c.k16.ends = reinterpret_cast<float*>(static_cast<char*>(workspace) + at.split);
         c.k16.turns = reinterpret_cast<float*>(static_cast<char*>(workspace) + at.split + at.turns);
-        Args& a = c.a;
-        char* to = static_cast<char*>(workspace) + at.packed;
-        I6TRAIN_TRY(pack(a, to, a.k, a.k_b, a.k_t, a.k_g, a.G, a.K, (hipStream_t)stream));
-        I6TRAIN_TRY(pack(a, to, a.q, a.q_b, a.q_t, a.q_g, a.G, a.K, (hipStream_t)stream));
-        I6TRAIN_TRY(pack(a, to, a.v, a.v_b, a.v_t, a.v_h, a.H, a.V, (hipStream_t)stream));
+        if (p->dtype == I6TRAIN_BF16) {
+            Args& a = c.a;
+            char* to = static_cast<char*>(workspace) + at.packed;
+            I6TRAIN_TRY(pack(a, to, a.k, a.k_b, a.k_t, a.k_g, a.G, a.K, (hipStream_t)stream));
+            I6TRAIN_TRY(pack(a, to, a.q, a.q_b, a.q_t, a.q_g, a.G, a.K, (hipStream_t)stream));
+            I6TRAIN_TRY(pack(a, to, a.v, a.v_b, a.v_t, a.v_h, a.H, a.V, (hipStream_t)stream));
+        }
     }
     return p->dtype == I6TRAIN_F32 ? forward_of<float>(c, (hipStream_t)stream) : forward_of<bf16>(c, (hipStream_t)stream);
 }
@@ -1161,6 +912,7 @@ int i6delta_backward(const i6delta_problem* p, const void* grad_o, int64_t grad_
     Args& a = c.a;
     a.d_o = grad_o; a.do_b = grad_stride_b; a.do_t = grad_stride_t; a.do_h = grad_stride_h;
     a.d_last = grad_last;
+    c.whole_v = whole_floats(grad_o, grad_stride_b, grad_stride_t, grad_stride_h);
     a.d_q = grad_q; a.d_k = grad_k; a.d_v = grad_v; a.d_gate = grad_gate; a.d_beta = grad_beta; a.d_initial = grad_initial;
     char* base = static_cast<char*>(workspace);
     a.ends = reinterpret_cast<float*>(base + at.ends);

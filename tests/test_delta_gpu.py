@@ -200,10 +200,11 @@ def test_frames_that_reach_far(T, K, V, dtype):
     check(p, run(p), expected(p))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("K,V,lens", [(64, 64, [1300, 1217]), (128, 128, [1300, 640]), (32, 40, [1281, 0]), (128, 64, [1000, 1300]), (64, 128, [1300, 1])])
-def test_sequences_in_segments(K, V, lens):
+def test_sequences_in_segments(K, V, lens, dtype):
     """Few heads and many frames: a sequence's parts are worked on at the same time.  Ends at and off a segment's, and sequences that end segments before the longest."""
-    p = problem(2, 1300, 2, 1, K, V, torch.bfloat16, lens=lens)
+    p = problem(2, 1300, 2, 1, K, V, dtype, lens=lens)
     p["gate"] += 3
     check(p, run(p), expected(p))
 
