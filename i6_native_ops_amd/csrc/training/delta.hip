@@ -307,18 +307,27 @@ __device__ __forceinline__ void store_columns(const acc_t (&v)[M][NT], T* p, int
 // Few frames, no training: 64 columns of a head, KP / 4 rows of the state in the registers of each of four waves.  The state is read and written once; with
 // x = S^T k and y = S^T q of the state in front of a frame,  u = w (v - f x),  o = f y + (k.q) u.
 template <typename T, int KP>
-__global__ __launch_bounds__(kThreads) void delta_frames(Args a) {
+__global__ __launch_bounds__(kThreads, 4) void delta_frames(Args a) {
     constexpr int R = KP / 4;
     __shared__ __align__(16) float key[KP], query[KP], sums[4][2][64], dots[2][3];
     const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
     const int len = len_of(a, b), g = h / (a.H / a.G);
     const int64_t head = (int64_t)b * a.H + h;
     const bool mine = col < a.V;
+    // whole rows, as they mostly are: one address for all
+    const int64_t from = (head * a.K + wave * R) * a.V + col;
+    const bool whole = a.K == KP && blockIdx.x * 64 + 64 <= a.V;
     float state[R];
+    if (a.initial && whole) {
+        const float* p = a.initial + from;
 #pragma unroll
-    for (int i = 0; i < R; i++) {
-        const int row = wave * R + i;
-        state[i] = a.initial && mine && row < a.K ? a.initial[(head * a.K + row) * a.V + col] : 0.f;
+        for (int i = 0; i < R; i++) {
+            state[i] = *p;
+            p += a.V;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < R; i++) state[i] = a.initial && mine && wave * R + i < a.K ? a.initial[from + (int64_t)i * a.V] : 0.f;
     }
     for (int t = 0; t < a.T; t++) {
         T* o = static_cast<T*>(a.o) + (((int64_t)b * a.T + t) * a.H + h) * a.V;
@@ -366,10 +375,17 @@ __global__ __launch_bounds__(kThreads) void delta_frames(Args a) {
 #pragma unroll
         for (int i = 0; i < R; i++) state[i] = fmaf(kv[i], uk, f * state[i]);
     }
+    if (whole) {
+        float* p = a.last + from;
 #pragma unroll
-    for (int i = 0; i < R; i++) {
-        const int row = wave * R + i;
-        if (mine && row < a.K) a.last[(head * a.K + row) * a.V + col] = state[i];
+        for (int i = 0; i < R; i++) {
+            *p = state[i];
+            p += a.V;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < R; i++)
+            if (mine && wave * R + i < a.K) a.last[from + (int64_t)i * a.V] = state[i];
     }
 }
 
