@@ -1,11 +1,11 @@
 // Orthogonal factors of matrices by Newton-Schulz products, and the optimiser's step on them (include/i6orth.h).
 //
 // X has n rows and m >= n columns.  An iteration is three products for all matrices of the call, a launch each:  A = X X^T,
-// B = b A + c A A,  X = a X + B X.  A and B are symmetric: of the first two only the tiles on and below the diagonal are formed, and written to both
+// B = a + b A + c A A,  X = B X.  A and B are symmetric: of the first two only the tiles on and below the diagonal are formed, and written to both
 // places.  X is kept as it is and transposed, so that both operands of every product have consecutive k.
 //
 // Operands are two 16-bit floating-point halves, x = x1 + x2, of 22 bits, times a power of two that brings the largest value they can have (X: 1.21, A: 1.46,
-// B: 2.9) below 2^16; of (x1 + x2)(y1 + y2) the last term is below the precision.  Half the bits would do for the products, but not for what becomes of them: an error in A is one of
+// B: 3.45) below 2^16; of (x1 + x2)(y1 + y2) the last term is below the precision.  Half the bits would do for the products, but not for what becomes of them: an error in A is one of
 // left singular vectors of all sizes, and the small ones grow 3.4 times in each iteration, 485 times in five.
 #include <cmath>
 
@@ -275,11 +275,45 @@ template <typename T, int KIND, int S, int kHalves> __device__ __forceinline__ v
 #endif
         }
     }
-    // What becomes of a tile.  A lane has four values of a column of C, which stand side by side in C's transpose; rows go through LDS, where a wave has room for 64 of them.
+    // What becomes of a tile: 64 of a wave's rows at a time go through LDS, from where lanes take eight values side by side, of rows and of columns.  A row's words are turned by
+    // its number, so that neither way two lanes meet in a bank.
     const int at = 4 * (lane >> 4), ci0 = i0 + wi * 16 * S, cj0 = j0 + wj * 16 * S;
-    const bool wide = t.rows <= t.cols, whole = t.cols % 4 == 0 && (uintptr_t)t.result % (4 * sizeof(T)) == 0;
+    const bool wide = t.rows <= t.cols, whole = t.cols % 8 == 0 && (uintptr_t)t.result % 16 == 0;
     constexpr int kWidth = 16 * S;
     uint32_t* mine = reinterpret_cast<uint32_t*>(lds) + wave * 64 * kWidth;
+    const auto turn = [](int r) { return ((r >> 3 & 7) << 3) ^ ((r >> 2 & 3) << 4); };
+    // halves of eight packed words
+    const auto store_halves = [&](f16* to, const uint32_t (&w)[8]) {
+        const auto first = [&](int i) { return __builtin_amdgcn_perm(w[i + 1], w[i], 0x05040100); };
+        const auto second = [&](int i) { return __builtin_amdgcn_perm(w[i + 1], w[i], 0x07060302); };
+        *reinterpret_cast<uint4*>(to) = make_uint4(first(0), first(2), first(4), first(6));
+        *reinterpret_cast<uint4*>(to + 32) = make_uint4(second(0), second(2), second(4), second(6));
+    };
+    const auto store_result = [&](int r, int c, const uint32_t (&w)[8]) {
+        if (r >= t.rows || c >= t.cols) return;
+        T* to = static_cast<T*>(t.result) + (int64_t)r * t.cols + c;
+        const int left = t.cols - c;
+        float was[8];
+        if (t.momentum) {
+            load_some(was, to, left, whole);
+#pragma unroll
+            for (int e = 0; e < 8; e++) was[e] = fmaf(-t.rate, __uint_as_float(w[e]), was[e] * t.keep);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) was[e] = __uint_as_float(w[e]);
+        }
+        if (whole) {
+            using T8 = T __attribute__((ext_vector_type(8)));
+            T8 v;
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = (T)was[e];
+            *reinterpret_cast<T8*>(to) = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (e < left) to[e] = (T)was[e];
+        }
+    };
     wait_and_meet<0>();
 #pragma unroll
     for (int strip = 0; strip < S / 4; strip++) {
@@ -292,77 +326,49 @@ template <typename T, int KIND, int S, int kHalves> __device__ __forceinline__ v
                 const bool there = cj < rows_q && ci < t.np;
                 acc_t v = acc[i][j];
                 if (KIND == kGram) v *= kScaleA / (kScaleX * kScaleX);
-                else {
-                    const f16* own = (KIND == kFactor ? t.a : t.xt) + place(there ? cj : 0, there ? ci : 0, t.np);
+                if (KIND == kFactor) {   // A is symmetric: a lane's four rows of a column are four columns of a row
+                    const f16* own = t.a + place(there ? cj : 0, there ? ci : 0, t.np);
                     const acc_t x = __builtin_convertvector(*reinterpret_cast<const f16x4*>(own), acc_t) + __builtin_convertvector(*reinterpret_cast<const f16x4*>(own + 32), acc_t);
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        v[e] = KIND == kFactor ? fmaf(kC * (kScaleB / (kScaleA * kScaleA)), v[e], kB * (kScaleB / kScaleA) * x[e]) : fmaf(v[e], 1.f / kScaleB, kA * x[e]);
-                }
-                uint32_t words[4];
-                if (KIND == kLast) {
-                    const acc_t o = v * (1.f / kScaleX);
-                    if (!wide && whole) {        // the result's rows are C's columns
-                        if (cj < t.m && ci < t.cols) {
-                            using T4 = T __attribute__((ext_vector_type(4)));
-                            T4* to = reinterpret_cast<T4*>(static_cast<T*>(t.result) + (int64_t)cj * t.cols + ci);
-                            T4 r = __builtin_convertvector(o, T4);
-                            if (t.momentum) {
-                                const acc_t was = __builtin_convertvector(*to, acc_t);
-#pragma unroll
-                                for (int e = 0; e < 4; e++) r[e] = (T)fmaf(-t.rate, o[e], was[e] * t.keep);
-                            }
-                            *to = r;
-                        }
-                        continue;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; e++) words[e] = __float_as_uint(o[e]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) words[e] = there && ci + e < t.n ? packed(v[e]) : 0;
-                    if (there && (!kSymmetric || ti != tj)) {
-                        f16* to = (KIND == kGram ? t.a : (KIND == kFactor ? t.b : t.xt_next)) + place(cj, ci, t.np);
-                        *reinterpret_cast<uint2*>(to) = make_uint2(__builtin_amdgcn_perm(words[1], words[0], 0x05040100), __builtin_amdgcn_perm(words[3], words[2], 0x05040100));
-                        *reinterpret_cast<uint2*>(to + 32) = make_uint2(__builtin_amdgcn_perm(words[1], words[0], 0x07060302), __builtin_amdgcn_perm(words[3], words[2], 0x07060302));
+                    for (int e = 0; e < 4; e++) {
+                        v[e] = fmaf(kC * (kScaleB / (kScaleA * kScaleA)), v[e], kB * (kScaleB / kScaleA) * x[e]);
+                        if (ci + e == cj) v[e] += kA * kScaleB;
                     }
                 }
+                if (KIND == kUpdate) v *= 1.f / kScaleB;
+                if (KIND == kLast) v *= 1.f / (kScaleB * kScaleX);
+                const int turned = (j * 16 + (lane & 15)) ^ turn(i4 * 16 + at);
 #pragma unroll
-                for (int e = 0; e < 4; e++) mine[(i4 * 16 + at + e) * kWidth + ((j * 16 + (lane & 15)) ^ (at << 2))] = words[e];
+                for (int e = 0; e < 4; e++) mine[(i4 * 16 + at + e) * kWidth + turned] = KIND == kLast ? __float_as_uint(v[e]) : (there && ci + e < t.n ? packed(v[e]) : 0);
             }
-            if (S == 8) __builtin_amdgcn_sched_barrier(0);       // or what all 16 x 16 tiles load is loaded first
         }
         asm volatile("" ::: "memory");   // a wave's own part of LDS, which it reads in the order of its writes
-        if (KIND == kLast) {
-            const auto put = [&](int r, int c) {
-                const int ci = ci0 + strip * 64 + r, cj = cj0 + c;
-                if (ci >= t.n || cj >= t.m) return;
-                const float o = __uint_as_float(mine[r * kWidth + (c ^ ((r & 12) << 2))]);
-                T* to = static_cast<T*>(t.result) + (wide ? (int64_t)ci * t.cols + cj : (int64_t)cj * t.cols + ci);
-                *to = t.momentum ? (T)fmaf(-t.rate, o, (float)*to * t.keep) : (T)o;
-            };
-            if (wide) {
-                for (int x = lane; x < 64 * kWidth; x += 64) put(x / kWidth, x % kWidth);
-            } else if (!whole) {
-                for (int c = 0; c < kWidth; c++) put(lane, c);
-            }
-            continue;
-        }
-        const int stride = kSymmetric ? t.np : t.mp;
-        f16* out = KIND == kGram ? t.a : (KIND == kFactor ? t.b : t.x);
+        if (KIND != kLast || wide) {
+            const int stride = kSymmetric ? t.np : t.mp;
+            f16* out = KIND == kGram ? t.a : (KIND == kFactor ? t.b : t.x);
 #pragma unroll 4
-        for (int x = lane; x < 64 * (kWidth / 8); x += 64) {
-            const int r = x / (kWidth / 8), c = x % (kWidth / 8) * 8, ci = ci0 + strip * 64 + r, cj = cj0 + c;
-            if (ci >= t.n || cj >= stride) continue;
-            const uint4* w = reinterpret_cast<const uint4*>(mine + r * kWidth + (c ^ ((r & 12) << 2)));
-            const uint4 u = w[0], v = w[1];
-            f16* to = out + place(ci, cj, stride);
-            *reinterpret_cast<uint4*>(to) = make_uint4(__builtin_amdgcn_perm(u.y, u.x, 0x05040100), __builtin_amdgcn_perm(u.w, u.z, 0x05040100), __builtin_amdgcn_perm(v.y, v.x, 0x05040100),
-                                                       __builtin_amdgcn_perm(v.w, v.z, 0x05040100));
-            *reinterpret_cast<uint4*>(to + 32) = make_uint4(__builtin_amdgcn_perm(u.y, u.x, 0x07060302), __builtin_amdgcn_perm(u.w, u.z, 0x07060302),
-                                                            __builtin_amdgcn_perm(v.y, v.x, 0x07060302), __builtin_amdgcn_perm(v.w, v.z, 0x07060302));
+            for (int x = lane; x < 64 * (kWidth / 8); x += 64) {
+                const int r = x / (kWidth / 8), c = x % (kWidth / 8) * 8, ci = ci0 + strip * 64 + r, cj = cj0 + c;
+                const uint4* from = reinterpret_cast<const uint4*>(mine + r * kWidth + (c ^ turn(r)));
+                const uint4 u = from[0], v = from[1];
+                const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+                if (KIND == kLast) store_result(ci, cj, w);
+                else if (ci < t.n && cj < stride) store_halves(out + place(ci, cj, stride), w);
+            }
+        }
+        if (KIND == kLast ? !wide : !kSymmetric || ti != tj) {
+            f16* out = KIND == kGram ? t.a : (KIND == kFactor ? t.b : t.xt_next);
+#pragma unroll 4
+            for (int x = lane; x < 8 * kWidth; x += 64) {
+                const int r = x >> 3, c = (x & 7) * 8, cj = cj0 + r, ci = ci0 + strip * 64 + c;
+                const uint32_t *from0 = mine + c * kWidth + (r ^ turn(c)), *from1 = mine + (c + 4) * kWidth + (r ^ turn(c + 4));
+                const uint32_t w[8] = {from0[0], from0[kWidth], from0[2 * kWidth], from0[3 * kWidth], from1[0], from1[kWidth], from1[2 * kWidth], from1[3 * kWidth]};
+                if (KIND == kLast) store_result(cj, ci, w);
+                else if (cj < rows_q && ci < t.np) store_halves(out + place(cj, ci, t.np), w);
+            }
         }
         asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
