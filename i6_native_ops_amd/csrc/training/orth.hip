@@ -7,6 +7,7 @@
 // Operands are two 16-bit floating-point halves, x = x1 + x2, of 22 bits, times a power of two that brings the largest value they can have (X: 1.21, A: 1.46,
 // B: 3.45) below 2^16; of (x1 + x2)(y1 + y2) the last term is below the precision.  Half the bits would do for the products, but not for what becomes of them: an error in A is one of
 // left singular vectors of all sizes, and the small ones grow 3.4 times in each iteration, 485 times in five.
+#include <algorithm>
 #include <cmath>
 
 #include "lds_loads.h"
@@ -26,7 +27,8 @@ constexpr float kScaleX = 0x1p15f, kScaleA = 0x1p15f, kScaleB = 0x1p14f;
 constexpr int kMaxTensors = 40;          // x 96 bytes: the arguments of a kernel may have 4 KB
 constexpr int kThreads = 256;
 constexpr int kRowPad = 64;               // of columns: what the products run over
-constexpr double kLargeTiles = 1.6;      // a round of large tiles to one of small ones, measured
+constexpr int kCus = 256;
+constexpr double kSmallRound = 0.62;     // of tiles of 128 x 128, two a unit, to one of 256 x 256
 constexpr int kParts = 256;              // partial sums of squares of a matrix
 
 struct Matrix {
@@ -44,6 +46,7 @@ static_assert(sizeof(Matrix) <= 112, "kernel arguments");
 struct Table {
     Matrix t[kMaxTensors - 6];
     int count, groups;
+    int quarters;                        // of the tiles of 256 x 256 from this one on; -1: tiles of the kernel's own size
     float mu;
     int nesterov;
 };
@@ -379,23 +382,30 @@ template <typename T, int KIND, int S, int kHalves> __global__ __launch_bounds__
     // neighbours in the order of the tiles go to the same eighth of the card, which has a cache of its own
     const int per = ceil_div(tab.groups, 8), wg = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
     if (wg >= tab.groups) return;
-    const Matrix& t = find(tab, wg);
-    int tile = wg - t.first, ti = 0, tj = 0;
+    const bool quarter = S == 4 && tab.quarters >= 0;
+    const int number = quarter ? tab.quarters + wg / 4 : wg, side = quarter ? 256 : kTile;
+    const Matrix& t = find(tab, number);
+    int tile = number - t.first, ti = 0, tj = 0;
     if (KIND == kGram || KIND == kFactor) {
         while ((ti + 1) * (ti + 2) / 2 <= tile) ti++;
         tj = tile - ti * (ti + 1) / 2;
     } else {                             // four rows of tiles side by side
-        const int tiles_i = ceil_div(t.n, kTile), tiles_j = ceil_div(t.m, kTile), four_rows = tile / (4 * tiles_j), high = min(4, tiles_i - 4 * four_rows);
+        const int tiles_i = ceil_div(t.n, side), tiles_j = ceil_div(t.m, side), four_rows = tile / (4 * tiles_j), high = min(4, tiles_i - 4 * four_rows);
         tile -= four_rows * 4 * tiles_j;
         ti = 4 * four_rows + tile % high;
         tj = tile / high;
+    }
+    if (quarter) {
+        ti = 2 * ti + (wg >> 1 & 1);
+        tj = 2 * tj + (wg & 1);
+        if (KIND == kGram || KIND == kFactor ? tj > ti || ti * kTile >= t.n : ti * kTile >= t.n || tj * kTile >= t.m) return;
     }
     product_of<T, KIND, S, kHalves>(t, ti, tj, lds);
 }
 
 // Small matrices: a workgroup does all of it for one, X and A (then B) in LDS.  A wave has sixteen rows of X, or a part of their columns, in 32 bits in its registers.
 // All four products of the halves: short sums have little error of their own beside that of the last one, and matrix instructions are not what is waited for.
-// What bounds it are the waits of a chain of products that has 15 links: two matrices of 128 x 64 take %%SMALL%%.
+// What bounds it are the waits of a chain of products that has 15 links: two matrices of 128 x 64 take 40 us.
 constexpr int kSmallThreads = 512, kSmallBytes = 140 * 1024, kSmallTiles = 8;
 __host__ __device__ constexpr int small_parts(int n) { return n <= 16 ? 8 : (n <= 32 ? 4 : (n <= 64 ? 2 : 1)); }     // waves of sixteen rows
 __host__ __device__ constexpr int up32(int n) { return (n + 31) / 32 * 32; }
@@ -623,24 +633,37 @@ template <typename Groups, typename Launch> int over(Table& tab, Groups groups, 
 }
 
 // A product over all matrices.  Tiles of 256 x 256 keep the matrix units busier, one workgroup a unit; tiles of 128 x 128, two a unit, waste less of small matrices and of the
-// last round.
+// last round.  So there are whole rounds of large tiles, and the rest is large ones or their quarters; or all tiles are small.  A round of small tiles takes 0.62 of one of large
+// ones (2048 columns: 89 us and 146).
 template <typename T, int KIND, int kHalves> int multiply(Table& tab, hipStream_t s) {
     constexpr bool kSymmetric = KIND == kGram || KIND == kFactor;
     const auto tiles = [](const Matrix& t, int side) {
         const int64_t i = ceil_div(t.n, side);
         return kSymmetric ? i * (i + 1) / 2 : i * ceil_div(t.m, side);
     };
-    const auto in_all = [&](int side) {
-        int64_t all = 0;
-        for (int i = 0; i < tab.count; i++) all += tiles(tab.t[i], side);
-        return all;
+    int64_t large = 0, small = 0;
+    for (int i = 0; i < tab.count; i++) {
+        large += tiles(tab.t[i], 256);
+        small += tiles(tab.t[i], 128);
+    }
+    const auto small_rounds = [](int64_t n) { return kSmallRound * (double)ceil_div(n, (int64_t)(2 * kCus)); };
+    const int64_t rounds = large / kCus, rest = large - rounds * kCus;
+    const double with_quarters = (double)rounds + small_rounds(rest * 4), all_large = (double)ceil_div(large, (int64_t)kCus);
+    const auto launch_large = [&](int64_t n) {
+        tab.groups = (int)n;
+        tab.quarters = -1;
+        orth_product<T, KIND, 8, kHalves><<<dim3((unsigned)(ceil_div(n, (int64_t)8) * 8)), dim3(kThreads), 0, s>>>(tab);
     };
-    const bool large = kLargeTiles * (double)ceil_div(in_all(256), (int64_t)256) <= (double)ceil_div(in_all(128), (int64_t)512);
-    return over(tab, [&](const Matrix& t) { return tiles(t, large ? 256 : 128); }, [&](dim3 g) {
-        tab.groups = (int)g.x;
-        const dim3 grid(ceil_div(g.x, 8u) * 8);
-        if (large) orth_product<T, KIND, 8, kHalves><<<grid, dim3(kThreads), 0, s>>>(tab);
-        else orth_product<T, KIND, 4, kHalves><<<grid, dim3(kThreads), 0, s>>>(tab);
+    const auto launch_small = [&](int64_t n, int64_t quarters) {
+        tab.groups = (int)n;
+        tab.quarters = (int)quarters;
+        orth_product<T, KIND, 4, kHalves><<<dim3((unsigned)(ceil_div(n, (int64_t)8) * 8)), dim3(kThreads), 0, s>>>(tab);
+    };
+    if (small_rounds(small) < std::min(with_quarters, all_large)) return over(tab, [&](const Matrix& t) { return tiles(t, 128); }, [&](dim3 g) { launch_small(g.x, -1); });
+    return over(tab, [&](const Matrix& t) { return tiles(t, 256); }, [&](dim3) {
+        if (all_large <= with_quarters) return launch_large(large);
+        if (rounds) launch_large(rounds * kCus);
+        launch_small(rest * 4, rounds * kCus);
     });
 }
 
@@ -657,8 +680,8 @@ template <typename T> int run(Table& tab, bool small, int iterations, hipStream_
     for (int i = 0; i < iterations; i++) {
         I6TRAIN_TRY((multiply<T, kGram, 2>(tab, s)));
         I6TRAIN_TRY((multiply<T, kFactor, 2>(tab, s)));
-        // 16-bit results: nothing follows in which an error of the last product grows.  Half the bits, 2^-12 of B's and X's values, add 0.1 to what the rounding of the result
-        // is off by (relative 2-norm 1.66e-3 -> 1.85e-3) and make it 1.5 times as fast.
+        // 16-bit results: nothing follows in which an error of the last product grows.  Half the bits of B's and X's values change what the result is off by from 1.66e-3 (its
+        // rounding alone) to 1.69e-3, relative 2-norm, and the product takes 1.16 ms instead of 1.98 (24 matrices of 4096 x 2048).
         if (i + 1 < iterations) I6TRAIN_TRY((multiply<T, kUpdate, 2>(tab, s)));
         else I6TRAIN_TRY((multiply<T, kLast, sizeof(T) == 2 ? 1 : 2>(tab, s)));
         for (int j = 0; j < tab.count; j++) {
