@@ -661,7 +661,7 @@ int checked(const i6delta_problem* p) {
     if (!p || p->B <= 0 || p->T <= 0 || p->H <= 0 || p->G <= 0 || p->K <= 0 || p->V <= 0 || p->H % p->G || !valid_dtype(p->dtype) || !p->q || !p->k || !p->v || !p->gate ||
         !p->beta)
         return I6TRAIN_ERR_INVALID_ARGUMENT;
-    if (p->B > 65535 || p->H > 65535 || p->K > 128 || p->V > 128 || p->T > (1 << 30) || (int64_t)p->B * p->H * ceil_div(p->T, kC) >= (1 << 24)) return I6TRAIN_ERR_TOO_LARGE;
+    if (p->B > 65535 || p->H > 65535 || p->K > 128 || p->V > 128 || p->T > (1 << 28) || (int64_t)p->B * p->H * ceil_div(p->T, kC) > (1 << 23)) return I6TRAIN_ERR_TOO_LARGE;
     return I6TRAIN_OK;
 }
 

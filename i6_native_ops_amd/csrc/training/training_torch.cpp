@@ -1,6 +1,7 @@
 // PyTorch-ROCm binding of libi6train.so: module `training_core`.  torch is used for device memory, the current
 // stream and the autograd graph; all arithmetic is behind the C ABI declared in include/i6train.h.  The graph's nodes
 // are C++: the smallest training steps take as long as their host work, of which nodes in Python would be the larger part.
+#include <algorithm>
 #include <optional>
 #include <string>
 #include <tuple>

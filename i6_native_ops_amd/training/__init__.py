@@ -254,7 +254,7 @@ def muon_step(
 
     :param params: contiguous matrices, all float32 or all bfloat16
     :param grads: of the same types and sizes
-    :param momenta: averages of the gradients, float32, of the same sizes
+    :param momenta: averages of the gradients, float32, of the same sizes.  Params, grads and momenta have memory of their own
     :param adjust_lr: the rate is multiplied by sqrt(max(1, rows / columns)) ("original") or by 0.2 sqrt(max(rows, columns)) ("match_rms_adamw")
     """
     rates = [_rate(lr, p.shape, adjust_lr) if p.dim() == 2 else lr for p in params]

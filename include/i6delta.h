@@ -13,8 +13,8 @@
  *   q, k [B, T, G, K], v [B, T, H, V], gate, beta [B, T, H], all of `dtype`, with strides (q, k, v: the last one is 1); H is a multiple
  *   of G, and head h has keys and queries h / (H / G).  initial, last float [B, H, K, V] contiguous;  o [B, T, H, V] contiguous, of `dtype`.
  *
- * States, sums and decays are held in 32 bits.  Sizes: B and H up to 65 535, K and V up to 128, T up to 2^30, B H ceil(T / 32) below 2^24;
- * larger ones are I6TRAIN_ERR_TOO_LARGE.
+ * States, sums and decays are held in 32 bits.  Sizes: B and H up to 65 535, K and V up to 128, B H ceil(T / 32) up to 2^23; larger ones
+ * are I6TRAIN_ERR_TOO_LARGE.
  *
  * A forward call for training leaves in `kept` what i6delta_backward needs (null otherwise).  Gradients: grad_o (strided, last stride 1, `dtype`)
  * and grad_last (float, contiguous) may be null; grad_q, grad_k [B, T, G, K], grad_v [B, T, H, V], grad_gate and grad_beta [B, T, H] of `dtype`
@@ -41,7 +41,8 @@ typedef struct {
     const float* initial;
 } i6delta_problem;
 
-/* Bytes of `kept` and of the workspaces of a forward call, with `train` or without, and of a backward call; each may be 0. */
+/* Bytes of `kept` and of the workspaces of a forward call, with `train` or without, and of a backward call; each may be 0.  They are those of calls with this very problem: with
+ * other places and strides of q, k and v they may be others. */
 int i6delta_sizes(const i6delta_problem* p, int train, size_t* kept_bytes, size_t* forward_bytes, size_t* backward_bytes);
 int i6delta_forward(const i6delta_problem* p, void* o, float* last, void* kept, size_t kept_bytes, void* workspace, size_t workspace_bytes,
                     void* stream);

@@ -72,8 +72,9 @@ def test_delta_refusals(lib):
     assert delta_sizes(lib, None)[0] == INVALID
     for bad in (dict(B=0), dict(T=0), dict(H=0), dict(G=3), dict(K=0), dict(V=0), dict(dtype=7), dict(q=None), dict(beta=None)):
         assert delta_sizes(lib, delta(**bad))[0] == INVALID, bad
-    for bad in (dict(B=65536), dict(K=129), dict(V=129), dict(H=65536, G=1), dict(T=(1 << 30) + 1), dict(B=65535, H=65535, G=1, T=1), dict(B=1, T=1 << 30, H=2)):
+    for bad in (dict(B=65536), dict(K=129), dict(V=129), dict(H=65536, G=1), dict(T=(1 << 28) + 1), dict(B=1, T=(1 << 28), H=2), dict(B=1, H=1, G=1, T=(1 << 28) + 1), dict(B=65535, H=65535, G=1, T=1), dict(B=1, T=1 << 30, H=2)):
         assert delta_sizes(lib, delta(**bad))[0] == TOO_LARGE, bad
+    assert delta_sizes(lib, delta(B=1, H=1, G=1, T=1 << 28))[0] == 0
     rc, (kept, forward, backward) = delta_sizes(lib, delta())
     assert rc == 0 and kept > 0 and backward > 0
     assert delta_sizes(lib, delta(), 0)[1][0] == 0
