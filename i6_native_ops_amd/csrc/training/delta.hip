@@ -691,9 +691,9 @@ int padded_keys(int K) { return K <= 32 ? 32 : (K <= 64 ? 64 : 128); }
 
 // Where the parts of a call's memory are.
 struct Places {
-    size_t rows, states, states_factor, u, u_factor, kept;           // kept; rows are in the forward workspace where nothing is
-    size_t blocks, packed, forward;                                  // the forward workspace
-    size_t ends, ends_factor, dr, dr_factor, d_q, d_k, back_blocks, back_packed, back;      // the backward workspace
+    size_t rows, states, states_factor, u, u_factor, blocks, kept;   // kept; rows and blocks are in the forward workspace where nothing is
+    size_t packed, forward;                                          // the forward workspace
+    size_t ends, ends_factor, dr, dr_factor, d_q, d_k, back_packed, back;       // the backward workspace
     size_t split, turns;                                             // of the forward workspace, and turns behind split
     size_t back_split;
     int pairs, segments = 1, per;
@@ -710,7 +710,9 @@ struct Places {
         states_factor = states + s;
         u = states_factor + f;
         u_factor = u + r;
-        kept = u_factor + f;
+        const size_t block_bytes = align256(x16 ? n * chunk_blocks(train) * sizeof(bf16) : n * kBlocks32 * 256 * sizeof(float));
+        blocks = train ? u_factor + f : states;
+        kept = blocks + block_bytes;
         ends = 0;
         ends_factor = s;
         dr = ends_factor + f;
@@ -721,8 +723,7 @@ struct Places {
         const size_t k = packed_bytes(p, p.G, p.K), v = packed_bytes(p, p.H, p.V);
         const size_t copy_k = whole_rows(p.k, p.k_stride_b, p.k_stride_t, p.k_stride_g, p.K) ? 0 : k, copy_q = whole_rows(p.q, p.q_stride_b, p.q_stride_t, p.q_stride_g, p.K) ? 0 : k;
         const size_t copy_v = whole_rows(p.v, p.v_stride_b, p.v_stride_t, p.v_stride_h, p.V) ? 0 : v;
-        back_blocks = d_k + heads;
-        back_packed = back_blocks + align256(x16 ? n * kChunkBlocks<true> * sizeof(bf16) : n * kBlocks32 * 256 * sizeof(float));
+        back_packed = d_k + heads;
         back_split = back_packed + (x16 ? copy_k + copy_q + v : 0);
         // Segments: as many as fill the card, and no more than pay for going along them one after the other; below three the second pass costs what the first one saves, and
         // a short sequence does not pay for the launches.  Without and with them, heads of 64 (128): 8 of 2048 frames 142 -> 54 us (225 -> 87), of 512 45 -> 37 (66 -> 52),
@@ -743,8 +744,7 @@ struct Places {
         back = back_split + split_bytes;
         // frame by frame nothing is needed
         const bool chunked = train || p.T > kMostFrames;
-        blocks = chunked && !train ? states : 0;
-        packed = chunked ? blocks + align256(x16 ? n * kChunkBlocks<false> * sizeof(bf16) : n * kBlocks32 * 256 * sizeof(float)) : 0;
+        packed = chunked && !train ? kept : 0;
         split = chunked ? packed + (x16 ? copy_k + copy_q + copy_v : 0) : 0;
         forward = chunked ? split + split_bytes : 0;
     }
@@ -763,7 +763,7 @@ bool wide(const Call& c) { return c.a.V > 64 && (int64_t)c.a.B * c.a.H * c.k16.s
 template <int KP> void run_forward(const Call& c, hipStream_t s, float) {
     const Args16& k = c.k16;
     float* blocks = reinterpret_cast<float*>(c.blocks);
-    delta_prepare32<KP, false><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, blocks, c.whole);
+    delta_prepare32<KP><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, blocks, c.whole);
     const int groups = ceil_div(32 * k.pairs + KP, 128);
     if (k.segments > 1) {
         delta_forward32<KP, 8, true><<<dim3(c.a.H * groups, c.a.B, k.segments - 1), dim3(512), 0, s>>>(c.a, k, blocks, c.whole, c.whole_v);
@@ -773,20 +773,20 @@ template <int KP> void run_forward(const Call& c, hipStream_t s, float) {
     else delta_forward32<KP, 4, false><<<dim3(c.a.H * ceil_div(c.a.V, 64), c.a.B, k.segments), dim3(256), 0, s>>>(c.a, k, blocks, c.whole, c.whole_v);
 }
 template <int KP> void run_forward(const Call& c, hipStream_t s, bf16) {
-    delta_prepare16<KP, false><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.blocks);
+    delta_prepare16<KP><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.blocks, c.train);
+    const int stride = chunk_blocks(c.train);
     const Args16& k = c.k16;
     const int groups = ceil_div(32 * k.pairs + KP, 128);
     if (k.segments > 1) {
-        delta_forward16<KP, 8, true><<<dim3(c.a.H * groups, c.a.B, k.segments - 1), dim3(512), 0, s>>>(c.a, k, c.blocks);
+        delta_forward16<KP, 8, true><<<dim3(c.a.H * groups, c.a.B, k.segments - 1), dim3(512), 0, s>>>(c.a, k, c.blocks, stride);
         delta_join16<KP, kC16><<<dim3(ceil_div(c.a.V, 16), c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, k, false);
     }
-    if (wide(c)) delta_forward16<KP, 8, false><<<dim3(c.a.H, c.a.B, k.segments), dim3(512), 0, s>>>(c.a, k, c.blocks);
-    else delta_forward16<KP, 4, false><<<dim3(c.a.H * ceil_div(c.a.V, 64), c.a.B, k.segments), dim3(256), 0, s>>>(c.a, k, c.blocks);
+    if (wide(c)) delta_forward16<KP, 8, false><<<dim3(c.a.H, c.a.B, k.segments), dim3(512), 0, s>>>(c.a, k, c.blocks, stride);
+    else delta_forward16<KP, 4, false><<<dim3(c.a.H * ceil_div(c.a.V, 64), c.a.B, k.segments), dim3(256), 0, s>>>(c.a, k, c.blocks, stride);
 }
 template <int KP> void run_backward(const Call& c, hipStream_t s, float) {
     const Args16& k = c.k16;
     float* blocks = reinterpret_cast<float*>(c.blocks);
-    delta_prepare32<KP, true><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, blocks, c.whole);
     const int groups = ceil_div(32 * k.pairs + KP, 128);
     if (k.segments > 1) {
         delta_backward32<KP, 8, true><<<dim3(c.a.H * groups, c.a.B, k.segments - 1), dim3(512), 0, s>>>(c.a, k, blocks, c.whole, c.whole_v);
@@ -797,7 +797,6 @@ template <int KP> void run_backward(const Call& c, hipStream_t s, float) {
     delta_gradients<float, KP><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a);
 }
 template <int KP> void run_backward(const Call& c, hipStream_t s, bf16) {
-    delta_prepare16<KP, true><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.blocks);
     const Args16& k = c.k16;
     const int groups = ceil_div(32 * k.pairs + KP, 128);
     if (k.segments > 1) {
@@ -869,6 +868,7 @@ Call call_of(const i6delta_problem& p, const Places& at, void* kept) {
     if (kept) {
         char* base = static_cast<char*>(kept);
         c.a.rows = reinterpret_cast<Rows*>(base + at.rows);
+        c.blocks = reinterpret_cast<bf16*>(base + at.blocks);
         c.a.states = reinterpret_cast<float*>(base + at.states);
         c.a.u = reinterpret_cast<float*>(base + at.u);
         c.k16.states = {reinterpret_cast<f16*>(base + at.states), reinterpret_cast<float*>(base + at.states_factor)};
@@ -902,8 +902,10 @@ int i6delta_forward(const i6delta_problem* p, void* o, float* last, void* kept, 
     Call c = call_of(*p, at, kept);
     c.a.o = o; c.a.last = last;
     if (at.forward) {
-        c.blocks = reinterpret_cast<bf16*>(static_cast<char*>(workspace) + at.blocks);
-        if (!kept) c.a.rows = static_cast<Rows*>(workspace);
+        if (!kept) {
+            c.a.rows = static_cast<Rows*>(workspace);
+            c.blocks = reinterpret_cast<bf16*>(static_cast<char*>(workspace) + at.blocks);
+        }
         c.k16.ends = reinterpret_cast<float*>(static_cast<char*>(workspace) + at.split);
         c.k16.turns = reinterpret_cast<float*>(static_cast<char*>(workspace) + at.split + at.turns);
         if (p->dtype == I6TRAIN_BF16) {
@@ -935,7 +937,6 @@ int i6delta_backward(const i6delta_problem* p, const void* grad_o, int64_t grad_
     a.dr = reinterpret_cast<float*>(base + at.dr);
     c.k16.left = {reinterpret_cast<f16*>(base + at.ends), reinterpret_cast<float*>(base + at.ends_factor)};
     c.k16.dr = {reinterpret_cast<f16*>(base + at.dr), reinterpret_cast<float*>(base + at.dr_factor)};
-    c.blocks = reinterpret_cast<bf16*>(base + at.back_blocks);
     c.k16.ends = reinterpret_cast<float*>(base + at.back_split);
     c.k16.turns = reinterpret_cast<float*>(base + at.back_split + at.turns);
     if (p->dtype == I6TRAIN_BF16) {
