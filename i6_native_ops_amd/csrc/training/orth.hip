@@ -7,6 +7,9 @@
 // Operands are two 16-bit floating-point halves, x = x1 + x2, of 22 bits, times a power of two that brings the largest value they can have (X: 1.21, A: 1.46,
 // B: 3.45) below 2^16; of (x1 + x2)(y1 + y2) the last term is below the precision.  Half the bits would do for the products, but not for what becomes of them: an error in A is one of
 // left singular vectors of all sizes, and the small ones grow 3.4 times in each iteration, 485 times in five.
+//
+// 24 matrices of 4096 x 2048 in 16 bits: 19.2 ms, of which 0.45 norms and operands, 4 x 1.98 + 1.16 X = B X, 5 x 1.08 A, 5 x 0.66 B: 20 PFLOP of 16-bit products at 1050 TFLOP/s, where a
+// library's product of this kind reaches 1390; both are bound by the matrix units and the clock that the card holds under them.  What is between is each tile's way in and out.
 #include <algorithm>
 #include <cmath>
 
