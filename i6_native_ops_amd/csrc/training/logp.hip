@@ -10,8 +10,9 @@
 // kCandidates scores reach the bound (masked, equal or ordered scores), the k-th largest score itself is found bit by bit, and then the index up to
 // which scores equal to it count: what is left are k candidates.
 //
-// 28 900 frames of 12 001 classes in 32 bits: 245 us, 5.7 TB/s; training on 44 800 frames of 5001 in 16 bits: 193 us forward (2.3 TB/s: 13 instructions and an exponential a score
-// issue for half of it) and 180 backward (5.3 TB/s with what is written); the next frame of 64 streams: 15 us, most of which two barriers, reductions and a row's first bytes take.
+// 28 900 frames of 12 001 classes in 32 bits: 250 us, 5.5 TB/s, and all of the time vector instructions are issued, too.  Training on 44 800 frames of 5001 in 16 bits: 150 us
+// forward (3 TB/s; ten instructions and an exponential a score) and 198 backward (4.8 TB/s with what is written).  The next frame of 64 streams: 15 us, most of which two barriers,
+// the reductions and a row's first bytes take.
 #include "train_common.h"
 #include "../../../include/i6logp.h"
 
