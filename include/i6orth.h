@@ -5,7 +5,8 @@
  * X = u / max(|u|, 1e-7), |u| the root of the sum of squares; `iterations` times
  *   A = X X^T,   X = 3.4445 X + (-4.7750 A + 2.0315 A A) X
  * (u transposed where it has more rows than columns, and the result back).  Singular values of X end near one.
- * X, A and the factors are held in 22 bits relative to the largest value they can have (2^-39 at least), sums in 32.
+ * X, A and the factors are held in 22 bits relative to the largest value they can have (2^-39 at least), sums in 32.  For 16-bit results the
+ * last product takes 11 bits of its operands.
  *
  * Where `momentum` is given, u comes from the gradient g and is applied to the parameter p:
  *   m = mu m + (1 - mu) g,   u = nesterov ? mu m + (1 - mu) g : m,   p = p keep - rate X

@@ -270,9 +270,10 @@ def test_single_incoming_gradients_and_repeats(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_captured_calls(dtype):
-    """Forward and backward replayed with new inputs, eager calls in between; two graphs in turn."""
-    p = problem(2, 70, 4, 2, 64, 64, dtype, lens=[70, 41])
+@pytest.mark.parametrize("T,lens", [(70, [70, 41]), (1100, [1100, 700])])
+def test_captured_calls(T, lens, dtype):
+    """Forward and backward replayed with new inputs, eager calls in between; two graphs in turn.  In one piece, and in segments."""
+    p = problem(2, T, 4, 2, 64, 64, dtype, lens=lens)
     leaves = [p[n].detach().clone().requires_grad_() for n in NAMES]
     from i6_native_ops_amd.training import gated_delta_rule
 
@@ -291,7 +292,7 @@ def test_captured_calls(dtype):
         with torch.cuda.graph(graphs[-1]):
             outs.append(step())
     for seed in range(3):
-        new = problem(2, 70, 4, 2, 64, 64, dtype, seed=20 + seed, lens=[70, 41])
+        new = problem(2, T, 4, 2, 64, 64, dtype, seed=20 + seed, lens=lens)
         with torch.no_grad():
             for leaf, n in zip(leaves, NAMES):
                 leaf.copy_(new[n])
@@ -303,8 +304,9 @@ def test_captured_calls(dtype):
                 assert torch.equal(x, want[n]), (seed, n)
 
 
-def test_on_another_stream():
-    p = problem(2, 100, 2, 2, 64, 64, torch.bfloat16)
+@pytest.mark.parametrize("T", [100, 900])
+def test_on_another_stream(T):
+    p = problem(2, T, 2, 2, 64, 64, torch.bfloat16)
     want = run(p)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -313,6 +315,22 @@ def test_on_another_stream():
     side.synchronize()
     for n in want:
         assert torch.equal(got[n], want[n]), n
+
+
+def test_two_calls_at_once():
+    """Calls in flight on two streams have workspaces of their own."""
+    p, q = problem(1, 2000, 2, 2, 64, 64, torch.bfloat16, seed=5, lens="all"), problem(3, 700, 4, 4, 128, 128, torch.float32, seed=6, lens="all")
+    want = run(p), run(q)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(a):
+            x = run(p)
+        with torch.cuda.stream(b):
+            y = run(q)
+        torch.cuda.synchronize()
+        for got, right in zip((x, y), want):
+            assert all(torch.equal(got[n], right[n]) for n in right)
 
 
 def test_second_derivatives_and_tangents_are_refused():
