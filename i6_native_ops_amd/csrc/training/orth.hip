@@ -32,6 +32,7 @@ constexpr int kThreads = 256;
 constexpr int kRowPad = 64;               // of columns: what the products run over
 constexpr int kCus = 256;
 constexpr double kSmallRound = 0.62;     // of tiles of 128 x 128, two a unit, to one of 256 x 256
+constexpr int kPartSteps = 16;
 constexpr int kParts = 256;              // partial sums of squares of a matrix
 
 struct Matrix {
@@ -50,6 +51,8 @@ struct Table {
     Matrix t[kMaxTensors - 6];
     int count, groups;
     int quarters;                        // of the tiles of 256 x 256 from this one on; -1: tiles of the kernel's own size
+    int parts;                           // of the columns that a product runs over, where tiles are few
+    acc_t* partial;                      // [tiles][parts][a tile's accumulators]
     float mu;
     int nesterov;
 };
@@ -197,6 +200,11 @@ template <typename T> __global__ __launch_bounds__(kThreads) void orth_operands(
 
 enum Kind { kGram, kFactor, kUpdate, kLast };
 
+// Few tiles of long products: parts of the columns by workgroups of their own, kPart, whose sums kJoin adds up in their order.
+enum Mode { kWhole, kPart, kJoin };
+// Halves of the operands that a product takes: the first ones alone; both, without the product of the second ones; all four products.
+constexpr int kOne = 1, kThree = 2, kFour = 3;
+
 // The packed halves of a value, and four of them side by side.
 __device__ __forceinline__ uint32_t packed(float v) {
     f16 hi, lo;
@@ -207,10 +215,10 @@ __device__ __forceinline__ uint32_t packed(float v) {
 // C[i][j] = sum_k P[i][k] Q[j][k]: P = Q = X, P = Q = A, and P = B, Q = X^T.  Tiles of 32 S x 32 S, four waves with 16 S x 16 S each.  A stage has of every row 128 bytes:
 // 32 k, first and second halves (kHalves = 2), or the first halves of 64 k.  In LDS a row's eight pieces of 16 bytes are turned by the row, so that eight lanes that read
 // eight rows' pieces reach all banks; the loads, which write LDS in order, take them from the turned places.
-template <typename T, int KIND, int S, int kHalves> __device__ __forceinline__ void product_of(const Matrix& t, int ti, int tj, char* lds) {
+template <typename T, int KIND, int S, int kHalves, Mode MODE> __device__ __forceinline__ void product_of(const Matrix& t, int ti, int tj, char* lds, int parts, int part, acc_t* partial) {
     constexpr int kTile = 32 * S, kSide = kTile * 128, kStage = 2 * kSide, kLoads = S;       // per wave, stage and operand
     constexpr bool kSymmetric = KIND == kGram || KIND == kFactor;
-    constexpr int kStep = kHalves == 2 ? 32 : 64;
+    constexpr int kStep = kHalves == kOne ? 64 : 32;
     const f16* p = KIND == kGram ? t.x : (KIND == kFactor ? t.a : t.b);
     const f16* q = KIND == kGram ? t.x : (KIND == kFactor ? t.a : t.xt);
     const int rows_q = kSymmetric ? t.n : t.m, k_all = KIND == kGram ? t.mp : t.np;
@@ -223,25 +231,27 @@ template <typename T, int KIND, int S, int kHalves> __device__ __forceinline__ v
     uint32_t from;                       // of the lane's piece: 8 rows a load
     {
         const int row = wave * kLoads * 8 + (lane >> 3), piece = (lane & 7) ^ (lane >> 3);
-        from = (uint32_t)(row * row_bytes) + (kHalves == 2 ? piece * 16 : (piece >> 2) * 128 + (piece & 3) * 16);
+        from = (uint32_t)(row * row_bytes) + (kHalves == kOne ? (piece >> 2) * 128 + (piece & 3) * 16 : piece * 16);
     }
     const uint32_t lds0 = lds_address(lds) + wave * kLoads * 1024, eight_rows = (uint32_t)(8 * row_bytes);
     const auto fetch = [&](int i, int stage, uint32_t offset) {
         const uint32_t to = lds0 + stage * kStage + (i & 1) * kSide + (i >> 1) * 1024;
         load_to_lds(i & 1 ? from_q : from_p, to, from + (i >> 1) * eight_rows, offset);
     };
-    constexpr uint32_t kStepBytes = kHalves == 2 ? 128 : 256;
+    constexpr uint32_t kStepBytes = kHalves == kOne ? 256 : 128;
     acc_t acc[S][S];
 #pragma unroll
     for (int i = 0; i < S; i++)
 #pragma unroll
         for (int j = 0; j < S; j++) acc[i][j] = 0.f;
+    const int steps = k_all / kStep, per = MODE == kPart ? ceil_div(steps, parts) : steps, begin = MODE == kPart ? min(part * per, steps) : 0, end = min(begin + per, steps);
+    if (MODE != kJoin && begin < end) {
 #pragma unroll
-    for (int i = 0; i < 2 * kLoads; i++) fetch(i, 0, 0);
-    const int steps = k_all / kStep;
+        for (int i = 0; i < 2 * kLoads; i++) fetch(i, 0, (uint32_t)begin * kStepBytes);
+    }
     // fragments: the lane's row, and pieces 0 .. 3 and 4 .. 7
     const uint32_t read0 = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) * 16), read1 = read0 ^ 64;
-    for (int k = 0; k < steps; k++) {
+    for (int k = 0; MODE != kJoin && k < end - begin; k++) {
         wait_and_meet<0>();
         const char* sp = lds + (k & 1) * kStage + wi * (16 * S * 128);
         const char* sq = lds + (k & 1) * kStage + kSide + wj * (16 * S * 128);
@@ -253,8 +263,8 @@ template <typename T, int KIND, int S, int kHalves> __device__ __forceinline__ v
         }
         fp[0][0] = *reinterpret_cast<const f16x8*>(sp + read0);
         fp[0][1] = *reinterpret_cast<const f16x8*>(sp + read1);
-        const uint32_t offset = (uint32_t)(k + 1) * kStepBytes;
-        const bool more = k + 1 < steps;
+        const uint32_t offset = (uint32_t)(begin + k + 1) * kStepBytes;
+        const bool more = k + 1 < end - begin;
 #pragma unroll
         for (int i = 0; i < S; i++) {
             if (i + 1 < S) {
@@ -267,7 +277,11 @@ template <typename T, int KIND, int S, int kHalves> __device__ __forceinline__ v
             }
             const f16x8 p0 = fp[i & 1][0], p1 = fp[i & 1][1];
 #if __HIP_DEVICE_COMPILE__
-            if (kHalves == 2) {
+            if (kHalves != kOne) {
+                if (kHalves == kFour) {
+#pragma unroll
+                    for (int j = 0; j < S; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p1, fq[1][j], acc[i][j], 0, 0, 0);
+                }
 #pragma unroll
                 for (int j = 0; j < S; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p0, fq[1][j], acc[i][j], 0, 0, 0);
 #pragma unroll
@@ -280,6 +294,21 @@ template <typename T, int KIND, int S, int kHalves> __device__ __forceinline__ v
             for (int j = 0; j < S; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p0, fq[0][j], acc[i][j], 0, 0, 0);
 #endif
         }
+    }
+    if (MODE != kWhole) {
+        constexpr int kTileSums = 4 * S * S * 64;
+        acc_t* mine = partial + (MODE == kPart ? (int64_t)part * kTileSums : 0) + wave * S * S * 64 + lane;
+#pragma unroll 2
+        for (int x = 0; x < (MODE == kPart ? 1 : parts); x++)
+#pragma unroll
+            for (int i = 0; i < S; i++)
+#pragma unroll
+                for (int j = 0; j < S; j++) {
+                    acc_t* at = mine + (int64_t)x * kTileSums + (i * S + j) * 64;
+                    if (MODE == kPart) *at = acc[i][j];
+                    else acc[i][j] += *at;
+                }
+        if (MODE == kPart) return;
     }
     // What becomes of a tile: 64 of a wave's rows at a time go through LDS, from where lanes take eight values side by side, of rows and of columns.  A row's words are turned by
     // its number, so that neither way two lanes meet in a bank.
@@ -379,14 +408,14 @@ template <typename T, int KIND, int S, int kHalves> __device__ __forceinline__ v
 }
 
 constexpr int stages_bytes(int S) { return 2 * 2 * 32 * S * 128; }
-template <typename T, int KIND, int S, int kHalves> __global__ __launch_bounds__(kThreads, S == 8 ? 1 : 2) void orth_product(Table tab) {
+template <typename T, int KIND, int S, int kHalves, Mode MODE> __global__ __launch_bounds__(kThreads, S == 8 ? 1 : 2) void orth_product(Table tab) {
     constexpr int kTile = 32 * S;
     __shared__ __align__(128) char lds[stages_bytes(S)];
     // neighbours in the order of the tiles go to the same eighth of the card, which has a cache of its own
     const int per = ceil_div(tab.groups, 8), wg = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
     if (wg >= tab.groups) return;
-    const bool quarter = S == 4 && tab.quarters >= 0;
-    const int number = quarter ? tab.quarters + wg / 4 : wg, side = quarter ? 256 : kTile;
+    const bool quarter = S == 4 && MODE == kWhole && tab.quarters >= 0;
+    const int number = quarter ? tab.quarters + wg / 4 : (MODE == kPart ? wg / tab.parts : wg), side = quarter ? 256 : kTile;
     const Matrix& t = find(tab, number);
     int tile = number - t.first, ti = 0, tj = 0;
     if (KIND == kGram || KIND == kFactor) {
@@ -403,7 +432,7 @@ template <typename T, int KIND, int S, int kHalves> __global__ __launch_bounds__
         tj = 2 * tj + (wg & 1);
         if (KIND == kGram || KIND == kFactor ? tj > ti || ti * kTile >= t.n : ti * kTile >= t.n || tj * kTile >= t.m) return;
     }
-    product_of<T, KIND, S, kHalves>(t, ti, tj, lds);
+    product_of<T, KIND, S, kHalves, MODE>(t, ti, tj, lds, tab.parts, MODE == kPart ? wg % tab.parts : 0, tab.partial + (int64_t)number * tab.parts * (4 * S * S * 64));
 }
 
 // Small matrices: a workgroup does all of it for one, X and A (then B) in LDS.  A wave has sixteen rows of X, or a part of their columns, in 32 bits in its registers.
@@ -635,6 +664,29 @@ template <typename Groups, typename Launch> int over(Table& tab, Groups groups, 
     return launched();
 }
 
+// Tiles that do not fill the card: how many parts of its columns a product is formed in.  A step takes 0.8 us, a part's sums are read in half of that, another launch takes 7: so no
+// parts below 16 steps of 32 columns, four steps at least in each, and about the root of their number of them.  Without and with, in 32 bits: one matrix of 200 x 4096 656 -> 310 us,
+// of 1024 x 1024 497 -> 405, 8 of 60 x 2000 332 -> 225.  Sums in parts are also nearer: with all four products 3.0e-6 -> 1.4e-6 off 64 bits in the last of these.
+struct Parts {
+    bool few;
+    int parts;
+    size_t bytes;
+};
+Parts parts_of(const Table& tab, bool gram, bool symmetric) {
+    int64_t tiles = 0;
+    int steps = 0;
+    for (int i = 0; i < tab.count; i++) {
+        const Matrix& t = tab.t[i];
+        const int64_t r = ceil_div(t.n, 128);
+        tiles += symmetric ? r * (r + 1) / 2 : r * ceil_div(t.m, 128);
+        steps = std::max(steps, (gram ? t.mp : t.np) / 32);
+    }
+    Parts p{tiles > 0 && tiles <= kCus, 1, 0};
+    if (p.few && steps >= kPartSteps) p.parts = (int)std::max<int64_t>(1, std::min<int64_t>({2 * kCus / tiles, steps / 4, (int64_t)sqrt(1.6 * steps)}));
+    if (p.parts > 1) p.bytes = (size_t)tiles * p.parts * 128 * 128 * sizeof(float);
+    return p;
+}
+
 // A product over all matrices.  Tiles of 256 x 256 keep the matrix units busier, one workgroup a unit; tiles of 128 x 128, two a unit, waste less of small matrices and of the
 // last round.  So there are whole rounds of large tiles, and the rest is large ones or their quarters; or all tiles are small.  A round of small tiles takes 0.62 of one of large
 // ones (2048 columns: 89 us and 146).
@@ -644,6 +696,22 @@ template <typename T, int KIND, int kHalves> int multiply(Table& tab, hipStream_
         const int64_t i = ceil_div(t.n, side);
         return kSymmetric ? i * (i + 1) / 2 : i * ceil_div(t.m, side);
     };
+    const Parts split = parts_of(tab, KIND == kGram, kSymmetric);
+    if (split.few) {                     // all four products: matrix instructions are not what is waited for, and short sums have little error beside that of the last one
+        constexpr int kAll = kHalves == kOne ? kOne : kFour;
+        tab.quarters = -1;
+        tab.parts = split.parts;
+        return over(tab, [&](const Matrix& t) { return tiles(t, 128); }, [&](dim3 g) {
+            const auto grid = [](unsigned n) { return dim3(ceil_div(n, 8u) * 8); };
+            if (split.parts > 1) {
+                tab.groups = (int)g.x * split.parts;
+                orth_product<T, KIND, 4, kAll, kPart><<<grid(tab.groups), dim3(kThreads), 0, s>>>(tab);
+            }
+            tab.groups = (int)g.x;
+            if (split.parts > 1) orth_product<T, KIND, 4, kAll, kJoin><<<grid(g.x), dim3(kThreads), 0, s>>>(tab);
+            else orth_product<T, KIND, 4, kAll, kWhole><<<grid(g.x), dim3(kThreads), 0, s>>>(tab);
+        });
+    }
     int64_t large = 0, small = 0;
     for (int i = 0; i < tab.count; i++) {
         large += tiles(tab.t[i], 256);
@@ -655,12 +723,12 @@ template <typename T, int KIND, int kHalves> int multiply(Table& tab, hipStream_
     const auto launch_large = [&](int64_t n) {
         tab.groups = (int)n;
         tab.quarters = -1;
-        orth_product<T, KIND, 8, kHalves><<<dim3((unsigned)(ceil_div(n, (int64_t)8) * 8)), dim3(kThreads), 0, s>>>(tab);
+        orth_product<T, KIND, 8, kHalves, kWhole><<<dim3((unsigned)(ceil_div(n, (int64_t)8) * 8)), dim3(kThreads), 0, s>>>(tab);
     };
     const auto launch_small = [&](int64_t n, int64_t quarters) {
         tab.groups = (int)n;
         tab.quarters = (int)quarters;
-        orth_product<T, KIND, 4, kHalves><<<dim3((unsigned)(ceil_div(n, (int64_t)8) * 8)), dim3(kThreads), 0, s>>>(tab);
+        orth_product<T, KIND, 4, kHalves, kWhole><<<dim3((unsigned)(ceil_div(n, (int64_t)8) * 8)), dim3(kThreads), 0, s>>>(tab);
     };
     if (small_rounds(small) < std::min(with_quarters, all_large)) return over(tab, [&](const Matrix& t) { return tiles(t, 128); }, [&](dim3 g) { launch_small(g.x, -1); });
     return over(tab, [&](const Matrix& t) { return tiles(t, 256); }, [&](dim3) {
@@ -681,12 +749,12 @@ template <typename T> int run(Table& tab, bool small, int iterations, hipStream_
     if (iterations == 0)
         return over(tab, [](const Matrix& t) { return ceil_div((int64_t)t.rows * t.cols, (int64_t)kThreads); }, [&](dim3 g) { orth_copy<T><<<g, threads, 0, s>>>(tab); });
     for (int i = 0; i < iterations; i++) {
-        I6TRAIN_TRY((multiply<T, kGram, 2>(tab, s)));
-        I6TRAIN_TRY((multiply<T, kFactor, 2>(tab, s)));
+        I6TRAIN_TRY((multiply<T, kGram, kThree>(tab, s)));
+        I6TRAIN_TRY((multiply<T, kFactor, kThree>(tab, s)));
         // 16-bit results: nothing follows in which an error of the last product grows.  Half the bits of B's and X's values change what the result is off by from 1.66e-3 (its
         // rounding alone) to 1.69e-3, relative 2-norm, and the product takes 1.16 ms instead of 1.98 (24 matrices of 4096 x 2048).
-        if (i + 1 < iterations) I6TRAIN_TRY((multiply<T, kUpdate, 2>(tab, s)));
-        else I6TRAIN_TRY((multiply<T, kLast, sizeof(T) == 2 ? 1 : 2>(tab, s)));
+        if (i + 1 < iterations) I6TRAIN_TRY((multiply<T, kUpdate, kThree>(tab, s)));
+        else I6TRAIN_TRY((multiply<T, kLast, sizeof(T) == 2 ? kOne : kThree>(tab, s)));
         for (int j = 0; j < tab.count; j++) {
             f16* xt = tab.t[j].xt;
             tab.t[j].xt = tab.t[j].xt_next;
@@ -696,42 +764,22 @@ template <typename T> int run(Table& tab, bool small, int iterations, hipStream_
     return I6TRAIN_OK;
 }
 
-}  // namespace
-}  // namespace i6train
+// What all matrices of a table share.
+size_t shared_bytes(const Table& tab) { return std::max(parts_of(tab, true, true).bytes, std::max(parts_of(tab, false, true).bytes, parts_of(tab, false, false).bytes)); }
 
-using namespace i6train;
-
-extern "C" {
-
-int i6orth_workspace_size(const i6orth_tensor* tensors, int n_tensors, int dtype, size_t* bytes) {
-    I6TRAIN_TRY(checked(tensors, n_tensors, dtype));
-    if (!bytes) return I6TRAIN_ERR_INVALID_ARGUMENT;
-    size_t all = 0;
-    for (int i = 0; i < n_tensors; i++)
-        if (tensors[i].rows > 0 && tensors[i].cols > 0) all += Places(tensors[i]).all;
-    *bytes = all;
-    return I6TRAIN_OK;
-}
-
-int i6orth_step(const i6orth_tensor* tensors, int n_tensors, int dtype, int iterations, double mu, int nesterov, void* workspace, size_t workspace_bytes, void* stream) {
-    size_t need = 0;
-    I6TRAIN_TRY(i6orth_workspace_size(tensors, n_tensors, dtype, &need));
-    if (iterations < 0 || !(mu >= 0 && mu < 1)) return I6TRAIN_ERR_INVALID_ARGUMENT;
-    if (need == 0) return I6TRAIN_OK;
-    if (!workspace || workspace_bytes < need) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
-    Table tab;
-    tab.count = 0;
-    tab.mu = (float)mu;
-    tab.nesterov = nesterov;
-    // which way a matrix goes depends on it alone, and so does its result
+// f(table, small) for the matrices of a call, as many at once as a table has room for; `all` receives the bytes of what they have of their own.  Which way a matrix goes
+// depends on it alone.
+template <typename F> int in_tables(const i6orth_tensor* tensors, int n_tensors, int iterations, char* workspace, size_t* all, F f) {
+    Table tab{};
     for (const bool small : {true, false}) {
+        char* at = workspace;
+        *all = 0;
         const auto flush = [&]() {
             if (tab.count == 0) return I6TRAIN_OK;
-            const int rc = dtype == I6TRAIN_BF16 ? run<bf16>(tab, small, iterations, (hipStream_t)stream) : run<float>(tab, small, iterations, (hipStream_t)stream);
+            const int rc = f(tab, small);
             tab.count = 0;
             return rc;
         };
-        char* at = static_cast<char*>(workspace);
         for (int i = 0; i < n_tensors; i++) {
             const i6orth_tensor& t = tensors[i];
             if (t.rows == 0 || t.cols == 0) continue;
@@ -747,10 +795,46 @@ int i6orth_step(const i6orth_tensor* tensors, int n_tensors, int dtype, int iter
                 m.keep = t.keep; m.rate = t.rate; m.parts_n = p.parts_n;
             }
             at += p.all;
+            *all += p.all;
         }
         I6TRAIN_TRY(flush());
     }
     return I6TRAIN_OK;
+}
+
+}  // namespace
+}  // namespace i6train
+
+using namespace i6train;
+
+extern "C" {
+
+int i6orth_workspace_size(const i6orth_tensor* tensors, int n_tensors, int dtype, size_t* bytes) {
+    I6TRAIN_TRY(checked(tensors, n_tensors, dtype));
+    if (!bytes) return I6TRAIN_ERR_INVALID_ARGUMENT;
+    size_t all = 0, shared = 0;
+    I6TRAIN_TRY(in_tables(tensors, n_tensors, 1, nullptr, &all, [&](Table& tab, bool small) {
+        if (!small) shared = std::max(shared, shared_bytes(tab));
+        return I6TRAIN_OK;
+    }));
+    *bytes = all + align256(shared);
+    return I6TRAIN_OK;
+}
+
+int i6orth_step(const i6orth_tensor* tensors, int n_tensors, int dtype, int iterations, double mu, int nesterov, void* workspace, size_t workspace_bytes, void* stream) {
+    size_t need = 0, all = 0;
+    I6TRAIN_TRY(i6orth_workspace_size(tensors, n_tensors, dtype, &need));
+    if (iterations < 0 || !(mu >= 0 && mu < 1)) return I6TRAIN_ERR_INVALID_ARGUMENT;
+    if (need == 0) return I6TRAIN_OK;
+    if (!workspace || workspace_bytes < need) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
+    for (int i = 0; i < n_tensors; i++)
+        if (tensors[i].rows > 0 && tensors[i].cols > 0) all += Places(tensors[i]).all;
+    return in_tables(tensors, n_tensors, iterations, static_cast<char*>(workspace), &all, [&](Table& tab, bool small) {
+        tab.mu = (float)mu;
+        tab.nesterov = nesterov;
+        tab.partial = reinterpret_cast<acc_t*>(static_cast<char*>(workspace) + all);
+        return dtype == I6TRAIN_BF16 ? run<bf16>(tab, small, iterations, (hipStream_t)stream) : run<float>(tab, small, iterations, (hipStream_t)stream);
+    });
 }
 
 }  // extern "C"

@@ -76,9 +76,9 @@ def test_many_matrices_of_all_sizes(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("n,rows,cols", [(20, 1000, 1100), (16, 1024, 1300), (3, 2100, 1500), (5, 257, 513), (70, 130, 600)])
+@pytest.mark.parametrize("n,rows,cols", [(20, 1000, 1100), (16, 1024, 1300), (3, 2100, 1500), (5, 257, 513), (70, 130, 600), (1, 200, 4096), (2, 3000, 70), (1, 8, 30000), (1, 700, 520), (3, 513, 511)])
 def test_many_large_matrices(n, rows, cols, dtype):
-    """Large tiles, large ones and their quarters, quarters alone, small ones; more than a launch's table."""
+    """Large tiles, large ones and their quarters, quarters alone, small ones; more than a launch's table; few tiles, whose sums are formed in parts."""
     from i6_native_ops_amd.training import orthogonalize
     updates = [matrix(rows, cols, dtype, seed=i) for i in range(n)]
     got, again = orthogonalize(updates), orthogonalize(updates)
