@@ -17,6 +17,16 @@ DTYPES = [torch.float32, torch.bfloat16]
 NAMES = ("q", "k", "v", "gate", "beta", "initial")
 
 
+STREAMS = {}
+
+
+def stream_of(name):
+    """One stream for a name: streams share a few hardware queues, and what else runs in this process should find them as free as it can."""
+    if name not in STREAMS:
+        STREAMS[name] = torch.cuda.Stream()
+    return STREAMS[name]
+
+
 def gen(seed):
     return torch.Generator(device="cuda").manual_seed(seed)
 
@@ -281,7 +291,7 @@ def test_captured_calls(T, lens, dtype):
         o, last = gated_delta_rule(*leaves[:5], seq_lens=p["lens"], initial_state=leaves[5])
         return (o, last) + torch.autograd.grad([o, last], leaves, [p["grad_o"], p["grad_last"]])
 
-    side = torch.cuda.Stream()
+    side = stream_of(dtype)
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
         step()
@@ -308,7 +318,7 @@ def test_captured_calls(T, lens, dtype):
 def test_on_another_stream(T):
     p = problem(2, T, 2, 2, 64, 64, torch.bfloat16)
     want = run(p)
-    side = torch.cuda.Stream()
+    side = stream_of("another")
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
         got = run(p)
@@ -321,7 +331,7 @@ def test_two_calls_at_once():
     """Calls in flight on two streams have workspaces of their own."""
     p, q = problem(1, 2000, 2, 2, 64, 64, torch.bfloat16, seed=5, lens="all"), problem(3, 700, 4, 4, 128, 128, torch.float32, seed=6, lens="all")
     want = run(p), run(q)
-    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    a, b = stream_of(torch.float32), stream_of(torch.bfloat16)
     torch.cuda.synchronize()
     for _ in range(3):
         with torch.cuda.stream(a):
