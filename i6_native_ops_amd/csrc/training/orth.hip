@@ -829,7 +829,8 @@ int i6orth_step(const i6orth_tensor* tensors, int n_tensors, int dtype, int iter
     if (!workspace || workspace_bytes < need) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
     for (int i = 0; i < n_tensors; i++)
         if (tensors[i].rows > 0 && tensors[i].cols > 0) all += Places(tensors[i]).all;
-    return in_tables(tensors, n_tensors, iterations, static_cast<char*>(workspace), &all, [&](Table& tab, bool small) {
+    size_t so_far = 0;
+    return in_tables(tensors, n_tensors, iterations, static_cast<char*>(workspace), &so_far, [&](Table& tab, bool small) {
         tab.mu = (float)mu;
         tab.nesterov = nesterov;
         tab.partial = reinterpret_cast<acc_t*>(static_cast<char*>(workspace) + all);
