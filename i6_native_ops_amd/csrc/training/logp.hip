@@ -443,10 +443,10 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_backward
         for (int i = 0; i <= k; i++) more += classes[i] == c ? mores[i] : 0.f;
         return more;
     };
-    // - p (gl + sum gt + ge (log p + entropy))
+    // - p (gl + sum gt + ge (log p + entropy)).  Below -200 p is 0 and log p only has to be a number whose product with ge is one, too
     const auto share = [&](float z) {
         const float log_p = (z - m) - log_total, p = exp2_fast(log_p * kLog2e);
-        return -p * fmaf(ge, fmaxf(log_p, -1e30f) + entropy, sum);
+        return -p * fmaf(ge, fmaxf(log_p, -200.f) + entropy, sum);
     };
     const T* from = static_cast<const T*>(a.logits) + b * a.l_b + t * a.l_t;
     const auto one = [&](int i) {

@@ -323,3 +323,23 @@ def test_second_derivatives_tangents_and_refusals():
     ]:
         with pytest.raises(RuntimeError, match=match):
             target_log_probs(*args)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("F", [20, 700, 5000, 30001])
+def test_large_incoming_gradients_leave_ruled_out_classes_alone(F, dtype):
+    """-inf and scores far below the others have no share, whatever comes in: their gradients are 0 and not a product of 0 and infinity."""
+    logits, targets, lens, k, grads = problem(1, 4, F, 2, dtype, lens=[4])
+    logits[0, 0, ::3] = -INF
+    logits[0, 1, ::3] = torch.finfo(dtype).min
+    logits[0, 2, ::3] = -1e30
+    targets[:] = 1
+    grads = [g * 1e12 for g in grads]
+    got = run(logits, targets, lens, k, grads)
+    assert torch.isfinite(got["logits"]).all()
+    for t in range(3):
+        ruled_out = torch.zeros(F, dtype=torch.bool, device="cuda")
+        ruled_out[::3] = True
+        ruled_out[got["classes"][0, t].long()] = False
+        assert (got["logits"][0, t, ruled_out] == 0).all()
+    check(got, expected(logits, targets, lens, k, grads))
