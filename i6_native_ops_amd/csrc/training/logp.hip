@@ -389,20 +389,16 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_forward(
 
 // ------------------------------------------------------------------------------------------------------------ backward
 
-// A target and alternatives are found by the pieces they are in: a bit for each piece, modulo kMarks, and those whose bit is set look through the list.
-constexpr int kMarks = 2048;
-
+// What every class has of the frame's sums is written first, then the classes that something comes in for are written again.
 template <typename T, int kThreads>
 __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_backward(Args a) {
     using G = Team<kThreads>;
     constexpr int kTeams = G::kWaves == 1 ? 4 : 1, P = kPiece<T>, kList = I6LOGP_MOST_ALTERNATIVES + 1;
-    __shared__ uint32_t all_marks[kTeams][kMarks / 32];
     __shared__ int all_class[kTeams][kList];
     __shared__ float all_more[kTeams][kList];
     const int team = kTeams == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t frame = (int64_t)blockIdx.x * kTeams + team;
     if (frame >= (int64_t)a.B * a.T) return;
-    uint32_t* marks = all_marks[team];
     int* classes = all_class[team];
     float* mores = all_more[team];
     const int thread = G::thread(), b = (int)((uint32_t)frame / (uint32_t)a.T), t = (int)((uint32_t)frame % (uint32_t)a.T), k = a.k;
@@ -425,55 +421,44 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_backward
     const float gl = a.g_log_prob && y >= 0 ? a.g_log_prob[frame] : 0.f, ge = a.g_entropy ? a.g_entropy[frame] : 0.f;
     const int lane = threadIdx.x & 63;
     const float gt = a.g_top && lane < k ? a.g_top[frame * k + lane] : 0.f, sum = gl + wave_sum(gt);
-    for (int i = thread; i < kMarks / 32; i += kThreads) marks[i] = 0;
-    G::meet();
-    // number of the piece of a class; the single ones in front and behind have numbers of their own
-    const auto piece_of = [&](int c) { return (uint32_t)(c - out.head + P) / P; };
-    const auto list = [&](int i, int c, float more) {
-        classes[i] = c;
-        mores[i] = more;
-        if (c >= 0) atomicOr(&marks[piece_of(c) / 32 % (kMarks / 32)], 1u << (piece_of(c) & 31));
-    };
-    if (thread < k) list(thread, a.top_class[frame * k + thread], gt);
-    if (thread == 0) list(k, y, gl);
-    G::meet();
-    const auto marked = [&](int c) { return marks[piece_of(c) / 32 % (kMarks / 32)] >> (piece_of(c) & 31) & 1; };
-    const auto listed = [&](int c) {
-        float more = 0.f;
-        for (int i = 0; i <= k; i++) more += classes[i] == c ? mores[i] : 0.f;
-        return more;
-    };
+    if (thread < k) {
+        classes[thread] = a.top_class[frame * k + thread];
+        mores[thread] = gt;
+    }
+    if (thread == 0) {
+        classes[k] = y;
+        mores[k] = gl;
+    }
     // - p (gl + sum gt + ge (log p + entropy)).  Below -200 p is 0 and log p only has to be a number whose product with ge is one, too
     const auto share = [&](float z) {
         const float log_p = (z - m) - log_total, p = exp2_fast(log_p * kLog2e);
         return -p * fmaf(ge, fmaxf(log_p, -200.f) + entropy, sum);
     };
     const T* from = static_cast<const T*>(a.logits) + b * a.l_b + t * a.l_t;
-    const auto one = [&](int i) {
-        float g = share((float)from[i]);
-        if (marked(i)) g += listed(i);
-        to[i] = (T)g;
-    };
     if ((((uintptr_t)from ^ (uintptr_t)to) & 15) == 0) {
 #pragma unroll 4
         for (int i = thread; i < out.pieces; i += kThreads) {
             const int at = out.head + i * P;
             const Vector<T> z = *reinterpret_cast<const Vector<T>*>(from + at);
-            float g[P];
-#pragma unroll
-            for (int e = 0; e < P; e++) g[e] = share((float)z[e]);
-            if (marked(at)) {
-#pragma unroll
-                for (int e = 0; e < P; e++) g[e] += listed(at + e);
-            }
             Vector<T> v;
 #pragma unroll
-            for (int e = 0; e < P; e++) v[e] = (T)g[e];
+            for (int e = 0; e < P; e++) v[e] = (T)share((float)z[e]);
             *reinterpret_cast<Vector<T>*>(to + at) = v;
         }
-        if (single >= 0) one(single);
+        if (single >= 0) to[single] = (T)share((float)from[single]);
     } else {
-        for (int i = thread; i < a.F; i += kThreads) one(i);
+        for (int i = thread; i < a.F; i += kThreads) to[i] = (T)share((float)from[i]);
+    }
+    G::meet();
+    for (int i = thread; i <= k; i += kThreads) {
+        const int c = classes[i];
+        if (c < 0) continue;
+        float more = 0.f;                // a target may be an alternative; then both write the same
+        for (int j = 0; j <= k; j++) more += classes[j] == c ? mores[j] : 0.f;
+        // Where p is next to 1 with 1 - p from log p, so that a confident frame's difference keeps its relative precision; below one half more - p (...) is one rounding and
+        // nothing cancels
+        const float log_p = ((float)from[c] - m) - log_total, p = exp2_fast(log_p * kLog2e), of_entropy = fmaxf(log_p, -200.f) + entropy;
+        to[c] = (T)(p > 0.5f ? fmaf(-p, fmaf(ge, of_entropy, sum - more), -more * expm1f(log_p)) : fmaf(-p, fmaf(ge, of_entropy, sum), more));
     }
 }
 

@@ -343,3 +343,24 @@ def test_large_incoming_gradients_leave_ruled_out_classes_alone(F, dtype):
         ruled_out[got["classes"][0, t].long()] = False
         assert (got["logits"][0, t, ruled_out] == 0).all()
     check(got, expected(logits, targets, lens, k, grads))
+
+
+@pytest.mark.parametrize("F,k", [(100, 0), (1003, 1), (9001, 3)])
+def test_confident_frames_keep_their_small_gradients(F, k):
+    """1 - p is the others' sum, not the difference of two numbers next to 1.  An exponential's argument, at most 90 / ln 2, is rounded to 2^-24 of it: 130 * 0.7 EPS32 of the exponential;
+    sums of them take (64 + 2 * 10) EPS32 more, log1p, expm1 and the products 20."""
+    from i6_native_ops_amd.training import target_log_probs
+    sizes = [10.0, 25.0, 45.0, 80.0]
+    logits = torch.zeros((1, 4, F), device="cuda")
+    logits[0, :, F - 3] = torch.tensor(sizes, device="cuda")
+    logits.requires_grad_()
+    targets, lens = torch.full((1, 4), F - 3, dtype=torch.int32, device="cuda"), torch.tensor([4], dtype=torch.int32, device="cuda")
+    log_prob, _, top, classes = target_log_probs(logits, targets, lens, alternatives=k)
+    loss = log_prob.sum() + (0.5 * top[:, :, 0].sum() if k else 0.0)      # the best alternative is the target
+    grad, = torch.autograd.grad(loss, logits)
+    if k:
+        assert (classes[0, :, 0] == F - 3).all()
+    for t, x in enumerate(sizes):
+        others = (F - 1) * math.exp(-x)
+        want = (1.5 if k else 1.0) * others / (1.0 + others)
+        assert abs(float(grad[0, t, F - 3]) - want) <= want * 200 * EPS32, (x, float(grad[0, t, F - 3]), want)
