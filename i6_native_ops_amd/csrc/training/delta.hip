@@ -304,6 +304,40 @@ __device__ __forceinline__ void store_columns(const acc_t (&v)[M][NT], T* p, int
     }
 }
 
+// A value that is no number belongs to its frame and those behind it, but products of whole blocks would take it to the frames of its block in front of it, too: there it is multiplied
+// by 0, and that is NaN.  So from the first such row of R on, in its column, rows are 0 while the chunk's system is solved and read, and NaN behind that.  A sum with 0 times each
+// value says whether there is one, which is all that a chunk pays for it.  Whether: the whole wave; `first`: the lane's column.
+__device__ __forceinline__ void fill_from(acc_t& v, int m, int first, float by) {
+    const int at = 16 * m + 4 * ((threadIdx.x & 63) >> 4);
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (at + e >= first) v[e] = by;
+}
+template <int M> __device__ __forceinline__ bool take_out(acc_t (&r)[M], int& first) {
+    float probe = 0.f;
+#pragma unroll
+    for (int m = 0; m < M; m++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) probe = fmaf(r[m][e], 0.f, probe);
+    if (!__any(probe != probe)) return false;
+    const int at = 4 * ((threadIdx.x & 63) >> 4);
+    first = 16 * M;
+#pragma unroll
+    for (int m = M - 1; m >= 0; m--)
+#pragma unroll
+        for (int e = 3; e >= 0; e--)
+            if (!(fabsf(r[m][e]) < INFINITY)) first = 16 * m + at + e;
+    first = min(first, __shfl_xor(first, 16));
+    first = min(first, __shfl_xor(first, 32));
+#pragma unroll
+    for (int m = 0; m < M; m++) fill_from(r[m], m, first, 0.f);
+    return true;
+}
+template <int M> __device__ __forceinline__ void put_back(acc_t (&r)[M], int first) {
+#pragma unroll
+    for (int m = 0; m < M; m++) fill_from(r[m], m, first, __builtin_nanf(""));
+}
+
 // ------------------------------------------------------------------------------------------------------ frame by frame
 
 // Few frames, no training: 64 columns of a head, KP / 4 rows of the state in the registers of each of four waves.  The state is read and written once; with

@@ -1,0 +1,37 @@
+"""The gated delta rule with values of very different sizes, and with values that are no numbers."""
+import pytest
+import torch
+
+from tests.test_delta_gpu import DTYPES, NAMES, problem
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,K,V,at", [(70, 16, 16, (0, 21)), (70, 64, 40, (15, 16, 31, 63, 64)), (130, 128, 128, (33, 127)), (1300, 64, 64, (700,))])
+def test_what_is_no_number_stays_out_of_the_frames_in_front_of_it(T, K, V, at, dtype):
+    """A value that is NaN or infinite spoils its column from its frame on, a key or share all columns: never a frame in front of it, another column or another sequence."""
+    from i6_native_ops_amd.training import gated_delta_rule
+
+    def outputs(p):
+        with torch.no_grad():
+            plain = gated_delta_rule(*(p[n] for n in NAMES[:5]), initial_state=p["initial"])
+        trained = gated_delta_rule(*(p[n].requires_grad_(n == "v") for n in NAMES[:5]), initial_state=p["initial"])
+        assert all(torch.equal(a.nan_to_num(7.0), b.detach().nan_to_num(7.0)) for a, b in zip(plain, trained))
+        return plain
+
+    p = problem(2, T, 2, 2, K, V, dtype, lens="all")
+    want = outputs({n: x.clone() if torch.is_tensor(x) else x for n, x in p.items()})
+    for t in at:
+        for name, bad in (("v", float("nan")), ("v", float("inf")), ("k", float("nan")), ("beta", float("nan"))):
+            q = {n: x.clone() if torch.is_tensor(x) else x for n, x in p.items()}
+            q[name][(0, t, 1, 3) if name == "v" else (0, t, 1)] = bad
+            o, last = outputs(q)
+            columns = [3] if name == "v" else list(range(V))
+            spoilt = torch.zeros(o.shape, dtype=torch.bool, device="cuda")
+            spoilt[0, t:, 1, columns] = True
+            assert not torch.isfinite(o[spoilt]).any(), (name, t)
+            assert torch.equal(o[~spoilt], want[0][~spoilt]), (name, t)
+            of_state = torch.zeros(last.shape, dtype=torch.bool, device="cuda")
+            of_state[0, 1, :, columns] = True
+            assert not torch.isfinite(last[of_state]).any() and torch.equal(last[~of_state], want[1][~of_state]), (name, t)
