@@ -61,6 +61,11 @@ __device__ __forceinline__ int len_of(const Args& a, int b) {
     return n < 0 ? 0 : (n > a.T ? a.T : n);
 }
 __device__ __forceinline__ float log_sigmoid(float x) { return fminf(x, 0.f) - log1pf(expf(-fabsf(x))); }
+// For sums over a chunk.  A gate of -inf: a factor that is 0, and sums that stay numbers; one that is no number stays that.
+__device__ __forceinline__ float log_kept(float gate) {
+    const float x = log_sigmoid(gate);
+    return x < -1e6f ? -1e6f : x;
+}
 __device__ __forceinline__ float sigmoid(float x) {
     const float e = expf(-fabsf(x));
     return (x >= 0.f ? 1.f : e) / (1.f + e);
@@ -189,8 +194,7 @@ template <typename T, int KP> struct Ahead {
         if (threadIdx.x < kWave) {
             const int i = threadIdx.x;
             const bool there = i < kC && first + i < len;
-            // a gate of -inf: a factor that is 0, and sums that stay numbers
-            double c = there ? (double)fmaxf(log_sigmoid(gate), -1e6f) : 0.0;
+            double c = there ? (double)log_kept(gate) : 0.0;
 #pragma unroll
             for (int m = 1; m < kC; m *= 2) {
                 const double before = __shfl_up(c, m);

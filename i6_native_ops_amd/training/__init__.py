@@ -121,7 +121,8 @@ def gated_delta_rule(
     :param seq_lens: int32 [B]; all T frames without.  Frames behind the end are not looked at
     :param initial_state: float32 [B, H, K, V], the state in front of the first frame; zeros without
     :return: o [B, T, H, V] in the type of v, 0 behind the end, and the state after the last frame of every sequence, float32 [B, H, K, V].
-        The next frames of the same streams start from it
+        The next frames of the same streams start from it.  What is no number in v spoils its column of the head from its frame on, in k, gate or beta all of the head from the frame
+        on, in q the frame's output; nothing in front of the frame.  Gradients of such a sequence's head are not defined
     """
     return core.gated_delta_rule(q, k, v, gate, beta, seq_lens, initial_state)
 

@@ -35,3 +35,20 @@ def test_what_is_no_number_stays_out_of_the_frames_in_front_of_it(T, K, V, at, d
             of_state = torch.zeros(last.shape, dtype=torch.bool, device="cuda")
             of_state[0, 1, :, columns] = True
             assert not torch.isfinite(last[of_state]).any() and torch.equal(last[~of_state], want[1][~of_state]), (name, t)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,K,V,t", [(10, 16, 16, 4), (40, 16, 16, 5), (70, 64, 40, 63), (130, 128, 128, 64), (1300, 64, 64, 700)])
+def test_a_gate_that_is_no_number(T, K, V, t, dtype):
+    """It is none of the gates that forget: all of the head is spoilt from its frame on, and not replaced by what looks like results.  In chunks as frame by frame."""
+    from i6_native_ops_amd.training import gated_delta_rule
+    p = problem(2, T, 2, 2, K, V, dtype, lens="all")
+    with torch.no_grad():
+        want = gated_delta_rule(*(p[n] for n in NAMES[:5]), initial_state=p["initial"])
+        p["gate"][1, t, 0] = float("nan")
+        o, last = gated_delta_rule(*(p[n] for n in NAMES[:5]), initial_state=p["initial"])
+    trained = gated_delta_rule(*(p[n].requires_grad_(n == "v") for n in NAMES[:5]), initial_state=p["initial"])[0].detach()
+    assert torch.isnan(o[1, t:, 0]).all() and torch.isnan(trained[1, t:, 0]).all() and torch.isnan(last[1, 0]).all()
+    o[1, t:, 0] = want[0][1, t:, 0]
+    last[1, 0] = want[1][1, 0]
+    assert torch.equal(o, want[0]) and torch.equal(last, want[1])
