@@ -6,7 +6,7 @@
 //   O = exp(c) Q S0 + P U,  P_ij = D_ij q_i.k_j (j <= i);   S1 = exp(c_C) S0 + (exp(c_C - c) K)^T U
 // Backward, with G1 the gradient of S1, from the last chunk to the first:
 //   dU = P^T dO + exp(c_C - c) K G1,  (1 + A)^T dR = dU,  dV = w dR,  G0 = exp(c_C) G1 + (exp(c) Q)^T dO - (w exp(c) K)^T dR
-// and from S0, G1, U and dR of a chunk all gradients of its q, k, gates, for all chunks at once (delta_gradients).
+// and from S0, G1, U and dR of a chunk all gradients of its q, k, gates, for all chunks at once (delta_gradients32, delta_gradients16).
 //
 // Every column of the state goes its own way: a wave has columns of its own, their states in registers as they come out of the matrix
 // instructions, which is also how these take them for their second operand (with the order of k that both operands share), so states, R, U, O and their
@@ -43,8 +43,8 @@ struct Args {
     int B, T, H, G, K, V, chunks;
     void* o;
     float* last;
-    Rows* rows;                          // null: not for training
-    float *states, *u;                   // [B][H][chunks][K][V], [B][H][chunks C][V]
+    Rows* rows;                          // of all chunks; null: frame by frame
+    float *states, *u;                   // [B][H][chunks][K][V], [B][H][chunks C][V]; null: not for training
     // backward
     const void* d_o;
     int64_t do_b, do_t, do_h;
@@ -71,17 +71,12 @@ __device__ __forceinline__ float sigmoid(float x) {
     return (x >= 0.f ? 1.f : e) / (1.f + e);
 }
 
-// 16 bytes of a row of `n` values from value `at` on; zeros behind them.
-template <typename T> struct Piece {
-    static constexpr int kN = 16 / sizeof(T);
-    using type = T __attribute__((ext_vector_type(kN)));
-};
-template <typename T> __device__ __forceinline__ typename Piece<T>::type load_piece(const T* row, int at, int n, bool whole) {
-    using P = typename Piece<T>::type;
-    if (whole && at + Piece<T>::kN <= n) return *reinterpret_cast<const P*>(row + at);
-    P p;
+// Four values of a row of `n` from value `at` on; zeros behind them.
+__device__ __forceinline__ acc_t load_piece(const float* row, int at, int n, bool whole) {
+    if (whole && at + 4 <= n) return *reinterpret_cast<const acc_t*>(row + at);
+    acc_t p;
 #pragma unroll
-    for (int i = 0; i < Piece<T>::kN; i++) p[i] = at + i < n ? row[at + i] : (T)0.f;
+    for (int i = 0; i < 4; i++) p[i] = at + i < n ? row[at + i] : 0.f;
     return p;
 }
 
@@ -138,19 +133,19 @@ template <int KP> struct Chunk {
 };
 
 // Keys and queries of a chunk, loaded ahead: kPer pieces of each for a thread.
-template <typename T, int KP> struct Ahead {
-    static constexpr int kPieces = KP / Piece<T>::kN, kThreadsPerRow = kThreads / kC, kPer = (kPieces + kThreadsPerRow - 1) / kThreadsPerRow;
-    typename Piece<T>::type k[kPer], q[kPer];
+template <int KP> struct Ahead {
+    static constexpr int kPieces = KP / 4, kThreadsPerRow = kThreads / kC, kPer = (kPieces + kThreadsPerRow - 1) / kThreadsPerRow;
+    acc_t k[kPer], q[kPer];
     float gate, beta;
     __device__ __forceinline__ void fetch(const Args& a, int b, int h, int first, int len, bool whole) {
         const int row = threadIdx.x / kThreadsPerRow, j = threadIdx.x % kThreadsPerRow, t = first + row;
         const int g = h / (a.H / a.G);
-        const T* kr = static_cast<const T*>(a.k) + b * a.k_b + t * a.k_t + g * a.k_g;
-        const T* qr = static_cast<const T*>(a.q) + b * a.q_b + t * a.q_t + g * a.q_g;
-        const typename Piece<T>::type none = {};
+        const float* kr = static_cast<const float*>(a.k) + b * a.k_b + t * a.k_t + g * a.k_g;
+        const float* qr = static_cast<const float*>(a.q) + b * a.q_b + t * a.q_t + g * a.q_g;
+        const acc_t none = 0.f;
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
-            const int at = (i * kThreadsPerRow + j) * Piece<T>::kN;
+            const int at = (i * kThreadsPerRow + j) * 4;
             const bool there = t < len && at < a.K;
             k[i] = there ? load_piece(kr, at, a.K, whole) : none;
             q[i] = there ? load_piece(qr, at, a.K, whole) : none;
@@ -158,8 +153,8 @@ template <typename T, int KP> struct Ahead {
         if (threadIdx.x < kC) {
             const int tt = first + threadIdx.x;
             const bool there = tt < len;
-            gate = there ? (float)static_cast<const T*>(a.gate)[b * a.gate_b + tt * a.gate_t + h * a.gate_h] : 0.f;
-            beta = there ? (float)static_cast<const T*>(a.beta)[b * a.beta_b + tt * a.beta_t + h * a.beta_h] : 0.f;
+            gate = there ? static_cast<const float*>(a.gate)[b * a.gate_b + tt * a.gate_t + h * a.gate_h] : 0.f;
+            beta = there ? static_cast<const float*>(a.beta)[b * a.beta_b + tt * a.beta_t + h * a.beta_h] : 0.f;
         }
     }
     // to LDS, with lengths, shares and decays.  The sum of log f is taken in 64 bits: differences of it are what counts, and it may be far larger.
@@ -168,17 +163,17 @@ template <typename T, int KP> struct Ahead {
         float kk = 0.f, qq = 0.f;
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
-            const int at = (i * kThreadsPerRow + j) * Piece<T>::kN;
+            const int at = (i * kThreadsPerRow + j) * 4;
 #pragma unroll
-            for (int e = 0; e < Piece<T>::kN; e++) {
-                kk = fmaf((float)k[i][e], (float)k[i][e], kk);
-                qq = fmaf((float)q[i][e], (float)q[i][e], qq);
+            for (int e = 0; e < 4; e++) {
+                kk = fmaf(k[i][e], k[i][e], kk);
+                qq = fmaf(q[i][e], q[i][e], qq);
             }
             if (at < KP) {
 #pragma unroll
-                for (int e = 0; e < Piece<T>::kN; e++) {
-                    s.k[row * Chunk<KP>::kStride + at + e] = (float)k[i][e];
-                    s.q[row * Chunk<KP>::kStride + at + e] = (float)q[i][e];
+                for (int e = 0; e < 4; e++) {
+                    s.k[row * Chunk<KP>::kStride + at + e] = k[i][e];
+                    s.q[row * Chunk<KP>::kStride + at + e] = q[i][e];
                 }
             }
         }
@@ -271,9 +266,9 @@ template <int KP> __device__ __forceinline__ void invert(Chunk<KP>& s) {
     Tile<20>{s.inverse}.put(wave, 0, t);
 }
 
-// Values of `T` at rows 16 m + 4 (lane >> 4) + r of a matrix, as accumulators.
-template <typename T, int NT, int M>
-__device__ __forceinline__ void load_columns(acc_t (&v)[M][NT], const T* p, int64_t stride, int rows, int col, int cols) {
+// Values at rows 16 m + 4 (lane >> 4) + r of a matrix, as accumulators.
+template <int NT, int M>
+__device__ __forceinline__ void load_columns(acc_t (&v)[M][NT], const float* p, int64_t stride, int rows, int col, int cols) {
     const int at = 4 * ((threadIdx.x & 63) >> 4);
     p += at * stride + col;
     asm volatile("" : "+v"(p));       // rows' addresses are formed here, or the compiler keeps them all from chunk to chunk
@@ -283,14 +278,14 @@ __device__ __forceinline__ void load_columns(acc_t (&v)[M][NT], const T* p, int6
         for (int e = 0; e < 4; e++) {
             const bool there = 16 * m + at + e < rows;
 #pragma unroll
-            for (int j = 0; j < NT; j++) v[m][j][e] = there && col + j < cols ? (float)p[j] : 0.f;
+            for (int j = 0; j < NT; j++) v[m][j][e] = there && col + j < cols ? p[j] : 0.f;
             p += stride;
         }
         p += 12 * stride;
     }
 }
-template <typename T, int NT, int M>
-__device__ __forceinline__ void store_columns(const acc_t (&v)[M][NT], T* p, int64_t stride, int rows, int col, int cols) {
+template <int NT, int M>
+__device__ __forceinline__ void store_columns(const acc_t (&v)[M][NT], float* p, int64_t stride, int rows, int col, int cols) {
     const int at = 4 * ((threadIdx.x & 63) >> 4);
     p += at * stride + col;
     asm volatile("" : "+v"(p));       // rows' addresses are formed here, or the compiler keeps them all from chunk to chunk
@@ -301,7 +296,7 @@ __device__ __forceinline__ void store_columns(const acc_t (&v)[M][NT], T* p, int
             const bool there = 16 * m + at + e < rows;
 #pragma unroll
             for (int j = 0; j < NT; j++)
-                if (there && col + j < cols) p[j] = (T)v[m][j][e];
+                if (there && col + j < cols) p[j] = v[m][j][e];
             p += stride;
         }
         p += 12 * stride;
@@ -440,12 +435,12 @@ __device__ __forceinline__ acc_t load_four(const float* row, int at, int n, bool
     return v;
 }
 
-// All other gradients of a chunk, from the state in front of it, the gradient of that behind it, U and dR:
+// 32 bits: all other gradients of a chunk, from the state in front of it, the gradient of that behind it, U and dR:
 //   dq^ = exp(c) dO S0^T + Z K^,   dk^ = exp(c_C - c) U G1^T - w exp(c) dR S0^T + Z^T Q^ + (E + E^T) K^,   Z = D (dO U^T),  E = - w D (dR U^T)
 // (lower triangles, E's without its diagonal).  What decays with c_i is a row's dot product with its query's gradient and the part of its key's that stands on
 // the left; what decays with - c_j that with the other part; so the gradient of c needs no products of its own, nor A and P.
-template <typename T, int KP>
-__global__ __launch_bounds__(kThreads, 2) void delta_gradients(Args a) {
+template <int KP>
+__global__ __launch_bounds__(kThreads, 2) void delta_gradients32(Args a) {
     constexpr int M = kC / 16, N = KP == 128 ? 2 : 1, kV = 128 + 4, kSquare = kC + 4;
     __shared__ __align__(16) float s_o[kC * kV], s_u[kC * kV], s_r[kC * kV], s_z[kC * kSquare], s_e[kC * kSquare];
     __shared__ __align__(16) float s_c[kC], s_rest[kC], s_w[kC], s_rk[kC], s_rq[kC], s_start[kC], s_end[kC], s_dots[4][kC][4], s_whole[4], s_gate[kC];
@@ -454,16 +449,16 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients(Args a) {
     const int len = len_of(a, b), live = min(kC, len - first), rows = min(kC, a.T - first), g = h / (a.H / a.G);
     const int64_t head = (int64_t)b * a.H + h, frame = (int64_t)b * a.T + first;
     const int col = wave * 16 * N + (lane & 15) * N;
-    T* dq = static_cast<T*>(a.d_q) + (frame * a.G + g) * a.K;
-    T* dk = static_cast<T*>(a.d_k) + (frame * a.G + g) * a.K;
+    float* dq = static_cast<float*>(a.d_q) + (frame * a.G + g) * a.K;
+    float* dk = static_cast<float*>(a.d_k) + (frame * a.G + g) * a.K;
     float* dq_head = a.d_q_head + (frame * a.H + h) * a.K;
     float* dk_head = a.d_k_head + (frame * a.H + h) * a.K;
     const auto store = [&](const acc_t (&v)[M][N], bool keys) {
-        if (a.d_q_head) store_columns<float, N, M>(v, keys ? dk_head : dq_head, (int64_t)a.H * a.K, rows, col, a.K);
-        else store_columns<T, N, M>(v, keys ? dk : dq, (int64_t)a.G * a.K, rows, col, a.K);
+        if (a.d_q_head) store_columns<N, M>(v, keys ? dk_head : dq_head, (int64_t)a.H * a.K, rows, col, a.K);
+        else store_columns<N, M>(v, keys ? dk : dq, (int64_t)a.G * a.K, rows, col, a.K);
     };
-    T* d_gate = static_cast<T*>(a.d_gate) + frame * a.H + h;
-    T* d_beta = static_cast<T*>(a.d_beta) + frame * a.H + h;
+    float* d_gate = static_cast<float*>(a.d_gate) + frame * a.H + h;
+    float* d_beta = static_cast<float*>(a.d_beta) + frame * a.H + h;
     if (live <= 0) {
         acc_t none[M][N] = {};
         if (col < KP) {
@@ -471,8 +466,8 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients(Args a) {
             store(none, true);
         }
         if ((int)threadIdx.x < rows) {
-            d_gate[threadIdx.x * a.H] = (T)0.f;
-            d_beta[threadIdx.x * a.H] = (T)0.f;
+            d_gate[threadIdx.x * a.H] = 0.f;
+            d_beta[threadIdx.x * a.H] = 0.f;
         }
         return;
     }
@@ -484,14 +479,14 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients(Args a) {
         const int row = threadIdx.x / kPerRow, j = threadIdx.x % kPerRow;
         const float* u = a.u + (head * a.chunks * kC + first + row) * a.V;
         const float* r = a.dr + (head * a.chunks * kC + first + row) * a.V;
-        const T* d_o = static_cast<const T*>(a.d_o) + b * a.do_b + (first + row) * a.do_t + h * a.do_h;
+        const float* d_o = static_cast<const float*>(a.d_o) + b * a.do_b + (first + row) * a.do_t + h * a.do_h;
         float ru = 0.f;
         for (int c = j * 4; c < cols; c += kPerRow * 4) {
             const acc_t uv = load_four(u, c, a.V, whole), rv = load_four(r, c, a.V, whole);
             acc_t ov;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                ov[i] = a.d_o && row < live && c + i < a.V ? (float)d_o[c + i] : 0.f;
+                ov[i] = a.d_o && row < live && c + i < a.V ? d_o[c + i] : 0.f;
                 ru = fmaf(uv[i], rv[i], ru);
             }
             *reinterpret_cast<acc_t*>(s_u + row * kV + c) = uv;
@@ -502,8 +497,8 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients(Args a) {
         for (int m = 1; m < kPerRow; m *= 2) ru += __shfl_xor(ru, m);
         // u = w (v - ...), so dw = dR.u / w, times w (1 - w)
         if (j == 0 && row < rows) {
-            const float beta = row < live ? (float)static_cast<const T*>(a.beta)[b * a.beta_b + (first + row) * a.beta_t + h * a.beta_h] : 0.f;
-            d_beta[row * a.H] = (T)(row < live ? ru * sigmoid(-beta) : 0.f);
+            const float beta = row < live ? static_cast<const float*>(a.beta)[b * a.beta_b + (first + row) * a.beta_t + h * a.beta_h] : 0.f;
+            d_beta[row * a.H] = row < live ? ru * sigmoid(-beta) : 0.f;
         }
         if (threadIdx.x < kC) {
             const int i = threadIdx.x;
@@ -573,8 +568,8 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients(Args a) {
     __syncthreads();
     acc_t kv[M][N], qv[M][N];
     if (col < KP) {
-        load_columns<T, N, M>(kv, static_cast<const T*>(a.k) + b * a.k_b + first * a.k_t + g * a.k_g, a.k_t, live, col, a.K);
-        load_columns<T, N, M>(qv, static_cast<const T*>(a.q) + b * a.q_b + first * a.q_t + g * a.q_g, a.q_t, live, col, a.K);
+        load_columns<N, M>(kv, static_cast<const float*>(a.k) + b * a.k_b + first * a.k_t + g * a.k_g, a.k_t, live, col, a.K);
+        load_columns<N, M>(qv, static_cast<const float*>(a.q) + b * a.q_b + first * a.q_t + g * a.q_g, a.q_t, live, col, a.K);
 #pragma unroll
         for (int m = 0; m < M; m++) {
             const acc_t start = four(s_start + 16 * m + at), rk = four(s_rk + 16 * m + at);
@@ -665,8 +660,8 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients(Args a) {
             if (lane + m < kC) d += behind;
         }
         if (lane < rows) {
-            const float gate = lane < live ? (float)static_cast<const T*>(a.gate)[b * a.gate_b + (first + lane) * a.gate_t + h * a.gate_h] : 0.f;
-            d_gate[lane * a.H] = (T)(lane < live ? d * sigmoid(-gate) : 0.f);
+            const float gate = lane < live ? static_cast<const float*>(a.gate)[b * a.gate_b + (first + lane) * a.gate_t + h * a.gate_h] : 0.f;
+            d_gate[lane * a.H] = lane < live ? d * sigmoid(-gate) : 0.f;
         }
     }
 }
@@ -834,7 +829,7 @@ template <int KP> void run_backward(const Call& c, hipStream_t s, float) {
     }
     if (wide(c)) delta_backward32<KP, 8, false><<<dim3(c.a.H, c.a.B, k.segments), dim3(512), 0, s>>>(c.a, k, blocks, c.whole, c.whole_v);
     else delta_backward32<KP, 4, false><<<dim3(c.a.H * ceil_div(c.a.V, 64), c.a.B, k.segments), dim3(256), 0, s>>>(c.a, k, blocks, c.whole, c.whole_v);
-    delta_gradients<float, KP><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a);
+    delta_gradients32<KP><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a);
 }
 template <int KP> void run_backward(const Call& c, hipStream_t s, bf16) {
     const Args16& k = c.k16;
