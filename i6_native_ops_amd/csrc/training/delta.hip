@@ -426,6 +426,80 @@ __global__ __launch_bounds__(kThreads, 4) void delta_frames(Args a) {
 
 // ------------------------------------------------------------------------------------------------------------ backward
 
+// Sums over sixteen lanes of four values each: lanes with e in their last two bits get the sum of value e.
+__device__ __forceinline__ float sum_of_16(acc_t v, int lane) {
+#define I6_TURN(x, ctrl) __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), ctrl, 0xf, 0xf, false))
+    const bool odd = lane & 1, high = lane & 2;
+    const float lo = (odd ? v[1] : v[0]) + I6_TURN(odd ? v[0] : v[1], 0xb1), hi = (odd ? v[3] : v[2]) + I6_TURN(odd ? v[2] : v[3], 0xb1);      // with the neighbour
+    float x = (high ? hi : lo) + I6_TURN(high ? lo : hi, 0x4e);                                                                               // with the one two further
+    x += I6_TURN(x, 0x124);
+    x += I6_TURN(x, 0x128);
+#undef I6_TURN
+    return x;
+}
+
+// The gradient of log f of a frame t is what decays over it:  what frames i >= t take from the state in front of the chunk, what frames j < t leave behind it, what goes from the one to
+// the other, and M_ij of all pairs j < t <= i within the chunk.  Each of these is added up by itself, of terms that cross the frame and no others.  (Sums over all frames from t on
+// of what decays with c_i, less what decays with -c_j, have the same value, but between frames of very different sizes, and where little is left of anything, what cancels
+// there is far larger than the result.)
+//
+// Of a block of M, as an accumulator: on the diagonal the sums for its sixteen t; below it those of its rows, and of its columns.
+__device__ __forceinline__ void store_crossing(acc_t v, bool diagonal, float* rows, float* columns) {
+    const int lane = threadIdx.x & 63, group = lane >> 4, at = 4 * group;
+    const float sum = (v[0] + v[1]) + (v[2] + v[3]);
+    const float next = __shfl_down(sum, 16), second = __shfl_down(sum, 32), third = __shfl_down(sum, 48);
+    if (diagonal) {
+        float below = (group < 3 ? next : 0.f) + (group < 2 ? second : 0.f) + (group < 1 ? third : 0.f);
+#pragma unroll
+        for (int e = 3; e >= 0; e--) {
+            below += v[e];
+            v[e] = (lane & 15) < at + e ? below : 0.f;
+        }
+    } else if (lane < 16) {
+        columns[lane] = (sum + next) + (second + third);
+    }
+    const float of_rows = sum_of_16(v, lane);
+    if ((lane & 12) == 0) rows[at + (lane & 3)] = of_rows;
+}
+// What crosses frame t = lane of a chunk of M blocks; slot(which, block, 0: rows, 1: columns) is where sixteen of these sums are.
+template <int M, typename F> __device__ __forceinline__ float crossing(F slot, int lane) {
+    const int own = min(lane >> 4, M - 1), r = lane & 15;
+    float rows = 0.f, columns = 0.f, across = 0.f, sum = 0.f;
+#pragma unroll
+    for (int which = 0; which < 2; which++) {
+        sum += slot(which, own * (own + 3) / 2, 0)[r];
+#pragma unroll
+        for (int i = 1; i < M; i++)
+#pragma unroll
+            for (int j = 0; j < i; j++) {
+                const float of_row = slot(which, i * (i + 1) / 2 + j, 0)[r], of_column = slot(which, i * (i + 1) / 2 + j, 1)[r];
+                rows += i == own ? of_row : 0.f;
+                columns += j == own ? of_column : 0.f;
+                across += j < own && own < i ? of_row : 0.f;
+            }
+    }
+#pragma unroll
+    for (int m = 1; m < 16; m *= 2) {
+        const float behind = __shfl_down(rows, m), before = __shfl_up(columns, m);
+        rows += r + m < 16 ? behind : 0.f;
+        columns += r >= m ? before : 0.f;
+        across += __shfl_xor(across, m);
+    }
+    const float in_front = __shfl_up(columns, 1);
+    return (sum + across) + (rows + (r ? in_front : 0.f));
+}
+// And of what begins in front of the chunk or ends behind it: of frame t = lane what it takes from the state in front, what it leaves behind the chunk.
+template <int C> __device__ __forceinline__ float reaching(float takes, float leaves, int lane) {
+#pragma unroll
+    for (int m = 1; m < C; m *= 2) {
+        const float behind = __shfl_down(takes, m), before = __shfl_up(leaves, m);
+        takes += lane + m < C ? behind : 0.f;
+        leaves += lane >= m ? before : 0.f;
+    }
+    const float in_front = __shfl_up(leaves, 1);
+    return takes + (lane ? in_front : 0.f);
+}
+
 // Four values of a row of a float matrix with V columns; zeros behind them.
 __device__ __forceinline__ acc_t load_four(const float* row, int at, int n, bool whole) {
     if (whole) return at < n ? *reinterpret_cast<const acc_t*>(row + at) : acc_t{0.f, 0.f, 0.f, 0.f};
@@ -437,13 +511,12 @@ __device__ __forceinline__ acc_t load_four(const float* row, int at, int n, bool
 
 // 32 bits: all other gradients of a chunk, from the state in front of it, the gradient of that behind it, U and dR:
 //   dq^ = exp(c) dO S0^T + Z K^,   dk^ = exp(c_C - c) U G1^T - w exp(c) dR S0^T + Z^T Q^ + (E + E^T) K^,   Z = D (dO U^T),  E = - w D (dR U^T)
-// (lower triangles, E's without its diagonal).  What decays with c_i is a row's dot product with its query's gradient and the part of its key's that stands on
-// the left; what decays with - c_j that with the other part; so the gradient of c needs no products of its own, nor A and P.
+// (lower triangles, E's without its diagonal);  M_ij = Z_ij q_i.k_j + E_ij k_i.k_j.
 template <int KP>
-__global__ __launch_bounds__(kThreads, 2) void delta_gradients32(Args a) {
+__global__ __launch_bounds__(kThreads, 2) void delta_gradients32(Args a, bool whole_k) {
     constexpr int M = kC / 16, N = KP == 128 ? 2 : 1, kV = 128 + 4, kSquare = kC + 4;
     __shared__ __align__(16) float s_o[kC * kV], s_u[kC * kV], s_r[kC * kV], s_z[kC * kSquare], s_e[kC * kSquare];
-    __shared__ __align__(16) float s_c[kC], s_rest[kC], s_w[kC], s_rk[kC], s_rq[kC], s_start[kC], s_end[kC], s_dots[4][kC][4], s_whole[4], s_gate[kC];
+    __shared__ __align__(16) float s_c[kC], s_rest[kC], s_w[kC], s_rk[kC], s_rq[kC], s_start[kC], s_end[kC], s_dots[4][kC][4], s_whole[4], s_cross[2][M * (M + 1) / 2][2][16];
     const int b = blockIdx.z, h = blockIdx.y, n = blockIdx.x, first = n * kC;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = 4 * (lane >> 4);
     const int len = len_of(a, b), live = min(kC, len - first), rows = min(kC, a.T - first), g = h / (a.H / a.G);
@@ -474,6 +547,8 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients32(Args a) {
 
     const bool whole = a.V % 4 == 0;
     const int cols = (a.V + 15) / 16 * 16;
+    Ahead<KP> in;                        // keys and queries, on their way to where dO and U are first
+    in.fetch(a, b, h, first, len, whole_k);
     {
         constexpr int kPerRow = kThreads / kC;
         const int row = threadIdx.x / kPerRow, j = threadIdx.x % kPerRow;
@@ -513,7 +588,7 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients32(Args a) {
     const Tile<kSquare> tz{s_z}, te{s_e};
     const int blocks = cols / 16;
     acc_t yq[M][N] = {}, yp[M][N] = {}, ym[M][N] = {};
-    float crossed = 0.f;                 // <S1, G1>, what decays with c_C
+    float crossed = 0.f;                 // <S0, G1>, what decays with c_C
     if (col < KP) {
         const float* states = a.states + (head * a.chunks + n) * a.K * a.V;
         const float* ends = a.ends + (head * a.chunks + n) * a.K * a.V;
@@ -541,35 +616,60 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients32(Args a) {
         }
         crossed *= s_start[kC - 1];
     }
-    {
-        int c = 0;
+    acc_t square[2];                     // of Z and E, blocks of the lower triangles in turn
 #pragma unroll
-        for (int i = 0; i < M; i++)
-#pragma unroll
-            for (int j = 0; j <= i; j++)
-#pragma unroll
-                for (int which = 0; which < 2; which++) {
-                    if ((c++ & 3) != wave) continue;
-                    acc_t v = 0.f;
+    for (int y = 0; y < 2; y++) {
+        const int c = wave + 4 * y, which = c & 1, i = block_row(c >> 1), j = (c >> 1) - i * (i + 1) / 2;
+        if (c >= M * (M + 1)) continue;
+        acc_t v = 0.f;
 #pragma unroll 1
-                    for (int x = 0; x < blocks; x++) v = product(which ? tr.rows(i, x) : to.rows(i, x), tu.rows(j, x), v);
-                    const int column = 16 * j + (lane & 15), row = 16 * i + at;
-                    const float cc = s_c[column], rest = s_rest[column], rk = s_rk[column];
+        for (int x = 0; x < blocks; x++) v = product(which ? tr.rows(i, x) : to.rows(i, x), tu.rows(j, x), v);
+        const int column = 16 * j + (lane & 15), row = 16 * i + at;
+        const float cc = s_c[column], rest = s_rest[column], rk = s_rk[column];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int t = row + e;
-                        const float decay = exp_fast((s_c[t] - cc) + (s_rest[t] - rest));
-                        const float by = which ? -s_w[t] * s_rk[t] : s_rq[t];
-                        v[e] = (which ? column < t : column <= t) ? v[e] * decay * rk * by : 0.f;
-                    }
-                    (which ? te : tz).put(i, j, v);
-                }
+        for (int e = 0; e < 4; e++) {
+            const int t = row + e;
+            const float decay = exp_fast((s_c[t] - cc) + (s_rest[t] - rest));
+            const float by = which ? -s_w[t] * s_rk[t] : s_rq[t];
+            v[e] = (which ? column < t : column <= t) ? v[e] * decay * rk * by : 0.f;
+        }
+        (which ? te : tz).put(i, j, v);
+        square[y] = v;
     }
     __syncthreads();
+    const Tile<kV> tk{s_o}, tq{s_u};     // of dO and U nothing is used any more
+    {
+        constexpr int kPerRow = Ahead<KP>::kThreadsPerRow;
+        const int row = threadIdx.x / kPerRow, j = threadIdx.x % kPerRow;
+#pragma unroll
+        for (int i = 0; i < Ahead<KP>::kPer; i++) {
+            const int c = (i * kPerRow + j) * 4;
+            if (c >= KP) continue;
+            *reinterpret_cast<acc_t*>(s_o + row * kV + c) = in.k[i];
+            *reinterpret_cast<acc_t*>(s_u + row * kV + c) = in.q[i];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int y = 0; y < 2; y++) {        // blocks of M
+        const int c = wave + 4 * y, which = c & 1, i = block_row(c >> 1), j = (c >> 1) - i * (i + 1) / 2;
+        if (c >= M * (M + 1)) continue;
+        acc_t v = 0.f;
+#pragma unroll
+        for (int x = 0; x < KP / 16; x++) v = product(which ? tk.rows(i, x) : tq.rows(i, x), tk.rows(j, x), v);
+        store_crossing(square[y] * v, i == j, s_cross[which][c >> 1][0], s_cross[which][c >> 1][1]);
+    }
     acc_t kv[M][N], qv[M][N];
     if (col < KP) {
-        load_columns<N, M>(kv, static_cast<const float*>(a.k) + b * a.k_b + first * a.k_t + g * a.k_g, a.k_t, live, col, a.K);
-        load_columns<N, M>(qv, static_cast<const float*>(a.q) + b * a.q_b + first * a.q_t + g * a.q_g, a.q_t, live, col, a.K);
+#pragma unroll
+        for (int m = 0; m < M; m++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    kv[m][j][e] = s_o[(16 * m + at + e) * kV + col + j];
+                    qv[m][j][e] = s_u[(16 * m + at + e) * kV + col + j];
+                }
 #pragma unroll
         for (int m = 0; m < M; m++) {
             const acc_t start = four(s_start + 16 * m + at), rk = four(s_rk + 16 * m + at);
@@ -579,8 +679,20 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients32(Args a) {
                 yq[m][j] *= by_q;
                 yp[m][j] *= by_p;
                 ym[m][j] *= by_m;
+            }
+            const auto store_dots = [&](int which, acc_t v) {
+                const float sum = sum_of_16(v, lane);
+                if ((lane & 12) == 0) s_dots[wave][16 * m + at + (lane & 3)][which] = sum;
+            };
+            {
+                acc_t takes = 0.f, leaves = 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; e++) crossed = fmaf(ym[m][j][e], kv[m][j][e], crossed);
+                for (int j = 0; j < N; j++) {
+                    takes += qv[m][j] * yq[m][j] + kv[m][j] * yp[m][j];
+                    leaves += kv[m][j] * ym[m][j];
+                }
+                store_dots(2, takes);
+                store_dots(3, leaves);
             }
 #pragma unroll
             for (int x = 0; x <= m; x++) {
@@ -600,31 +712,21 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients32(Args a) {
                     ym[m][j] = product(e, kv[x][j], ym[m][j]);
                 }
             }
+            acc_t of_q = 0.f, of_k = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                float dots[3] = {0.f, 0.f, 0.f};
-#pragma unroll
-                for (int j = 0; j < N; j++) {
-                    dots[0] = fmaf(qv[m][j][e], yq[m][j][e], dots[0]);
-                    dots[1] = fmaf(kv[m][j][e], yp[m][j][e], dots[1]);
-                    dots[2] = fmaf(kv[m][j][e], ym[m][j][e], dots[2]);
-                }
-#pragma unroll
-                for (int i = 0; i < 3; i++) {
-#pragma unroll
-                    for (int x = 1; x < 16; x *= 2) dots[i] += __shfl_xor(dots[i], x);
-                    if ((lane & 15) == 0) s_dots[wave][16 * m + at + e][i] = dots[i];
-                }
+            for (int j = 0; j < N; j++) {
+                yp[m][j] += ym[m][j];
+                of_q += qv[m][j] * yq[m][j];
+                of_k += kv[m][j] * yp[m][j];
             }
+            store_dots(0, of_q);
+            store_dots(1, of_k);
         }
-    } else {
+    } else if ((lane & 15) < 4) {
 #pragma unroll
         for (int m = 0; m < M; m++)
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-#pragma unroll
-                for (int i = 0; i < 3; i++)
-                    if ((lane & 15) == 0) s_dots[wave][16 * m + at + e][i] = 0.f;
+            for (int e = 0; e < 4; e++) s_dots[wave][16 * m + at + e][lane & 15] = 0.f;
     }
     crossed = wave_sum(crossed);
     if (lane == 0) s_whole[wave] = crossed;
@@ -637,28 +739,20 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients32(Args a) {
             for (int e = 0; e < 4; e++) {
                 const int row = 16 * m + at + e;
                 const float rq = s_rq[row], rk = s_rk[row];
-                const float q_off = rq * rq * dot(row, 0), k_off = rk * rk * (dot(row, 1) + dot(row, 2));
+                const float q_off = rq * rq * dot(row, 0), k_off = rk * rk * dot(row, 1);
 #pragma unroll
                 for (int j = 0; j < N; j++) {
                     yq[m][j][e] = yq[m][j][e] - qv[m][j][e] * q_off;
-                    yp[m][j][e] = (yp[m][j][e] + ym[m][j][e]) - kv[m][j][e] * k_off;
+                    yp[m][j][e] = yp[m][j][e] - kv[m][j][e] * k_off;
                 }
             }
         store(yq, false);
         store(yp, true);
     }
     if (wave == 0) {
-        // of log f: what decays over the frame, a sum over the frames from it to the chunk's end
-        float d = 0.f;
-        if (lane < kC) {
-            d = (dot(lane, 0) + dot(lane, 1)) - dot(lane, 2);
-            if (lane == kC - 1) d += (s_whole[0] + s_whole[1]) + (s_whole[2] + s_whole[3]);
-        }
-#pragma unroll
-        for (int m = 1; m < kC; m *= 2) {
-            const float behind = __shfl_down(d, m);
-            if (lane + m < kC) d += behind;
-        }
+        const int t = lane & (kC - 1);
+        const float whole_chunk = (s_whole[0] + s_whole[1]) + (s_whole[2] + s_whole[3]);
+        const float d = (reaching<kC>(dot(t, 2), dot(t, 3), t) + whole_chunk) + crossing<M>([&](int which, int block, int part) { return s_cross[which][block][part]; }, t);
         if (lane < rows) {
             const float gate = lane < live ? static_cast<const float*>(a.gate)[b * a.gate_b + (first + lane) * a.gate_t + h * a.gate_h] : 0.f;
             d_gate[lane * a.H] = lane < live ? d * sigmoid(-gate) : 0.f;
@@ -829,7 +923,7 @@ template <int KP> void run_backward(const Call& c, hipStream_t s, float) {
     }
     if (wide(c)) delta_backward32<KP, 8, false><<<dim3(c.a.H, c.a.B, k.segments), dim3(512), 0, s>>>(c.a, k, blocks, c.whole, c.whole_v);
     else delta_backward32<KP, 4, false><<<dim3(c.a.H * ceil_div(c.a.V, 64), c.a.B, k.segments), dim3(256), 0, s>>>(c.a, k, blocks, c.whole, c.whole_v);
-    delta_gradients32<KP><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a);
+    delta_gradients32<KP><<<dim3(c.a.chunks, c.a.H, c.a.B), dim3(kThreads), 0, s>>>(c.a, c.whole);
 }
 template <int KP> void run_backward(const Call& c, hipStream_t s, bf16) {
     const Args16& k = c.k16;

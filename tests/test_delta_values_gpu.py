@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests.test_delta_gpu import DTYPES, NAMES, problem
+from tests.test_delta_gpu import DTYPES, NAMES, check, expected, problem, run
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +52,26 @@ def test_a_gate_that_is_no_number(T, K, V, t, dtype):
     o[1, t:, 0] = want[0][1, t:, 0]
     last[1, 0] = want[1][1, 0]
     assert torch.equal(o, want[0]) and torch.equal(last, want[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,K,V", [(40, 16, 16), (64, 64, 40), (130, 128, 128), (150, 32, 100)])
+def test_gates_of_frames_in_front_of_a_far_larger_one(T, K, V, dtype):
+    """Their gradients are sums of what decays over them, none of which a later frame's value enters: as right as without it.  (The incoming gradients do not depend on it.)"""
+    p = problem(2, T, 2, 1, K, V, dtype, lens="all")
+    t = T - 11
+    p["v"][:, t] *= 2.0 ** 20
+    want, got = expected(p), run(p)
+    n = slice(0, t + 1)
+    check(p, {"gate": got["gate"][:, n]}, {"gate": want["gate"][:, n]})
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gate", [-3.0, -10.0, -20.0, -60.0])
+@pytest.mark.parametrize("K,V", [(16, 16), (128, 128)])
+def test_gates_that_leave_little(gate, K, V, dtype):
+    """The gradients of gates are in proportion to what is left, e^gate of the other sums, and right in that proportion."""
+    p = problem(2, 100, 2, 1, K, V, dtype, lens="all")
+    p["gate"][:] = gate
+    p["gate"][:, ::7] += 2.0
+    check(p, run(p), expected(p))
