@@ -820,9 +820,9 @@ int padded_keys(int K) { return K <= 32 ? 32 : (K <= 64 ? 64 : 128); }
 
 // Where the parts of a call's memory are.
 struct Places {
-    size_t rows, states, states_factor, u, u_factor, blocks, kept;   // kept; rows and blocks are in the forward workspace where nothing is
+    size_t rows, states, u, blocks, kept;                            // kept; rows and blocks are in the forward workspace where nothing is
     size_t packed, forward;                                          // the forward workspace
-    size_t ends, ends_factor, dr, dr_factor, d_q, d_k, back_packed, back;       // the backward workspace
+    size_t ends, dr, d_q, d_k, back_packed, back;                    // the backward workspace
     size_t split, turns;                                             // of the forward workspace, and turns behind split
     size_t back_split;
     int pairs, segments = 1, per;
@@ -831,22 +831,18 @@ struct Places {
         const int C = x16 ? kC16 : kC, KP = padded_keys(p.K);
         const size_t n = (size_t)p.B * p.H * ceil_div(p.T, C);
         pairs = p.V > 64 ? 4 : 2;
-        const size_t s = align256(x16 ? n * KP * pairs * 32 * sizeof(f16) : n * p.K * p.V * sizeof(float)), f = x16 ? align256(n * 2 * pairs * sizeof(float)) : 0;
-        const size_t r = align256(x16 ? n * C * pairs * 32 * sizeof(f16) : n * C * p.V * sizeof(float));
+        const size_t s = align256(x16 ? n * (KP / 16) * pairs * kKept * sizeof(bf16) : n * p.K * p.V * sizeof(float));
+        const size_t r = align256(x16 ? n * (C / 16) * pairs * kKept * sizeof(bf16) : n * C * p.V * sizeof(float));
         const size_t heads = p.H > p.G ? align256((size_t)p.B * p.T * p.H * p.K * sizeof(float)) : 0;
         rows = 0;
         states = align256(n * C * sizeof(Rows));
-        states_factor = states + s;
-        u = states_factor + f;
-        u_factor = u + r;
+        u = states + s;
         const size_t block_bytes = align256(x16 ? n * chunk_blocks(train) * sizeof(bf16) : n * kBlocks32 * 256 * sizeof(float));
-        blocks = train ? u_factor + f : states;
+        blocks = train ? u + r : states;
         kept = blocks + block_bytes;
         ends = 0;
-        ends_factor = s;
-        dr = ends_factor + f;
-        dr_factor = dr + r;
-        d_q = dr_factor + f;
+        dr = s;
+        d_q = dr + r;
         d_k = d_q + heads;
         // whatever their strides are: those of the incoming gradient are not known before it is there
         const size_t k = packed_bytes(p, p.G, p.K), v = packed_bytes(p, p.H, p.V);
@@ -1000,8 +996,8 @@ Call call_of(const i6delta_problem& p, const Places& at, void* kept) {
         c.blocks = reinterpret_cast<bf16*>(base + at.blocks);
         c.a.states = reinterpret_cast<float*>(base + at.states);
         c.a.u = reinterpret_cast<float*>(base + at.u);
-        c.k16.states = {reinterpret_cast<f16*>(base + at.states), reinterpret_cast<float*>(base + at.states_factor)};
-        c.k16.u = {reinterpret_cast<f16*>(base + at.u), reinterpret_cast<float*>(base + at.u_factor)};
+        c.k16.states = reinterpret_cast<Kept16>(base + at.states);
+        c.k16.u = reinterpret_cast<Kept16>(base + at.u);
     }
     return c;
 }
@@ -1064,8 +1060,8 @@ int i6delta_backward(const i6delta_problem* p, const void* grad_o, int64_t grad_
     char* base = static_cast<char*>(workspace);
     a.ends = reinterpret_cast<float*>(base + at.ends);
     a.dr = reinterpret_cast<float*>(base + at.dr);
-    c.k16.left = {reinterpret_cast<f16*>(base + at.ends), reinterpret_cast<float*>(base + at.ends_factor)};
-    c.k16.dr = {reinterpret_cast<f16*>(base + at.dr), reinterpret_cast<float*>(base + at.dr_factor)};
+    c.k16.left = reinterpret_cast<Kept16>(base + at.ends);
+    c.k16.dr = reinterpret_cast<Kept16>(base + at.dr);
     c.k16.ends = reinterpret_cast<float*>(base + at.back_split);
     c.k16.turns = reinterpret_cast<float*>(base + at.back_split + at.turns);
     if (p->dtype == I6TRAIN_BF16) {

@@ -13,7 +13,8 @@
  *   q, k [B, T, G, K], v [B, T, H, V], gate, beta [B, T, H], all of `dtype`, with strides (q, k, v: the last one is 1); H is a multiple
  *   of G, and head h has keys and queries h / (H / G).  initial, last float [B, H, K, V] contiguous;  o [B, T, H, V] contiguous, of `dtype`.
  *
- * States, sums and decays are held in 32 bits.  Sizes: B and H up to 65 535, K and V up to 128, B H ceil(T / 32) up to 2^23; larger ones
+ * States, sums and decays are held in 32 bits.  Of bfloat16 inputs, products take their 32-bit operands in three bfloat16 parts (24 bits) where results are of 32 bits and in two (16 bits) where
+ * they are of bfloat16, and a forward call for training keeps states and written rows in two such parts for the gradients.  Sums of squares of q and of k have to be below 2^127.  Sizes: B and H up to 65 535, K and V up to 128, B H ceil(T / 32) up to 2^23; larger ones
  * are I6TRAIN_ERR_TOO_LARGE.
  *
  * A forward call for training leaves in `kept` what i6delta_backward needs (null otherwise).  Gradients: grad_o (strided, last stride 1, `dtype`)

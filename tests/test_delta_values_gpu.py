@@ -75,3 +75,38 @@ def test_gates_that_leave_little(gate, K, V, dtype):
     p["gate"][:] = gate
     p["gate"][:, ::7] += 2.0
     check(p, run(p), expected(p))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,K,V", [(40, 16, 16), (100, 64, 64), (130, 128, 128), (70, 32, 100), (1300, 64, 40)])
+def test_columns_of_very_different_sizes(T, K, V, dtype):
+    """Values times powers of two, incoming gradients divided by them: every product of the one with the other is what it was, and so is every result, to the last bit."""
+    p = problem(2, T, 2, 1, K, V, dtype, lens="all")
+    plain = run(p)
+    if T < 1000:
+        check(p, plain, expected(p))
+    sizes = torch.tensor([2.0 ** i for i in torch.randint(-20, 41, (V,), generator=torch.Generator().manual_seed(5)).tolist()], device="cuda")    # (the card's powers are not exact)
+    moved = dict(p, v=(p["v"].float() * sizes).to(dtype), initial=p["initial"] * sizes, grad_o=(p["grad_o"].float() / sizes).to(dtype), grad_last=p["grad_last"] / sizes)
+    got = run(moved)
+    for n in ("q", "k", "gate", "beta"):
+        assert torch.equal(got[n], plain[n]), n
+    for n, by in (("o", 1 / sizes), ("last", 1 / sizes), ("v", sizes), ("initial", sizes)):
+        assert torch.equal((got[n].float() * by).to(got[n].dtype), plain[n]), n
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,K,V", [(40, 16, 16), (100, 64, 64), (130, 128, 128), (70, 32, 100)])
+def test_frames_of_very_different_sizes(T, K, V, dtype):
+    """What a far larger value or incoming gradient does not enter is as right as without it: results of frames in front of the value, gradients of frames behind the incoming one."""
+    t = T - 21
+    p = problem(2, T, 2, 1, K, V, dtype, lens="all")
+    p["v"][:, t] *= 2.0 ** 40
+    want, got = expected(p), run(p)
+    for n in ("o", "q", "k", "beta", "gate"):
+        check(p, {n: got[n][:, :t]}, {n: want[n][:, :t]})
+    check(p, {"v": got["v"]}, {"v": want["v"]})
+    p = problem(2, T, 2, 1, K, V, dtype, lens="all")
+    p["grad_o"][:, t] *= 2.0 ** 40
+    want, got = expected(p), run(p)
+    for n in ("q", "k", "v", "beta", "gate"):
+        check(p, {n: got[n][:, t + 1:]}, {n: want[n][:, t + 1:]})
