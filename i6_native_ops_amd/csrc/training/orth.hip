@@ -642,11 +642,13 @@ struct Places {
 
 int checked(const i6orth_tensor* tensors, int n, int dtype) {
     if (n < 0 || (n > 0 && !tensors) || !valid_dtype(dtype)) return I6TRAIN_ERR_INVALID_ARGUMENT;
+    const i6orth_tensor* first = nullptr;        // of those that have values; the others' pointers mean nothing
     for (int i = 0; i < n; i++) {
         const i6orth_tensor& t = tensors[i];
         if (t.rows < 0 || t.cols < 0) return I6TRAIN_ERR_INVALID_ARGUMENT;
         if (t.rows == 0 || t.cols == 0) continue;
-        if (!t.update || !t.result || (t.momentum == nullptr) != (tensors[0].momentum == nullptr)) return I6TRAIN_ERR_INVALID_ARGUMENT;
+        if (!first) first = &t;
+        if (!t.update || !t.result || (t.momentum == nullptr) != (first->momentum == nullptr)) return I6TRAIN_ERR_INVALID_ARGUMENT;
         if (t.rows > 32768 || t.cols > 32768) return I6TRAIN_ERR_TOO_LARGE;
     }
     return I6TRAIN_OK;

@@ -24,7 +24,7 @@ extern "C" {
 typedef struct {
     const void* update;      /* u, or g where there is a momentum: [rows][cols] contiguous, dtype */
     void* result;            /* X, or p, which is read too: [rows][cols] contiguous, dtype */
-    float* momentum;         /* m [rows][cols], or null: for all tensors of a call or none */
+    float* momentum;         /* m [rows][cols], or null: for all tensors of a call that have values, or none */
     int rows, cols;          /* up to 2^15 each; 0 is allowed */
     float keep, rate;
 } i6orth_tensor;

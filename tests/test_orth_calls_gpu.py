@@ -1,0 +1,36 @@
+"""Muon and orthogonalised updates as calls go: matrices without values, many at once, captured."""
+import pytest
+import torch
+
+from tests.test_orth_gpu import DTYPES, check, expected, matrix
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("at", [0, 1, 2])
+def test_matrices_without_values_among_others(at, dtype):
+    """As if they were not there, first, in the middle or last; a call that is refused raises no version."""
+    from i6_native_ops_amd.training import Muon, muon_step
+    shapes = [(64, 40), (30, 90)]
+    shapes.insert(at, (0, 8))
+    params = [matrix(r, c, dtype, seed=i, size=0.05) if r else torch.zeros((r, c), dtype=dtype, device="cuda") for i, (r, c) in enumerate(shapes)]
+    grads = [matrix(r, c, dtype, seed=10 + i) if r else torch.zeros_like(p) for i, ((r, c), p) in enumerate(zip(shapes, params))]
+    others = [i for i in range(3) if i != at]
+    alone = [p.clone() for p in params]
+    moved = [torch.zeros(s, device="cuda") for s in shapes]
+    muon_step([alone[i] for i in others], [grads[i] for i in others], [moved[i] for i in others], lr=0.02)
+    momenta = [torch.zeros(s, device="cuda") for s in shapes]
+    muon_step(params, grads, momenta, lr=0.02)
+    for p, q, m, n in zip(params, alone, momenta, moved):
+        assert torch.equal(p, q) and torch.equal(m, n)
+    weights = [torch.nn.Parameter(p.clone()) for p in params]
+    for w, g in zip(weights, grads):
+        w.grad = g
+    Muon(weights, lr=0.02).step()
+    versions = [p._version for p in params]
+    with pytest.raises(RuntimeError, match="momentum must be"):
+        muon_step(params, grads, momenta, lr=0.02, momentum=1.0)
+    with pytest.raises(RuntimeError, match="steps must be"):
+        muon_step(params, grads, momenta, lr=0.02, steps=-1)
+    assert versions == [p._version for p in params]
