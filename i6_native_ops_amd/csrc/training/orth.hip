@@ -27,7 +27,9 @@ using acc_t = float __attribute__((ext_vector_type(4)));
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr double kLeastNorm = 1e-7;
 constexpr float kScaleX = 0x1p15f, kScaleA = 0x1p15f, kScaleB = 0x1p14f;
-constexpr int kMaxTensors = 40;          // x 96 bytes: the arguments of a kernel may have 4 KB
+constexpr int kMaxTensors = 34;          // x 112 bytes: the arguments of a kernel may have 4 KB
+// Of a table's workspace, unless one matrix alone has more.  More at once is no faster: of 4096 x 2048 in 16 bits 24 matrices take 19.3 ms, 12 of them 9.7; of 4096 x 11008 24 take 185, 6 of them 46.
+constexpr size_t kTableBytes = (size_t)4 << 30;
 constexpr int kThreads = 256;
 constexpr int kRowPad = 64;               // of columns: what the products run over
 constexpr int kCus = 256;
@@ -48,7 +50,7 @@ struct Matrix {
 };
 static_assert(sizeof(Matrix) <= 112, "kernel arguments");
 struct Table {
-    Matrix t[kMaxTensors - 6];
+    Matrix t[kMaxTensors];
     int count, groups;
     int quarters;                        // of the tiles of 256 x 256 from this one on; -1: tiles of the kernel's own size
     int parts;                           // of the columns that a product runs over, where tiles are few
@@ -769,35 +771,35 @@ template <typename T> int run(Table& tab, bool small, int iterations, hipStream_
 // What all matrices of a table share.
 size_t shared_bytes(const Table& tab) { return std::max(parts_of(tab, true, true).bytes, std::max(parts_of(tab, false, true).bytes, parts_of(tab, false, false).bytes)); }
 
-// f(table, small) for the matrices of a call, as many at once as a table has room for; `all` receives the bytes of what they have of their own.  Which way a matrix goes
-// depends on it alone.
-template <typename F> int in_tables(const i6orth_tensor* tensors, int n_tensors, int iterations, char* workspace, size_t* all, F f) {
+// f(table, small, bytes) for the matrices of a call, as many at once as a table has room for and kTableBytes hold; bytes are those of the workspace that they have of their own, from its
+// start on: one table follows the other on the stream, and small matrices need none.  Which way a matrix goes depends on it alone.
+template <typename F> int in_tables(const i6orth_tensor* tensors, int n_tensors, int iterations, char* workspace, F f) {
     Table tab{};
     for (const bool small : {true, false}) {
-        char* at = workspace;
-        *all = 0;
+        size_t own = 0;
         const auto flush = [&]() {
             if (tab.count == 0) return I6TRAIN_OK;
-            const int rc = f(tab, small);
+            const int rc = f(tab, small, own);
             tab.count = 0;
+            own = 0;
             return rc;
         };
         for (int i = 0; i < n_tensors; i++) {
             const i6orth_tensor& t = tensors[i];
             if (t.rows == 0 || t.cols == 0) continue;
             const Places p(t);
-            if (small == (iterations > 0 && is_small(p.n, p.m))) {
-                if (tab.count == (int)(sizeof(tab.t) / sizeof(tab.t[0]))) I6TRAIN_TRY(flush());
-                Matrix& m = tab.t[tab.count++];
-                m.update = t.update; m.result = t.result; m.momentum = t.momentum;
-                m.x = reinterpret_cast<f16*>(at + p.x); m.xt = reinterpret_cast<f16*>(at + p.xt); m.xt_next = reinterpret_cast<f16*>(at + p.xt_next);
-                m.a = reinterpret_cast<f16*>(at + p.a); m.b = reinterpret_cast<f16*>(at + p.b);
-                m.parts = reinterpret_cast<double*>(at + p.parts);
-                m.rows = t.rows; m.cols = t.cols; m.n = p.n; m.m = p.m; m.np = p.np; m.mp = p.mp;
-                m.keep = t.keep; m.rate = t.rate; m.parts_n = p.parts_n;
-            }
-            at += p.all;
-            *all += p.all;
+            if (small != (iterations > 0 && is_small(p.n, p.m))) continue;
+            const size_t more = small ? 0 : p.all;
+            if (tab.count == kMaxTensors || (tab.count > 0 && own + more > kTableBytes)) I6TRAIN_TRY(flush());
+            char* at = workspace + own;
+            Matrix& m = tab.t[tab.count++];
+            m.update = t.update; m.result = t.result; m.momentum = t.momentum;
+            m.x = reinterpret_cast<f16*>(at + p.x); m.xt = reinterpret_cast<f16*>(at + p.xt); m.xt_next = reinterpret_cast<f16*>(at + p.xt_next);
+            m.a = reinterpret_cast<f16*>(at + p.a); m.b = reinterpret_cast<f16*>(at + p.b);
+            m.parts = reinterpret_cast<double*>(at + p.parts);
+            m.rows = t.rows; m.cols = t.cols; m.n = p.n; m.m = p.m; m.np = p.np; m.mp = p.mp;
+            m.keep = t.keep; m.rate = t.rate; m.parts_n = p.parts_n;
+            own += more;
         }
         I6TRAIN_TRY(flush());
     }
@@ -814,28 +816,26 @@ extern "C" {
 int i6orth_workspace_size(const i6orth_tensor* tensors, int n_tensors, int dtype, size_t* bytes) {
     I6TRAIN_TRY(checked(tensors, n_tensors, dtype));
     if (!bytes) return I6TRAIN_ERR_INVALID_ARGUMENT;
-    size_t all = 0, shared = 0;
-    I6TRAIN_TRY(in_tables(tensors, n_tensors, 1, nullptr, &all, [&](Table& tab, bool small) {
-        if (!small) shared = std::max(shared, shared_bytes(tab));
-        return I6TRAIN_OK;
-    }));
-    *bytes = all + align256(shared);
+    size_t most = 0;
+    for (const int iterations : {0, 1})          // without iterations small matrices go the others' way
+        I6TRAIN_TRY(in_tables(tensors, n_tensors, iterations, nullptr, [&](Table& tab, bool small, size_t own) {
+            most = std::max(most, own + (small || iterations == 0 ? 0 : align256(shared_bytes(tab))));
+            return I6TRAIN_OK;
+        }));
+    *bytes = most;
     return I6TRAIN_OK;
 }
 
 int i6orth_step(const i6orth_tensor* tensors, int n_tensors, int dtype, int iterations, double mu, int nesterov, void* workspace, size_t workspace_bytes, void* stream) {
-    size_t need = 0, all = 0;
+    size_t need = 0;
     I6TRAIN_TRY(i6orth_workspace_size(tensors, n_tensors, dtype, &need));
     if (iterations < 0 || !(mu >= 0 && mu < 1)) return I6TRAIN_ERR_INVALID_ARGUMENT;
     if (need == 0) return I6TRAIN_OK;
     if (!workspace || workspace_bytes < need) return I6TRAIN_ERR_WORKSPACE_TOO_SMALL;
-    for (int i = 0; i < n_tensors; i++)
-        if (tensors[i].rows > 0 && tensors[i].cols > 0) all += Places(tensors[i]).all;
-    size_t so_far = 0;
-    return in_tables(tensors, n_tensors, iterations, static_cast<char*>(workspace), &so_far, [&](Table& tab, bool small) {
+    return in_tables(tensors, n_tensors, iterations, static_cast<char*>(workspace), [&](Table& tab, bool small, size_t own) {
         tab.mu = (float)mu;
         tab.nesterov = nesterov;
-        tab.partial = reinterpret_cast<acc_t*>(static_cast<char*>(workspace) + all);
+        tab.partial = reinterpret_cast<acc_t*>(static_cast<char*>(workspace) + own);
         return dtype == I6TRAIN_BF16 ? run<bf16>(tab, small, iterations, (hipStream_t)stream) : run<float>(tab, small, iterations, (hipStream_t)stream);
     });
 }

@@ -29,7 +29,8 @@ typedef struct {
     float keep, rate;
 } i6orth_tensor;
 
-/* `tensors` is a host array; `workspace` has i6orth_workspace_size bytes. */
+/* `tensors` is a host array; `workspace` has i6orth_workspace_size bytes.  That is 12 to 20 bytes a value (rows and columns rounded up to 64) of as many matrices as are worked on at the same time: up to 34 and 4 GB of it, or one matrix that
+ * has more alone, and up to 32 MB that they share.  Other matrices of the call follow in the same memory. */
 int i6orth_workspace_size(const i6orth_tensor* tensors, int n_tensors, int dtype, size_t* bytes);
 int i6orth_step(const i6orth_tensor* tensors, int n_tensors, int dtype, int iterations, double mu, int nesterov, void* workspace,
                 size_t workspace_bytes, void* stream);

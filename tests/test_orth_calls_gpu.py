@@ -34,3 +34,26 @@ def test_matrices_without_values_among_others(at, dtype):
     with pytest.raises(RuntimeError, match="steps must be"):
         muon_step(params, grads, momenta, lr=0.02, steps=-1)
     assert versions == [p._version for p in params]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("count,rows,cols", [(36, 130, 300), (70, 140, 136), (34, 200, 129), (35, 129, 200), (5, 257, 513), (3, 513, 511)])
+def test_every_matrix_of_calls_that_take_several_launches(count, rows, cols, dtype):
+    """Matrices of one launch follow those of another in the same memory.  All of them, and again."""
+    from i6_native_ops_amd.training import orthogonalize
+    updates = [matrix(rows + i % 3, cols, dtype, seed=i) for i in range(count)]
+    got, again = orthogonalize(updates), orthogonalize(updates)
+    for u, x, y in zip(updates, got, again):
+        assert torch.equal(x, y)
+        check(x, expected(u), max(u.shape))
+
+
+@pytest.mark.parametrize("steps", [0, 1, 5])
+def test_many_small_matrices_with_and_without_iterations(steps):
+    from i6_native_ops_amd.training import orthogonalize
+    sizes = [(20 + i % 9, 30 + i % 7) for i in range(80)] + [(150, 170), (0, 3)]
+    updates = [matrix(r, c, torch.float32, seed=i) if r else torch.zeros((r, c), device="cuda") for i, (r, c) in enumerate(sizes)]
+    for u, x in zip(updates, orthogonalize(updates, steps=steps)):
+        assert x.shape == u.shape
+        if u.numel():
+            check(x, expected(u, steps), max(u.shape))

@@ -34,3 +34,25 @@ def test_matrices_without_values_say_nothing_about_momenta(sizes, order):
     without = [matrix(5, 9), matrix(300, 200)]
     assert sizes(*without[:at], Orth(rows=0, cols=5, momentum=256), *without[at:])[0] == 0
     assert sizes(empty, matrix(5, 9), matrix(5, 9, 256))[0] == INVALID
+
+
+def test_workspace_is_that_of_the_matrices_at_work(sizes):
+    """Three times the matrix (as it is and twice turned) and two square ones, 4 bytes a value each, sides rounded up to 64: for the matrices of one launch, not for all of the call."""
+    def own(rows, cols):
+        up = lambda n: (n + 63) // 64 * 64  # noqa: E731
+        n, m = min(rows, cols), max(rows, cols)
+        return 4 * (n * up(m) + 2 * m * up(n) + 2 * n * up(n)) + 8 * 256 + 8 * 256     # and sums; each part rounded up to 256 bytes
+
+    shared = 64 << 20
+    for rows, cols in [(4096, 11008), (300, 200), (2048, 1024)]:
+        one = sizes(matrix(rows, cols))[1]
+        assert 0.99 * own(rows, cols) <= one <= own(rows, cols) + shared
+        for count in (2, 34, 35, 200):
+            need = sizes(*[matrix(rows, cols)] * count)[1]
+            at_work = min(count, 34, max(1, (4 << 30) // own(rows, cols)))
+            assert 0.99 * at_work * own(rows, cols) <= need <= at_work * own(rows, cols) + shared, (rows, cols, count)
+    # matrices that a workgroup does alone need none but where they go the others' way, without iterations
+    assert sizes(*[matrix(64, 64)] * 1000)[1] <= 34 * own(64, 64) + shared
+    assert sizes(*[matrix(64, 64)] * 1000)[1] == sizes(*[matrix(64, 64)] * 34)[1]
+    # one larger than 4 GB is worked on alone
+    assert sizes(matrix(20000, 20000), matrix(20000, 20000), matrix(5, 5))[1] <= own(20000, 20000) + shared
