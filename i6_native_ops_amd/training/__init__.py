@@ -263,7 +263,8 @@ def muon_step(
 
 
 class Muon(torch.optim.Optimizer):
-    """Muon on ``muon_step``: averaged gradients of matrices, orthogonalised.  For the weights between layers; biases, gains and output layers are for ``AdamW``."""
+    """Muon on ``muon_step``: averaged gradients of matrices, orthogonalised.  For the weights between layers; biases, gains and output layers are for ``AdamW``.  ``step`` can be
+    captured into a graph once every parameter has had one, or its state has been loaded."""
 
     def __init__(self, params: Iterable, lr: float = 1e-3, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.1, steps: int = 5,
                  adjust_lr: str = "original"):
@@ -278,6 +279,7 @@ class Muon(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
+        capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -291,6 +293,8 @@ class Muon(torch.optim.Optimizer):
                     raise RuntimeError("Muon does not take sparse gradients")
                 state = self.state[p]
                 if not state:
+                    if capturing:
+                        raise RuntimeError("Muon.step makes the averages of a parameter's gradients in its first step, which cannot be captured: every replay would begin them anew")
                     state["momentum"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 calls.setdefault((p.device, p.dtype), []).append((p, state["momentum"]))
             for items in calls.values():

@@ -57,3 +57,29 @@ def test_many_small_matrices_with_and_without_iterations(steps):
         assert x.shape == u.shape
         if u.numel():
             check(x, expected(u, steps), max(u.shape))
+
+
+def test_a_captured_optimiser_goes_on_with_its_averages():
+    """The step that makes them is refused under capture (each replay would begin them anew); behind it replays are the steps that eager calls are."""
+    from i6_native_ops_amd.training import Muon
+    weights = [torch.nn.Parameter(matrix(60, 40, torch.float32, seed=1, size=0.05)) for _ in range(2)]
+    for w in weights:
+        w.grad = matrix(60, 40, torch.float32, seed=2)
+    captured, eager = Muon(weights[:1], lr=0.02), Muon(weights[1:], lr=0.02)
+    graph = torch.cuda.CUDAGraph()
+    before = weights[0].detach().clone()
+    with pytest.raises(RuntimeError, match="first step"):
+        with torch.cuda.graph(graph):
+            captured.step()
+    assert torch.equal(weights[0], before)
+    captured.step(), eager.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured.step()
+    for step in range(3):
+        for w in weights:
+            w.grad.copy_(matrix(60, 40, torch.float32, seed=3 + step))
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        assert torch.equal(weights[0], weights[1]) and torch.equal(captured.state[weights[0]]["momentum"], eager.state[weights[1]]["momentum"]), step
