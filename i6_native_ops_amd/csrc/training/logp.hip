@@ -452,7 +452,7 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_backward
     G::meet();
     for (int i = thread; i <= k; i += kThreads) {
         const int c = classes[i];
-        if (c < 0) continue;
+        if (c < 0 || c >= a.F) continue; // (none: a caller's alternatives may be anything)
         float more = 0.f;                // a target may be an alternative; then both write the same
         for (int j = 0; j <= k; j++) more += classes[j] == c ? mores[j] : 0.f;
         // Where p is next to 1 with 1 - p from log p, so that a confident frame's difference keeps its relative precision; below one half more - p (...) is one rounding and

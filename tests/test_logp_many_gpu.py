@@ -55,3 +55,32 @@ def test_many_frames_that_are_no_distribution(dtype, F):
     keep = torch.ones(4100, dtype=torch.bool, device="cuda")
     keep[bad] = False
     check({n: x[:, keep] for n, x in got.items()}, {n: (w[:, keep], b[:, keep] if b is not None else None) for n, (w, b) in want.items()})
+
+
+def test_alternatives_that_are_no_classes_are_passed_over():
+    """At the C level a caller may hand over any alternatives: those outside of the row's classes count for nothing, and nothing is written for them."""
+    import ctypes
+
+    import i6_native_ops_amd.training as training
+    from tests.test_more_training_cpu import Logp
+    lib = ctypes.CDLL(training.__file__.replace("__init__.py", "libi6train.so"))
+    B, T, F, k = 1, 3, 37, 4
+    logits, targets, lens, _, grads = problem(B, T, F, k, FEW, lens=[T])
+    room = torch.full((3, T, F), 5.0, device="cuda")                 # memory of its own on both sides
+    floats = [torch.empty(n, device="cuda") for n in (B * T, B * T, B * T * k, B * T * 4)]
+    classes = torch.empty(B * T * k, dtype=torch.int32, device="cuda")
+    at = lambda x: ctypes.c_void_p(x.data_ptr())  # noqa: E731
+    p = Logp(B=B, T=T, F=F, k=k, dtype=0, logits=logits.data_ptr(), targets=targets.data_ptr(), lens=lens.data_ptr(), l_b=T * F, l_t=F, t_b=T, t_t=1)
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert lib.i6logp_forward(ctypes.byref(p), at(floats[0]), at(floats[1]), at(floats[2]), at(classes), at(floats[3]), stream) == 0
+    gt = grads[2].clone()
+    classes.view(T, k)[:, 1], classes.view(T, k)[:, 3] = F, -7       # both would be within `room`
+    assert lib.i6logp_backward(ctypes.byref(p), at(floats[3]), at(classes), None, None, at(gt), at(room[1]), stream) == 0
+    torch.cuda.synchronize()
+    assert (room[0] == 5.0).all() and (room[2] == 5.0).all()
+    # what comes in for them is in the frame's sum, but no class has it
+    z = logits[0].double()
+    direct = torch.zeros_like(z)
+    direct.scatter_add_(1, classes.view(T, k)[:, ::2].long(), gt[0, :, ::2].double())
+    want = direct - torch.softmax(z, -1) * gt[0].double().sum(-1, keepdim=True)
+    assert float((room[1].double() - want).abs().max()) <= 2.0 ** -20 * float(gt.abs().sum(-1).max())
