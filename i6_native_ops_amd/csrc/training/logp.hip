@@ -5,14 +5,18 @@
 // of e = exp(z - m) and e (z - m), the terms that are equal to the largest apart from the others, so that log p of a confident frame's class, log1p of the others'
 // sum, and its entropy keep their relative precision; and the alternatives.
 //
-// Alternatives: the k-th largest of a wave's 64 lanes' largest scores is a bound that at least k scores of the row reach, and that few others do.  What reaches the
+// Alternatives: the k-th largest of a wave's 64 lanes' largest scores is a bound that at least k scores of the row reach.  What reaches the
 // largest such bound of the row's waves is a candidate; candidates go to LDS, and a candidate's place is the number of those before it.  Where more than
-// kCandidates scores reach the bound (masked, equal or ordered scores), the k-th largest score itself is found bit by bit, and then the index up to
-// which scores equal to it count: what is left are k candidates.
+// kCandidates scores reach the bound, the k-th largest score itself is found bit by bit, and then the index up to
+// which scores equal to it count: what is left are k candidates.  That is so for masked, equal and ordered scores, and also for any with many alternatives, as the bound is one
+// wave's and more scores reach it the more waves a row has: from about 60 alternatives on where a row is one wave's, 45 at 12 001 classes, 30 at 20 000, 20 at 30 000 and more.  It
+// takes some forty passes over the row: 4096 rows of 12 001 in 32 bits 43 us with 8 alternatives, 82 with 32 and 1000 with 48, of 30 000 257 with 16 and 2700 with 24.
 //
-// 28 900 frames of 12 001 classes in 32 bits: 250 us, 5.5 TB/s, and all of the time vector instructions are issued, too.  Training on 44 800 frames of 5001 in 16 bits: 150 us
-// forward (3 TB/s; ten instructions and an exponential a score) and 198 backward (4.8 TB/s with what is written).  The next frame of 64 streams: 15 us, most of which two barriers,
-// the reductions and a row's first bytes take.
+// Backward, what every class has of the frame's sums is written, and then the classes that something comes in for are written again, by their numbers.
+//
+// 28 900 frames of 12 001 classes in 32 bits: 250 us, 5.5 TB/s, and all of the time vector instructions are issued, too.  Training on 44 800 frames of 5001 in 16 bits: 151 us
+// forward (3 TB/s; ten instructions and an exponential a score) and 177 backward (5.4 TB/s with what is written).  The next frame of 64 streams: 15 us, most of which two barriers,
+// the reductions and a row's first bytes take.  Rows of more than 24 576 classes (bfloat16 49 152) are not held: 4096 of 128 256 in 32 bits 855 us with 8 alternatives, 2.5 TB/s; 64 of them 44 us.
 #include "train_common.h"
 #include "../../../include/i6logp.h"
 
@@ -322,7 +326,7 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_forward(
     }
     int count = (int)s.count;
     if (count > kCandidates) {
-        // from memory, all scores: rows of this kind are few, and with what this needs the others would not keep theirs in registers
+        // from memory, all scores: with what this needs, rows that never come here would not keep theirs in registers
         const auto each = [&](auto f) I6_INLINE {
             read_pieces([&](const Vector<T>& v, int at) I6_INLINE {
 #pragma unroll
@@ -389,7 +393,6 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_forward(
 
 // ------------------------------------------------------------------------------------------------------------ backward
 
-// What every class has of the frame's sums is written first, then the classes that something comes in for are written again.
 template <typename T, int kThreads>
 __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void logp_backward(Args a) {
     using G = Team<kThreads>;
@@ -509,8 +512,8 @@ template <typename T> int forward(const Args& a, hipStream_t s) {
 
 template <typename T> int backward(const Args& a, hipStream_t s) {
     const int64_t frames = (int64_t)a.B * a.T;
-    // a wave for rows of up to 4 KB, with many rows 10 KB: 16 384 rows of 5001 in 16 bits 104 us by workgroups, 85 by waves; in 32 bits 133 and 181
-    if (a.F * sizeof(T) <= (many(a) ? 10240 : 4096)) logp_backward<T, 64><<<dim3((unsigned)ceil_div(frames, (int64_t)4)), dim3(256), 0, s>>>(a);
+    // many rows of up to 10 KB have a wave each: 16 384 of 5001 in 16 bits 72 us by workgroups, 68 by waves, of 1000 27 and 15, but of 5001 in 32 bits 124 and 175, and 1024 of 1000 4.7 and 5.9
+    if (many(a) && a.F * sizeof(T) <= 10240) logp_backward<T, 64><<<dim3((unsigned)ceil_div(frames, (int64_t)4)), dim3(256), 0, s>>>(a);
     else logp_backward<T, 256><<<dim3((unsigned)frames), dim3(256), 0, s>>>(a);
     return launched();
 }

@@ -8,8 +8,9 @@
 // B: 3.45) below 2^16; of (x1 + x2)(y1 + y2) the last term is below the precision.  Half the bits would do for the products, but not for what becomes of them: an error in A is one of
 // left singular vectors of all sizes, and the small ones grow 3.4 times in each iteration, 485 times in five.
 //
-// 24 matrices of 4096 x 2048 in 16 bits: 19.2 ms, of which 0.45 norms and operands, 4 x 1.98 + 1.16 X = B X, 5 x 1.08 A, 5 x 0.66 B: 20 TFLOP of 16-bit products at 1050 TFLOP/s, where
-// the library's product of 8192 x 8192 reaches 1135 on such values; both are bound by the matrix units and the clock that the card holds under them (2.05 - 2.15 GHz).
+// 24 matrices of 4096 x 2048 in 16 bits: 19.1 - 19.4 ms, of which 0.46 norms and operands, 4 x 2.18 + 1.19 X = B X, 5 x 1.14 A, 5 x 0.69 B: 20 TFLOP of 16-bit products at 1040 TFLOP/s, where
+// the library's product of 8192 x 8192 reaches 1135 on such values; both are bound by the matrix units and the clock that the card holds under them (1.96 - 2.15 GHz).  With the step
+// on momenta and parameters 19.9 ms.
 #include <algorithm>
 #include <cmath>
 
@@ -669,8 +670,8 @@ template <typename Groups, typename Launch> int over(Table& tab, Groups groups, 
 }
 
 // Tiles that do not fill the card: how many parts of its columns a product is formed in.  A step takes 0.8 us, a part's sums are read in half of that, another launch takes 7: so no
-// parts below 16 steps of 32 columns, four steps at least in each, and about the root of their number of them.  Without and with, in 32 bits: one matrix of 200 x 4096 656 -> 310 us,
-// of 1024 x 1024 497 -> 405, 8 of 60 x 2000 332 -> 225.  Sums in parts are also nearer: with all four products 3.0e-6 -> 1.4e-6 off 64 bits in the last of these.
+// parts below 16 steps of 32 columns, four steps at least in each, and about the root of their number of them.  Without and with, in 32 bits: one matrix of 200 x 4096 656 -> 308 us,
+// of 1024 x 1024 497 -> 404, 8 of 60 x 2000 332 -> 212.  Sums in parts are also nearer: with all four products 3.0e-6 -> 1.4e-6 off 64 bits in the last of these.
 struct Parts {
     bool few;
     int parts;
