@@ -113,7 +113,7 @@ def gated_delta_rule(
     length one (``k / sqrt(sum(k**2) + 1e-6)``): the state fades, ``S = f S``; what the key holds is replaced to the share w, ``S = S + outer(k, w (v - S.T @ k))``;
     and the query reads, ``o = S.T @ q``.
 
-    :param q: [B, T, G, K], float32 or bfloat16, K up to 128
+    :param q: [B, T, G, K], float32 or bfloat16, K up to 128; sums of squares below 2^127, as those of k
     :param k: of the same shape and type
     :param v: [B, T, H, V], of the same type, V up to 128; H is a multiple of G, and H / G neighbouring heads share a query and a key
     :param gate: [B, T, H], before the sigmoid, of the same type
